@@ -6,7 +6,7 @@ A case is a dict of plain values. "op" says which entry point it runs:
   quantize  quantize_fp8: one scale per 1 x 128 (block_rows 1) or 128 x 128 (block_rows 128, with the transposed copy) elements
   product   grouped_gemm_fp8 on operands that are in 8 bits already: a serving product
   linear    grouped_linear_fp8, forward and backward: output, gradients of the rows and of the weights
-  swiglu    swiglu_packed with its input kept in 8 bits, forward and backward
+  swiglu    swiglu_packed_fp8, the activation that keeps its input in 8 bits, forward and backward
   infer     swiglu_experts_fp8 on weights that are in 8 bits already, no backward
   train     swiglu_experts_fp8 on 16-bit weights, forward and backward: output, gradients of tokens, router weights and both weights
 
@@ -330,7 +330,7 @@ def _own(s):
         return dict(y=y.detach(), x_grad=x.grad, w_grad=w.grad)
     if op == "swiglu":
         x = _leaf(s["x"])
-        y = fma.swiglu_packed(x, checkpoint_fp8=True)
+        y = fma.swiglu_packed_fp8(x)
         y.backward(s["dy"])
         return dict(y=y.detach(), x_grad=x.grad)
     if op == "infer":
