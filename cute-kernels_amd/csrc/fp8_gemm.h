@@ -1,0 +1,540 @@
+// Grouped product of 8-bit operands, D_e = A_e B_e^T, in the block format of fp8_parts.h: tiles of 256 x 256 by v_mfma_scale_f32_16x16x128_f8f6f4,
+// which multiplies 128 elements of reduction at a time (one block) and applies both operands' scales, fp32 sums throughout.
+//
+//  * A K step is one block of 128: 32 KB of each operand, brought into one of two LDS stages by direct global -> LDS loads (addresses are a
+//    descriptor in scalar registers, one lane offset and a scalar offset; rows and columns past the end arrive as zeros). Eight wavefronts,
+//    2 x 4, 128 x 64 each, 32 matrix instructions a step; their operands are two 16-byte LDS reads per 16 rows. The instruction wants 32
+//    consecutive k a lane; both operands are given the same permutation of the block's k instead (bytes 16 q and 64 + 16 q), which leaves
+//    every sum what it is and makes the reads free of bank conflicts.
+//  * The 16 rows of B that make a fragment are not neighbours but rows 8 a + b (a, b = 0 .. 3) and, in the next fragment, 8 a + 4 + b:
+//    a lane's results of two fragments are then eight neighbouring columns, and every epilogue stores from registers: 16 bytes of a 16-bit
+//    result, 8 of an 8-bit one, with no trip through LDS.
+//  * The loads are one stream over the steps of all tiles of a workgroup, two steps ahead: the last two steps of a tile load the first
+//    two of the next. They are written in assembly, so the compiler places no waits for them; the one wait of a step, in front of its
+//    last sixteenth-row block, is written by hand, and behind it the step's own stage is free again.
+//  * Scales: a dword of four blocks per row of A (and per 128 rows of B) goes to LDS the same way every fourth step.
+//  * A reduction may be cut into segments (the two halves of a pre-activation): blocks begin anew in each.
+//  * GLU: the tile holds 128 "up" and 128 "gate" columns; the activation, 128 columns or one block, is quantised from the fp32 sums: the
+//    largest magnitude of a row goes from wavefront to wavefront through LDS. With KEEP the pre-activation is kept in 8 bits too.
+//  * GLU_BWD: the product is the gradient of the activation; the pre-activation's gradient leaves, once rounded to 16 bits for the weight
+//    gradient and once, from the unrounded values, in 8 bits for the input gradient.
+#pragma once
+
+#include "fp8_parts.h"
+#include "gemm_parts.h"
+
+namespace fmahip {
+namespace fp8 {
+
+using ::fmahip::gemm::kOutOfRange;
+using ::fmahip::gemm::lds_address;
+using ::fmahip::gemm::make_rsrc_words;
+using ::fmahip::gemm::u32x4;
+using ::fmahip::gemm::uniform;
+using ::fmahip::gemm::wait_lds;
+using ::fmahip::gemm::wait_vm;
+
+typedef __attribute__((ext_vector_type(4))) float f32x4;
+typedef __attribute__((ext_vector_type(16))) float f32x16;
+typedef __attribute__((ext_vector_type(4))) int i32x4;
+typedef __attribute__((ext_vector_type(8))) int i32x8;
+
+constexpr int kTileM = 256, kTileN = 256;
+constexpr int kWavesM = 2, kWavesN = 4, kWaves = kWavesM * kWavesN, kGemmThreads = kWaves * 64;
+constexpr int kRowBlocks = 8, kColBlocks = 4;  // 16 x 16 blocks of a wavefront's 128 x 64
+constexpr uint32_t kOperandBytes = 256 * kBlock, kStage = 2 * kOperandBytes;
+constexpr uint32_t kScaleWords = 320;  // per buffer: 256 rows of A, two blocks of B, the rest of the fifth wavefront's load
+constexpr uint32_t kMaxGroups = FMA_MAX_GROUPS;
+
+enum Epilogue { EPI_BF16, EPI_F16, EPI_F32, EPI_GLU, EPI_GLU_KEEP, EPI_GLU_BWD_BF16, EPI_GLU_BWD_F16 };
+
+struct GemmArgs {
+    const uint8_t *A, *A_s, *B, *B_s;
+    const uint32_t* sizes;      // [E] rows per group; NULL: one group of R rows
+    const int32_t* row_index;   // not NULL: row i of A is row row_index[i] / divisor of a_rows
+    uint32_t divisor, a_rows;
+    uint32_t E, R, N, K, segs;  // K: elements of a segment of the reduction
+    uint32_t a_pitch, a_seg, as_pitch, as_seg;            // bytes from row to row, from segment to segment
+    uint32_t b_seg, bs_pitch, bs_seg, b_half, bs_half;    // half: from an expert's "up" matrix to its "gate" matrix
+    uint64_t b_group, bs_group;
+    void* D;                    // plain: [R, N]; GLU_BWD: [R, 2 N], the pre-activation's gradient
+    uint8_t *out, *out_s;       // GLU: activation [R, N]; GLU_BWD: the pre-activation's gradient [R, 2, N]
+    uint8_t *h, *h_s;           // pre-activation [R, 2, N]: written by GLU_KEEP, read by GLU_BWD
+    uint32_t o_pitch_s;         // bytes of scales of N elements
+};
+
+__device__ __forceinline__ void load_lds16(u32x4 rsrc, uint32_t voff, uint32_t soff, uint32_t lds) {
+    ::fmahip::gemm::buffer_load_lds_quiet(rsrc, voff, soff, lds);
+}
+__device__ __forceinline__ void fence_lds() { asm volatile("" ::: "memory"); }
+// every LDS access of the workgroup in front of it is done (global stores stay in flight)
+__device__ __forceinline__ void lds_barrier() {
+    wait_lds();
+    __builtin_amdgcn_s_barrier();
+    fence_lds();
+}
+__device__ __forceinline__ u32x4 rsrc_at(uint64_t base, uint32_t bytes) {
+    return u32x4{(uint32_t)base, (uint32_t)(base >> 32) & 0xffffu, bytes, 0x00020000u};
+}
+__device__ __forceinline__ uint64_t uniform64(uint64_t x) { return ((uint64_t)uniform((uint32_t)(x >> 32)) << 32) | uniform((uint32_t)x); }
+
+template <int EPI, bool GATHER>
+__global__ __launch_bounds__(kGemmThreads) void fp8_gemm_kernel(const GemmArgs args) {
+    constexpr bool kGlu = EPI == EPI_GLU || EPI == EPI_GLU_KEEP;
+    constexpr bool kBwd = EPI == EPI_GLU_BWD_BF16 || EPI == EPI_GLU_BWD_F16;
+    constexpr uint32_t kCols = kGlu ? kTileN / 2 : kTileN;  // columns of the output grid per tile
+    constexpr int kMaxima = EPI == EPI_GLU_KEEP ? 3 : (kGlu ? 1 : (kBwd ? 1 : 0));
+
+    __shared__ __attribute__((aligned(1024))) uint8_t s_op[2 * kStage];
+    __shared__ __attribute__((aligned(256))) uint32_t s_scale[2 * kScaleWords];
+    __shared__ __attribute__((aligned(16))) uint32_t s_max[kMaxima ? kMaxima * 256 * 4 : 4];
+    __shared__ uint32_t s_tiles[kMaxGroups + 1];  // row tiles of the groups before
+    __shared__ uint32_t s_first[kMaxGroups + 1];  // first row of the group
+
+    const uint32_t tid = threadIdx.x, lane = tid & 63u;
+    const uint32_t wave = uniform(tid >> 6);
+    const uint32_t wm = wave / kWavesN, wn = wave % kWavesN;
+    const uint32_t r16 = lane & 15u, q = lane >> 4;
+    const uint32_t E = args.E, N = args.N, K = args.K;
+
+    // ---- group table: rows past R do not exist, whatever the sizes say ----
+    if (wave == 0) {
+        uint32_t tiles = 0, rows = 0;
+        for (uint32_t base = 0; base < E; base += 64) {
+            const uint32_t e = base + lane;
+            uint32_t m = e < E ? (args.sizes ? args.sizes[e] : args.R) : 0u;
+            m = m < args.R ? m : args.R;
+            // (sums of 64 values of at most R fit 64 bits; what counts is clamped to R)
+            const uint64_t end = rows + wave_inclusive_scan<uint64_t>(m);
+            const uint32_t last = end < args.R ? (uint32_t)end : args.R;
+            const uint64_t before = end - m;
+            const uint32_t first = before < args.R ? (uint32_t)before : args.R;
+            const uint32_t t = (last - first + kTileM - 1) / kTileM;
+            const uint32_t it = wave_inclusive_scan<uint32_t>(t);
+            if (e < E) {
+                s_tiles[e] = tiles + it - t;
+                s_first[e] = first;
+            }
+            tiles += __shfl(it, 63, 64);
+            rows = __shfl(last, 63, 64);
+        }
+        if (lane == 0) {
+            s_tiles[E] = tiles;
+            s_first[E] = rows;
+        }
+    }
+    __syncthreads();
+    const uint32_t col_tiles = (N + kCols - 1) / kCols;
+    const uint32_t total = uniform(s_tiles[E]) * col_tiles;
+    const uint32_t grid = gridDim.x, per_xcd = grid / 8u;
+    const uint32_t slot = grid % 8u == 0 ? (blockIdx.x % 8u) * per_xcd + blockIdx.x / 8u : blockIdx.x;
+    if (slot >= total) return;
+
+    const uint32_t k_blocks = (K + kBlock - 1) / kBlock;
+    const uint32_t steps = k_blocks * args.segs;
+
+    struct Tile {
+        uint32_t e, row0, rows, n0;  // group, first packed row, rows, first column
+    };
+    // tile t (below `total`) of the sequence: a group's tiles one after the other, in blocks of eight row tiles, column by column
+    auto find = [&](uint32_t t) -> Tile {
+        const uint32_t row_tile = t / col_tiles;
+        uint32_t e = 0;
+        for (uint32_t base = 0; base < E; base += 64) {
+            const bool before = base + lane < E && s_tiles[base + lane + 1] <= row_tile;
+            const uint32_t n = (uint32_t)__popcll(__ballot(before));
+            e += n;
+            if (n < 64) break;
+        }
+        e = uniform(e);
+        const uint32_t t0 = uniform(s_tiles[e]), mt = uniform(s_tiles[e + 1]) - t0;
+        const uint32_t first = uniform(s_first[e]), end = uniform(s_first[e + 1]);
+        const uint32_t in = t - t0 * col_tiles;
+        const uint32_t block = in / (8u * col_tiles), at = in - block * 8u * col_tiles;
+        const uint32_t height = mt - block * 8u < 8u ? mt - block * 8u : 8u;
+        const uint32_t n = at / height, m = block * 8u + at - n * height;
+        Tile tile;
+        tile.e = e;
+        tile.row0 = first + m * kTileM;
+        tile.rows = end - tile.row0 < (uint32_t)kTileM ? end - tile.row0 : (uint32_t)kTileM;
+        tile.n0 = n * kCols;
+        return tile;
+    };
+
+    // ---- the load stream ----
+    const uint32_t lr = lane >> 3, lp = lane & 7u;
+    const uint32_t a_chunk = (lp ^ (((wave * 8u + lr) >> 1) & 7u)) * 16u;
+    const uint32_t b_chunk = (lp ^ ((wave & 3u) * 2u + ((lr >> 1) & 1u))) * 16u;
+    const uint32_t a_lane = (wave * 8u + lr) * args.a_pitch + a_chunk;
+    const uint32_t b_lane = (wave * 8u + lr) * K + b_chunk;
+    const uint32_t lds0 = lds_address(s_op);
+    const uint32_t lds_scale = lds_address(reinterpret_cast<const uint8_t*>(s_scale)) + wave * 256u;
+    uint32_t l_tile = slot, l_ks = 0, l_seg = 0, l_stage = 0, l_quad = 0;  // next step to be loaded
+    uint64_t l_a = 0, l_b = 0, l_b2 = 0, l_s = 0;  // addresses of the operands and of this wavefront's scales, at the current segment
+    uint32_t l_a_bytes = 0, l_b_bytes = 0;
+    uint32_t l_gather[4] = {0u, 0u, 0u, 0u};
+    uint32_t l_scale = kOutOfRange;  // this lane's offset into the scales
+    auto aim = [&]() {
+        if (l_tile >= total) {
+            l_a_bytes = l_b_bytes = 0;
+            l_scale = kOutOfRange;
+            if constexpr (GATHER) {
+#pragma unroll
+                for (int i = 0; i < 4; ++i) l_gather[i] = kOutOfRange;
+            }
+            return;
+        }
+        const Tile t = find(l_tile);
+        const uint32_t n_block = t.n0 / kBlock;
+        l_b = uniform64((uint64_t)(uintptr_t)args.B + t.e * args.b_group + (uint64_t)t.n0 * K);
+        const uint32_t cols = N - t.n0 < kCols ? N - t.n0 : kCols;
+        l_b_bytes = uniform(cols * K);
+        if constexpr (kGlu) l_b2 = uniform64(l_b + args.b_half);
+        if constexpr (GATHER) {
+            l_a = uniform64((uint64_t)(uintptr_t)args.A);
+            l_a_bytes = args.a_rows * args.a_pitch;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const uint32_t r = i * 64u + wave * 8u + lr;
+                const uint32_t src = r < t.rows ? (uint32_t)args.row_index[t.row0 + r] / args.divisor : args.a_rows;
+                l_gather[i] = src < args.a_rows ? src * args.a_pitch + a_chunk : kOutOfRange;
+            }
+        } else {
+            l_a = uniform64((uint64_t)(uintptr_t)args.A + (uint64_t)t.row0 * args.a_pitch);
+            l_a_bytes = uniform(t.rows * args.a_pitch);
+        }
+        if (wave < 4) {
+            const uint32_t r = wave * 64u + lane;
+            l_s = (uint64_t)(uintptr_t)args.A_s;
+            if constexpr (GATHER) {
+                const uint32_t src = r < t.rows ? (uint32_t)args.row_index[t.row0 + r] / args.divisor : args.a_rows;
+                l_scale = src < args.a_rows ? src * args.as_pitch : kOutOfRange;
+            } else {
+                l_s += (uint64_t)t.row0 * args.as_pitch;
+                l_scale = r < t.rows ? r * args.as_pitch : kOutOfRange;
+            }
+        } else {
+            l_s = (uint64_t)(uintptr_t)args.B_s + t.e * args.bs_group + (uint64_t)n_block * args.bs_pitch;
+            l_scale = lane == 0 ? 0u : kOutOfRange;
+            if constexpr (kGlu) {
+                if (lane == 1) l_scale = args.bs_half;
+            } else {
+                if (lane == 1 && t.n0 + kBlock < N) l_scale = args.bs_pitch;
+            }
+        }
+        l_s = uniform64(l_s);
+    };
+    auto load_a = [&](int i) {
+        uint32_t v = GATHER ? l_gather[i] : a_lane;
+        if (l_ks * kBlock + a_chunk >= K) v = kOutOfRange;
+        load_lds16(rsrc_at(l_a, l_a_bytes), v, (GATHER ? 0u : (uint32_t)i * 64u * args.a_pitch) + l_ks * kBlock,
+                   lds0 + l_stage + ((uint32_t)i * 8u + wave) * 1024u);
+    };
+    auto load_b = [&](int i) {
+        const uint32_t v = l_ks * kBlock + b_chunk >= K ? kOutOfRange : b_lane;
+        const uint32_t rows = kGlu ? (uint32_t)(i & 1) * 64u : (uint32_t)i * 64u;
+        load_lds16(rsrc_at(kGlu && i >= 2 ? l_b2 : l_b, l_b_bytes), v, rows * K + l_ks * kBlock,
+                   lds0 + l_stage + kOperandBytes + ((uint32_t)i * 8u + wave) * 1024u);
+    };
+    auto load_scales = [&]() {  // at the first of four steps
+        if ((l_ks & 3u) == 0 && wave < 5)
+            ::fmahip::gemm::buffer_load_lds_quiet_b32(rsrc_at(l_s, 0x7fffffffu), l_scale, l_ks, lds_scale + l_quad * (kScaleWords * 4u));
+    };
+    auto next_load = [&]() {
+        l_stage ^= kStage;
+        ++l_ks;
+        if (l_ks == k_blocks) {
+            l_ks = 0;
+            ++l_seg;
+            if (l_seg == args.segs) {
+                l_seg = 0;
+                l_tile += grid;
+                aim();
+            } else {
+                l_a += args.a_seg;
+                l_b += args.b_seg;
+                l_s += wave < 4 ? args.as_seg : args.bs_seg;
+            }
+        }
+        if ((l_ks & 3u) == 0) l_quad ^= 1u;
+    };
+
+    // ---- fragments ----
+    const uint32_t a_key = (r16 >> 1) & 7u, b_key = (r16 >> 2) * 2u + ((r16 >> 1) & 1u);
+    const uint32_t a_off = (wm * 128u + r16) * kBlock + ((q ^ a_key) << 4);
+    const uint32_t b_base = kGlu ? wn * 32u : wn * 64u;
+    const uint32_t b_off = kOperandBytes + (b_base + (r16 >> 2) * 8u + (r16 & 3u)) * kBlock + ((q ^ b_key) << 4);
+    // bytes from fragment 0 of B to fragment j
+    auto b_step = [](int j) -> uint32_t { return (uint32_t)((kGlu ? (j >> 1) * 128 : (j >> 1) * 32) + (j & 1) * 4) * kBlock; };
+    const uint8_t* const sc = reinterpret_cast<const uint8_t*>(s_scale);
+    const uint32_t sa_off = (wm * 128u + r16) * 4u;
+    const uint32_t sb_off = (256u + (kGlu ? 0u : wn >> 1)) * 4u;
+    uint32_t c_stage = 0, c_ks = 0, c_quad = 0;  // the step whose fragments are read
+
+    auto read_frag = [&](uint32_t off) -> i32x8 {
+        const i32x4 lo = *reinterpret_cast<const i32x4*>(s_op + (c_stage + off));
+        const i32x4 hi = *reinterpret_cast<const i32x4*>(s_op + (c_stage + (off ^ 64u)));
+        return __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
+    };
+    auto read_scale = [&](uint32_t off) -> int { return (int)sc[c_quad * (kScaleWords * 4u) + off + (c_ks & 3u)]; };
+
+    // A row block's results are one 16-register value: the instruction's 4-register form has no variant whose result stays in place, and
+    // without the value being named after every instruction results wander through the register file until it spills.
+    f32x16 acc[kRowBlocks];
+    i32x8 fa[2], fb[kColBlocks];
+    int sa[2], sb[2];
+    auto read_a = [&](int i, int buf) {
+        fa[buf] = read_frag(a_off + (uint32_t)i * 16u * kBlock);
+        sa[buf] = read_scale(sa_off + (uint32_t)i * 64u);
+    };
+    auto read_b = [&](int j) { fb[j] = read_frag(b_off + b_step(j)); };
+    auto read_sb = [&]() {
+        sb[0] = read_scale(sb_off);
+        sb[1] = kGlu ? read_scale(sb_off + 4u) : sb[0];
+    };
+    auto mma = [&](int i, int j, int buf, int scale_b) {
+        f32x16& c = acc[i];
+        f32x4 v = {c[4 * j], c[4 * j + 1], c[4 * j + 2], c[4 * j + 3]};
+        v = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(fb[j], fa[buf], v, 0, 0, 0, scale_b, 0, sa[buf]);
+        c[4 * j] = v[0];
+        c[4 * j + 1] = v[1];
+        c[4 * j + 2] = v[2];
+        c[4 * j + 3] = v[3];
+        asm("" : "+v"(c));
+    };
+    auto next_step = [&]() {  // of the fragments
+        c_stage ^= kStage;
+        ++c_ks;
+        if (c_ks == k_blocks) c_ks = 0;
+        if ((c_ks & 3u) == 0) c_quad ^= 1u;
+    };
+
+    // ---- the first two steps ----
+    aim();
+#pragma unroll 1
+    for (int s = 0; s < 2; ++s) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) load_b(i);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) load_a(i);
+        load_scales();
+        next_load();
+    }
+    wait_vm<0>();
+    lds_barrier();
+    read_sb();
+#pragma unroll
+    for (int j = 0; j < kColBlocks; ++j) read_b(j);
+    read_a(0, 0);
+
+    for (uint32_t c_tile = slot; c_tile < total; c_tile += grid) {
+#pragma unroll
+        for (int i = 0; i < kRowBlocks; ++i)
+#pragma unroll
+            for (int x = 0; x < 16; ++x) acc[i][x] = 0.f;
+
+        for (uint32_t step = 0; step < steps; ++step) {
+#pragma unroll
+            for (int i = 0; i < kRowBlocks - 1; ++i) {
+                read_a(i + 1, (i + 1) & 1);
+#pragma unroll
+                for (int j = 0; j < kColBlocks; ++j) mma(i, j, i & 1, sb[j >> 1]);
+                __builtin_amdgcn_sched_barrier(0);
+            }
+            // Every fragment of this step is read, and the next step has landed: its stage is read from here on, this step's is loaded into.
+            wait_vm<0>();
+            lds_barrier();
+            next_step();
+            {
+                constexpr int i = kRowBlocks - 1;
+                const int s0 = sb[0], s1 = sb[1];
+                read_sb();
+#pragma unroll
+                for (int j = 0; j < kColBlocks; ++j) {
+                    mma(i, j, i & 1, j < 2 ? s0 : s1);
+                    load_b(j);
+                    load_a(j);
+                    read_b(j);
+                }
+                read_a(0, 0);
+            }
+            load_scales();
+            next_load();
+        }
+
+        // ---- epilogue ----
+        const Tile t = find(c_tile);
+        if constexpr (EPI == EPI_BF16 || EPI == EPI_F16 || EPI == EPI_F32) {
+            using T = std::conditional_t<EPI == EPI_BF16, bf16_t, std::conditional_t<EPI == EPI_F16, f16_t, float>>;
+            T* const D = (T*)args.D;
+#pragma unroll
+            for (int i = 0; i < kRowBlocks; ++i) {
+                const uint32_t row = wm * 128u + (uint32_t)i * 16u + r16;
+                if (row < t.rows) {
+#pragma unroll
+                    for (int p = 0; p < 2; ++p) {
+                        const uint32_t col = t.n0 + wn * 64u + (uint32_t)p * 32u + q * 8u;
+                        float v[8];
+#pragma unroll
+                        for (int x = 0; x < 8; ++x) v[x] = acc[i][8 * p + x];
+                        T* const to = D + (uint64_t)(t.row0 + row) * N + col;
+                        if (N % 8u == 0) {
+                            if (col < N) {
+                                constexpr int V = Vec16<T>::N;
+#pragma unroll
+                                for (int c = 0; c < 8 / V; ++c) {
+                                    Vec16<T> o;
+#pragma unroll
+                                    for (int x = 0; x < V; ++x) o.v[x] = Num<T>::down(v[c * V + x]);
+                                    *(reinterpret_cast<Vec16<T>*>(to) + c) = o;
+                                }
+                            }
+                        } else {
+#pragma unroll
+                            for (int x = 0; x < 8; ++x)
+                                if (col + x < N) to[x] = Num<T>::down(v[x]);
+                        }
+                    }
+                }
+            }
+        } else if constexpr (kGlu) {
+            const uint32_t col = t.n0 + wn * 32u + q * 8u, block = t.n0 / kBlock;
+            // magnitudes of the row's columns of this wavefront
+            auto row_max = [&](uint32_t m) -> uint32_t {
+                m = max_u32(m, (uint32_t)__shfl_xor((int)m, 16, 64));
+                return max_u32(m, (uint32_t)__shfl_xor((int)m, 32, 64));
+            };
+            constexpr int kWhat = EPI == EPI_GLU_KEEP ? 3 : 1;
+            auto activation = [&](int i, int x) -> float {
+                const float u = acc[i][x], g = acc[i][8 + x];
+                return u * g * sigmoid_clamped_fast(g);
+            };
+#pragma unroll
+            for (int i = 0; i < kRowBlocks; ++i) {
+                uint32_t m[3] = {0u, 0u, 0u};
+#pragma unroll
+                for (int x = 0; x < 8; ++x) {
+                    m[0] = max_u32(m[0], magnitude_bits(activation(i, x)));
+                    if constexpr (kWhat == 3) {
+                        m[1] = max_u32(m[1], magnitude_bits(acc[i][x]));
+                        m[2] = max_u32(m[2], magnitude_bits(acc[i][8 + x]));
+                    }
+                }
+#pragma unroll
+                for (int w = 0; w < kWhat; ++w) {
+                    const uint32_t v = row_max(m[w]);
+                    if (q == 0) s_max[((uint32_t)w * 256u + wm * 128u + (uint32_t)i * 16u + r16) * 4u + wn] = v;
+                }
+                __builtin_amdgcn_sched_barrier(0);
+            }
+            lds_barrier();
+            // (activations are computed anew rather than kept: 64 more registers)
+#pragma unroll
+            for (int i = 0; i < kRowBlocks; ++i) asm("" : "+v"(acc[i]));
+#pragma unroll
+            for (int i = 0; i < kRowBlocks; ++i) {
+                const uint32_t row = wm * 128u + (uint32_t)i * 16u + r16;
+                if (row < t.rows) {
+                    const uint64_t to = t.row0 + row;
+#pragma unroll
+                    for (int w = 0; w < kWhat; ++w) {
+                        const uint4 m = *reinterpret_cast<const uint4*>(s_max + ((uint32_t)w * 256u + row) * 4u);
+                        const uint32_t byte = scale_byte(max_u32(max_u32(m.x, m.y), max_u32(m.z, m.w)));
+                        const float inverse = scale_inverse(byte);
+                        float v[8];
+#pragma unroll
+                        for (int x = 0; x < 8; ++x)
+                            v[x] = (w == 0 ? activation(i, x) : acc[i][(w == 2 ? 8 : 0) + x]) * inverse;
+                        uint2 o;
+                        o.x = pack4(v[0], v[1], v[2], v[3]);
+                        o.y = pack4(v[4], v[5], v[6], v[7]);
+                        uint8_t* const values = w == 0 ? args.out + to * N : args.h + to * (2u * (uint64_t)N) + (w == 2 ? N : 0u);
+                        uint8_t* const scales = w == 0 ? args.out_s + to * args.o_pitch_s : args.h_s + to * (2u * (uint64_t)args.o_pitch_s) + (w == 2 ? args.o_pitch_s : 0u);
+                        if (col < N) *reinterpret_cast<uint2*>(values + col) = o;
+                        if (q == 0 && wn == 0) scales[block] = (uint8_t)byte;
+                    }
+                }
+                __builtin_amdgcn_sched_barrier(0);
+            }
+        } else {
+            using T = std::conditional_t<EPI == EPI_GLU_BWD_BF16, bf16_t, f16_t>;
+            // columns of block wn / 2 of the tile's two
+            const uint32_t block = t.n0 / kBlock + (wn >> 1);
+            const uint32_t s_pitch = args.o_pitch_s;
+#pragma unroll
+            for (int i = 0; i < kRowBlocks; ++i) {
+                const uint32_t row = wm * 128u + (uint32_t)i * 16u + r16;
+                const bool live = row < t.rows;
+                const uint64_t to = t.row0 + (live ? row : 0u);
+                float d[2][2][8];  // [half][columns p][x]
+                uint32_t m[2] = {0u, 0u};
+                const bool in = t.n0 + (wn >> 1) * kBlock < N;
+                const float su = in ? scale_value(args.h_s[to * (2u * (uint64_t)s_pitch) + block]) : 0.f;
+                const float sg = in ? scale_value(args.h_s[to * (2u * (uint64_t)s_pitch) + s_pitch + block]) : 0.f;
+#pragma unroll
+                for (int p = 0; p < 2; ++p) {
+                    const uint32_t col = t.n0 + wn * 64u + (uint32_t)p * 32u + q * 8u;
+                    uint2 hu = {0u, 0u}, hg = {0u, 0u};
+                    if (col < N) {
+                        hu = *reinterpret_cast<const uint2*>(args.h + to * (2u * (uint64_t)N) + col);
+                        hg = *reinterpret_cast<const uint2*>(args.h + to * (2u * (uint64_t)N) + N + col);
+                    }
+                    float u[8], g[8];
+                    unpack4(hu.x, *reinterpret_cast<float(*)[4]>(u));
+                    unpack4(hu.y, *reinterpret_cast<float(*)[4]>(u + 4));
+                    unpack4(hg.x, *reinterpret_cast<float(*)[4]>(g));
+                    unpack4(hg.y, *reinterpret_cast<float(*)[4]>(g + 4));
+#pragma unroll
+                    for (int x = 0; x < 8; ++x) {
+                        swiglu_b<T>(g[x] * sg, u[x] * su, acc[i][8 * p + x], d[1][p][x], d[0][p][x]);
+                        m[0] = max_u32(m[0], magnitude_bits(d[0][p][x]));
+                        m[1] = max_u32(m[1], magnitude_bits(d[1][p][x]));
+                    }
+                }
+                // the other wavefront of the block has its half of the row: slots alternate, so one barrier per row block is enough
+                uint32_t* const slots = s_max + (uint32_t)(i & 1) * 256u;  // [wave][half][16]
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    m[h] = max_u32(m[h], (uint32_t)__shfl_xor((int)m[h], 16, 64));
+                    m[h] = max_u32(m[h], (uint32_t)__shfl_xor((int)m[h], 32, 64));
+                    if (q == 0) slots[(wave * 2u + (uint32_t)h) * 16u + r16] = m[h];
+                }
+                lds_barrier();
+                if (live) {
+#pragma unroll
+                    for (int h = 0; h < 2; ++h) {
+                        const uint32_t byte = scale_byte(max_u32(m[h], slots[((wave ^ 1u) * 2u + (uint32_t)h) * 16u + r16]));
+                        const float inverse = scale_inverse(byte);
+                        if (q == 0 && (wn & 1u) == 0 && in) args.out_s[to * (2u * (uint64_t)s_pitch) + (uint32_t)h * s_pitch + block] = (uint8_t)byte;
+#pragma unroll
+                        for (int p = 0; p < 2; ++p) {
+                            const uint32_t col = t.n0 + wn * 64u + (uint32_t)p * 32u + q * 8u;
+                            const float(&v)[8] = d[h][p];
+                            if (col < N) {
+                                const uint64_t at = to * (2u * (uint64_t)N) + (uint32_t)h * (uint64_t)N + col;
+                                Vec16<T> o;
+#pragma unroll
+                                for (int x = 0; x < 8; ++x) o.v[x] = Num<T>::down(v[x]);
+                                *reinterpret_cast<Vec16<T>*>((T*)args.D + at) = o;
+                                uint2 o8;
+                                o8.x = pack4(v[0] * inverse, v[1] * inverse, v[2] * inverse, v[3] * inverse);
+                                o8.y = pack4(v[4] * inverse, v[5] * inverse, v[6] * inverse, v[7] * inverse);
+                                *reinterpret_cast<uint2*>(args.out + at) = o8;
+                            }
+                        }
+                    }
+                }
+                __builtin_amdgcn_sched_barrier(0);
+            }
+            // the next tile's first fragments once more: 42 registers that this epilogue uses meanwhile
+            read_sb();
+#pragma unroll
+            for (int j = 0; j < kColBlocks; ++j) read_b(j);
+            read_a(0, 0);
+        }
+    }
+    wait_vm<0>();  // loads past the last step write zeros into LDS: they are done when the workgroup ends
+}
+
+}  // namespace fp8
+}  // namespace fmahip

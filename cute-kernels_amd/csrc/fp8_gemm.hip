@@ -1,0 +1,76 @@
+// Launches of the grouped product of 8-bit operands (fp8_gemm.h) and its C entry point.
+#include "fp8_gemm_launch.h"
+
+namespace fmahip {
+namespace fp8 {
+
+int check_gemm(const char* who, int64_t E, int64_t R, int64_t N, int64_t K, int64_t segs) {
+    FMA_REQUIRE(E >= 0 && R >= 0 && N >= 0 && K >= 1, FMA_ERR_BAD_SIZE, "%s: bad size E=%lld R=%lld N=%lld K=%lld", who, (long long)E,
+                (long long)R, (long long)N, (long long)K);
+    FMA_REQUIRE(E <= FMA_MAX_GROUPS, FMA_ERR_TOO_MANY_EXPERTS, "%s: E=%lld, at most %d groups", who, (long long)E, FMA_MAX_GROUPS);
+    FMA_REQUIRE(K % 16 == 0, FMA_ERR_BAD_SIZE, "%s: rows of whole 16-byte pieces: K=%lld is no multiple of 16", who, (long long)K);
+    FMA_REQUIRE(K < (1 << 21) && N < (1 << 23) && R < (1ll << 31), FMA_ERR_TOO_MANY_ELEMENTS, "%s: K < 2^21, N < 2^23, R < 2^31", who);
+    const int64_t row_tiles = R / kTileM + E + 1, col_tiles = (N + kTileN / 2 - 1) / (kTileN / 2);
+    FMA_REQUIRE(row_tiles * col_tiles < (1ll << 30), FMA_ERR_TOO_MANY_ELEMENTS, "%s: more than 2^30 tiles", who);
+    FMA_REQUIRE(segs * N * K < (1ll << 32), FMA_ERR_TOO_MANY_ELEMENTS, "%s: a group's matrix has 2^32 bytes or more", who);
+    return FMA_OK;
+}
+
+int launch_gemm(const char* who, int epilogue, const GemmArgs& args, hipStream_t st) {
+    const bool glu = epilogue == EPI_GLU || epilogue == EPI_GLU_KEEP;
+    const int64_t cols = glu ? kTileN / 2 : kTileN;
+    // the host does not know the sizes: as many workgroups as the rows could make tiles, or one per compute unit
+    const int64_t tiles = ((int64_t)args.R / kTileM + (args.E < args.R ? args.E : args.R)) * ((args.N + cols - 1) / cols);
+    const int64_t cus = num_compute_units() > 0 ? num_compute_units() : 256;
+    const dim3 grid((uint32_t)(tiles < cus ? tiles : cus)), block(kGemmThreads);
+    auto run = [&](auto kernel) { hipLaunchKernelGGL(kernel, grid, block, 0, st, args); };
+    const bool gather = args.row_index != nullptr;
+    switch (epilogue) {
+        case EPI_BF16: run(fp8_gemm_kernel<EPI_BF16, false>); break;
+        case EPI_F16: run(fp8_gemm_kernel<EPI_F16, false>); break;
+        case EPI_F32: run(fp8_gemm_kernel<EPI_F32, false>); break;
+        case EPI_GLU: gather ? run(fp8_gemm_kernel<EPI_GLU, true>) : run(fp8_gemm_kernel<EPI_GLU, false>); break;
+        case EPI_GLU_KEEP: gather ? run(fp8_gemm_kernel<EPI_GLU_KEEP, true>) : run(fp8_gemm_kernel<EPI_GLU_KEEP, false>); break;
+        case EPI_GLU_BWD_BF16: run(fp8_gemm_kernel<EPI_GLU_BWD_BF16, false>); break;
+        default: run(fp8_gemm_kernel<EPI_GLU_BWD_F16, false>); break;
+    }
+    return launch_status(who);
+}
+
+}  // namespace fp8
+}  // namespace fmahip
+
+extern "C" {
+
+int fma_grouped_gemm_fp8(const void* A, const void* A_scales, const void* B, const void* B_scales, void* D, const uint32_t* M_arr, int64_t E,
+                         int64_t R, int64_t N, int64_t K, int dtype, void* stream) {
+    using namespace fmahip;
+    using namespace fmahip::fp8;
+    FMA_REQUIRE(dtype_bytes(dtype) != 0, FMA_ERR_BAD_DTYPE, "grouped_gemm_fp8: dtype code %d", dtype);
+    if (const int rc = check_gemm("grouped_gemm_fp8", E, R, N, K, 1)) return rc;
+    FMA_REQUIRE(M_arr || E <= 1, FMA_ERR_NULL_POINTER, "grouped_gemm_fp8: M_arr is NULL, and there are %lld groups", (long long)E);
+    if (E == 0 || R == 0 || N == 0) return FMA_OK;
+    FMA_REQUIRE(A && A_scales && B && B_scales && D, FMA_ERR_NULL_POINTER, "grouped_gemm_fp8: an operand is NULL");
+    FMA_REQUIRE(aligned16(A) && aligned16(B) && aligned16(D), FMA_ERR_MISALIGNED, "grouped_gemm_fp8: A, B and D must be aligned to 16 bytes");
+    FMA_REQUIRE(((reinterpret_cast<uintptr_t>(A_scales) | reinterpret_cast<uintptr_t>(B_scales)) & 3u) == 0, FMA_ERR_MISALIGNED,
+                "grouped_gemm_fp8: scales must be aligned to 4 bytes");
+    GemmArgs a = {};
+    a.A = (const uint8_t*)A;
+    a.A_s = (const uint8_t*)A_scales;
+    a.B = (const uint8_t*)B;
+    a.B_s = (const uint8_t*)B_scales;
+    a.sizes = M_arr;
+    a.E = (uint32_t)E;
+    a.R = (uint32_t)R;
+    a.N = (uint32_t)N;
+    a.K = (uint32_t)K;
+    a.segs = 1;
+    a.a_pitch = (uint32_t)K;
+    a.as_pitch = a.bs_pitch = (uint32_t)scale_pitch(K);
+    a.b_group = (uint64_t)N * K;
+    a.bs_group = (uint64_t)((N + kBlock - 1) / kBlock) * a.bs_pitch;
+    a.D = D;
+    return launch_gemm("grouped_gemm_fp8", dtype == FMA_F32 ? EPI_F32 : (dtype == FMA_F16 ? EPI_F16 : EPI_BF16), a, (hipStream_t)stream);
+}
+
+}  // extern "C"

@@ -3,6 +3,18 @@ signatures for the ops and the module on that path, computed by hand-written HIP
 
 from .kernel_backend import KernelBackend
 from .math import ceil_divide, divide_if_divisible
-from .modules import MoE
-from .ops import continuous_count, fused_residual_add_rmsnorm, grouped_gemm, swiglu, swiglu_packed
+from .modules import MoE, quantize_expert_weights, swiglu_experts_fp8
+from .ops import (
+    Fp8Blocks,
+    continuous_count,
+    dequantize_fp8,
+    fused_residual_add_rmsnorm,
+    grouped_gemm,
+    grouped_gemm_fp8,
+    grouped_linear_fp8,
+    quantize_fp8,
+    swiglu,
+    swiglu_packed,
+    swiglu_packed_fp8,
+)
 from .utils import ensure_contiguous, set_seed

@@ -15,6 +15,7 @@ from torch.autograd import forward_ad
 
 from ...kernel_backend import KernelBackend, is_hip_kernel_backend
 from ...ops.swiglu import swiglu_packed
+from .fp8_implementation import quantize_expert_weights, swiglu_experts_fp8
 from .cuda_implementation import (
     add_expert_bias,
     build_routing_index,
@@ -205,6 +206,10 @@ class MoE(nn.Module):
         # the activation's backward inside the second projection's input-gradient GEMM (see _runs_swiglu_experts_as_one_node)
         self.fuse_swiglu_backward = True
 
+        # the experts' products in 8 bits (swiglu_experts_fp8): a SwiGLU layer without biases in a 16-bit type
+        self.fp8_experts = False
+        self._fp8_weights: tuple | None = None  # what quantize_experts() made, and the versions it made it of
+
         self.act = activation_function
         # swiglu_packed as the activation of a GLU layer is computed inside the up-projection's epilogue (a kernel for
         # rows of whole 16-byte pieces; other sizes run the GEMM's element-wise path and the activation after it)
@@ -306,6 +311,9 @@ class MoE(nn.Module):
         if not is_hip_kernel_backend(kernel_backend):
             raise ValueError(f"unexpected kernel_backend ({kernel_backend})")
 
+        if self.fp8_experts:
+            return self._compute_experts_fp8(hidden_states, router_weights, selected_experts)
+
         # counts, offsets and the stable expert-major order of the (token, choice) slots, with its inverse
         expert_frequency, expert_offsets, sorted_scattered_idxs, _, inverse = build_routing_index(
             selected_experts, self.num_experts, token_block_histogram
@@ -362,6 +370,41 @@ class MoE(nn.Module):
 
         return hidden_states
 
+    def quantize_experts(self) -> "MoE":
+        """Switches the experts' products to 8 bits (fp8_experts) and lays both projections out in 8 bits once, for calls that no backward
+        pass follows: a serving program calls it after loading the weights, and again after changing them (a forward pass on weights that
+        have changed since quantises them in the call, as one without this call does)."""
+        self._check_fp8_experts(self.c_fc.weight.dtype)
+        self.fp8_experts = True
+        with torch.no_grad():
+            self._fp8_weights = (self._weight_versions(), quantize_expert_weights(self.c_fc.weight, self.c_proj.weight))
+        return self
+
+    def _weight_versions(self) -> tuple:
+        # (module.to() puts other memory behind a parameter without advancing its version)
+        return tuple((t, t._version, t.data_ptr(), t.dtype) for t in (self.c_fc.weight, self.c_proj.weight))
+
+    def _check_fp8_experts(self, dtype: torch.dtype) -> None:
+        if not (self.c_fc.out_features == 2 * self.intermediate_size and _is_swiglu_packed(self.act)):
+            raise ValueError("fp8_experts: the layer's activation should be swiglu_packed")
+        if self.c_fc.bias is not None or self.c_proj.bias is not None:
+            raise ValueError("fp8_experts: a layer with biases has no 8-bit path")
+        if dtype not in (torch.bfloat16, torch.float16) or not self.c_fc.weight.dtype == self.c_proj.weight.dtype == dtype:
+            raise ValueError("fp8_experts: tokens and weights should both be bfloat16 or float16")
+        if self.hidden_size % 16 != 0 or self.intermediate_size % 16 != 0:
+            raise ValueError("fp8_experts: hidden and intermediate size should be multiples of 16")
+
+    def _compute_experts_fp8(
+        self, hidden_states: torch.Tensor, router_weights: torch.Tensor, selected_experts: torch.Tensor
+    ) -> torch.Tensor:
+        self._check_fp8_experts(hidden_states.dtype)
+        weights = self.c_fc.weight, self.c_proj.weight
+        if self._fp8_weights is not None and not torch.is_grad_enabled():
+            made_of, blocks = self._fp8_weights
+            if all(a[0] is b[0] and a[1:] == b[1:] for a, b in zip(made_of, self._weight_versions())):
+                weights = blocks
+        return swiglu_experts_fp8(hidden_states, router_weights, selected_experts, *weights)
+
     def _decode_operands(self, hidden_states: torch.Tensor, kernel_backend: KernelBackend) -> tuple | None:
         """The weights and biases of the layer if the whole forward pass is one native call: no backward, up to 32 rows per expert
         on average (the line of _runs_thin_experts, whose kernel it runs) and up to 1024 (token, choice) slots (one workgroup sorts
@@ -376,6 +419,7 @@ class MoE(nn.Module):
             and self.fuse_router
             and self.fuse_swiglu
             and self.gather_in_gemm is not False
+            and not self.fp8_experts
         ):
             return None
         parameters, gate_weight = self._expert_parameters(), self.gate.weight
@@ -412,6 +456,7 @@ class MoE(nn.Module):
             and self.fuse_router
             and self.fuse_swiglu
             and self.fuse_swiglu_backward
+            and not self.fp8_experts
             and self.num_experts <= 1024
             and self.top_k <= 64
             and self.hidden_size <= (1 << 24)

@@ -84,3 +84,42 @@ def swiglu_backward_cuda(
             cols, gs, us, ds, ggs, ugs, _lib.dtype_code(gate.dtype), _lib.current_stream(gate.device),
         )
     _lib.check(rc, "swiglu_backward_cuda")
+
+
+def _check_packed_rows(x: torch.Tensor, half: torch.Tensor, values: torch.Tensor, scales: torch.Tensor) -> tuple[int, int]:
+    R, I = half.shape
+    assert x.shape == (R, 2 * I) and values.shape == (R, 2, I) and scales.shape == (R, 2, 4 * -(-I // 512))
+    assert x.dtype == half.dtype and values.dtype == torch.float8_e4m3fn and scales.dtype == torch.float8_e8m0fnu
+    for t in (x, half, values, scales):
+        assert t.is_contiguous()
+    return R, I
+
+
+@hip_op("swiglu_fp8_forward_cuda", mutates_args={"output", "values", "scales"})
+def swiglu_fp8_forward_cuda(x: torch.Tensor, output: torch.Tensor, values: torch.Tensor, scales: torch.Tensor) -> None:
+    """output [R, I] = the activation of x [R, 2 I] = [up | gate], and x in 8-bit blocks: values [R, 2, I] with their scales
+    (fma_swiglu_fp8_forward)"""
+    _lib.require_gpu(x, output, values, scales)
+    R, I = _check_packed_rows(x, output, values, scales)
+    if output.numel() == 0:
+        return
+    with _lib.on_device(x.device):
+        rc = _lib.load().fma_swiglu_fp8_forward(
+            x.data_ptr(), output.data_ptr(), values.data_ptr(), scales.data_ptr(), R, I, _lib.dtype_code(x.dtype),
+            _lib.current_stream(x.device),
+        )  # fmt: skip
+    _lib.check(rc, "swiglu_fp8_forward_cuda")
+
+
+@hip_op("swiglu_fp8_backward_cuda", mutates_args={"x_grad"})
+def swiglu_fp8_backward_cuda(values: torch.Tensor, scales: torch.Tensor, output_grad: torch.Tensor, x_grad: torch.Tensor) -> None:
+    _lib.require_gpu(values, scales, output_grad, x_grad)
+    R, I = _check_packed_rows(x_grad, output_grad, values, scales)
+    if output_grad.numel() == 0:
+        return
+    with _lib.on_device(values.device):
+        rc = _lib.load().fma_swiglu_fp8_backward(
+            values.data_ptr(), scales.data_ptr(), output_grad.data_ptr(), x_grad.data_ptr(), R, I, _lib.dtype_code(x_grad.dtype),
+            _lib.current_stream(values.device),
+        )  # fmt: skip
+    _lib.check(rc, "swiglu_fp8_backward_cuda")

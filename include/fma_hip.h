@@ -435,6 +435,55 @@ int fma_fused_residual_add_rmsnorm_bwd(const void* added_x_residual, const void*
                                        float eps, float multiplier, void* workspace, int64_t workspace_bytes,
                                        int dtype, void* stream);
 
+/* ---- 8-bit blocks -------------------------------------------------------------------------------
+ * e4m3 values (1 byte) and one scale, a power of two as an e8m0 byte b = 2^(b - 127), per block of 128 elements along a row or,
+ * block_rows = 128, per 128 x 128 elements of a matrix (the last block of a row or a column is shorter): the smallest power of two
+ * that brings the block's largest magnitude to 448 or less, 2^-126 at the least; value = x / scale rounded to nearest even. A block
+ * with an infinity or a NaN: scale byte 255 (NaN), every value NaN. A row's scales are fma_fp8_scale_pitch(K) bytes,
+ * ceil(K / 128) of them filled up with 127 to a multiple of four. No counterpart in the reference. */
+int64_t fma_fp8_scale_pitch(int64_t K);
+
+/* x [E, N, K] of dtype -> values [E, N, K], scales [E, N, pitch(K)] (block_rows 1) or [E, ceil(N / 128), pitch(K)] (block_rows 128).
+ * With 128 x 128 blocks a transposed copy too, values_t [E, K, N] with scales_t [E, ceil(K / 128), pitch(N)], unless both are NULL.
+ * Any size and alignment; rows of multiples of 16 (8 with 128 x 128 blocks) elements, aligned, take the 16-byte kernels. */
+int fma_quantize_fp8(const void* x, void* values, void* scales, void* values_t, void* scales_t, int64_t E, int64_t N, int64_t K,
+                     int64_t block_rows, int dtype, void* stream);
+/* out [E, N, K] = value * scale, rounded to dtype once (exact in fp32 and bf16). */
+int fma_dequantize_fp8(const void* values, const void* scales, void* out, int64_t E, int64_t N, int64_t K, int64_t block_rows,
+                       int dtype, void* stream);
+
+/* D_e = A_e B_e^T, fp32 sums, one rounding to dtype (FMA_F32 / FMA_F16 / FMA_BF16): A [R, K] with scales [R, pitch(K)], rows of the
+ * groups back to back; B [E, N, K] with scales [E, ceil(N / 128), pitch(K)]; D [R, N]. M_arr: rows of every group, in device memory,
+ * or NULL for one group of R rows. Rows past the last group are not written, rows past R do not exist whatever M_arr says.
+ * K % 16 == 0, K < 2^21, N < 2^23, N * K < 2^32; A, B and D aligned to 16 bytes, scales to 4. */
+int fma_grouped_gemm_fp8(const void* A, const void* A_scales, const void* B, const void* B_scales, void* D, const uint32_t* M_arr,
+                         int64_t E, int64_t R, int64_t N, int64_t K, int dtype, void* stream);
+
+/* y [R, I] = up * gate * sigmoid(gate) of x [R, 2 I] = [up | gate], and x in 8-bit blocks along each half: values [R, 2, I],
+ * scales [R, 2, pitch(I)]; any I. The backward reads those: dx [R, 2 I] from dy [R, I]. */
+int fma_swiglu_fp8_forward(const void* x, void* y, void* values, void* scales, int64_t R, int64_t I, int dtype, void* stream);
+int fma_swiglu_fp8_backward(const void* values, const void* scales, const void* dy, void* dx, int64_t R, int64_t I, int dtype, void* stream);
+
+/* The experts of a SwiGLU layer with 8-bit products: y [T, H] = the gated sum over every token's top_k choices of
+ * q(swiglu(q(x) W1_e^T)) W2_e^T, q = quantisation to blocks of 128. ids [T, top_k] (id_bytes 4 or 8; one that names no expert
+ * contributes nothing), gates [T, top_k] of dtype; W1 [E, 2, I, H] ("up", then "gate"), W2 [E, H, I] in 128 x 128 blocks.
+ * buffer: fma_swiglu_experts_fp8_buffer_bytes, 16-byte aligned, no initialisation; with keep it holds what the backward call reads
+ * (tokens, pre-activation and activation in 8 bits, the experts' output, the routing index) and must not be touched in between.
+ * The backward takes the transposed copies W1t [E, 2, H, I] and W2t [E, I, H]; dx, d_gates, dW1 [E, 2 I, H], dW2 [E, H, I] of dtype
+ * are each computed unless NULL. H % 16 == I % 16 == 0, T * H < 2^30, I < 2^20, 2 * I * H < 2^32, E <= FMA_MAX_GROUPS;
+ * dtype FMA_BF16 or FMA_F16. */
+int64_t fma_swiglu_experts_fp8_buffer_bytes(int64_t T, int64_t top_k, int64_t E, int64_t H, int64_t I, int keep);
+int64_t fma_swiglu_experts_fp8_workspace_bytes(int64_t T, int64_t top_k, int64_t E);
+int fma_swiglu_experts_fp8(const void* x, const void* gates, const void* ids, int id_bytes, const void* W1, const void* W1_scales,
+                           const void* W2, const void* W2_scales, void* y, int64_t T, int64_t top_k, int64_t E, int64_t H, int64_t I,
+                           int keep, void* buffer, int64_t buffer_bytes, void* workspace, int64_t workspace_bytes, int dtype,
+                           void* stream);
+int64_t fma_swiglu_experts_fp8_bwd_workspace_bytes(int64_t T, int64_t top_k, int64_t H, int64_t I);
+int fma_swiglu_experts_fp8_bwd(const void* dy, const void* gates, const void* ids, int id_bytes, const void* W1t, const void* W1t_scales,
+                               const void* W2t, const void* W2t_scales, const void* buffer, int64_t buffer_bytes, void* dx, void* d_gates,
+                               void* dW1, void* dW2, int64_t T, int64_t top_k, int64_t E, int64_t H, int64_t I, void* workspace,
+                               int64_t workspace_bytes, int dtype, void* stream);
+
 #ifdef __cplusplus
 }
 #endif
