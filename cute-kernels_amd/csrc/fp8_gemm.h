@@ -76,13 +76,26 @@ __device__ __forceinline__ void lds_barrier() {
 __device__ __forceinline__ u32x4 rsrc_at(uint64_t base, uint32_t bytes) {
     return u32x4{(uint32_t)base, (uint32_t)(base >> 32) & 0xffffu, bytes, 0x00020000u};
 }
+// everything from `base` on, for stores whose lanes have been checked (one that has nothing to store takes kOutOfRange)
+__device__ __forceinline__ __amdgpu_buffer_rsrc_t buffer_at(uint64_t base) {
+    return __builtin_amdgcn_make_buffer_rsrc((void*)(uintptr_t)base, 0, (int)0x7fffffff, 0x00020000);
+}
 __device__ __forceinline__ uint64_t uniform64(uint64_t x) { return ((uint64_t)uniform((uint32_t)(x >> 32)) << 32) | uniform((uint32_t)x); }
+
+// two floats rounded to T, the first in the low half
+template <typename T>
+__device__ __forceinline__ uint32_t pack_pair(float lo, float hi) {
+    if constexpr (std::is_same_v<T, bf16_t>) return ::fmahip::gemm::ElemBf16::pack2(lo, hi);
+    else return ::fmahip::gemm::ElemF16::pack2(lo, hi);
+}
 
 template <int EPI, bool GATHER>
 __global__ __launch_bounds__(kGemmThreads) void fp8_gemm_kernel(const GemmArgs args) {
     constexpr bool kGlu = EPI == EPI_GLU || EPI == EPI_GLU_KEEP;
     constexpr bool kBwd = EPI == EPI_GLU_BWD_BF16 || EPI == EPI_GLU_BWD_F16;
     constexpr uint32_t kCols = kGlu ? kTileN / 2 : kTileN;  // columns of the output grid per tile
+    // Stores of an epilogue per wavefront, at least (0, 59: an epilogue that has waited for all loads in front of them itself)
+    constexpr int kStores = EPI == EPI_BF16 || EPI == EPI_F16 ? 2 * kRowBlocks : (EPI == EPI_GLU ? 2 * kRowBlocks : (EPI == EPI_GLU_KEEP ? 6 * kRowBlocks : (kBwd ? 59 : 0)));
     constexpr int kMaxima = EPI == EPI_GLU_KEEP ? 3 : (kGlu ? 1 : (kBwd ? 1 : 0));
 
     __shared__ __attribute__((aligned(1024))) uint8_t s_op[2 * kStage];
@@ -336,13 +349,24 @@ __global__ __launch_bounds__(kGemmThreads) void fp8_gemm_kernel(const GemmArgs a
         for (uint32_t step = 0; step < steps; ++step) {
 #pragma unroll
             for (int i = 0; i < kRowBlocks - 1; ++i) {
+                if (i == 1) {
+                    // The step's fragments of B are in registers, in every wavefront (its first products have used them): the loads of B
+                    // two steps on may fill their place.
+                    lds_barrier();
+                }
                 read_a(i + 1, (i + 1) & 1);
 #pragma unroll
-                for (int j = 0; j < kColBlocks; ++j) mma(i, j, i & 1, sb[j >> 1]);
+                for (int j = 0; j < kColBlocks; ++j) {
+                    mma(i, j, i & 1, sb[j >> 1]);
+                    if (i == 1) load_b(j);
+                }
                 __builtin_amdgcn_sched_barrier(0);
             }
-            // Every fragment of this step is read, and the next step has landed: its stage is read from here on, this step's is loaded into.
-            wait_vm<0>();
+            // Every fragment of the step is read, and the next step has landed (all but the loads of B just issued): the next step's
+            // fragments are read from here on, and the loads of A two steps on fill this step's place.
+            // In a tile's first step the stores of the epilogue before it are younger than what is waited for, and stay outstanding.
+            if (step == 0) wait_vm<4 + kStores>();
+            else wait_vm<4>();
             lds_barrier();
             next_step();
             {
@@ -352,7 +376,6 @@ __global__ __launch_bounds__(kGemmThreads) void fp8_gemm_kernel(const GemmArgs a
 #pragma unroll
                 for (int j = 0; j < kColBlocks; ++j) {
                     mma(i, j, i & 1, j < 2 ? s0 : s1);
-                    load_b(j);
                     load_a(j);
                     read_b(j);
                 }
@@ -364,39 +387,70 @@ __global__ __launch_bounds__(kGemmThreads) void fp8_gemm_kernel(const GemmArgs a
 
         // ---- epilogue ----
         const Tile t = find(c_tile);
-        if constexpr (EPI == EPI_BF16 || EPI == EPI_F16 || EPI == EPI_F32) {
-            using T = std::conditional_t<EPI == EPI_BF16, bf16_t, std::conditional_t<EPI == EPI_F16, f16_t, float>>;
-            T* const D = (T*)args.D;
+        if constexpr (EPI == EPI_BF16 || EPI == EPI_F16) {
+            using T = std::conditional_t<EPI == EPI_BF16, bf16_t, f16_t>;
+            uint16_t* const tile = (uint16_t*)args.D + (uint64_t)t.row0 * N + t.n0;
+            if (N % 8u == 0) {
+                // A lane has twice eight neighbouring columns of row r16, 32 columns apart. Of a pair of rows the even one's lanes store the first eight
+                // of both rows, the odd one's the second: a store then writes eight whole lines of 128 bytes, not sixteen halves.
+                const __amdgpu_buffer_rsrc_t rsrc = ::fmahip::gemm::make_rsrc(tile, uniform(t.rows * N - t.n0) * 2u);
+                const bool odd = (r16 & 1u) != 0;
+                const uint32_t col = wn * 64u + (odd ? 32u : 0u) + q * 8u;
+                const bool in = t.n0 + col < N;
+#pragma unroll
+                for (int i = 0; i < kRowBlocks; ++i) {
+                    u32x4 v[2];
+#pragma unroll
+                    for (int p = 0; p < 2; ++p)
+#pragma unroll
+                        for (int x = 0; x < 4; ++x)
+                            v[p][x] = pack_pair<T>(acc[i][8 * p + 2 * x], acc[i][8 * p + 2 * x + 1]);
+                    u32x4 even_row, odd_row;  // columns `col` of this pair's rows
+#pragma unroll
+                    for (int x = 0; x < 4; ++x) {
+                        const uint32_t mine = odd ? v[0][x] : v[1][x];  // what the other row's lane stores
+                        const uint32_t other = (uint32_t)__builtin_amdgcn_mov_dpp((int)mine, 0xb1, 0xf, 0xf, true);
+                        even_row[x] = odd ? other : v[0][x];
+                        odd_row[x] = odd ? v[1][x] : other;
+                    }
+                    const uint32_t row = wm * 128u + (uint32_t)i * 16u + (r16 & ~1u);
+                    const uint32_t at = (row * N + col) * 2u;
+                    ::fmahip::gemm::store_tile16<false>(rsrc, in ? at : kOutOfRange, __builtin_bit_cast(uint4, even_row));
+                    ::fmahip::gemm::store_tile16<false>(rsrc, in ? at + N * 2u : kOutOfRange, __builtin_bit_cast(uint4, odd_row));
+                }
+            } else {
+#pragma unroll
+                for (int i = 0; i < kRowBlocks; ++i) {
+                    const uint32_t row = wm * 128u + (uint32_t)i * 16u + r16;
+#pragma unroll
+                    for (int x = 0; x < 16; ++x) {
+                        const uint32_t col = wn * 64u + (uint32_t)(x / 8) * 32u + q * 8u + (uint32_t)(x % 8);
+                        if (row < t.rows && t.n0 + col < N) ((T*)tile)[(uint64_t)row * N + col] = Num<T>::down(acc[i][x]);
+                    }
+                }
+                wait_vm<0>();
+            }
+        } else if constexpr (EPI == EPI_F32) {
+            float* const tile = (float*)args.D + (uint64_t)t.row0 * N + t.n0;
 #pragma unroll
             for (int i = 0; i < kRowBlocks; ++i) {
                 const uint32_t row = wm * 128u + (uint32_t)i * 16u + r16;
-                if (row < t.rows) {
 #pragma unroll
-                    for (int p = 0; p < 2; ++p) {
-                        const uint32_t col = t.n0 + wn * 64u + (uint32_t)p * 32u + q * 8u;
-                        float v[8];
-#pragma unroll
-                        for (int x = 0; x < 8; ++x) v[x] = acc[i][8 * p + x];
-                        T* const to = D + (uint64_t)(t.row0 + row) * N + col;
-                        if (N % 8u == 0) {
-                            if (col < N) {
-                                constexpr int V = Vec16<T>::N;
-#pragma unroll
-                                for (int c = 0; c < 8 / V; ++c) {
-                                    Vec16<T> o;
-#pragma unroll
-                                    for (int x = 0; x < V; ++x) o.v[x] = Num<T>::down(v[c * V + x]);
-                                    *(reinterpret_cast<Vec16<T>*>(to) + c) = o;
-                                }
-                            }
+                for (int x = 0; x < 16; x += 4) {
+                    const uint32_t col = wn * 64u + (uint32_t)(x / 8) * 32u + q * 8u + (uint32_t)(x % 8);
+                    float* const to = tile + (uint64_t)row * N + col;
+                    if (row < t.rows) {
+                        if (N % 4u == 0) {
+                            if (t.n0 + col < N) *reinterpret_cast<f32x4*>(to) = f32x4{acc[i][x], acc[i][x + 1], acc[i][x + 2], acc[i][x + 3]};
                         } else {
 #pragma unroll
-                            for (int x = 0; x < 8; ++x)
-                                if (col + x < N) to[x] = Num<T>::down(v[x]);
+                            for (int y = 0; y < 4; ++y)
+                                if (t.n0 + col + y < N) to[y] = acc[i][x + y];
                         }
                     }
                 }
             }
+            wait_vm<0>();
         } else if constexpr (kGlu) {
             const uint32_t col = t.n0 + wn * 32u + q * 8u, block = t.n0 / kBlock;
             // magnitudes of the row's columns of this wavefront
@@ -432,35 +486,37 @@ __global__ __launch_bounds__(kGemmThreads) void fp8_gemm_kernel(const GemmArgs a
 #pragma unroll
             for (int i = 0; i < kRowBlocks; ++i) asm("" : "+v"(acc[i]));
 #pragma unroll
-            for (int i = 0; i < kRowBlocks; ++i) {
-                const uint32_t row = wm * 128u + (uint32_t)i * 16u + r16;
-                if (row < t.rows) {
-                    const uint64_t to = t.row0 + row;
+            for (int w = 0; w < kWhat; ++w) {
+                // values of this tile's rows from its first column on (the rows' ends are the descriptor's), and their scales
+                const uint32_t pitch = w == 0 ? N : 2u * N, s_pitch = w == 0 ? args.o_pitch_s : 2u * args.o_pitch_s;
+                const uint64_t values = w == 0 ? (uint64_t)(uintptr_t)args.out + (uint64_t)t.row0 * pitch
+                                               : (uint64_t)(uintptr_t)args.h + (uint64_t)t.row0 * pitch + (w == 2 ? N : 0u);
+                const uint64_t scales = w == 0 ? (uint64_t)(uintptr_t)args.out_s + (uint64_t)t.row0 * s_pitch
+                                               : (uint64_t)(uintptr_t)args.h_s + (uint64_t)t.row0 * s_pitch + (w == 2 ? args.o_pitch_s : 0u);
+                const __amdgpu_buffer_rsrc_t rv = buffer_at(values), rs = buffer_at(scales);
 #pragma unroll
-                    for (int w = 0; w < kWhat; ++w) {
-                        const uint4 m = *reinterpret_cast<const uint4*>(s_max + ((uint32_t)w * 256u + row) * 4u);
-                        const uint32_t byte = scale_byte(max_u32(max_u32(m.x, m.y), max_u32(m.z, m.w)));
-                        const float inverse = scale_inverse(byte);
-                        float v[8];
+                for (int i = 0; i < kRowBlocks; ++i) {
+                    const uint32_t row = wm * 128u + (uint32_t)i * 16u + r16;
+                    const uint4 m = *reinterpret_cast<const uint4*>(s_max + ((uint32_t)w * 256u + row) * 4u);
+                    const uint32_t byte = scale_byte(max_u32(max_u32(m.x, m.y), max_u32(m.z, m.w)));
+                    const float inverse = scale_inverse(byte);
+                    float v[8];
 #pragma unroll
-                        for (int x = 0; x < 8; ++x)
-                            v[x] = (w == 0 ? activation(i, x) : acc[i][(w == 2 ? 8 : 0) + x]) * inverse;
-                        uint2 o;
-                        o.x = pack4(v[0], v[1], v[2], v[3]);
-                        o.y = pack4(v[4], v[5], v[6], v[7]);
-                        uint8_t* const values = w == 0 ? args.out + to * N : args.h + to * (2u * (uint64_t)N) + (w == 2 ? N : 0u);
-                        uint8_t* const scales = w == 0 ? args.out_s + to * args.o_pitch_s : args.h_s + to * (2u * (uint64_t)args.o_pitch_s) + (w == 2 ? args.o_pitch_s : 0u);
-                        if (col < N) *reinterpret_cast<uint2*>(values + col) = o;
-                        if (q == 0 && wn == 0) scales[block] = (uint8_t)byte;
-                    }
+                    for (int x = 0; x < 8; ++x) v[x] = (w == 0 ? activation(i, x) : acc[i][(w == 2 ? 8 : 0) + x]) * inverse;
+                    typedef __attribute__((ext_vector_type(2))) uint32_t u32x2;
+                    const u32x2 o = {pack4(v[0], v[1], v[2], v[3]), pack4(v[4], v[5], v[6], v[7])};
+                    const bool live = row < t.rows;
+                    __builtin_amdgcn_raw_buffer_store_b64(o, rv, (int)(live && col < N ? row * pitch + col : kOutOfRange), 0, 0);
+                    __builtin_amdgcn_raw_buffer_store_b8((uint8_t)byte, rs, (int)(live && q == 0 && wn == 0 ? row * s_pitch + block : kOutOfRange), 0, 0);
+                    __builtin_amdgcn_sched_barrier(0);
                 }
-                __builtin_amdgcn_sched_barrier(0);
             }
         } else {
             using T = std::conditional_t<EPI == EPI_GLU_BWD_BF16, bf16_t, f16_t>;
             // columns of block wn / 2 of the tile's two
             const uint32_t block = t.n0 / kBlock + (wn >> 1);
             const uint32_t s_pitch = args.o_pitch_s;
+            wait_vm<0>();
 #pragma unroll
             for (int i = 0; i < kRowBlocks; ++i) {
                 const uint32_t row = wm * 128u + (uint32_t)i * 16u + r16;

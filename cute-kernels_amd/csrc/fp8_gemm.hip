@@ -9,7 +9,7 @@ int check_gemm(const char* who, int64_t E, int64_t R, int64_t N, int64_t K, int6
                 (long long)R, (long long)N, (long long)K);
     FMA_REQUIRE(E <= FMA_MAX_GROUPS, FMA_ERR_TOO_MANY_EXPERTS, "%s: E=%lld, at most %d groups", who, (long long)E, FMA_MAX_GROUPS);
     FMA_REQUIRE(K % 16 == 0, FMA_ERR_BAD_SIZE, "%s: rows of whole 16-byte pieces: K=%lld is no multiple of 16", who, (long long)K);
-    FMA_REQUIRE(K < (1 << 21) && N < (1 << 23) && R < (1ll << 31), FMA_ERR_TOO_MANY_ELEMENTS, "%s: K < 2^21, N < 2^23, R < 2^31", who);
+    FMA_REQUIRE(K < (1 << 21) && N < (1 << 21) && R < (1ll << 31), FMA_ERR_TOO_MANY_ELEMENTS, "%s: K < 2^21, N < 2^21, R < 2^31", who);
     const int64_t row_tiles = R / kTileM + E + 1, col_tiles = (N + kTileN / 2 - 1) / (kTileN / 2);
     FMA_REQUIRE(row_tiles * col_tiles < (1ll << 30), FMA_ERR_TOO_MANY_ELEMENTS, "%s: more than 2^30 tiles", who);
     FMA_REQUIRE(segs * N * K < (1ll << 32), FMA_ERR_TOO_MANY_ELEMENTS, "%s: a group's matrix has 2^32 bytes or more", who);

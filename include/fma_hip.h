@@ -455,7 +455,7 @@ int fma_dequantize_fp8(const void* values, const void* scales, void* out, int64_
 /* D_e = A_e B_e^T, fp32 sums, one rounding to dtype (FMA_F32 / FMA_F16 / FMA_BF16): A [R, K] with scales [R, pitch(K)], rows of the
  * groups back to back; B [E, N, K] with scales [E, ceil(N / 128), pitch(K)]; D [R, N]. M_arr: rows of every group, in device memory,
  * or NULL for one group of R rows. Rows past the last group are not written, rows past R do not exist whatever M_arr says.
- * K % 16 == 0, K < 2^21, N < 2^23, N * K < 2^32; A, B and D aligned to 16 bytes, scales to 4. */
+ * K % 16 == 0, K < 2^21, N < 2^21, N * K < 2^32; A, B and D aligned to 16 bytes, scales to 4. */
 int fma_grouped_gemm_fp8(const void* A, const void* A_scales, const void* B, const void* B_scales, void* D, const uint32_t* M_arr,
                          int64_t E, int64_t R, int64_t N, int64_t K, int dtype, void* stream);
 

@@ -64,7 +64,7 @@ def test_product_validation(lib):
     assert product(p, p, p, p, p, p, 1025, 10, 64, 128, 2, None) == -4
     assert product(p, p, p, p, p, p, 4, 10, 64, 1 << 21, 2, None) == -5
     assert product(p, p, p, p, p, p, 4, 1 << 31, 64, 128, 2, None) == -5
-    assert product(p, p, p, p, p, p, 1, 10, 1 << 22, 1 << 12, 2, None) == -5  # a matrix of 2^34 bytes
+    assert product(p, p, p, p, p, p, 1, 10, 1 << 20, 1 << 12, 2, None) == -5  # a matrix of 2^32 bytes
     assert product(p, p, p, p, p, p, 4, 10, 64, 128, 9, None) == -2
     assert product(p, p, p, p, p, None, 4, 10, 64, 128, 2, None) == -1  # several groups without their sizes
     assert product(p, None, p, p, p, p, 4, 10, 64, 128, 2, None) == -1
