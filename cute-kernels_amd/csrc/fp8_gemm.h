@@ -101,6 +101,7 @@ __global__ __launch_bounds__(kGemmThreads) void fp8_gemm_kernel(const GemmArgs a
     __shared__ __attribute__((aligned(1024))) uint8_t s_op[2 * kStage];
     __shared__ __attribute__((aligned(256))) uint32_t s_scale[2 * kScaleWords];
     __shared__ __attribute__((aligned(16))) uint32_t s_max[kMaxima ? kMaxima * 256 * 4 : 4];
+    __shared__ __attribute__((aligned(1024))) uint8_t s_out[EPI == EPI_BF16 || EPI == EPI_F16 ? kWaves * 2048 : 16];
     __shared__ uint32_t s_tiles[kMaxGroups + 1];  // row tiles of the groups before
     __shared__ uint32_t s_first[kMaxGroups + 1];  // first row of the group
 
@@ -187,6 +188,7 @@ __global__ __launch_bounds__(kGemmThreads) void fp8_gemm_kernel(const GemmArgs a
     uint32_t l_a_bytes = 0, l_b_bytes = 0;
     uint32_t l_gather[4] = {0u, 0u, 0u, 0u};
     uint32_t l_scale = kOutOfRange;  // this lane's offset into the scales
+    Tile l_found = {0u, 0u, 0u, 0u};  // the tile that the loads are in
     auto aim = [&]() {
         if (l_tile >= total) {
             l_a_bytes = l_b_bytes = 0;
@@ -198,6 +200,7 @@ __global__ __launch_bounds__(kGemmThreads) void fp8_gemm_kernel(const GemmArgs a
             return;
         }
         const Tile t = find(l_tile);
+        l_found = t;
         const uint32_t n_block = t.n0 / kBlock;
         l_b = uniform64((uint64_t)(uintptr_t)args.B + t.e * args.b_group + (uint64_t)t.n0 * K);
         const uint32_t cols = N - t.n0 < kCols ? N - t.n0 : kCols;
@@ -305,9 +308,10 @@ __global__ __launch_bounds__(kGemmThreads) void fp8_gemm_kernel(const GemmArgs a
         sb[0] = read_scale(sb_off);
         sb[1] = kGlu ? read_scale(sb_off + 4u) : sb[0];
     };
-    auto mma = [&](int i, int j, int buf, int scale_b) {
+    auto mma = [&](auto first_c, int i, int j, int buf, int scale_b) {
         f32x16& c = acc[i];
-        f32x4 v = {c[4 * j], c[4 * j + 1], c[4 * j + 2], c[4 * j + 3]};
+        f32x4 v = {0.f, 0.f, 0.f, 0.f};  // (a tile's first step: the instruction takes the constant)
+        if constexpr (!decltype(first_c)::value) v = f32x4{c[4 * j], c[4 * j + 1], c[4 * j + 2], c[4 * j + 3]};
         v = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(fb[j], fa[buf], v, 0, 0, 0, scale_b, 0, sa[buf]);
         c[4 * j] = v[0];
         c[4 * j + 1] = v[1];
@@ -335,88 +339,85 @@ __global__ __launch_bounds__(kGemmThreads) void fp8_gemm_kernel(const GemmArgs a
     }
     wait_vm<0>();
     lds_barrier();
-    read_sb();
+    auto first_fragments = [&]() {
+        read_sb();
 #pragma unroll
-    for (int j = 0; j < kColBlocks; ++j) read_b(j);
-    read_a(0, 0);
+        for (int j = 0; j < kColBlocks; ++j) read_b(j);
+        read_a(0, 0);
+    };
+    first_fragments();
 
-    for (uint32_t c_tile = slot; c_tile < total; c_tile += grid) {
+    // One K step of a tile; FIRST: of its first, whose sums begin at zero.
+    auto k_step = [&](auto first_c) {
+        constexpr bool FIRST = decltype(first_c)::value;
 #pragma unroll
-        for (int i = 0; i < kRowBlocks; ++i)
+        for (int i = 0; i < kRowBlocks - 1; ++i) {
+            // The step's fragments of B are in registers, in every wavefront (its first products have used them): the loads of B two steps
+            // on may fill their place.
+            if (i == 1) lds_barrier();
+            read_a(i + 1, (i + 1) & 1);
 #pragma unroll
-            for (int x = 0; x < 16; ++x) acc[i][x] = 0.f;
-
-        for (uint32_t step = 0; step < steps; ++step) {
-#pragma unroll
-            for (int i = 0; i < kRowBlocks - 1; ++i) {
-                if (i == 1) {
-                    // The step's fragments of B are in registers, in every wavefront (its first products have used them): the loads of B
-                    // two steps on may fill their place.
-                    lds_barrier();
-                }
-                read_a(i + 1, (i + 1) & 1);
-#pragma unroll
-                for (int j = 0; j < kColBlocks; ++j) {
-                    mma(i, j, i & 1, sb[j >> 1]);
-                    if (i == 1) load_b(j);
-                }
-                __builtin_amdgcn_sched_barrier(0);
+            for (int j = 0; j < kColBlocks; ++j) {
+                mma(first_c, i, j, i & 1, sb[j >> 1]);
+                if (i == 1) load_b(j);
             }
-            // Every fragment of the step is read, and the next step has landed (all but the loads of B just issued): the next step's
-            // fragments are read from here on, and the loads of A two steps on fill this step's place.
-            // In a tile's first step the stores of the epilogue before it are younger than what is waited for, and stay outstanding.
-            if (step == 0) wait_vm<4 + kStores>();
-            else wait_vm<4>();
-            lds_barrier();
-            next_step();
-            {
-                constexpr int i = kRowBlocks - 1;
-                const int s0 = sb[0], s1 = sb[1];
-                read_sb();
-#pragma unroll
-                for (int j = 0; j < kColBlocks; ++j) {
-                    mma(i, j, i & 1, j < 2 ? s0 : s1);
-                    load_a(j);
-                    read_b(j);
-                }
-                read_a(0, 0);
-            }
-            load_scales();
-            next_load();
+            __builtin_amdgcn_sched_barrier(0);
         }
+        // Every fragment of the step is read, and the next step has landed (all but the loads of B just issued): the next step's fragments
+        // are read from here on, and the loads of A two steps on fill this step's place. In a tile's first step the stores of the
+        // epilogue before it are younger than what is waited for, and stay outstanding.
+        wait_vm<(FIRST ? (4 + kStores < 63 ? 4 + kStores : 63) : 4)>();
+        lds_barrier();
+        next_step();
+        {
+            constexpr int i = kRowBlocks - 1;
+            const int s0 = sb[0], s1 = sb[1];
+            read_sb();
+#pragma unroll
+            for (int j = 0; j < kColBlocks; ++j) {
+                mma(first_c, i, j, i & 1, j < 2 ? s0 : s1);
+                load_a(j);
+                read_b(j);
+            }
+            read_a(0, 0);
+        }
+        load_scales();
+        next_load();
+    };
+
+    Tile t = l_found;
+    for (uint32_t c_tile = slot; c_tile < total; c_tile += grid) {
+        if (steps < 3) t = find(c_tile);  // (the loads are two steps ahead: with three and more they are in this tile when it begins)
+        else t = l_found;
+        k_step(std::integral_constant<bool, true>{});
+        for (uint32_t step = 1; step < steps; ++step) k_step(std::integral_constant<bool, false>{});
 
         // ---- epilogue ----
-        const Tile t = find(c_tile);
         if constexpr (EPI == EPI_BF16 || EPI == EPI_F16) {
             using T = std::conditional_t<EPI == EPI_BF16, bf16_t, f16_t>;
             uint16_t* const tile = (uint16_t*)args.D + (uint64_t)t.row0 * N + t.n0;
             if (N % 8u == 0) {
-                // A lane has twice eight neighbouring columns of row r16, 32 columns apart. Of a pair of rows the even one's lanes store the first eight
-                // of both rows, the odd one's the second: a store then writes eight whole lines of 128 bytes, not sixteen halves.
+                // Through 2 KB of LDS per wavefront, 16 rows at a time, so that eight neighbouring lanes store a line of 128 bytes: straight from the
+                // registers neighbouring lanes are in different rows, and a store takes as many turns of the address unit as it has lines.
                 const __amdgpu_buffer_rsrc_t rsrc = ::fmahip::gemm::make_rsrc(tile, uniform(t.rows * N - t.n0) * 2u);
-                const bool odd = (r16 & 1u) != 0;
-                const uint32_t col = wn * 64u + (odd ? 32u : 0u) + q * 8u;
+                uint8_t* const image = s_out + wave * 2048u;
+                const uint32_t chunk = lane & 7u, line = lane >> 3;
+                const uint32_t col = wn * 64u + chunk * 8u;
                 const bool in = t.n0 + col < N;
+                const uint32_t put = r16 * 128u + ((q ^ (r16 & 7u)) << 4), get = line * 128u + ((chunk ^ line) << 4);
 #pragma unroll
                 for (int i = 0; i < kRowBlocks; ++i) {
                     u32x4 v[2];
 #pragma unroll
                     for (int p = 0; p < 2; ++p)
 #pragma unroll
-                        for (int x = 0; x < 4; ++x)
-                            v[p][x] = pack_pair<T>(acc[i][8 * p + 2 * x], acc[i][8 * p + 2 * x + 1]);
-                    u32x4 even_row, odd_row;  // columns `col` of this pair's rows
-#pragma unroll
-                    for (int x = 0; x < 4; ++x) {
-                        const uint32_t mine = odd ? v[0][x] : v[1][x];  // what the other row's lane stores
-                        const uint32_t other = (uint32_t)__builtin_amdgcn_mov_dpp((int)mine, 0xb1, 0xf, 0xf, true);
-                        even_row[x] = odd ? other : v[0][x];
-                        odd_row[x] = odd ? v[1][x] : other;
-                    }
-                    const uint32_t row = wm * 128u + (uint32_t)i * 16u + (r16 & ~1u);
-                    const uint32_t at = (row * N + col) * 2u;
-                    ::fmahip::gemm::store_tile16<false>(rsrc, in ? at : kOutOfRange, __builtin_bit_cast(uint4, even_row));
-                    ::fmahip::gemm::store_tile16<false>(rsrc, in ? at + N * 2u : kOutOfRange, __builtin_bit_cast(uint4, odd_row));
+                        for (int x = 0; x < 4; ++x) v[p][x] = pack_pair<T>(acc[i][8 * p + 2 * x], acc[i][8 * p + 2 * x + 1]);
+                    *reinterpret_cast<u32x4*>(image + put) = v[0];
+                    *reinterpret_cast<u32x4*>(image + (put ^ 64u)) = v[1];
+                    const u32x4 low = *reinterpret_cast<const u32x4*>(image + get), high = *reinterpret_cast<const u32x4*>(image + 1024u + get);
+                    const uint32_t at = ((wm * 128u + (uint32_t)i * 16u + line) * N + col) * 2u;
+                    ::fmahip::gemm::store_tile16<false>(rsrc, in ? at : kOutOfRange, __builtin_bit_cast(uint4, low));
+                    ::fmahip::gemm::store_tile16<false>(rsrc, in ? at + N * 16u : kOutOfRange, __builtin_bit_cast(uint4, high));
                 }
             } else {
 #pragma unroll
@@ -582,12 +583,9 @@ __global__ __launch_bounds__(kGemmThreads) void fp8_gemm_kernel(const GemmArgs a
                 }
                 __builtin_amdgcn_sched_barrier(0);
             }
-            // the next tile's first fragments once more: 42 registers that this epilogue uses meanwhile
-            read_sb();
-#pragma unroll
-            for (int j = 0; j < kColBlocks; ++j) read_b(j);
-            read_a(0, 0);
         }
+        // The next tile's first fragments once more: 42 registers that these epilogues use meanwhile.
+        if constexpr (kGlu || kBwd) first_fragments();
     }
     wait_vm<0>();  // loads past the last step write zeros into LDS: they are done when the workgroup ends
 }
