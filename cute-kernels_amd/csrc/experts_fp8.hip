@@ -9,6 +9,7 @@
 // gates' gradient reads, in 16). The weight gradients are products in 16 bits: of the unrounded gradients' 16-bit form and the 8-bit
 // activations, which are exact in bf16 (in fp16 as far as its exponents reach).
 #include "fp8_gemm_launch.h"
+#include "fp8_thin.h"
 
 namespace fmahip {
 namespace {
@@ -23,9 +24,9 @@ __device__ __forceinline__ bool names_expert(const void* ids, int id_bytes, int6
 }
 
 // ---- y[t] = sum_j gates[t, j] * o[inv[t, j]], fp32 sums in ascending j; gates NULL: ones ------------------------------
-// One workgroup per token; KC choices (top_k, or 4 at a time) of a vector are loaded before the first is added.
-template <typename T, int KC>
-__global__ __launch_bounds__(kThreads) void sum_choices_kernel(const T* __restrict__ o, const void* __restrict__ ids, int id_bytes,
+// o in type O; inv NULL: the row of a slot is the slot. One workgroup per token; KC choices (top_k, or 4 at a time) of a vector are loaded before the first is added.
+template <typename T, typename O, int KC>
+__global__ __launch_bounds__(kThreads) void sum_choices_kernel(const O* __restrict__ o, const void* __restrict__ ids, int id_bytes,
                                                                const int32_t* __restrict__ inv, const T* __restrict__ gates, uint32_t top_k,
                                                                uint32_t E, uint32_t H, int64_t slots, T* __restrict__ y) {
     const int64_t t = blockIdx.x;
@@ -34,18 +35,20 @@ __global__ __launch_bounds__(kThreads) void sum_choices_kernel(const T* __restri
 #pragma unroll
         for (int i = 0; i < 8; ++i) sum[i] = 0.f;
         for (uint32_t j0 = 0; j0 < top_k; j0 += KC) {
-            Vec16<T> v[KC];
+            constexpr int V = Vec16<O>::N;
+            Vec16<O> v[KC][8 / V];
             float g[KC];
 #pragma unroll
             for (int j = 0; j < KC; ++j) {
                 const int64_t slot = t * top_k + j0 + j;
                 g[j] = 0.f;
 #pragma unroll
-                for (int i = 0; i < 8; ++i) v[j].v[i] = Num<T>::down(0.f);
+                for (int i = 0; i < 8; ++i) v[j][i / V].v[i % V] = Num<O>::down(0.f);
                 if (j0 + j < top_k && names_expert(ids, id_bytes, slot, E)) {
-                    const int64_t row = inv[slot];
+                    const int64_t row = inv ? inv[slot] : slot;
                     if ((uint64_t)row < (uint64_t)slots) {
-                        v[j] = load_streaming16(reinterpret_cast<const Vec16<T>*>(o + row * H + h));
+#pragma unroll
+                        for (int c = 0; c < 8 / V; ++c) v[j][c] = load_streaming16(reinterpret_cast<const Vec16<O>*>(o + row * H + h) + c);
                         g[j] = gates ? Num<T>::up(gates[slot]) : 1.0f;
                     }
                 }
@@ -53,7 +56,7 @@ __global__ __launch_bounds__(kThreads) void sum_choices_kernel(const T* __restri
 #pragma unroll
             for (int j = 0; j < KC; ++j)
 #pragma unroll
-                for (int i = 0; i < 8; ++i) sum[i] = fmaf(g[j], Num<T>::up(v[j].v[i]), sum[i]);
+                for (int i = 0; i < 8; ++i) sum[i] = fmaf(g[j], Num<O>::up(v[j][i / V].v[i % V]), sum[i]);
         }
         Vec16<T> w;
 #pragma unroll
@@ -62,17 +65,17 @@ __global__ __launch_bounds__(kThreads) void sum_choices_kernel(const T* __restri
     }
 }
 
-template <typename T>
+template <typename T, typename O = T>
 int sum_choices(const void* o, const void* ids, int id_bytes, const int32_t* inv, const void* gates, int64_t T_, int64_t top_k, int64_t E,
                 int64_t H, void* y, hipStream_t st) {
     auto run = [&](auto kernel) {
-        hipLaunchKernelGGL(kernel, dim3((uint32_t)T_), dim3(kThreads), 0, st, (const T*)o, ids, id_bytes, inv, (const T*)gates, (uint32_t)top_k,
+        hipLaunchKernelGGL(kernel, dim3((uint32_t)T_), dim3(kThreads), 0, st, (const O*)o, ids, id_bytes, inv, (const T*)gates, (uint32_t)top_k,
                            (uint32_t)E, (uint32_t)H, T_ * top_k, (T*)y);
     };
-    if (top_k == 1) run(sum_choices_kernel<T, 1>);
-    else if (top_k == 2) run(sum_choices_kernel<T, 2>);
-    else if (top_k <= 4 || top_k % 8 != 0) run(sum_choices_kernel<T, 4>);
-    else run(sum_choices_kernel<T, 8>);
+    if (top_k == 1) run(sum_choices_kernel<T, O, 1>);
+    else if (top_k == 2) run(sum_choices_kernel<T, O, 2>);
+    else if (top_k <= 4 || top_k % 8 != 0) run(sum_choices_kernel<T, O, 4>);
+    else run(sum_choices_kernel<T, O, 8>);
     return launch_status("swiglu_experts_fp8");
 }
 
@@ -156,6 +159,8 @@ struct Shape {
     int64_t T, k, E, H, I, R;
 };
 
+int64_t thin_output_offset(const Shape& s) { return (s.R * s.I * 4 + 255) & ~(int64_t)255; }
+
 // The pieces of one buffer, each at a multiple of 256 bytes. keep: the pre-activation among them.
 Buffers lay_out(uint8_t* base, const Shape& s, bool keep) {
     Buffers b = {};
@@ -179,6 +184,10 @@ Buffers lay_out(uint8_t* base, const Shape& s, bool keep) {
         b.h8_s = take(s.R * 2 * scale_pitch(s.I));
     }
     b.bytes = at;
+    if (!keep && are_thin_experts(s.E, s.R, s.H, s.I)) {  // few rows: activation and output in fp32 take the place of all that
+        const int64_t thin = thin_output_offset(s) + s.R * s.H * 4;
+        if (b.bytes < thin) b.bytes = thin;
+    }
     return b;
 }
 
@@ -269,6 +278,13 @@ int fma_swiglu_experts_fp8(const void* x, const void* gates, const void* ids, in
     FMA_REQUIRE(workspace_bytes >= needed, FMA_ERR_WORKSPACE_TOO_SMALL, "swiglu_experts_fp8: workspace of %lld bytes, %lld needed",
                 (long long)workspace_bytes, (long long)needed);
     hipStream_t st = (hipStream_t)stream;
+    if (!keep && are_thin_experts(E, s.R, H, I)) {
+        float* const act = (float*)buffer;
+        float* const o = (float*)((uint8_t*)buffer + thin_output_offset(s));
+        if (const int rc = launch_thin_experts(x, ids, id_bytes, W1, W1_scales, W2, W2_scales, act, o, T, top_k, E, H, I, dtype, st)) return rc;
+        return dtype == FMA_BF16 ? sum_choices<bf16_t, float>(o, ids, id_bytes, nullptr, gates, T, top_k, E, H, y, st)
+                                 : sum_choices<f16_t, float>(o, ids, id_bytes, nullptr, gates, T, top_k, E, H, y, st);
+    }
     if (const int rc = fma_quantize_fp8(x, b.x8, b.x8_s, nullptr, nullptr, 1, T, H, 1, dtype, stream)) return rc;
     const int64_t eid_bytes = index_rows_bytes(s.R);
     if (const int rc = fma_moe_build_index(ids, id_bytes, s.R, E, b.counts, b.offsets, b.perm, (int32_t*)workspace, b.inv,

@@ -1,5 +1,6 @@
 // Launches of the grouped product of 8-bit operands (fp8_gemm.h) and its C entry point.
 #include "fp8_gemm_launch.h"
+#include "fp8_thin.h"
 
 namespace fmahip {
 namespace fp8 {
@@ -54,6 +55,7 @@ int fma_grouped_gemm_fp8(const void* A, const void* A_scales, const void* B, con
     FMA_REQUIRE(aligned16(A) && aligned16(B) && aligned16(D), FMA_ERR_MISALIGNED, "grouped_gemm_fp8: A, B and D must be aligned to 16 bytes");
     FMA_REQUIRE(((reinterpret_cast<uintptr_t>(A_scales) | reinterpret_cast<uintptr_t>(B_scales)) & 3u) == 0, FMA_ERR_MISALIGNED,
                 "grouped_gemm_fp8: scales must be aligned to 4 bytes");
+    if (is_thin_product(E, R, N, K)) return launch_thin_product(A, A_scales, B, B_scales, D, M_arr, E, R, N, K, dtype, (hipStream_t)stream);
     GemmArgs a = {};
     a.A = (const uint8_t*)A;
     a.A_s = (const uint8_t*)A_scales;

@@ -205,15 +205,16 @@ def test_layer(dtype, T):
     exact = _oracle(x.cpu(), gates.detach().cpu(), ids.cpu(), moe.c_fc.weight.detach().cpu(), moe.c_proj.weight.detach().cpu())[0]
     _close(y, exact, dtype, 1, "y")
     with torch.no_grad():
-        assert torch.equal(moe(x, kernel_backend=KernelBackend.cuda)[0], y)
+        alone = moe(x, kernel_backend=KernelBackend.cuda)[0]  # (no backward follows: another kernel for few tokens)
+        _close(alone, exact, dtype, 1, "alone")
         served = moe.quantize_experts()(x, kernel_backend=KernelBackend.cuda)[0]
-        assert torch.equal(served, y)
+        assert torch.equal(served, alone)
         # 8-bit products against 16-bit ones: three quantised operands on the way, each off by 2^-5.2 of itself in the norm (uniform
         # within half a step of 2^-3 .. 2^-4), and twice that
         assert float((served - sixteen).float().norm() / sixteen.float().norm()) <= 2 * 5**0.5 * 2.0**-5.2
         # weights that have changed since are used as they are
         moe.c_proj.weight.mul_(2)
-        assert torch.allclose(moe(x, kernel_backend=KernelBackend.cuda)[0].float(), 2 * y.float(), rtol=2.0**-7, atol=1e-3)
+        assert torch.allclose(moe(x, kernel_backend=KernelBackend.cuda)[0].float(), 2 * alone.float(), rtol=2.0**-7, atol=1e-3)
         assert torch.equal(moe.quantize_experts()(x, kernel_backend=KernelBackend.cuda)[0], moe(x, kernel_backend=KernelBackend.cuda)[0])
     other = copy.deepcopy(moe)
     with torch.no_grad():
