@@ -75,4 +75,51 @@ int fma_grouped_gemm_fp8(const void* A, const void* A_scales, const void* B, con
     return launch_gemm("grouped_gemm_fp8", dtype == FMA_F32 ? EPI_F32 : (dtype == FMA_F16 ? EPI_F16 : EPI_BF16), a, (hipStream_t)stream);
 }
 
+// ---- the product of 16-bit tensors, quantised on the way, and its gradients ----
+
+int fma_grouped_linear_fp8(const void* x, const void* W, void* x_values, void* x_scales, void* W_values, void* W_scales, void* Wt_values,
+                           void* Wt_scales, void* y, const uint32_t* M_arr, int64_t E, int64_t R, int64_t N, int64_t K, int dtype,
+                           void* stream) {
+    using namespace fmahip;
+    FMA_REQUIRE(dtype == FMA_BF16 || dtype == FMA_F16, FMA_ERR_BAD_DTYPE, "grouped_linear_fp8: 16-bit tensors only, got dtype code %d", dtype);
+    if (const int rc = fmahip::fp8::check_gemm("grouped_linear_fp8", E, R, N, K, 1)) return rc;
+    if (const int rc = fma_quantize_fp8(W, W_values, W_scales, Wt_values, Wt_scales, E, N, K, 128, dtype, stream)) return rc;
+    if (const int rc = fma_quantize_fp8(x, x_values, x_scales, nullptr, nullptr, 1, R, K, 1, dtype, stream)) return rc;
+    return fma_grouped_gemm_fp8(x_values, x_scales, W_values, W_scales, y, M_arr, E, R, N, K, dtype, stream);
+}
+
+int64_t fma_grouped_linear_fp8_bwd_workspace_bytes(int64_t R, int64_t N, int64_t K) {
+    if (R < 0 || N < 1 || K < 1) return 0;
+    auto whole = [](int64_t n) { return (n + 255) & ~(int64_t)255; };
+    return whole(R * N) + whole(R * fmahip::fp8::scale_pitch(N)) + whole(R * K * 2);
+}
+
+int fma_grouped_linear_fp8_bwd(const void* dy, const void* x_values, const void* x_scales, const void* Wt_values, const void* Wt_scales,
+                               void* dx, void* dW, const uint32_t* M_arr, int64_t E, int64_t R, int64_t N, int64_t K, void* workspace,
+                               int64_t workspace_bytes, int dtype, void* stream) {
+    using namespace fmahip;
+    FMA_REQUIRE(dtype == FMA_BF16 || dtype == FMA_F16, FMA_ERR_BAD_DTYPE, "grouped_linear_fp8_bwd: 16-bit tensors only, got dtype code %d", dtype);
+    if (const int rc = fmahip::fp8::check_gemm("grouped_linear_fp8_bwd", E, R, K, N, 1)) return rc;
+    if (E == 0 || R == 0 || N == 0) return FMA_OK;
+    FMA_REQUIRE(dy && M_arr && workspace && (!dx || (Wt_values && Wt_scales)) && (!dW || (x_values && x_scales)), FMA_ERR_NULL_POINTER,
+                "grouped_linear_fp8_bwd: a tensor is NULL");
+    FMA_REQUIRE(aligned16(dy) && aligned16(workspace) && aligned16(dx) && aligned16(dW), FMA_ERR_MISALIGNED,
+                "grouped_linear_fp8_bwd: tensors must be aligned to 16 bytes");
+    const int64_t needed = fma_grouped_linear_fp8_bwd_workspace_bytes(R, N, K);
+    FMA_REQUIRE(workspace_bytes >= needed, FMA_ERR_WORKSPACE_TOO_SMALL, "grouped_linear_fp8_bwd: workspace of %lld bytes, %lld needed",
+                (long long)workspace_bytes, (long long)needed);
+    uint8_t* const dy8 = (uint8_t*)workspace;
+    uint8_t* const dy8_s = dy8 + ((R * N + 255) & ~(int64_t)255);
+    uint8_t* const x16 = dy8_s + ((R * fmahip::fp8::scale_pitch(N) + 255) & ~(int64_t)255);
+    if (dx) {
+        if (const int rc = fma_quantize_fp8(dy, dy8, dy8_s, nullptr, nullptr, 1, R, N, 1, dtype, stream)) return rc;
+        if (const int rc = fma_grouped_gemm_fp8(dy8, dy8_s, Wt_values, Wt_scales, dx, M_arr, E, R, K, N, dtype, stream)) return rc;
+    }
+    if (dW) {
+        if (const int rc = fma_dequantize_fp8(x_values, x_scales, x16, 1, R, K, 1, dtype, stream)) return rc;
+        return fma_grouped_gemm_ragged(dy, x16, dW, M_arr, nullptr, E, /*FMA_VARY_K*/ 1, N, K, 0, 1, 0, 1.0f, dtype, stream);
+    }
+    return FMA_OK;
+}
+
 }  // extern "C"

@@ -3,8 +3,10 @@
 //
 // The unit of work is 32 weight rows of one expert (16 of "up" and 16 of "gate" with the activation) against up to 16 or 32 rows, the
 // reduction in KS parts, one wavefront each, whose sums are added up through LDS in a fixed order. Weights go straight to registers, 16 bytes a lane, as
-// the matrix instruction takes them (16 rows x 64 bytes a load, two loads a line) and with the non-temporal hint: nothing reads them
-// twice. Many small wavefronts keep the loads in flight; there is no barrier in the loop.
+// the matrix instruction takes them (16 rows x 64 bytes a load, two loads a line). Without the non-temporal hint: the line is asked for
+// twice, and with it the halves come from memory one by one (128 x 4 rows, 4096 x 1536, 174 -> 140 us without; 8 x 4, 4096 x 14336, 98 -> 83).
+// Many small wavefronts keep the loads in flight; there is no barrier in the loop. (Rows in LDS for eight units at a time, with a barrier
+// per 512 elements: 8 x 4 rows, 28672 x 4096, 212 us against 168.)
 //
 // The rows come from memory in 8 bits (the product of quantised operands), or are quantised on the way to the instruction: the tokens of a
 // layer (16 bits) and the activation between its two products (fp32). Each lane has 32 elements of a block of 128, its three neighbours
@@ -44,11 +46,9 @@ struct ThinArgs {
 __device__ __forceinline__ __amdgpu_buffer_rsrc_t buffer(const void* p, uint32_t bytes) {
     return __builtin_amdgcn_make_buffer_rsrc(const_cast<void*>(p), 0, (int)bytes, 0x00020000);
 }
-template <int AUX>
 __device__ __forceinline__ u32x4 load16(__amdgpu_buffer_rsrc_t r, uint32_t at) {
-    return __builtin_amdgcn_raw_buffer_load_b128(r, (int)at, 0, AUX);
+    return __builtin_amdgcn_raw_buffer_load_b128(r, (int)at, 0, 0);
 }
-constexpr int kStream = 2;  // the non-temporal hint
 
 // One unit: rows `first` .. of the group's list (`rows` of them, at most 16 * TB).
 template <int SRC, int OUT, int TB, int KS>
@@ -109,8 +109,8 @@ struct Unit {
                 const bool lo = on && k * kBlock + q * 16u < K, hi = on && k * kBlock + 64u + q * 16u < K;
 #pragma unroll
                 for (int f = 0; f < 2; ++f) {
-                    wl[u][f][0] = load16<kStream>(f ? w1 : w0, lo ? w_off[f] + k * kBlock : kOutOfRange);
-                    wl[u][f][1] = load16<kStream>(f ? w1 : w0, hi ? w_off[f] + k * kBlock + 64u : kOutOfRange);
+                    wl[u][f][0] = load16(f ? w1 : w0, lo ? w_off[f] + k * kBlock : kOutOfRange);
+                    wl[u][f][1] = load16(f ? w1 : w0, hi ? w_off[f] + k * kBlock + 64u : kOutOfRange);
                 }
                 const uint32_t word = on ? k >> 2 : 0u, shift = (k & 3u) * 8u;
                 wsc[u][0] = on ? ws0[word] >> shift : 127u;
@@ -121,7 +121,7 @@ struct Unit {
                     for (int i = 0; i < 2 * kElem; ++i) {
                         const bool in = i < kElem ? lo : hi;
                         const uint32_t at = x_off[t] + (k * kBlock + (i < kElem ? 0u : 64u)) * (uint32_t)kElem + (uint32_t)(i % kElem) * 16u;
-                        xl[u][t][i] = load16<0>(xr, in && x_off[t] != kOutOfRange ? at : kOutOfRange);
+                        xl[u][t][i] = load16(xr, in && x_off[t] != kOutOfRange ? at : kOutOfRange);
                     }
                     if constexpr (SRC == ROWS_FP8)
                         xsc[u][t] = __builtin_amdgcn_raw_buffer_load_b32(xs, (int)(on && s_off[t] != kOutOfRange ? s_off[t] + word * 4u : kOutOfRange), 0, 0) >> shift;
@@ -284,10 +284,11 @@ int launch(const char* who, ThinArgs a, hipStream_t st) {
     a.col_blocks = (a.N + per - 1) / per;
     const int64_t groups = a.E < a.R ? a.E : a.R, cus = num_compute_units() > 0 ? num_compute_units() : 256;
     const bool wide = (int64_t)a.R > 8 * groups;
-    // parts of the reduction: as many as make eight wavefronts per compute unit, of two blocks at least
+    // parts of the reduction, of two blocks at least, until there are 32 wavefronts per compute unit, two rounds (12: 8 x 4 rows, 28672 x 4096,
+    // 179 -> 169 us; 64: 64 x 16 rows, 2816 x 2048, 84 -> 96)
     const int64_t units = groups * a.col_blocks, k_blocks = (a.K + kBlock - 1) / kBlock;
     int parts = 1;
-    while (parts < 8 && units * parts < 12 * cus && k_blocks >= 4 * parts) parts *= 2;
+    while (parts < 8 && units * parts < 32 * cus && k_blocks >= 4 * parts) parts *= 2;
     const dim3 grid(a.E * a.col_blocks);
     auto run = [&](auto kernel, int ks) { hipLaunchKernelGGL(kernel, grid, dim3(64 * ks), 0, st, a); };
     if (wide) {
@@ -306,19 +307,28 @@ int launch(const char* who, ThinArgs a, hipStream_t st) {
 
 }  // namespace
 
-#ifndef FMA_THIN_ROWS
-#define FMA_THIN_ROWS 16
-#endif
 namespace {
+// Whether this kernel is ahead of the tiles, of which a round takes 1.75 us a block of the reduction, one of a few tiles 1.3. Here the weights
+// stream at 5.4 TB/s, less an eightieth per row of the average group, and twice as long from 16 rows on. Weights from memory, this / tiles, us,
+// at 4, 8, 16 and 32 rows: 8 x 28672 x 4096 169, 171, 204, 325 / 232; 128 x 4096 x 1536 140, 157, 180, 256 / 160; 64 x 2816 x 2048 66, 70, 84, 127
+// / 81; 32 x 5760 x 2880 101, 111, 128, 174 / 110; 64 x 2048 x 1408 40, 42, 49, 76 / 42; 8 x 4096 x 14336 84, 89, 112, 192 / 144; 8 x 2048 x 8192
+// 33, 34, 41, 70 / 85.
+bool few_rows(int64_t E, int64_t R, int64_t N, int64_t K) {
+    const int64_t groups = E < R ? E : R, cus = num_compute_units() > 0 ? num_compute_units() : 256;
+    if (R > 32 * groups) return false;
+    const int64_t tiles = groups * ((N + 255) / 256), rounds = (tiles + cus - 1) / cus;
+    const double row = (double)R / groups, stream = (double)groups * N * K * (row > 16 ? 1.9 : 1 + row / 80) / 5.4e6;
+    return stream <= 3 + (double)rounds * ((K + kBlock - 1) / kBlock) * (tiles <= cus ? 1.3 : 1.75);
+}
+// lane offsets into the rows, and the number of threads of a launch
 bool fits(int64_t E, int64_t R, int64_t N, int64_t K, int64_t bytes, int64_t per) {
-    // few rows per group; lane offsets into the rows, and the number of threads of a launch
-    return R <= FMA_THIN_ROWS * (E < R ? E : R) && R * K * bytes < (1ll << 31) && E * ((N + per - 1) / per) < (1ll << 22);
+    return R * K * bytes < (1ll << 31) && E * ((N + per - 1) / per) < (1ll << 22);
 }
 }  // namespace
 
-bool is_thin_product(int64_t E, int64_t R, int64_t N, int64_t K) { return fits(E, R, N, K, 1, 32); }
+bool is_thin_product(int64_t E, int64_t R, int64_t N, int64_t K) { return fits(E, R, N, K, 1, 32) && few_rows(E, R, N, K); }
 bool are_thin_experts(int64_t E, int64_t R, int64_t H, int64_t I) {
-    return R <= kMaxThinSlots && fits(E, R, I, H, 2, 16) && fits(E, R, H, I, 4, 32);
+    return R <= kMaxThinSlots && fits(E, R, I, H, 2, 16) && fits(E, R, H, I, 4, 32) && few_rows(E, R, 2 * I, H);
 }
 
 int launch_thin_product(const void* A, const void* A_s, const void* B, const void* B_s, void* D, const uint32_t* sizes, int64_t E, int64_t R,

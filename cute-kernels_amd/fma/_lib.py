@@ -83,6 +83,9 @@ SIGNATURES = {
     "fma_quantize_fp8": (_i32, [_p] * 5 + [_i64] * 4 + [_i32, _p]),
     "fma_dequantize_fp8": (_i32, [_p] * 3 + [_i64] * 4 + [_i32, _p]),
     "fma_grouped_gemm_fp8": (_i32, [_p] * 6 + [_i64] * 4 + [_i32, _p]),
+    "fma_grouped_linear_fp8": (_i32, [_p] * 10 + [_i64] * 4 + [_i32, _p]),
+    "fma_grouped_linear_fp8_bwd_workspace_bytes": (_i64, [_i64] * 3),
+    "fma_grouped_linear_fp8_bwd": (_i32, [_p] * 8 + [_i64] * 4 + [_p, _i64, _i32, _p]),
     "fma_swiglu_fp8_forward": (_i32, [_p] * 4 + [_i64] * 2 + [_i32, _p]),
     "fma_swiglu_fp8_backward": (_i32, [_p] * 4 + [_i64] * 2 + [_i32, _p]),
     "fma_swiglu_experts_fp8_buffer_bytes": (_i64, [_i64] * 5 + [_i32]),

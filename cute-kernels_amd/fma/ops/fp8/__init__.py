@@ -14,7 +14,13 @@ import torch
 
 from ...math import ceil_divide
 from ...utils import ensure_contiguous
-from .cuda_implementation import dequantize_fp8_cuda, grouped_gemm_fp8_cuda, quantize_fp8_cuda
+from .cuda_implementation import (
+    dequantize_fp8_cuda,
+    grouped_gemm_fp8_cuda,
+    grouped_linear_fp8_backward_cuda,
+    grouped_linear_fp8_cuda,
+    quantize_fp8_cuda,
+)
 
 BLOCK_SIZE = 128
 _FLOATS = (torch.float32, torch.float16, torch.bfloat16)
@@ -40,8 +46,6 @@ def _empty_blocks(shape: tuple[int, ...], block_rows: int, device: torch.device)
     )
 
 
-@torch.no_grad()
-@ensure_contiguous
 def quantize_fp8(
     x: torch.Tensor, block_rows: int = 1, transposed: bool = False
 ) -> Fp8Blocks | tuple[Fp8Blocks, Fp8Blocks]:
@@ -52,12 +56,14 @@ def quantize_fp8(
     assert not transposed or block_rows == BLOCK_SIZE, "a transposed copy exists of 128 x 128 blocks only"
     assert x.dim() >= (1 if block_rows == 1 else 2), "x has too few dimensions"
     assert x.size(-1) > 0, "rows must not be empty"
-    shape = tuple(x.shape) if x.dim() > 1 else (1, x.size(0))
+    one_row = x.dim() == 1
+    shape = (1, x.size(0)) if one_row else tuple(x.shape)
     assert not transposed or shape[-2] > 0, "columns must not be empty"
+    x = x.detach().contiguous().view(shape)
     blocks = _empty_blocks(shape, block_rows, x.device)
     other = _empty_blocks((*shape[:-2], shape[-1], shape[-2]), block_rows, x.device) if transposed else None
-    quantize_fp8_cuda(x.view(shape), *blocks, *(other or (None, None)), block_rows)
-    if x.dim() == 1:
+    quantize_fp8_cuda(x, *blocks, *(other or (None, None)), block_rows)
+    if one_row:
         return Fp8Blocks(blocks.values[0], blocks.scales[0])
     return blocks if other is None else (blocks, other)
 
@@ -65,8 +71,8 @@ def quantize_fp8(
 def block_rows_of(blocks: Fp8Blocks) -> int:
     """1 or 128, from the shapes; raises if they do not fit each other"""
     values, scales = blocks
-    assert values.dtype == torch.float8_e4m3fn and scales.dtype == torch.float8_e8m0fnu, "values in e4m3, scales in e8m0"
-    assert values.dim() == scales.dim() >= 2, "values and scales should have the same number of dimensions, two at least"
+    assert values.dtype is torch.float8_e4m3fn and scales.dtype is torch.float8_e8m0fnu, "values in e4m3, scales in e8m0"
+    assert values.dim() >= 2, "values should have two dimensions at least"
     *batch, N, K = values.shape
     for block_rows in (1, BLOCK_SIZE):
         if K > 0 and scales.shape == (*batch, ceil_divide(N, block_rows), scale_columns(K)):
@@ -74,17 +80,16 @@ def block_rows_of(blocks: Fp8Blocks) -> int:
     raise AssertionError(f"scales of shape {tuple(scales.shape)} do not fit values of shape {tuple(values.shape)}")
 
 
-@torch.no_grad()
-@ensure_contiguous
 def dequantize_fp8(blocks: Fp8Blocks, dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
     """The numbers that the blocks stand for, rounded to dtype (exact in float32 and bfloat16)."""
     assert dtype in _FLOATS, f"dequantize_fp8 gives float32, float16 and bfloat16, not {dtype}"
-    one_row = blocks[0].dim() == 1
+    values, scales = (t.contiguous() for t in blocks)
+    one_row = values.dim() == 1
     if one_row:
-        blocks = Fp8Blocks(blocks[0][None], blocks[1][None])
-    block_rows = block_rows_of(blocks)
-    output = torch.empty(blocks[0].shape, dtype=dtype, device=blocks[0].device)
-    dequantize_fp8_cuda(*blocks, output, block_rows)
+        values, scales = values[None], scales[None]
+    block_rows = block_rows_of((values, scales))
+    output = torch.empty(values.shape, dtype=dtype, device=values.device)
+    dequantize_fp8_cuda(values, scales, output, block_rows)
     return output[0] if one_row else output
 
 
@@ -93,8 +98,6 @@ def _check_sizes(M_array: torch.Tensor | None, E: int) -> None:
         assert M_array.dtype == torch.uint32 and M_array.shape == (E,), "M_array should be uint32 with one entry per group"
 
 
-@torch.no_grad()
-@ensure_contiguous
 def grouped_gemm_fp8(
     A: Fp8Blocks, B: Fp8Blocks, M_array: torch.Tensor | None = None, output_dtype: torch.dtype = torch.bfloat16
 ) -> torch.Tensor:
@@ -104,21 +107,27 @@ def grouped_gemm_fp8(
     the rows of every group, on the device; None with one group (B may then be [N, K]): a plain matrix product. Rows past the last group are
     not written. K must be a multiple of 16. No gradients: grouped_linear_fp8 has them.
     """
-    A, B = Fp8Blocks(*A), Fp8Blocks(*B)
-    if B.values.dim() == 2 and B.scales.dim() == 2:
-        B = Fp8Blocks(B.values[None], B.scales[None])
-    assert A.values.dim() == 2 and B.values.dim() == 3, "A should be [R, K], B [E, N, K]"
-    E, N, K = B.values.shape
-    R = A.values.size(0)
-    assert A.values.size(1) == K, "A and B should have the same reduction length"
-    assert K % 16 == 0, "the reduction length should be a multiple of 16"
-    assert block_rows_of(A) == 1 or R == 1, "A should have a scale per row and 128 elements"
-    assert B.scales.shape == (E, ceil_divide(N, BLOCK_SIZE), scale_columns(K)) and block_rows_of(B), "B should have 128 x 128 blocks"
+    (a, a_scales), (b, b_scales) = A, B
+    if b.dim() == 2 and b_scales.dim() == 2:
+        b, b_scales = b[None], b_scales[None]
+    assert a.dim() == 2 and b.dim() == 3, "A should be [R, K], B [E, N, K]"
+    (R, K), (E, N, _) = a.shape, b.shape
+    assert b.size(2) == K, "A and B should have the same reduction length"
+    assert K > 0 and K % 16 == 0, "the reduction length should be a multiple of 16"
+    assert a.dtype is b.dtype is torch.float8_e4m3fn and a_scales.dtype is b_scales.dtype is torch.float8_e8m0fnu, (
+        "values in e4m3, scales in e8m0"
+    )
+    columns = scale_columns(K)
+    assert a_scales.shape == (R, columns), "A should have a scale per row and 128 elements"
+    assert b_scales.shape == (E, ceil_divide(N, BLOCK_SIZE), columns), "B should have 128 x 128 blocks"
     assert output_dtype in _FLOATS, f"grouped_gemm_fp8 gives float32, float16 and bfloat16, not {output_dtype}"
-    assert M_array is not None or E == 1, "several groups need M_array"
-    _check_sizes(M_array, E)
-    output = torch.empty(R, N, dtype=output_dtype, device=A.values.device)
-    grouped_gemm_fp8_cuda(*A, *B, M_array, output)
+    if M_array is not None:
+        _check_sizes(M_array, E)
+        M_array = M_array.contiguous()
+    else:
+        assert E == 1, "several groups need M_array"
+    output = torch.empty(R, N, dtype=output_dtype, device=a.device)
+    grouped_gemm_fp8_cuda(a.contiguous(), a_scales.contiguous(), b.contiguous(), b_scales.contiguous(), M_array, output)
     return output
 
 
@@ -127,31 +136,29 @@ class _GroupedLinearFp8(torch.autograd.Function):
     @ensure_contiguous
     def forward(ctx, x: torch.Tensor, weight: torch.Tensor, M_array: torch.Tensor, grad_enabled: bool) -> torch.Tensor:
         needs_x, needs_weight = (grad_enabled and n for n in ctx.needs_input_grad[:2])
-        x8 = quantize_fp8(x)
-        weight8, weight8_t = quantize_fp8(weight, BLOCK_SIZE, transposed=True) if needs_x else (quantize_fp8(weight, BLOCK_SIZE), None)
-        output = grouped_gemm_fp8(x8, weight8, M_array, x.dtype)
+        E, N, K = weight.shape
+        x8 = _empty_blocks(x.shape, 1, x.device)
+        weight8 = _empty_blocks(weight.shape, BLOCK_SIZE, x.device)
+        weight8_t = _empty_blocks((E, K, N), BLOCK_SIZE, x.device) if needs_x else (None, None)
+        output = x.new_empty(x.size(0), N)
+        grouped_linear_fp8_cuda(x, weight, M_array, *x8, *weight8, *weight8_t, output)
         if needs_x or needs_weight:
             # x is kept in 8 bits, for the weight's gradient; the weight as its transposed copy, for x's
-            ctx.save_for_backward(*(x8 if needs_weight else (None, None)), *(weight8_t or (None, None)), M_array)
+            ctx.save_for_backward(*(x8 if needs_weight else (None, None)), *weight8_t, M_array)
+            ctx.K = K
         return output
 
     @staticmethod
     @ensure_contiguous
     def backward(ctx, output_grad: torch.Tensor) -> tuple[torch.Tensor | None, ...]:
-        from ...modules.moe.cuda_implementation import grouped_gemm_ragged_cuda
-
-        x_values, x_scales, weight_values, weight_scales, M_array = ctx.saved_tensors
-        x_grad = weight_grad = None
-        if ctx.needs_input_grad[0]:
-            x_grad = grouped_gemm_fp8(quantize_fp8(output_grad), Fp8Blocks(weight_values, weight_scales), M_array, output_grad.dtype)
+        *saved, M_array = ctx.saved_tensors
+        (R, N), K = output_grad.shape, ctx.K
+        x_grad = output_grad.new_empty(R, K) if ctx.needs_input_grad[0] else None
+        weight_grad = None
         if ctx.needs_input_grad[1]:
-            x = dequantize_fp8(Fp8Blocks(x_values, x_scales), output_grad.dtype)
-            E, N, K = M_array.numel(), output_grad.size(1), x.size(1)
-            weight_grad = output_grad.new_empty(E, N, K)
-            if x.size(0) == 0:
-                weight_grad.zero_()
-            else:
-                grouped_gemm_ragged_cuda(output_grad, x, weight_grad, M_array, True, N, K, 0, True, False)
+            weight_grad = (output_grad.new_empty if R else output_grad.new_zeros)(M_array.numel(), N, K)
+        if R:
+            grouped_linear_fp8_backward_cuda(output_grad, *saved, M_array, K, x_grad, weight_grad)
         return x_grad, weight_grad, None, None
 
 

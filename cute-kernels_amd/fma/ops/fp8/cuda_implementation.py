@@ -90,3 +90,61 @@ def grouped_gemm_fp8_cuda(
             _lib.dtype_code(output.dtype), _lib.current_stream(A.device),
         )  # fmt: skip
     _lib.check(rc, "grouped_gemm_fp8_cuda")
+
+
+@hip_op("grouped_linear_fp8_cuda", mutates_args={"x_values", "x_scales", "weight_values", "weight_scales", "weight_t_values", "weight_t_scales", "output"})
+def grouped_linear_fp8_cuda(
+    x: torch.Tensor, weight: torch.Tensor, M_array: torch.Tensor, x_values: torch.Tensor, x_scales: torch.Tensor,
+    weight_values: torch.Tensor, weight_scales: torch.Tensor, weight_t_values: torch.Tensor | None, weight_t_scales: torch.Tensor | None,
+    output: torch.Tensor,
+) -> None:  # fmt: skip
+    """quantize_fp8 of x and of weight (with its transposed copy if that is asked for) and grouped_gemm_fp8 of the two, as one call"""
+    _lib.require_gpu(x, weight, M_array, x_values, x_scales, weight_values, weight_scales, weight_t_values, weight_t_scales, output)
+    E, N, K = weight.shape
+    R = x.size(0)
+    assert x.shape == (R, K) == x_values.shape and weight_values.shape == weight.shape and output.shape == (R, N)
+    assert x.dtype == weight.dtype == output.dtype and x.is_contiguous() and weight.is_contiguous() and output.is_contiguous()
+    assert M_array.dtype == torch.uint32 and M_array.numel() == E and M_array.is_contiguous()
+    _check_blocks(x_values, x_scales, R, K, 1)
+    _check_blocks(weight_values, weight_scales, N, K, 128)
+    if weight_t_values is not None:
+        assert weight_t_values.shape == (E, K, N)
+        _check_blocks(weight_t_values, weight_t_scales, K, N, 128)
+    for t in (weight, M_array, x_values, x_scales, weight_values, weight_scales, output):
+        assert t.device == x.device
+    with _lib.on_device(x.device):
+        rc = _lib.load().fma_grouped_linear_fp8(
+            x.data_ptr(), weight.data_ptr(), x_values.data_ptr(), x_scales.data_ptr(), weight_values.data_ptr(), weight_scales.data_ptr(),
+            _lib.ptr(weight_t_values), _lib.ptr(weight_t_scales), output.data_ptr(), M_array.data_ptr(), E, R, N, K,
+            _lib.dtype_code(x.dtype), _lib.current_stream(x.device),
+        )  # fmt: skip
+    _lib.check(rc, "grouped_linear_fp8_cuda")
+
+
+@hip_op("grouped_linear_fp8_backward_cuda", mutates_args={"x_grad", "weight_grad"})
+def grouped_linear_fp8_backward_cuda(
+    output_grad: torch.Tensor, x_values: torch.Tensor | None, x_scales: torch.Tensor | None, weight_t_values: torch.Tensor | None,
+    weight_t_scales: torch.Tensor | None, M_array: torch.Tensor, K: int, x_grad: torch.Tensor | None, weight_grad: torch.Tensor | None,
+) -> None:  # fmt: skip
+    _lib.require_gpu(output_grad, x_values, x_scales, weight_t_values, weight_t_scales, M_array, x_grad, weight_grad)
+    R, N = output_grad.shape
+    E = M_array.numel()
+    assert output_grad.is_contiguous() and M_array.dtype == torch.uint32 and M_array.is_contiguous()
+    if x_grad is not None:
+        assert x_grad.shape == (R, K) and x_grad.dtype == output_grad.dtype and x_grad.is_contiguous()
+        assert weight_t_values.shape == (E, K, N)
+        _check_blocks(weight_t_values, weight_t_scales, K, N, 128)
+    if weight_grad is not None:
+        assert weight_grad.shape == (E, N, K) and weight_grad.dtype == output_grad.dtype and weight_grad.is_contiguous()
+        assert x_values.shape == (R, K)
+        _check_blocks(x_values, x_scales, R, K, 1)
+    lib = _lib.load()
+    with _lib.on_device(output_grad.device):
+        nbytes = lib.fma_grouped_linear_fp8_bwd_workspace_bytes(R, N, K)
+        workspace = torch.empty(nbytes, dtype=torch.uint8, device=output_grad.device)
+        rc = lib.fma_grouped_linear_fp8_bwd(
+            output_grad.data_ptr(), _lib.ptr(x_values), _lib.ptr(x_scales), _lib.ptr(weight_t_values), _lib.ptr(weight_t_scales),
+            _lib.ptr(x_grad), _lib.ptr(weight_grad), M_array.data_ptr(), E, R, N, K, workspace.data_ptr(), nbytes,
+            _lib.dtype_code(output_grad.dtype), _lib.current_stream(output_grad.device),
+        )  # fmt: skip
+    _lib.check(rc, "grouped_linear_fp8_backward_cuda")

@@ -459,6 +459,18 @@ int fma_dequantize_fp8(const void* values, const void* scales, void* out, int64_
 int fma_grouped_gemm_fp8(const void* A, const void* A_scales, const void* B, const void* B_scales, void* D, const uint32_t* M_arr,
                          int64_t E, int64_t R, int64_t N, int64_t K, int dtype, void* stream);
 
+/* The product of 16-bit tensors, quantised on the way: y_e = q(x_e) q(W_e)^T, x [R, K], W [E, N, K], y [R, N] of dtype (FMA_BF16 or
+ * FMA_F16); x_values and W_values with their scales are written, Wt_values (the transposed copy, for dx) unless it is NULL.
+ * Backward: dx = q(dy_e) q(W_e) [R, K] and dW_e = dy_e^T x^_e [E, N, K], x^ the stored values, the second product in 16 bits; each is
+ * computed unless NULL. N % 16 == K % 16 == 0 there; R > 0 (dW is not written without rows). */
+int fma_grouped_linear_fp8(const void* x, const void* W, void* x_values, void* x_scales, void* W_values, void* W_scales, void* Wt_values,
+                           void* Wt_scales, void* y, const uint32_t* M_arr, int64_t E, int64_t R, int64_t N, int64_t K, int dtype,
+                           void* stream);
+int64_t fma_grouped_linear_fp8_bwd_workspace_bytes(int64_t R, int64_t N, int64_t K);
+int fma_grouped_linear_fp8_bwd(const void* dy, const void* x_values, const void* x_scales, const void* Wt_values, const void* Wt_scales,
+                               void* dx, void* dW, const uint32_t* M_arr, int64_t E, int64_t R, int64_t N, int64_t K, void* workspace,
+                               int64_t workspace_bytes, int dtype, void* stream);
+
 /* y [R, I] = up * gate * sigmoid(gate) of x [R, 2 I] = [up | gate], and x in 8-bit blocks along each half: values [R, 2, I],
  * scales [R, 2, pitch(I)]; any I. The backward reads those: dx [R, 2 I] from dy [R, I]. */
 int fma_swiglu_fp8_forward(const void* x, void* y, void* values, void* scales, int64_t R, int64_t I, int dtype, void* stream);

@@ -74,6 +74,20 @@ def test_product_validation(lib):
         assert product(None, None, None, None, None, p, *empty, 128, 2, None) == 0
 
 
+def test_linear_validation(lib):
+    buf, p = _pointer()
+
+    def backward(R=8, N=64, K=32, dtype=2, dy=p, x=p, wt=p, size=1 << 30):
+        return lib.fma_grouped_linear_fp8_bwd(dy, x, x, wt, wt, p, p, p, 2, R, N, K, p, size, dtype, None)
+
+    assert lib.fma_grouped_linear_fp8(p, p, p, p, p, p, None, None, p, p, 2, 8, 64, 32, 0, None) == -2
+    assert lib.fma_grouped_linear_fp8(p, p, p, p, p, p, None, None, p, p, 2, 8, 64, 24, 2, None) == -3
+    assert lib.fma_grouped_linear_fp8(p, p, p, p, p, p, p, None, p, p, 2, 8, 64, 32, 2, None) == -1
+    assert backward(dtype=0) == -2 and backward(N=40) == -3 and backward(dy=None) == -1 and backward(x=None) == -1 and backward(wt=None) == -1
+    assert backward(size=64) == -7 and backward(R=0) == 0
+    assert lib.fma_grouped_linear_fp8_bwd_workspace_bytes(8, 64, 32) == 512 + 256 + 512
+
+
 def test_experts_validation(lib):
     buf, p = _pointer()
 
@@ -94,7 +108,7 @@ def test_experts_validation(lib):
     assert forward(ids=None) == -1 and forward(buffer=None) == -1 and forward(ids=p + 2) == -6
     for sizes in ((1, 1, 1, 16, 16), (37, 2, 6, 256, 208), (8192, 8, 64, 2048, 1408), (3, 3, 5, 528, 1040)):
         assert lib.fma_swiglu_experts_fp8_buffer_bytes(*sizes, 1) == buffer_bytes(*sizes)
-        assert lib.fma_swiglu_experts_fp8_buffer_bytes(*sizes, 0) < buffer_bytes(*sizes)
+    assert lib.fma_swiglu_experts_fp8_buffer_bytes(8192, 8, 64, 2048, 1408, 0) < buffer_bytes(8192, 8, 64, 2048, 1408)
 
 
 def _blocks(*shape, rows=1, K=None):
