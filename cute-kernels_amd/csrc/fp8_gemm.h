@@ -13,6 +13,8 @@
 //    two of the next. They are written in assembly, so the compiler places no waits for them; the one wait of a step, in front of its
 //    last sixteenth-row block, is written by hand, and behind it the step's own stage is free again.
 //  * Scales: a dword of four blocks per row of A (and per 128 rows of B) goes to LDS the same way every fourth step.
+//  * Tall tiles (at most 256 groups): a tile may have 288 rows, 256 and one more row block per wavefront, whose 4 KB a step have stages of
+//    their own.
 //  * A reduction may be cut into segments (the two halves of a pre-activation): blocks begin anew in each.
 //  * GLU: the tile holds 128 "up" and 128 "gate" columns; the activation, 128 columns or one block, is quantised from the fp32 sums: the
 //    largest magnitude of a row goes from wavefront to wavefront through LDS. With KEEP the pre-activation is kept in 8 bits too.
@@ -43,7 +45,8 @@ constexpr int kTileM = 256, kTileN = 256;
 constexpr int kWavesM = 2, kWavesN = 4, kWaves = kWavesM * kWavesN, kGemmThreads = kWaves * 64;
 constexpr int kRowBlocks = 8, kColBlocks = 4;  // 16 x 16 blocks of a wavefront's 128 x 64
 constexpr uint32_t kOperandBytes = 256 * kBlock, kStage = 2 * kOperandBytes;
-constexpr uint32_t kScaleWords = 320;  // per buffer: 256 rows of A, two blocks of B, the rest of the fifth wavefront's load
+constexpr int kTallM = 288;               // rows of a tall tile: 256, and one more row block per wavefront
+constexpr uint32_t kTallGroups = 256;     // groups that a launch of the kernels for tall tiles may have (their table leaves room for the rows)
 constexpr uint32_t kMaxGroups = FMA_MAX_GROUPS;
 
 enum Epilogue { EPI_BF16, EPI_F16, EPI_F32, EPI_GLU, EPI_GLU_KEEP, EPI_GLU_BWD_BF16, EPI_GLU_BWD_F16 };
@@ -89,21 +92,28 @@ __device__ __forceinline__ uint32_t pack_pair(float lo, float hi) {
     else return ::fmahip::gemm::ElemF16::pack2(lo, hi);
 }
 
-template <int EPI, bool GATHER>
+template <int EPI, bool GATHER, bool TALL>
 __global__ __launch_bounds__(kGemmThreads) void fp8_gemm_kernel(const GemmArgs args) {
     constexpr bool kGlu = EPI == EPI_GLU || EPI == EPI_GLU_KEEP;
     constexpr bool kBwd = EPI == EPI_GLU_BWD_BF16 || EPI == EPI_GLU_BWD_F16;
     constexpr uint32_t kCols = kGlu ? kTileN / 2 : kTileN;  // columns of the output grid per tile
     // Stores of an epilogue per wavefront, at least (0, 59: an epilogue that has waited for all loads in front of them itself)
     constexpr int kStores = EPI == EPI_BF16 || EPI == EPI_F16 ? 2 * kRowBlocks : (EPI == EPI_GLU ? 2 * kRowBlocks : (EPI == EPI_GLU_KEEP ? 6 * kRowBlocks : (kBwd ? 59 : 0)));
+    constexpr uint32_t kMostGroups = TALL ? kTallGroups : kMaxGroups;
+    constexpr int kBlocks = TALL ? kRowBlocks + 1 : kRowBlocks;  // row blocks of a wavefront, at most
+    constexpr uint32_t kMostRows = TALL ? kTallM : kTileM;
+    // per buffer: the scales of 256 rows of A, of two blocks of B (with the rest of that wavefront's load), and of the rows past 256
+    constexpr uint32_t kScaleWords = TALL ? 384 : 320;
     constexpr int kMaxima = EPI == EPI_GLU_KEEP ? 3 : (kGlu ? 1 : (kBwd ? 1 : 0));
 
     __shared__ __attribute__((aligned(1024))) uint8_t s_op[2 * kStage];
     __shared__ __attribute__((aligned(256))) uint32_t s_scale[2 * kScaleWords];
-    __shared__ __attribute__((aligned(16))) uint32_t s_max[kMaxima ? kMaxima * 256 * 4 : 4];
+    __shared__ __attribute__((aligned(16))) uint32_t s_max[kMaxima ? kMaxima * kMostRows * 4 : 4];
+    __shared__ __attribute__((aligned(1024))) uint8_t s_x[TALL ? 2 * 32 * kBlock : 16];  // rows 256 .. 287 of A, per stage
+    __shared__ uint32_t s_height;
     __shared__ __attribute__((aligned(1024))) uint8_t s_out[EPI == EPI_BF16 || EPI == EPI_F16 ? kWaves * 2048 : 16];
-    __shared__ uint32_t s_tiles[kMaxGroups + 1];  // row tiles of the groups before
-    __shared__ uint32_t s_first[kMaxGroups + 1];  // first row of the group
+    __shared__ uint32_t s_tiles[kMostGroups + 1];  // row tiles of the groups before
+    __shared__ uint32_t s_first[kMostGroups + 1];  // first row of the group
 
     const uint32_t tid = threadIdx.x, lane = tid & 63u;
     const uint32_t wave = uniform(tid >> 6);
@@ -113,7 +123,25 @@ __global__ __launch_bounds__(kGemmThreads) void fp8_gemm_kernel(const GemmArgs a
 
     // ---- group table: rows past R do not exist, whatever the sizes say ----
     if (wave == 0) {
-        uint32_t tiles = 0, rows = 0;
+        uint32_t tiles = 0, rows = 0, height = kTileM;
+        if constexpr (TALL) {
+            // Tiles of up to 288 rows where they save more rounds of tiles than their longer steps cost, a tenth: experts of 256 or 512 +- 20 rows,
+            // as an even routing makes them, otherwise pay a nearly empty tile every other time.
+            uint32_t low = 0, high = 0;
+            for (uint32_t e = lane; e < E; e += 64) {
+                uint32_t m = args.sizes ? args.sizes[e] : args.R;
+                m = m < args.R ? m : args.R;
+                low += (m + kTileM - 1) / kTileM;
+                high += (m + kTallM - 1) / kTallM;
+            }
+#pragma unroll
+            for (int d = 32; d > 0; d >>= 1) {
+                low += (uint32_t)__shfl_xor((int)low, d, 64);
+                high += (uint32_t)__shfl_xor((int)high, d, 64);
+            }
+            const uint64_t columns = (N + kCols - 1) / kCols, g = gridDim.x;
+            if ((high * columns + g - 1) / g * 11u < (low * columns + g - 1) / g * 10u) height = kTallM;
+        }
         for (uint32_t base = 0; base < E; base += 64) {
             const uint32_t e = base + lane;
             uint32_t m = e < E ? (args.sizes ? args.sizes[e] : args.R) : 0u;
@@ -123,7 +151,7 @@ __global__ __launch_bounds__(kGemmThreads) void fp8_gemm_kernel(const GemmArgs a
             const uint32_t last = end < args.R ? (uint32_t)end : args.R;
             const uint64_t before = end - m;
             const uint32_t first = before < args.R ? (uint32_t)before : args.R;
-            const uint32_t t = (last - first + kTileM - 1) / kTileM;
+            const uint32_t t = (last - first + height - 1) / height;
             const uint32_t it = wave_inclusive_scan<uint32_t>(t);
             if (e < E) {
                 s_tiles[e] = tiles + it - t;
@@ -135,6 +163,7 @@ __global__ __launch_bounds__(kGemmThreads) void fp8_gemm_kernel(const GemmArgs a
         if (lane == 0) {
             s_tiles[E] = tiles;
             s_first[E] = rows;
+            s_height = height;
         }
     }
     __syncthreads();
@@ -170,7 +199,13 @@ __global__ __launch_bounds__(kGemmThreads) void fp8_gemm_kernel(const GemmArgs a
         Tile tile;
         tile.e = e;
         tile.row0 = first + m * kTileM;
-        tile.rows = end - tile.row0 < (uint32_t)kTileM ? end - tile.row0 : (uint32_t)kTileM;
+        uint32_t most = kTileM;
+        if constexpr (TALL) {  // of a group's tiles as few as its rows need are tall, the first ones
+            const uint32_t group = end - first, past = group > mt * kTileM ? (group - mt * kTileM + 31u) / 32u : 0u;
+            tile.row0 += 32u * (m < past ? m : past);
+            most += m < past ? 32u : 0u;
+        }
+        tile.rows = end - tile.row0 < most ? end - tile.row0 : most;
         tile.n0 = n * kCols;
         return tile;
     };
@@ -182,11 +217,13 @@ __global__ __launch_bounds__(kGemmThreads) void fp8_gemm_kernel(const GemmArgs a
     const uint32_t a_lane = (wave * 8u + lr) * args.a_pitch + a_chunk;
     const uint32_t b_lane = (wave * 8u + lr) * K + b_chunk;
     const uint32_t lds0 = lds_address(s_op);
+    const uint32_t lds_x = lds_address(s_x);
     const uint32_t lds_scale = lds_address(reinterpret_cast<const uint8_t*>(s_scale)) + wave * 256u;
     uint32_t l_tile = slot, l_ks = 0, l_seg = 0, l_stage = 0, l_quad = 0;  // next step to be loaded
     uint64_t l_a = 0, l_b = 0, l_b2 = 0, l_s = 0;  // addresses of the operands and of this wavefront's scales, at the current segment
     uint32_t l_a_bytes = 0, l_b_bytes = 0;
-    uint32_t l_gather[4] = {0u, 0u, 0u, 0u};
+    constexpr int kGathered = TALL ? 5 : 4;
+    uint32_t l_gather[kGathered] = {};
     uint32_t l_scale = kOutOfRange;  // this lane's offset into the scales
     Tile l_found = {0u, 0u, 0u, 0u};  // the tile that the loads are in
     auto aim = [&]() {
@@ -195,7 +232,7 @@ __global__ __launch_bounds__(kGemmThreads) void fp8_gemm_kernel(const GemmArgs a
             l_scale = kOutOfRange;
             if constexpr (GATHER) {
 #pragma unroll
-                for (int i = 0; i < 4; ++i) l_gather[i] = kOutOfRange;
+                for (int i = 0; i < kGathered; ++i) l_gather[i] = kOutOfRange;
             }
             return;
         }
@@ -210,8 +247,8 @@ __global__ __launch_bounds__(kGemmThreads) void fp8_gemm_kernel(const GemmArgs a
             l_a = uniform64((uint64_t)(uintptr_t)args.A);
             l_a_bytes = args.a_rows * args.a_pitch;
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const uint32_t r = i * 64u + wave * 8u + lr;
+            for (int i = 0; i < kGathered; ++i) {
+                const uint32_t r = i * 64u + wave * 8u + lr;  // (i == 4: four wavefronts load rows 256 .. 287)
                 const uint32_t src = r < t.rows ? (uint32_t)args.row_index[t.row0 + r] / args.divisor : args.a_rows;
                 l_gather[i] = src < args.a_rows ? src * args.a_pitch + a_chunk : kOutOfRange;
             }
@@ -219,8 +256,8 @@ __global__ __launch_bounds__(kGemmThreads) void fp8_gemm_kernel(const GemmArgs a
             l_a = uniform64((uint64_t)(uintptr_t)args.A + (uint64_t)t.row0 * args.a_pitch);
             l_a_bytes = uniform(t.rows * args.a_pitch);
         }
-        if (wave < 4) {
-            const uint32_t r = wave * 64u + lane;
+        if (wave < 4 || (TALL && wave == 5)) {
+            const uint32_t r = wave < 4 ? wave * 64u + lane : 256u + lane;
             l_s = (uint64_t)(uintptr_t)args.A_s;
             if constexpr (GATHER) {
                 const uint32_t src = r < t.rows ? (uint32_t)args.row_index[t.row0 + r] / args.divisor : args.a_rows;
@@ -252,8 +289,17 @@ __global__ __launch_bounds__(kGemmThreads) void fp8_gemm_kernel(const GemmArgs a
         load_lds16(rsrc_at(kGlu && i >= 2 ? l_b2 : l_b, l_b_bytes), v, rows * K + l_ks * kBlock,
                    lds0 + l_stage + kOperandBytes + ((uint32_t)i * 8u + wave) * 1024u);
     };
+    auto load_x = [&]() {  // rows past 256, where the tile has any
+        if constexpr (TALL) {
+            if (l_found.rows > (uint32_t)kTileM && wave < 4) {
+                uint32_t v = GATHER ? l_gather[kGathered - 1] : a_lane;
+                if (l_ks * kBlock + a_chunk >= K) v = kOutOfRange;
+                load_lds16(rsrc_at(l_a, l_a_bytes), v, (GATHER ? 0u : 256u * args.a_pitch) + l_ks * kBlock, lds_x + (l_stage ? 32u * kBlock : 0u) + wave * 1024u);
+            }
+        }
+    };
     auto load_scales = [&]() {  // at the first of four steps
-        if ((l_ks & 3u) == 0 && wave < 5)
+        if ((l_ks & 3u) == 0 && wave < (TALL ? 6u : 5u))
             ::fmahip::gemm::buffer_load_lds_quiet_b32(rsrc_at(l_s, 0x7fffffffu), l_scale, l_ks, lds_scale + l_quad * (kScaleWords * 4u));
     };
     auto next_load = [&]() {
@@ -269,7 +315,7 @@ __global__ __launch_bounds__(kGemmThreads) void fp8_gemm_kernel(const GemmArgs a
             } else {
                 l_a += args.a_seg;
                 l_b += args.b_seg;
-                l_s += wave < 4 ? args.as_seg : args.bs_seg;
+                l_s += wave < 4 || (TALL && wave == 5) ? args.as_seg : args.bs_seg;
             }
         }
         if ((l_ks & 3u) == 0) l_quad ^= 1u;
@@ -296,29 +342,35 @@ __global__ __launch_bounds__(kGemmThreads) void fp8_gemm_kernel(const GemmArgs a
 
     // A row block's results are one 16-register value: the instruction's 4-register form has no variant whose result stays in place, and
     // without the value being named after every instruction results wander through the register file until it spills.
-    f32x16 acc[kRowBlocks];
+    f32x16 acc[kBlocks];
     i32x8 fa[2], fb[kColBlocks];
     int sa[2], sb[2];
     auto read_a = [&](int i, int buf) {
         fa[buf] = read_frag(a_off + (uint32_t)i * 16u * kBlock);
         sa[buf] = read_scale(sa_off + (uint32_t)i * 64u);
     };
+    auto read_x = [&]() {  // the row block past 256, where block 6 was
+        const uint32_t off = (c_stage ? 32u * kBlock : 0u) + (wm * 16u + r16) * kBlock + ((q ^ a_key) << 4);
+        const i32x4 lo = *reinterpret_cast<const i32x4*>(s_x + off), hi = *reinterpret_cast<const i32x4*>(s_x + (off ^ 64u));
+        fa[0] = __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
+        sa[0] = read_scale((320u + wm * 16u + r16) * 4u);
+    };
     auto read_b = [&](int j) { fb[j] = read_frag(b_off + b_step(j)); };
     auto read_sb = [&]() {
         sb[0] = read_scale(sb_off);
         sb[1] = kGlu ? read_scale(sb_off + 4u) : sb[0];
     };
-    auto mma = [&](auto first_c, int i, int j, int buf, int scale_b) {
-        f32x16& c = acc[i];
+    auto mma_with = [&](auto first_c, f32x16& c, int j, i32x8 a, int scale_a, int scale_b) {
         f32x4 v = {0.f, 0.f, 0.f, 0.f};  // (a tile's first step: the instruction takes the constant)
         if constexpr (!decltype(first_c)::value) v = f32x4{c[4 * j], c[4 * j + 1], c[4 * j + 2], c[4 * j + 3]};
-        v = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(fb[j], fa[buf], v, 0, 0, 0, scale_b, 0, sa[buf]);
+        v = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(fb[j], a, v, 0, 0, 0, scale_b, 0, scale_a);
         c[4 * j] = v[0];
         c[4 * j + 1] = v[1];
         c[4 * j + 2] = v[2];
         c[4 * j + 3] = v[3];
         asm("" : "+v"(c));
     };
+    auto mma = [&](auto first_c, int i, int j, int buf, int scale_b) { mma_with(first_c, acc[i], j, fa[buf], sa[buf], scale_b); };
     auto next_step = [&]() {  // of the fragments
         c_stage ^= kStage;
         ++c_ks;
@@ -334,6 +386,7 @@ __global__ __launch_bounds__(kGemmThreads) void fp8_gemm_kernel(const GemmArgs a
         for (int i = 0; i < 4; ++i) load_b(i);
 #pragma unroll
         for (int i = 0; i < 4; ++i) load_a(i);
+        load_x();
         load_scales();
         next_load();
     }
@@ -348,7 +401,7 @@ __global__ __launch_bounds__(kGemmThreads) void fp8_gemm_kernel(const GemmArgs a
     first_fragments();
 
     // One K step of a tile; FIRST: of its first, whose sums begin at zero.
-    auto k_step = [&](auto first_c) {
+    auto k_step = [&](auto first_c, bool tall) {
         constexpr bool FIRST = decltype(first_c)::value;
 #pragma unroll
         for (int i = 0; i < kRowBlocks - 1; ++i) {
@@ -361,6 +414,7 @@ __global__ __launch_bounds__(kGemmThreads) void fp8_gemm_kernel(const GemmArgs a
                 mma(first_c, i, j, i & 1, sb[j >> 1]);
                 if (i == 1) load_b(j);
             }
+            if (TALL && i == kRowBlocks - 2 && tall) read_x();
             __builtin_amdgcn_sched_barrier(0);
         }
         // Every fragment of the step is read, and the next step has landed (all but the loads of B just issued): the next step's fragments
@@ -373,6 +427,12 @@ __global__ __launch_bounds__(kGemmThreads) void fp8_gemm_kernel(const GemmArgs a
             constexpr int i = kRowBlocks - 1;
             const int s0 = sb[0], s1 = sb[1];
             read_sb();
+            if constexpr (TALL) {
+                if (tall) {
+#pragma unroll
+                    for (int j = 0; j < kColBlocks; ++j) mma_with(first_c, acc[kBlocks - 1], j, fa[0], sa[0], j < 2 ? s0 : s1);
+                }
+            }
 #pragma unroll
             for (int j = 0; j < kColBlocks; ++j) {
                 mma(first_c, i, j, i & 1, j < 2 ? s0 : s1);
@@ -381,6 +441,7 @@ __global__ __launch_bounds__(kGemmThreads) void fp8_gemm_kernel(const GemmArgs a
             }
             read_a(0, 0);
         }
+        load_x();
         load_scales();
         next_load();
     };
@@ -389,8 +450,11 @@ __global__ __launch_bounds__(kGemmThreads) void fp8_gemm_kernel(const GemmArgs a
     for (uint32_t c_tile = slot; c_tile < total; c_tile += grid) {
         if (steps < 3) t = find(c_tile);  // (the loads are two steps ahead: with three and more they are in this tile when it begins)
         else t = l_found;
-        k_step(std::integral_constant<bool, true>{});
-        for (uint32_t step = 1; step < steps; ++step) k_step(std::integral_constant<bool, false>{});
+        const bool tall = TALL && t.rows > (uint32_t)kTileM;
+        k_step(std::integral_constant<bool, true>{}, tall);
+        for (uint32_t step = 1; step < steps; ++step) k_step(std::integral_constant<bool, false>{}, tall);
+        // first row of this wavefront's row block i
+        auto block_row = [&](int i) -> uint32_t { return i < kRowBlocks ? wm * 128u + (uint32_t)i * 16u : 256u + wm * 16u; };
 
         // ---- epilogue ----
         if constexpr (EPI == EPI_BF16 || EPI == EPI_F16) {
@@ -406,7 +470,8 @@ __global__ __launch_bounds__(kGemmThreads) void fp8_gemm_kernel(const GemmArgs a
                 const bool in = t.n0 + col < N;
                 const uint32_t put = r16 * 128u + ((q ^ (r16 & 7u)) << 4), get = line * 128u + ((chunk ^ line) << 4);
 #pragma unroll
-                for (int i = 0; i < kRowBlocks; ++i) {
+                for (int i = 0; i < kBlocks; ++i) {
+                if (i >= kRowBlocks && !tall) continue;
                     u32x4 v[2];
 #pragma unroll
                     for (int p = 0; p < 2; ++p)
@@ -415,18 +480,19 @@ __global__ __launch_bounds__(kGemmThreads) void fp8_gemm_kernel(const GemmArgs a
                     *reinterpret_cast<u32x4*>(image + put) = v[0];
                     *reinterpret_cast<u32x4*>(image + (put ^ 64u)) = v[1];
                     const u32x4 low = *reinterpret_cast<const u32x4*>(image + get), high = *reinterpret_cast<const u32x4*>(image + 1024u + get);
-                    const uint32_t at = ((wm * 128u + (uint32_t)i * 16u + line) * N + col) * 2u;
+                    const uint32_t at = ((block_row(i) + line) * N + col) * 2u;
                     ::fmahip::gemm::store_tile16<false>(rsrc, in ? at : kOutOfRange, __builtin_bit_cast(uint4, low));
                     ::fmahip::gemm::store_tile16<false>(rsrc, in ? at + N * 16u : kOutOfRange, __builtin_bit_cast(uint4, high));
                 }
             } else {
 #pragma unroll
-                for (int i = 0; i < kRowBlocks; ++i) {
-                    const uint32_t row = wm * 128u + (uint32_t)i * 16u + r16;
+                for (int i = 0; i < kBlocks; ++i) {
+                if (i >= kRowBlocks && !tall) continue;
+                    const uint32_t row = block_row(i) + r16;
 #pragma unroll
                     for (int x = 0; x < 16; ++x) {
                         const uint32_t col = wn * 64u + (uint32_t)(x / 8) * 32u + q * 8u + (uint32_t)(x % 8);
-                        if (row < t.rows && t.n0 + col < N) ((T*)tile)[(uint64_t)row * N + col] = Num<T>::down(acc[i][x]);
+                        if (row < t.rows && t.n0 + col < N) tile[(uint64_t)row * N + col] = (uint16_t)pack_pair<T>(acc[i][x], 0.f);
                     }
                 }
                 wait_vm<0>();
@@ -434,8 +500,9 @@ __global__ __launch_bounds__(kGemmThreads) void fp8_gemm_kernel(const GemmArgs a
         } else if constexpr (EPI == EPI_F32) {
             float* const tile = (float*)args.D + (uint64_t)t.row0 * N + t.n0;
 #pragma unroll
-            for (int i = 0; i < kRowBlocks; ++i) {
-                const uint32_t row = wm * 128u + (uint32_t)i * 16u + r16;
+            for (int i = 0; i < kBlocks; ++i) {
+                if (i >= kRowBlocks && !tall) continue;
+                const uint32_t row = block_row(i) + r16;
 #pragma unroll
                 for (int x = 0; x < 16; x += 4) {
                     const uint32_t col = wn * 64u + (uint32_t)(x / 8) * 32u + q * 8u + (uint32_t)(x % 8);
@@ -465,7 +532,8 @@ __global__ __launch_bounds__(kGemmThreads) void fp8_gemm_kernel(const GemmArgs a
                 return u * g * sigmoid_clamped_fast(g);
             };
 #pragma unroll
-            for (int i = 0; i < kRowBlocks; ++i) {
+            for (int i = 0; i < kBlocks; ++i) {
+                if (i >= kRowBlocks && !tall) continue;
                 uint32_t m[3] = {0u, 0u, 0u};
 #pragma unroll
                 for (int x = 0; x < 8; ++x) {
@@ -478,14 +546,14 @@ __global__ __launch_bounds__(kGemmThreads) void fp8_gemm_kernel(const GemmArgs a
 #pragma unroll
                 for (int w = 0; w < kWhat; ++w) {
                     const uint32_t v = row_max(m[w]);
-                    if (q == 0) s_max[((uint32_t)w * 256u + wm * 128u + (uint32_t)i * 16u + r16) * 4u + wn] = v;
+                    if (q == 0) s_max[((uint32_t)w * kMostRows + block_row(i) + r16) * 4u + wn] = v;
                 }
                 __builtin_amdgcn_sched_barrier(0);
             }
             lds_barrier();
             // (activations are computed anew rather than kept: 64 more registers)
 #pragma unroll
-            for (int i = 0; i < kRowBlocks; ++i) asm("" : "+v"(acc[i]));
+            for (int i = 0; i < kBlocks; ++i) asm("" : "+v"(acc[i]));
 #pragma unroll
             for (int w = 0; w < kWhat; ++w) {
                 // values of this tile's rows from its first column on (the rows' ends are the descriptor's), and their scales
@@ -496,9 +564,10 @@ __global__ __launch_bounds__(kGemmThreads) void fp8_gemm_kernel(const GemmArgs a
                                                : (uint64_t)(uintptr_t)args.h_s + (uint64_t)t.row0 * s_pitch + (w == 2 ? args.o_pitch_s : 0u);
                 const __amdgpu_buffer_rsrc_t rv = buffer_at(values), rs = buffer_at(scales);
 #pragma unroll
-                for (int i = 0; i < kRowBlocks; ++i) {
-                    const uint32_t row = wm * 128u + (uint32_t)i * 16u + r16;
-                    const uint4 m = *reinterpret_cast<const uint4*>(s_max + ((uint32_t)w * 256u + row) * 4u);
+                for (int i = 0; i < kBlocks; ++i) {
+                if (i >= kRowBlocks && !tall) continue;
+                    const uint32_t row = block_row(i) + r16;
+                    const uint4 m = *reinterpret_cast<const uint4*>(s_max + ((uint32_t)w * kMostRows + row) * 4u);
                     const uint32_t byte = scale_byte(max_u32(max_u32(m.x, m.y), max_u32(m.z, m.w)));
                     const float inverse = scale_inverse(byte);
                     float v[8];
@@ -519,8 +588,9 @@ __global__ __launch_bounds__(kGemmThreads) void fp8_gemm_kernel(const GemmArgs a
             const uint32_t s_pitch = args.o_pitch_s;
             wait_vm<0>();
 #pragma unroll
-            for (int i = 0; i < kRowBlocks; ++i) {
-                const uint32_t row = wm * 128u + (uint32_t)i * 16u + r16;
+            for (int i = 0; i < kBlocks; ++i) {
+                if (i >= kRowBlocks && !tall) continue;
+                const uint32_t row = block_row(i) + r16;
                 const bool live = row < t.rows;
                 const uint64_t to = t.row0 + (live ? row : 0u);
                 float d[2][2][8];  // [half][columns p][x]
@@ -569,10 +639,7 @@ __global__ __launch_bounds__(kGemmThreads) void fp8_gemm_kernel(const GemmArgs a
                             const float(&v)[8] = d[h][p];
                             if (col < N) {
                                 const uint64_t at = to * (2u * (uint64_t)N) + (uint32_t)h * (uint64_t)N + col;
-                                Vec16<T> o;
-#pragma unroll
-                                for (int x = 0; x < 8; ++x) o.v[x] = Num<T>::down(v[x]);
-                                *reinterpret_cast<Vec16<T>*>((T*)args.D + at) = o;
+                                *reinterpret_cast<u32x4*>((uint16_t*)args.D + at) = u32x4{pack_pair<T>(v[0], v[1]), pack_pair<T>(v[2], v[3]), pack_pair<T>(v[4], v[5]), pack_pair<T>(v[6], v[7])};
                                 uint2 o8;
                                 o8.x = pack4(v[0] * inverse, v[1] * inverse, v[2] * inverse, v[3] * inverse);
                                 o8.y = pack4(v[4] * inverse, v[5] * inverse, v[6] * inverse, v[7] * inverse);
