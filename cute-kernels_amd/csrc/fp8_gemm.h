@@ -457,6 +457,11 @@ __global__ __launch_bounds__(kGemmThreads) void fp8_gemm_kernel(const GemmArgs a
         auto block_row = [&](int i) -> uint32_t { return i < kRowBlocks ? wm * 128u + (uint32_t)i * 16u : 256u + wm * 16u; };
 
         // ---- epilogue ----
+        // (addresses that follow from the lane are computed here, anew for every tile: kept over the K loop they would be spilled)
+        uint32_t here = lane;
+        asm volatile("" : "+v"(here));
+        {
+        const uint32_t lane = here, r16 = lane & 15u, q = lane >> 4;
         if constexpr (EPI == EPI_BF16 || EPI == EPI_F16) {
             using T = std::conditional_t<EPI == EPI_BF16, bf16_t, f16_t>;
             uint16_t* const tile = (uint16_t*)args.D + (uint64_t)t.row0 * N + t.n0;
@@ -556,6 +561,8 @@ __global__ __launch_bounds__(kGemmThreads) void fp8_gemm_kernel(const GemmArgs a
             for (int i = 0; i < kBlocks; ++i) asm("" : "+v"(acc[i]));
 #pragma unroll
             for (int w = 0; w < kWhat; ++w) {
+                asm volatile("" : "+v"(here));  // (as above, for every one of the three)
+                const uint32_t lane = here, r16 = lane & 15u, q = lane >> 4, col = t.n0 + wn * 32u + q * 8u;
                 // values of this tile's rows from its first column on (the rows' ends are the descriptor's), and their scales
                 const uint32_t pitch = w == 0 ? N : 2u * N, s_pitch = w == 0 ? args.o_pitch_s : 2u * args.o_pitch_s;
                 const uint64_t values = w == 0 ? (uint64_t)(uintptr_t)args.out + (uint64_t)t.row0 * pitch
@@ -572,7 +579,10 @@ __global__ __launch_bounds__(kGemmThreads) void fp8_gemm_kernel(const GemmArgs a
                     const float inverse = scale_inverse(byte);
                     float v[8];
 #pragma unroll
-                    for (int x = 0; x < 8; ++x) v[x] = (w == 0 ? activation(i, x) : acc[i][(w == 2 ? 8 : 0) + x]) * inverse;
+                    for (int x = 0; x < 8; ++x) {
+                        const float kept = w == 1 ? acc[i][x] : acc[i][8 + x];
+                        v[x] = (w == 0 ? activation(i, x) : kept) * inverse;
+                    }
                     typedef __attribute__((ext_vector_type(2))) uint32_t u32x2;
                     const u32x2 o = {pack4(v[0], v[1], v[2], v[3]), pack4(v[4], v[5], v[6], v[7])};
                     const bool live = row < t.rows;
@@ -650,6 +660,7 @@ __global__ __launch_bounds__(kGemmThreads) void fp8_gemm_kernel(const GemmArgs a
                 }
                 __builtin_amdgcn_sched_barrier(0);
             }
+        }
         }
         // The next tile's first fragments once more: 42 registers that these epilogues use meanwhile.
         if constexpr (kGlu || kBwd) first_fragments();
