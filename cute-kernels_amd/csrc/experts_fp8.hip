@@ -24,13 +24,14 @@ __device__ __forceinline__ bool names_expert(const void* ids, int id_bytes, int6
 }
 
 // ---- y[t] = sum_j gates[t, j] * o[inv[t, j]], fp32 sums in ascending j; gates NULL: ones ------------------------------
-// o in type O; inv NULL: the row of a slot is the slot. One workgroup per token; KC choices (top_k, or 4 at a time) of a vector are loaded before the first is added.
-template <typename T, typename O, int KC>
+// o in type O; not INDEXED: the row of a slot is the slot. One workgroup per token and kThreads * 8 columns (64 * 8 of few tokens); KC choices (top_k, or 4 at a time) of a vector are loaded before the first is added.
+template <typename T, typename O, bool INDEXED, int KC>
 __global__ __launch_bounds__(kThreads) void sum_choices_kernel(const O* __restrict__ o, const void* __restrict__ ids, int id_bytes,
                                                                const int32_t* __restrict__ inv, const T* __restrict__ gates, uint32_t top_k,
                                                                uint32_t E, uint32_t H, int64_t slots, T* __restrict__ y) {
     const int64_t t = blockIdx.x;
-    for (uint32_t h = threadIdx.x * 8u; h < H; h += kThreads * 8u) {
+    const uint32_t h = (blockIdx.y * blockDim.x + threadIdx.x) * 8u;
+    if (h < H) {
         float sum[8];
 #pragma unroll
         for (int i = 0; i < 8; ++i) sum[i] = 0.f;
@@ -38,25 +39,24 @@ __global__ __launch_bounds__(kThreads) void sum_choices_kernel(const O* __restri
             constexpr int V = Vec16<O>::N;
             Vec16<O> v[KC][8 / V];
             float g[KC];
+            bool in[KC];
 #pragma unroll
             for (int j = 0; j < KC; ++j) {
-                const int64_t slot = t * top_k + j0 + j;
-                g[j] = 0.f;
+                // (loads first, looks after: a row that does not count is row 0, and what it holds is dropped)
+                const int64_t slot = t * top_k + (j0 + j < top_k ? j0 + j : 0);
+                const bool named = j0 + j < top_k && names_expert(ids, id_bytes, slot, E);
+                int64_t row = slot;
+                if constexpr (INDEXED) row = inv[slot];
+                in[j] = named && (uint64_t)row < (uint64_t)slots;
+                if (INDEXED && !in[j]) row = 0;
 #pragma unroll
-                for (int i = 0; i < 8; ++i) v[j][i / V].v[i % V] = Num<O>::down(0.f);
-                if (j0 + j < top_k && names_expert(ids, id_bytes, slot, E)) {
-                    const int64_t row = inv ? inv[slot] : slot;
-                    if ((uint64_t)row < (uint64_t)slots) {
-#pragma unroll
-                        for (int c = 0; c < 8 / V; ++c) v[j][c] = load_streaming16(reinterpret_cast<const Vec16<O>*>(o + row * H + h) + c);
-                        g[j] = gates ? Num<T>::up(gates[slot]) : 1.0f;
-                    }
-                }
+                for (int c = 0; c < 8 / V; ++c) v[j][c] = load_streaming16(reinterpret_cast<const Vec16<O>*>(o + row * H + h) + c);
+                g[j] = gates ? Num<T>::up(gates[slot]) : 1.0f;
             }
 #pragma unroll
             for (int j = 0; j < KC; ++j)
 #pragma unroll
-                for (int i = 0; i < 8; ++i) sum[i] = fmaf(g[j], Num<O>::up(v[j][i / V].v[i % V]), sum[i]);
+                for (int i = 0; i < 8; ++i) sum[i] = in[j] ? fmaf(g[j], Num<O>::up(v[j][i / V].v[i % V]), sum[i]) : sum[i];
         }
         Vec16<T> w;
 #pragma unroll
@@ -65,17 +65,20 @@ __global__ __launch_bounds__(kThreads) void sum_choices_kernel(const O* __restri
     }
 }
 
+// O = T: rows in the routing order, inv; O = float: rows by slot
 template <typename T, typename O = T>
 int sum_choices(const void* o, const void* ids, int id_bytes, const int32_t* inv, const void* gates, int64_t T_, int64_t top_k, int64_t E,
                 int64_t H, void* y, hipStream_t st) {
+    const uint32_t threads = T_ < 64 ? 64 : kThreads;
     auto run = [&](auto kernel) {
-        hipLaunchKernelGGL(kernel, dim3((uint32_t)T_), dim3(kThreads), 0, st, (const O*)o, ids, id_bytes, inv, (const T*)gates, (uint32_t)top_k,
-                           (uint32_t)E, (uint32_t)H, T_ * top_k, (T*)y);
+        hipLaunchKernelGGL(kernel, dim3((uint32_t)T_, (uint32_t)((H + threads * 8 - 1) / (threads * 8))), dim3(threads), 0, st, (const O*)o, ids, id_bytes,
+                           inv, (const T*)gates, (uint32_t)top_k, (uint32_t)E, (uint32_t)H, T_ * top_k, (T*)y);
     };
-    if (top_k == 1) run(sum_choices_kernel<T, O, 1>);
-    else if (top_k == 2) run(sum_choices_kernel<T, O, 2>);
-    else if (top_k <= 4 || top_k % 8 != 0) run(sum_choices_kernel<T, O, 4>);
-    else run(sum_choices_kernel<T, O, 8>);
+    constexpr bool kIndexed = std::is_same_v<T, O>;
+    if (top_k == 1) run(sum_choices_kernel<T, O, kIndexed, 1>);
+    else if (top_k == 2) run(sum_choices_kernel<T, O, kIndexed, 2>);
+    else if (top_k <= 4 || top_k % 8 != 0) run(sum_choices_kernel<T, O, kIndexed, 4>);
+    else run(sum_choices_kernel<T, O, kIndexed, 8>);
     return launch_status("swiglu_experts_fp8");
 }
 

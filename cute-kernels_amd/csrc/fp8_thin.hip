@@ -231,7 +231,8 @@ __global__ __launch_bounds__(64 * KS) void fp8_thin_kernel(const ThinArgs a) {
     __shared__ __attribute__((aligned(16))) float s_parts[KS > 1 ? (KS - 1) * TB * 2 * 64 * 4 : 4];
     __shared__ uint32_t s_count;
     const uint32_t lane = threadIdx.x & 63u;
-    const uint32_t e = blockIdx.x / a.col_blocks, n0 = (blockIdx.x - e * a.col_blocks) * (OUT == OUT_GLU ? 16u : 32u);
+    uint32_t e = blockIdx.x / a.col_blocks;
+    const uint32_t n0 = (blockIdx.x - e * a.col_blocks) * (OUT == OUT_GLU ? 16u : 32u);
     uint32_t rows, first = 0;
     if constexpr (SRC == ROWS_FP8) {
         if (a.sizes) {  // rows past R do not exist, whatever the sizes say
@@ -246,7 +247,32 @@ __global__ __launch_bounds__(64 * KS) void fp8_thin_kernel(const ThinArgs a) {
             rows = a.R;
         }
     } else {
-        // the slots of expert e, in their order
+        // `e` counts the experts that have a slot: which one it is, from a bit for each of them
+        constexpr uint32_t kWords = FMA_MAX_GROUPS / 32;
+        __shared__ uint32_t s_named[kWords];
+        if (threadIdx.x < 64) {
+            if (lane < kWords) s_named[lane] = 0u;
+            for (uint32_t s = lane; s < a.R; s += 64) {
+                const int64_t id = a.id_bytes == 8 ? ((const int64_t*)a.ids)[s] : (int64_t)((const int32_t*)a.ids)[s];
+                if ((uint64_t)id < a.E) atomicOr(&s_named[(uint32_t)id >> 5], 1u << ((uint32_t)id & 31u));
+            }
+            const uint32_t word = lane < kWords ? s_named[lane] : 0u;
+            const uint32_t n = (uint32_t)__popc(word), before = wave_inclusive_scan<uint32_t>(n) - n;
+            const uint64_t mine = __ballot(before <= e && e < before + n);
+            uint32_t found = a.E;
+            if (mine) {
+                const int src = (int)__builtin_ctzll(mine);
+                uint32_t bits = (uint32_t)__shfl((int)word, src, 64);
+                for (uint32_t skip = e - (uint32_t)__shfl((int)before, src, 64); skip; --skip) bits &= bits - 1u;
+                found = (uint32_t)src * 32u + (uint32_t)__builtin_ctz(bits);
+            }
+            if (lane == 0) s_count = found;
+        }
+        __syncthreads();
+        e = s_count;
+        if (e >= a.E) return;
+        __syncthreads();
+        // its slots, in their order
         if (threadIdx.x < 64) {
             uint32_t n = 0;
             for (uint32_t base = 0; base < a.R; base += 64) {
@@ -289,7 +315,7 @@ int launch(const char* who, ThinArgs a, hipStream_t st) {
     const int64_t units = groups * a.col_blocks, k_blocks = (a.K + kBlock - 1) / kBlock;
     int parts = 1;
     while (parts < 8 && units * parts < 32 * cus && k_blocks >= 4 * parts) parts *= 2;
-    const dim3 grid(a.E * a.col_blocks);
+    const dim3 grid((uint32_t)(SRC == ROWS_FP8 ? a.E : groups) * a.col_blocks);
     auto run = [&](auto kernel, int ks) { hipLaunchKernelGGL(kernel, grid, dim3(64 * ks), 0, st, a); };
     if (wide) {
         if (parts == 1) run(fp8_thin_kernel<SRC, OUT, 2, 1>, 1);
