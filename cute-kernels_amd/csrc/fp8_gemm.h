@@ -39,6 +39,7 @@ using ::fmahip::gemm::wait_vm;
 typedef __attribute__((ext_vector_type(4))) float f32x4;
 typedef __attribute__((ext_vector_type(16))) float f32x16;
 typedef __attribute__((ext_vector_type(4))) int i32x4;
+typedef __attribute__((ext_vector_type(2))) uint32_t u32x2;
 typedef __attribute__((ext_vector_type(8))) int i32x8;
 
 constexpr int kTileM = 256, kTileN = 256;
@@ -583,7 +584,6 @@ __global__ __launch_bounds__(kGemmThreads) void fp8_gemm_kernel(const GemmArgs a
                         const float kept = w == 1 ? acc[i][x] : acc[i][8 + x];
                         v[x] = (w == 0 ? activation(i, x) : kept) * inverse;
                     }
-                    typedef __attribute__((ext_vector_type(2))) uint32_t u32x2;
                     const u32x2 o = {pack4(v[0], v[1], v[2], v[3]), pack4(v[4], v[5], v[6], v[7])};
                     const bool live = row < t.rows;
                     __builtin_amdgcn_raw_buffer_store_b64(o, rv, (int)(live && col < N ? row * pitch + col : kOutOfRange), 0, 0);
@@ -597,30 +597,54 @@ __global__ __launch_bounds__(kGemmThreads) void fp8_gemm_kernel(const GemmArgs a
             const uint32_t block = t.n0 / kBlock + (wn >> 1);
             const uint32_t s_pitch = args.o_pitch_s;
             wait_vm<0>();
+            // The pre-activation of a row block: eight columns of each half twice, and the scales, requested two blocks ahead. Loads and stores
+            // are unconditional (a lane without work has an offset out of range): the compiler then counts them, and no block waits
+            // for the stores of the one before.
+            struct Kept {
+                u32x2 v[2][2];  // [half][columns p]
+                uint32_t s[2];
+            };
+            constexpr int kAhead = 2;
+            Kept kept[kAhead];
+            const bool in = t.n0 + (wn >> 1) * kBlock < N;
+            const uint64_t first_value = (uint64_t)t.row0 * (2u * (uint64_t)N), first_scale = (uint64_t)t.row0 * (2u * s_pitch);
+            const __amdgpu_buffer_rsrc_t r_h = buffer_at((uint64_t)(uintptr_t)args.h + first_value), r_hs = buffer_at((uint64_t)(uintptr_t)args.h_s + first_scale);
+            const __amdgpu_buffer_rsrc_t r_d = buffer_at((uint64_t)(uintptr_t)args.D + 2u * first_value);
+            const __amdgpu_buffer_rsrc_t r_o = buffer_at((uint64_t)(uintptr_t)args.out + first_value), r_os = buffer_at((uint64_t)(uintptr_t)args.out_s + first_scale);
+            auto value_at = [&](uint32_t row, int h, int p) -> uint32_t {
+                const uint32_t col = t.n0 + wn * 64u + (uint32_t)p * 32u + q * 8u;
+                return row < t.rows && col < N ? row * 2u * N + (uint32_t)h * N + col : kOutOfRange;
+            };
+            auto scale_at = [&](uint32_t row, int h) -> uint32_t { return row < t.rows && in ? row * 2u * s_pitch + (uint32_t)h * s_pitch + block : kOutOfRange; };
+            auto fetch = [&](int i) -> Kept {
+                const uint32_t row = block_row(i) + r16;
+                Kept k;
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    k.s[h] = __builtin_amdgcn_raw_buffer_load_b8(r_hs, (int)scale_at(row, h), 0, 0);
+#pragma unroll
+                    for (int p = 0; p < 2; ++p) k.v[h][p] = __builtin_amdgcn_raw_buffer_load_b64(r_h, (int)value_at(row, h, p), 0, 0);
+                }
+                return k;
+            };
+#pragma unroll
+            for (int i = 0; i < kAhead; ++i) kept[i] = fetch(i);
 #pragma unroll
             for (int i = 0; i < kBlocks; ++i) {
                 if (i >= kRowBlocks && !tall) continue;
                 const uint32_t row = block_row(i) + r16;
-                const bool live = row < t.rows;
-                const uint64_t to = t.row0 + (live ? row : 0u);
+                const Kept k = kept[i % kAhead];
+                if (i + kAhead < kBlocks) kept[i % kAhead] = fetch(i + kAhead);
                 float d[2][2][8];  // [half][columns p][x]
                 uint32_t m[2] = {0u, 0u};
-                const bool in = t.n0 + (wn >> 1) * kBlock < N;
-                const float su = in ? scale_value(args.h_s[to * (2u * (uint64_t)s_pitch) + block]) : 0.f;
-                const float sg = in ? scale_value(args.h_s[to * (2u * (uint64_t)s_pitch) + s_pitch + block]) : 0.f;
+                const float su = scale_value(k.s[0]), sg = scale_value(k.s[1]);
 #pragma unroll
                 for (int p = 0; p < 2; ++p) {
-                    const uint32_t col = t.n0 + wn * 64u + (uint32_t)p * 32u + q * 8u;
-                    uint2 hu = {0u, 0u}, hg = {0u, 0u};
-                    if (col < N) {
-                        hu = *reinterpret_cast<const uint2*>(args.h + to * (2u * (uint64_t)N) + col);
-                        hg = *reinterpret_cast<const uint2*>(args.h + to * (2u * (uint64_t)N) + N + col);
-                    }
                     float u[8], g[8];
-                    unpack4(hu.x, *reinterpret_cast<float(*)[4]>(u));
-                    unpack4(hu.y, *reinterpret_cast<float(*)[4]>(u + 4));
-                    unpack4(hg.x, *reinterpret_cast<float(*)[4]>(g));
-                    unpack4(hg.y, *reinterpret_cast<float(*)[4]>(g + 4));
+                    unpack4(k.v[0][p][0], *reinterpret_cast<float(*)[4]>(u));
+                    unpack4(k.v[0][p][1], *reinterpret_cast<float(*)[4]>(u + 4));
+                    unpack4(k.v[1][p][0], *reinterpret_cast<float(*)[4]>(g));
+                    unpack4(k.v[1][p][1], *reinterpret_cast<float(*)[4]>(g + 4));
 #pragma unroll
                     for (int x = 0; x < 8; ++x) {
                         swiglu_b<T>(g[x] * sg, u[x] * su, acc[i][8 * p + x], d[1][p][x], d[0][p][x]);
@@ -637,25 +661,20 @@ __global__ __launch_bounds__(kGemmThreads) void fp8_gemm_kernel(const GemmArgs a
                     if (q == 0) slots[(wave * 2u + (uint32_t)h) * 16u + r16] = m[h];
                 }
                 lds_barrier();
-                if (live) {
 #pragma unroll
-                    for (int h = 0; h < 2; ++h) {
-                        const uint32_t byte = scale_byte(max_u32(m[h], slots[((wave ^ 1u) * 2u + (uint32_t)h) * 16u + r16]));
-                        const float inverse = scale_inverse(byte);
-                        if (q == 0 && (wn & 1u) == 0 && in) args.out_s[to * (2u * (uint64_t)s_pitch) + (uint32_t)h * s_pitch + block] = (uint8_t)byte;
+                for (int h = 0; h < 2; ++h) {
+                    const uint32_t byte = scale_byte(max_u32(m[h], slots[((wave ^ 1u) * 2u + (uint32_t)h) * 16u + r16]));
+                    const float inverse = scale_inverse(byte);
+                    __builtin_amdgcn_raw_buffer_store_b8((uint8_t)byte, r_os, (int)(q == 0 && (wn & 1u) == 0 ? scale_at(row, h) : kOutOfRange), 0, 0);
 #pragma unroll
-                        for (int p = 0; p < 2; ++p) {
-                            const uint32_t col = t.n0 + wn * 64u + (uint32_t)p * 32u + q * 8u;
-                            const float(&v)[8] = d[h][p];
-                            if (col < N) {
-                                const uint64_t at = to * (2u * (uint64_t)N) + (uint32_t)h * (uint64_t)N + col;
-                                *reinterpret_cast<u32x4*>((uint16_t*)args.D + at) = u32x4{pack_pair<T>(v[0], v[1]), pack_pair<T>(v[2], v[3]), pack_pair<T>(v[4], v[5]), pack_pair<T>(v[6], v[7])};
-                                uint2 o8;
-                                o8.x = pack4(v[0] * inverse, v[1] * inverse, v[2] * inverse, v[3] * inverse);
-                                o8.y = pack4(v[4] * inverse, v[5] * inverse, v[6] * inverse, v[7] * inverse);
-                                *reinterpret_cast<uint2*>(args.out + at) = o8;
-                            }
-                        }
+                    for (int p = 0; p < 2; ++p) {
+                        const float(&v)[8] = d[h][p];
+                        const uint32_t at = value_at(row, h, p);
+                        const u32x4 o = {pack_pair<T>(v[0], v[1]), pack_pair<T>(v[2], v[3]), pack_pair<T>(v[4], v[5]), pack_pair<T>(v[6], v[7])};
+                        ::fmahip::gemm::store_tile16<false>(r_d, at == kOutOfRange ? kOutOfRange : 2u * at, __builtin_bit_cast(uint4, o));
+                        const u32x2 o8 = {pack4(v[0] * inverse, v[1] * inverse, v[2] * inverse, v[3] * inverse),
+                                          pack4(v[4] * inverse, v[5] * inverse, v[6] * inverse, v[7] * inverse)};
+                        __builtin_amdgcn_raw_buffer_store_b64(o8, r_o, (int)at, 0, 0);
                     }
                 }
                 __builtin_amdgcn_sched_barrier(0);

@@ -5,6 +5,7 @@
 // front. Weights: a workgroup takes one 128 x 128 block, eight by eight elements a thread; the transposed copy, which the input gradient's
 // product reads along its own reduction, is made from the same registers through 17 KB of LDS, so that the 16-bit weights are read once.
 #include "fp8_parts.h"
+#include "gemm_parts.h"
 
 namespace fmahip {
 namespace {
@@ -42,7 +43,7 @@ __global__ __launch_bounds__(kThreads) void quantize_rows_kernel(const T* __rest
                                                                  uint32_t* __restrict__ scales, int64_t total, uint32_t quads,
                                                                  int64_t K) {
     const uint32_t lane = threadIdx.x & 31u;
-    const int64_t first = ((int64_t)blockIdx.x * kThreads + threadIdx.x) / 32 + (int64_t)0;
+    const int64_t first = ((int64_t)blockIdx.x * kThreads + threadIdx.x) / 32;
     const int64_t step = (int64_t)gridDim.x * (kThreads / 32);
     float f[UNROLL][16];
     int64_t at[UNROLL], unit[UNROLL];
@@ -50,7 +51,7 @@ __global__ __launch_bounds__(kThreads) void quantize_rows_kernel(const T* __rest
 #pragma unroll
     for (int u = 0; u < UNROLL; ++u) {
         unit[u] = first + u * step;
-        const int64_t row = unit[u] / quads;
+        const int64_t row = total < (1ll << 31) ? (int64_t)((uint32_t)unit[u] / quads) : unit[u] / quads;
         const int64_t k = (unit[u] - row * quads) * 512 + lane * 16;
         in[u] = unit[u] < total && k < K;
         at[u] = row * K + k;
@@ -223,27 +224,61 @@ __global__ __launch_bounds__(kThreads) void quantize_blocks_generic_kernel(const
 
 // ---- back -----------------------------------------------------------------------------------------------------------
 
-// 16 elements a lane; row_shift: 0, or 7 where 128 rows share their scales (the rows of a matrix of N rows: `rows` = N)
-template <typename T>
+// 16 elements a lane, four times per workgroup with all loads in front. row_shift: 0, or 7 where 128 rows of a matrix of N rows share their
+// scales. Index arithmetic in 32 bits (I32) where the sizes allow it: a 64-bit division costs more than the rest of the kernel.
+// [65536, 1408] bf16: 95 -> 53 us (5.2 TB/s).
+constexpr int kDequantizeUnroll = 4;
+template <typename T, bool I32>
 __global__ __launch_bounds__(kThreads) void dequantize_kernel(const uint8_t* __restrict__ values, const uint8_t* __restrict__ scales,
                                                               T* __restrict__ out, int64_t total, uint32_t per_row, int64_t K,
                                                               int64_t pitch, int64_t N, int64_t scale_rows, int row_shift) {
-    const int64_t step = (int64_t)gridDim.x * kThreads;
-    for (int64_t u = (int64_t)blockIdx.x * kThreads + threadIdx.x; u < total; u += step) {
-        const int64_t row = u / per_row, k = (u - row * per_row) * 16;
-        const int64_t e = row / N, s_row = e * scale_rows + ((row - e * N) >> row_shift);
-        const float scale = scale_value(scales[s_row * pitch + k / kBlock]);
-        const uint4 q = load_streaming16(reinterpret_cast<const uint4*>(values + row * K + k));
-        const uint32_t w[4] = {q.x, q.y, q.z, q.w};
+    typedef std::conditional_t<I32, uint32_t, int64_t> index;
+    const int64_t first = (int64_t)blockIdx.x * (kDequantizeUnroll * kThreads) + threadIdx.x;
+    uint4 q[kDequantizeUnroll];
+    float scale[kDequantizeUnroll];
+    int64_t at[kDequantizeUnroll];
+#pragma unroll
+    for (int i = 0; i < kDequantizeUnroll; ++i) {
+        const int64_t u = first + i * kThreads;
+        at[i] = -1;
+        if (u < total) {
+            const index row = (index)u / (index)per_row, k = ((index)u - row * (index)per_row) * 16;
+            index s_row = row;
+            if (row_shift) {
+                const index e = row / (index)N;
+                s_row = e * (index)scale_rows + ((row - e * (index)N) >> row_shift);
+            }
+            at[i] = (int64_t)row * K + k;
+            q[i] = load_streaming16(reinterpret_cast<const uint4*>(values + at[i]));
+            scale[i] = scale_value(scales[(int64_t)s_row * pitch + k / kBlock]);
+        }
+    }
+#pragma unroll
+    for (int i = 0; i < kDequantizeUnroll; ++i) {
+        if (at[i] < 0) continue;
+        const uint32_t w[4] = {q[i].x, q[i].y, q[i].z, q[i].w};
         float f[16];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
+        for (int j = 0; j < 4; ++j) {
             float g[4];
-            unpack4(w[i], g);
+            unpack4(w[j], g);
 #pragma unroll
-            for (int j = 0; j < 4; ++j) f[4 * i + j] = g[j] * scale;
+            for (int x = 0; x < 4; ++x) f[4 * j + x] = g[x] * scale[i];
         }
-        store_floats(out + row * K + k, f);
+        if constexpr (sizeof(T) == 4) {
+            store_floats(out + at[i], f);
+        } else {
+            using EL = std::conditional_t<std::is_same_v<T, bf16_t>, ::fmahip::gemm::ElemBf16, ::fmahip::gemm::ElemF16>;
+#pragma unroll
+            for (int j = 0; j < 2; ++j) {
+                uint4 v;
+                v.x = EL::pack2(f[8 * j], f[8 * j + 1]);
+                v.y = EL::pack2(f[8 * j + 2], f[8 * j + 3]);
+                v.z = EL::pack2(f[8 * j + 4], f[8 * j + 5]);
+                v.w = EL::pack2(f[8 * j + 6], f[8 * j + 7]);
+                store_streaming16(reinterpret_cast<uint4*>(out + at[i]) + j, v);
+            }
+        }
     }
 }
 
@@ -303,10 +338,13 @@ int dequantize(const uint8_t* values, const uint8_t* scales, void* out, int64_t 
     const int64_t pitch = scale_pitch(K), scale_rows = (N + block_rows - 1) / block_rows;
     const int shift = block_rows == 1 ? 0 : 7;
     if (K % 16 == 0 && aligned16(values) && aligned16(out)) {
-        const int64_t total = E * N * (K / 16), blocks = (total + kThreads - 1) / kThreads;
-        const dim3 grid((uint32_t)(blocks < (1 << 20) ? blocks : (1 << 20)));
-        hipLaunchKernelGGL(dequantize_kernel<T>, grid, dim3(kThreads), 0, st, values, scales, (T*)out, total, (uint32_t)(K / 16), K, pitch, N,
-                           scale_rows, shift);
+        const int64_t total = E * N * (K / 16), per = kDequantizeUnroll * kThreads;
+        const dim3 grid((uint32_t)((total + per - 1) / per));
+        auto run = [&](auto kernel) {
+            hipLaunchKernelGGL(kernel, grid, dim3(kThreads), 0, st, values, scales, (T*)out, total, (uint32_t)(K / 16), K, pitch, N, scale_rows, shift);
+        };
+        if (total + per < (1ll << 31)) run(dequantize_kernel<T, true>);
+        else run(dequantize_kernel<T, false>);
     } else {
         const int64_t total = E * N * K, blocks = (total + kThreads - 1) / kThreads;
         const dim3 grid((uint32_t)(blocks < (1 << 20) ? blocks : (1 << 20)));

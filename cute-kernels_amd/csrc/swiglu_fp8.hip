@@ -69,7 +69,7 @@ __global__ __launch_bounds__(kThreads) void swiglu_fp8_fwd_kernel(const T* __res
 #pragma unroll
     for (int u = 0; u < UNROLL; ++u) {
         const int64_t unit = first + u * step;
-        row[u] = unit / quads;
+        row[u] = total < (1ll << 31) ? (int64_t)((uint32_t)unit / quads) : unit / quads;
         col[u] = (unit - row[u] * quads) * 512 + lane * 8;
         in[u] = unit < total && col[u] < I;
         if (in[u]) {
@@ -119,7 +119,7 @@ __global__ __launch_bounds__(kThreads) void swiglu_fp8_bwd_kernel(const uint8_t*
     for (int u = 0; u < UNROLL; ++u) {
         const int64_t v = first + u * kThreads;
         if (v < total) {
-            row[u] = v / vectors;
+            row[u] = total < (1ll << 31) ? (int64_t)((uint32_t)v / vectors) : v / vectors;
             col[u] = (v - row[u] * vectors) * 8;
             qu[u] = *reinterpret_cast<const uint2*>(values + row[u] * 2 * I + col[u]);
             qg[u] = *reinterpret_cast<const uint2*>(values + row[u] * 2 * I + I + col[u]);
