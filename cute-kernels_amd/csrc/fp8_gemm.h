@@ -99,7 +99,7 @@ __global__ __launch_bounds__(kGemmThreads) void fp8_gemm_kernel(const GemmArgs a
     constexpr bool kBwd = EPI == EPI_GLU_BWD_BF16 || EPI == EPI_GLU_BWD_F16;
     constexpr uint32_t kCols = kGlu ? kTileN / 2 : kTileN;  // columns of the output grid per tile
     // Stores of an epilogue per wavefront, at least (0, 59: an epilogue that has waited for all loads in front of them itself)
-    constexpr int kStores = EPI == EPI_BF16 || EPI == EPI_F16 ? 2 * kRowBlocks : (EPI == EPI_GLU ? 2 * kRowBlocks : (EPI == EPI_GLU_KEEP ? 6 * kRowBlocks : (kBwd ? 59 : 0)));
+    constexpr int kStores = EPI == EPI_BF16 || EPI == EPI_F16 ? 2 * kRowBlocks : (EPI == EPI_GLU ? kRowBlocks : (EPI == EPI_GLU_KEEP ? 3 * kRowBlocks : (kBwd ? 59 : 0)));
     constexpr uint32_t kMostGroups = TALL ? kTallGroups : kMaxGroups;
     constexpr int kBlocks = TALL ? kRowBlocks + 1 : kRowBlocks;  // row blocks of a wavefront, at most
     constexpr uint32_t kMostRows = TALL ? kTallM : kTileM;
@@ -526,71 +526,69 @@ __global__ __launch_bounds__(kGemmThreads) void fp8_gemm_kernel(const GemmArgs a
             }
             wait_vm<0>();
         } else if constexpr (kGlu) {
-            const uint32_t col = t.n0 + wn * 32u + q * 8u, block = t.n0 / kBlock;
+            const uint32_t block = t.n0 / kBlock;
             // magnitudes of the row's columns of this wavefront
             auto row_max = [&](uint32_t m) -> uint32_t {
                 m = max_u32(m, (uint32_t)__shfl_xor((int)m, 16, 64));
                 return max_u32(m, (uint32_t)__shfl_xor((int)m, 32, 64));
             };
-            constexpr int kWhat = EPI == EPI_GLU_KEEP ? 3 : 1;
-            auto activation = [&](int i, int x) -> float {
-                const float u = acc[i][x], g = acc[i][8 + x];
-                return u * g * sigmoid_clamped_fast(g);
-            };
+            // `what` 0: the activation, which has taken the place of the sums of "up" by then; 1, 2: the pre-activation's halves
+            auto maxima = [&](int what) {
 #pragma unroll
-            for (int i = 0; i < kBlocks; ++i) {
-                if (i >= kRowBlocks && !tall) continue;
-                uint32_t m[3] = {0u, 0u, 0u};
+                for (int i = 0; i < kBlocks; ++i) {
+                    if (i >= kRowBlocks && !tall) continue;
+                    uint32_t m = 0;
 #pragma unroll
-                for (int x = 0; x < 8; ++x) {
-                    m[0] = max_u32(m[0], magnitude_bits(activation(i, x)));
-                    if constexpr (kWhat == 3) {
-                        m[1] = max_u32(m[1], magnitude_bits(acc[i][x]));
-                        m[2] = max_u32(m[2], magnitude_bits(acc[i][8 + x]));
+                    for (int x = 0; x < 8; ++x) {
+                        if (what == 0) {
+                            const float g = acc[i][8 + x];
+                            acc[i][x] = acc[i][x] * g * sigmoid_clamped_fast(g);
+                        }
+                        m = max_u32(m, magnitude_bits(acc[i][(what == 2 ? 8 : 0) + x]));
                     }
+                    m = row_max(m);
+                    if (q == 0) s_max[((uint32_t)what * kMostRows + block_row(i) + r16) * 4u + wn] = m;
+                    __builtin_amdgcn_sched_barrier(0);
                 }
-#pragma unroll
-                for (int w = 0; w < kWhat; ++w) {
-                    const uint32_t v = row_max(m[w]);
-                    if (q == 0) s_max[((uint32_t)w * kMostRows + block_row(i) + r16) * 4u + wn] = v;
-                }
-                __builtin_amdgcn_sched_barrier(0);
-            }
-            lds_barrier();
-            // (activations are computed anew rather than kept: 64 more registers)
-#pragma unroll
-            for (int i = 0; i < kBlocks; ++i) asm("" : "+v"(acc[i]));
-#pragma unroll
-            for (int w = 0; w < kWhat; ++w) {
-                asm volatile("" : "+v"(here));  // (as above, for every one of the three)
+            };
+            auto store = [&](int what) {
+                asm volatile("" : "+v"(here));  // (as above, for every one of them)
                 const uint32_t lane = here, r16 = lane & 15u, q = lane >> 4, col = t.n0 + wn * 32u + q * 8u;
-                // values of this tile's rows from its first column on (the rows' ends are the descriptor's), and their scales
-                const uint32_t pitch = w == 0 ? N : 2u * N, s_pitch = w == 0 ? args.o_pitch_s : 2u * args.o_pitch_s;
-                const uint64_t values = w == 0 ? (uint64_t)(uintptr_t)args.out + (uint64_t)t.row0 * pitch
-                                               : (uint64_t)(uintptr_t)args.h + (uint64_t)t.row0 * pitch + (w == 2 ? N : 0u);
-                const uint64_t scales = w == 0 ? (uint64_t)(uintptr_t)args.out_s + (uint64_t)t.row0 * s_pitch
-                                               : (uint64_t)(uintptr_t)args.h_s + (uint64_t)t.row0 * s_pitch + (w == 2 ? args.o_pitch_s : 0u);
+                // values of this tile's rows (the rows' ends are looked at here), and their scales
+                const uint32_t pitch = what == 0 ? N : 2u * N, s_pitch = what == 0 ? args.o_pitch_s : 2u * args.o_pitch_s;
+                const uint64_t values = what == 0 ? (uint64_t)(uintptr_t)args.out + (uint64_t)t.row0 * pitch
+                                                  : (uint64_t)(uintptr_t)args.h + (uint64_t)t.row0 * pitch + (what == 2 ? N : 0u);
+                const uint64_t scales = what == 0 ? (uint64_t)(uintptr_t)args.out_s + (uint64_t)t.row0 * s_pitch
+                                                  : (uint64_t)(uintptr_t)args.h_s + (uint64_t)t.row0 * s_pitch + (what == 2 ? args.o_pitch_s : 0u);
                 const __amdgpu_buffer_rsrc_t rv = buffer_at(values), rs = buffer_at(scales);
 #pragma unroll
                 for (int i = 0; i < kBlocks; ++i) {
-                if (i >= kRowBlocks && !tall) continue;
+                    if (i >= kRowBlocks && !tall) continue;
                     const uint32_t row = block_row(i) + r16;
-                    const uint4 m = *reinterpret_cast<const uint4*>(s_max + ((uint32_t)w * kMostRows + row) * 4u);
+                    const uint4 m = *reinterpret_cast<const uint4*>(s_max + ((uint32_t)what * kMostRows + row) * 4u);
                     const uint32_t byte = scale_byte(max_u32(max_u32(m.x, m.y), max_u32(m.z, m.w)));
                     const float inverse = scale_inverse(byte);
                     float v[8];
 #pragma unroll
-                    for (int x = 0; x < 8; ++x) {
-                        const float kept = w == 1 ? acc[i][x] : acc[i][8 + x];
-                        v[x] = (w == 0 ? activation(i, x) : kept) * inverse;
-                    }
+                    for (int x = 0; x < 8; ++x) v[x] = acc[i][(what == 2 ? 8 : 0) + x] * inverse;
                     const u32x2 o = {pack4(v[0], v[1], v[2], v[3]), pack4(v[4], v[5], v[6], v[7])};
                     const bool live = row < t.rows;
                     __builtin_amdgcn_raw_buffer_store_b64(o, rv, (int)(live && col < N ? row * pitch + col : kOutOfRange), 0, 0);
-                    __builtin_amdgcn_raw_buffer_store_b8((uint8_t)byte, rs, (int)(live && q == 0 && wn == 0 ? row * s_pitch + block : kOutOfRange), 0, 0);
+                    if (wn == 0)
+                        __builtin_amdgcn_raw_buffer_store_b8((uint8_t)byte, rs, (int)(live && q == 0 ? row * s_pitch + block : kOutOfRange), 0, 0);
                     __builtin_amdgcn_sched_barrier(0);
                 }
+            };
+            if constexpr (EPI == EPI_GLU_KEEP) {
+                maxima(1);
+                maxima(2);
+                lds_barrier();
+                store(1);
+                store(2);
             }
+            maxima(0);
+            lds_barrier();
+            store(0);
         } else {
             using T = std::conditional_t<EPI == EPI_GLU_BWD_BF16, bf16_t, f16_t>;
             // columns of block wn / 2 of the tile's two

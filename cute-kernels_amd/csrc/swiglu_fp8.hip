@@ -12,12 +12,14 @@ using namespace fp8;
 
 constexpr int kThreads = 256;
 
+// (the non-temporal hint where an access takes whole lines, in the 16-bit types: halves of lines would go one by one)
 template <typename T>
 __device__ __forceinline__ void load8(const T* p, float (&f)[8]) {
     constexpr int V = Vec16<T>::N;
 #pragma unroll
     for (int i = 0; i < 8 / V; ++i) {
-        const Vec16<T> v = load_streaming16(reinterpret_cast<const Vec16<T>*>(p) + i);
+        const Vec16<T>* const from = reinterpret_cast<const Vec16<T>*>(p) + i;
+        const Vec16<T> v = V == 8 ? load_streaming16(from) : *from;
 #pragma unroll
         for (int e = 0; e < V; ++e) f[i * V + e] = Num<T>::up(v.v[e]);
     }
@@ -30,7 +32,8 @@ __device__ __forceinline__ void store8(T* p, const float (&f)[8]) {
         Vec16<T> v;
 #pragma unroll
         for (int e = 0; e < V; ++e) v.v[e] = Num<T>::down(f[i * V + e]);
-        store_streaming16(reinterpret_cast<Vec16<T>*>(p) + i, v);
+        if constexpr (V == 8) store_streaming16(reinterpret_cast<Vec16<T>*>(p) + i, v);
+        else *(reinterpret_cast<Vec16<T>*>(p) + i) = v;
     }
 }
 __device__ __forceinline__ uint2 pack8(const float (&f)[8], float inverse) {
