@@ -7,8 +7,7 @@
 //    consecutive k a lane; both operands are given the same permutation of the block's k instead (bytes 16 q and 64 + 16 q), which leaves
 //    every sum what it is and makes the reads free of bank conflicts.
 //  * The 16 rows of B that make a fragment are not neighbours but rows 8 a + b (a, b = 0 .. 3) and, in the next fragment, 8 a + 4 + b:
-//    a lane's results of two fragments are then eight neighbouring columns, and every epilogue stores from registers: 16 bytes of a 16-bit
-//    result, 8 of an 8-bit one, with no trip through LDS.
+//    a lane's results of two fragments are then eight neighbouring columns: 16 bytes of a 16-bit result, 8 of an 8-bit one.
 //  * The loads are one stream over the steps of all tiles of a workgroup, two steps ahead: the last two steps of a tile load the first
 //    two of the next. They are written in assembly, so the compiler places no waits for them; the one wait of a step, in front of its
 //    last sixteenth-row block, is written by hand, and behind it the step's own stage is free again.
@@ -16,6 +15,11 @@
 //  * Tall tiles (at most 256 groups): a tile may have 288 rows, 256 and one more row block per wavefront, whose 4 KB a step have stages of
 //    their own.
 //  * A reduction may be cut into segments (the two halves of a pre-activation): blocks begin anew in each.
+//  * The instruction's sums: eight neighbouring products are aligned to the largest of them and cut below 2^-13 of it before they are added
+//    to the fp32 sum (measured; the unscaled 8-bit instructions do the same), 2^-16 of a sum of random terms, root mean square. A result
+//    that leaves in 16 bits loses nothing by that, and where a result becomes e4m3 the next product's many terms average the roundings that
+//    fall to the other side (0.003 of the result instead of 0.0017). The pre-activation of a training pass, of which gradients are made
+//    element by element, takes the bfloat16 instruction instead (k_step_exact).
 //  * GLU: the tile holds 128 "up" and 128 "gate" columns; the activation, 128 columns or one block, is quantised from the fp32 sums: the
 //    largest magnitude of a row goes from wavefront to wavefront through LDS. With KEEP the pre-activation is kept in 8 bits too.
 //  * GLU_BWD: the product is the gradient of the activation; the pre-activation's gradient leaves, once rounded to 16 bits for the weight
@@ -55,7 +59,7 @@ enum Epilogue { EPI_BF16, EPI_F16, EPI_F32, EPI_GLU, EPI_GLU_KEEP, EPI_GLU_BWD_B
 struct GemmArgs {
     const uint8_t *A, *A_s, *B, *B_s;
     const uint32_t* sizes;      // [E] rows per group; NULL: one group of R rows
-    const int32_t* row_index;   // not NULL: row i of A is row row_index[i] / divisor of a_rows
+    const int32_t* row_index;   // GLU: row i of A is row row_index[i] / divisor of a_rows
     uint32_t divisor, a_rows;
     uint32_t E, R, N, K, segs;  // K: elements of a segment of the reduction
     uint32_t a_pitch, a_seg, as_pitch, as_seg;            // bytes from row to row, from segment to segment
@@ -93,11 +97,13 @@ __device__ __forceinline__ uint32_t pack_pair(float lo, float hi) {
     else return ::fmahip::gemm::ElemF16::pack2(lo, hi);
 }
 
-template <int EPI, bool GATHER, bool TALL>
+template <int EPI, bool TALL>
 __global__ __launch_bounds__(kGemmThreads) void fp8_gemm_kernel(const GemmArgs args) {
     constexpr bool kGlu = EPI == EPI_GLU || EPI == EPI_GLU_KEEP;
     constexpr bool kBwd = EPI == EPI_GLU_BWD_BF16 || EPI == EPI_GLU_BWD_F16;
+    constexpr bool kGather = kGlu;  // rows of A by index
     constexpr uint32_t kCols = kGlu ? kTileN / 2 : kTileN;  // columns of the output grid per tile
+    constexpr bool kExact = EPI == EPI_GLU_KEEP;  // sums of exact products (k_step_exact)
     // Stores of an epilogue per wavefront, at least (0, 59: an epilogue that has waited for all loads in front of them itself)
     constexpr int kStores = EPI == EPI_BF16 || EPI == EPI_F16 ? 2 * kRowBlocks : (EPI == EPI_GLU ? kRowBlocks : (EPI == EPI_GLU_KEEP ? 3 * kRowBlocks : (kBwd ? 59 : 0)));
     constexpr uint32_t kMostGroups = TALL ? kTallGroups : kMaxGroups;
@@ -231,7 +237,7 @@ __global__ __launch_bounds__(kGemmThreads) void fp8_gemm_kernel(const GemmArgs a
         if (l_tile >= total) {
             l_a_bytes = l_b_bytes = 0;
             l_scale = kOutOfRange;
-            if constexpr (GATHER) {
+            if constexpr (kGather) {
 #pragma unroll
                 for (int i = 0; i < kGathered; ++i) l_gather[i] = kOutOfRange;
             }
@@ -244,7 +250,7 @@ __global__ __launch_bounds__(kGemmThreads) void fp8_gemm_kernel(const GemmArgs a
         const uint32_t cols = N - t.n0 < kCols ? N - t.n0 : kCols;
         l_b_bytes = uniform(cols * K);
         if constexpr (kGlu) l_b2 = uniform64(l_b + args.b_half);
-        if constexpr (GATHER) {
+        if constexpr (kGather) {
             l_a = uniform64((uint64_t)(uintptr_t)args.A);
             l_a_bytes = args.a_rows * args.a_pitch;
 #pragma unroll
@@ -260,7 +266,7 @@ __global__ __launch_bounds__(kGemmThreads) void fp8_gemm_kernel(const GemmArgs a
         if (wave < 4 || (TALL && wave == 5)) {
             const uint32_t r = wave < 4 ? wave * 64u + lane : 256u + lane;
             l_s = (uint64_t)(uintptr_t)args.A_s;
-            if constexpr (GATHER) {
+            if constexpr (kGather) {
                 const uint32_t src = r < t.rows ? (uint32_t)args.row_index[t.row0 + r] / args.divisor : args.a_rows;
                 l_scale = src < args.a_rows ? src * args.as_pitch : kOutOfRange;
             } else {
@@ -279,9 +285,9 @@ __global__ __launch_bounds__(kGemmThreads) void fp8_gemm_kernel(const GemmArgs a
         l_s = uniform64(l_s);
     };
     auto load_a = [&](int i) {
-        uint32_t v = GATHER ? l_gather[i] : a_lane;
+        uint32_t v = kGather ? l_gather[i] : a_lane;
         if (l_ks * kBlock + a_chunk >= K) v = kOutOfRange;
-        load_lds16(rsrc_at(l_a, l_a_bytes), v, (GATHER ? 0u : (uint32_t)i * 64u * args.a_pitch) + l_ks * kBlock,
+        load_lds16(rsrc_at(l_a, l_a_bytes), v, (kGather ? 0u : (uint32_t)i * 64u * args.a_pitch) + l_ks * kBlock,
                    lds0 + l_stage + ((uint32_t)i * 8u + wave) * 1024u);
     };
     auto load_b = [&](int i) {
@@ -293,9 +299,9 @@ __global__ __launch_bounds__(kGemmThreads) void fp8_gemm_kernel(const GemmArgs a
     auto load_x = [&]() {  // rows past 256, where the tile has any
         if constexpr (TALL) {
             if (l_found.rows > (uint32_t)kTileM && wave < 4) {
-                uint32_t v = GATHER ? l_gather[kGathered - 1] : a_lane;
+                uint32_t v = kGather ? l_gather[kGathered - 1] : a_lane;
                 if (l_ks * kBlock + a_chunk >= K) v = kOutOfRange;
-                load_lds16(rsrc_at(l_a, l_a_bytes), v, (GATHER ? 0u : 256u * args.a_pitch) + l_ks * kBlock, lds_x + (l_stage ? 32u * kBlock : 0u) + wave * 1024u);
+                load_lds16(rsrc_at(l_a, l_a_bytes), v, (kGather ? 0u : 256u * args.a_pitch) + l_ks * kBlock, lds_x + (l_stage ? 32u * kBlock : 0u) + wave * 1024u);
             }
         }
     };
@@ -361,6 +367,16 @@ __global__ __launch_bounds__(kGemmThreads) void fp8_gemm_kernel(const GemmArgs a
         sb[0] = read_scale(sb_off);
         sb[1] = kGlu ? read_scale(sb_off + 4u) : sb[0];
     };
+    i32x4 ha[2];  // (a training pass's products: half of A's fragment, bytes h * 64 on)
+    auto read_half = [&](int h, int i, int buf) {
+        ha[buf] = *reinterpret_cast<const i32x4*>(s_op + (c_stage + ((a_off + (uint32_t)i * 16u * kBlock) ^ (h ? 64u : 0u))));
+        sa[buf] = read_scale(sa_off + (uint32_t)i * 64u);
+    };
+    auto read_half_x = [&](int h) {
+        const uint32_t off = (c_stage ? 32u * kBlock : 0u) + (wm * 16u + r16) * kBlock + ((q ^ a_key) << 4);
+        ha[0] = *reinterpret_cast<const i32x4*>(s_x + (off ^ (h ? 64u : 0u)));
+        sa[0] = read_scale((320u + wm * 16u + r16) * 4u);
+    };
     auto mma_with = [&](auto first_c, f32x16& c, int j, i32x8 a, int scale_a, int scale_b) {
         f32x4 v = {0.f, 0.f, 0.f, 0.f};  // (a tile's first step: the instruction takes the constant)
         if constexpr (!decltype(first_c)::value) v = f32x4{c[4 * j], c[4 * j + 1], c[4 * j + 2], c[4 * j + 3]};
@@ -397,9 +413,113 @@ __global__ __launch_bounds__(kGemmThreads) void fp8_gemm_kernel(const GemmArgs a
         read_sb();
 #pragma unroll
         for (int j = 0; j < kColBlocks; ++j) read_b(j);
-        read_a(0, 0);
+        if constexpr (kExact) read_half(0, 0, 0);
+        else read_a(0, 0);
     };
     first_fragments();
+
+    // The K step of a training pass's up projection (GLU_KEEP), whose result is rounded to e4m3 before a gradient is made of it. The 8-bit
+    // instruction's cut (2^-16 of a sum, root mean square) moves one rounding in 2000 by a whole step, an eighth of the value, and dh with it:
+    // weight gradients of a few rows, or of rows that cancel, then hold elements that are off by their size (0.46 of the tensor's root mean
+    // square was seen among sizes of 128 tokens and more). Here the operands become bfloat16 in registers, with their scales, which loses
+    // nothing, and the bfloat16 instruction sums them to 2^-26: 0.07 at most among thirty sizes. It costs half the matrix rate:
+    // 8192 tokens with 8 of 64 experts, 2048 x 1408, forward and backward take 3420 us instead of 3190. The gradient's product (GLU_BWD) has
+    // its result rounded to e4m3 for the input's gradient alone, where a row's many columns average it: it would take 110 us more.
+    // (Scaled values below bfloat16's smallest, 2^-133, are lost; their block's largest is below 2^-110.)
+    // Half a step's K at a time, so that the converted fragments fit beside the sums: both halves of B stay raw until their turn.
+    using gemm::bf16x8;
+    using gemm::bf16x2;
+    bf16x8 bx[kColBlocks][2], ax[2];
+    auto widen = [](bf16x8 (&to)[2], const int* raw, int scale) {
+        const float factor = __uint_as_float((uint32_t)scale << 23);
+#pragma unroll
+        for (int s = 0; s < 2; ++s) {
+#pragma unroll
+            for (int k = 0; k < 2; ++k) {
+                const bf16x2 lo = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(raw[2 * s + k], factor, false);
+                const bf16x2 hi = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(raw[2 * s + k], factor, true);
+                to[s][4 * k] = lo[0];
+                to[s][4 * k + 1] = lo[1];
+                to[s][4 * k + 2] = hi[0];
+                to[s][4 * k + 3] = hi[1];
+            }
+        }
+    };
+    auto widen_b = [&](int h) {
+#pragma unroll
+        for (int j = 0; j < kColBlocks; ++j) {
+            const int raw[4] = {fb[j][4 * h], fb[j][4 * h + 1], fb[j][4 * h + 2], fb[j][4 * h + 3]};
+            widen(bx[j], raw, sb[j >> 1]);
+        }
+    };
+    auto mma_half = [&](auto first_c, f32x16& c, int buf, auto&& between) {
+        const int raw[4] = {ha[buf][0], ha[buf][1], ha[buf][2], ha[buf][3]};
+        widen(ax, raw, sa[buf]);
+#pragma unroll
+        for (int s = 0; s < 2; ++s) {
+#pragma unroll
+            for (int j = 0; j < kColBlocks; ++j) {
+                f32x4 v = {0.f, 0.f, 0.f, 0.f};
+                if (s || !decltype(first_c)::value) v = f32x4{c[4 * j], c[4 * j + 1], c[4 * j + 2], c[4 * j + 3]};
+                v = __builtin_amdgcn_mfma_f32_16x16x32_bf16(bx[j][s], ax[s], v, 0, 0, 0);
+                c[4 * j] = v[0];
+                c[4 * j + 1] = v[1];
+                c[4 * j + 2] = v[2];
+                c[4 * j + 3] = v[3];
+                asm("" : "+v"(c));
+                if (s == 1) between(j);
+            }
+        }
+    };
+    auto k_step_exact = [&](auto first_c, bool tall) {
+        constexpr bool FIRST = decltype(first_c)::value;
+        using Sum = std::integral_constant<bool, false>;
+        const auto nothing = [](int) {};
+        // (the loads and barriers of the step below, with the same reasons)
+        widen_b(0);
+#pragma unroll
+        for (int i = 0; i < kRowBlocks; ++i) {
+            if (i == 1) lds_barrier();
+            if (i < kRowBlocks - 1) read_half(0, i + 1, (i + 1) & 1);
+            if (i == 1) mma_half(first_c, acc[i], i & 1, [&](int j) { load_b(j); });
+            else mma_half(first_c, acc[i], i & 1, nothing);
+            if (i == kRowBlocks - 2) {
+                if constexpr (TALL) {
+                    if (tall) {
+                        read_half_x(0);
+                        mma_half(first_c, acc[kBlocks - 1], 0, nothing);
+                    }
+                }
+                read_half(1, 0, 0);
+            }
+            __builtin_amdgcn_sched_barrier(0);
+        }
+        widen_b(1);
+#pragma unroll
+        for (int i = 0; i < kRowBlocks - 1; ++i) {
+            read_half(1, i + 1, (i + 1) & 1);
+            mma_half(Sum{}, acc[i], i & 1, nothing);
+            __builtin_amdgcn_sched_barrier(0);
+        }
+        if constexpr (TALL) {
+            if (tall) {
+                read_half_x(1);
+                mma_half(Sum{}, acc[kBlocks - 1], 0, nothing);
+            }
+        }
+        wait_vm<(FIRST ? (4 + kStores < 63 ? 4 + kStores : 63) : 4)>();
+        lds_barrier();
+        next_step();
+        mma_half(Sum{}, acc[kRowBlocks - 1], (kRowBlocks - 1) & 1, [&](int j) {
+            load_a(j);
+            read_b(j);
+        });
+        read_sb();
+        read_half(0, 0, 0);
+        load_x();
+        load_scales();
+        next_load();
+    };
 
     // One K step of a tile; FIRST: of its first, whose sums begin at zero.
     auto k_step = [&](auto first_c, bool tall) {
@@ -452,8 +572,13 @@ __global__ __launch_bounds__(kGemmThreads) void fp8_gemm_kernel(const GemmArgs a
         if (steps < 3) t = find(c_tile);  // (the loads are two steps ahead: with three and more they are in this tile when it begins)
         else t = l_found;
         const bool tall = TALL && t.rows > (uint32_t)kTileM;
-        k_step(std::integral_constant<bool, true>{}, tall);
-        for (uint32_t step = 1; step < steps; ++step) k_step(std::integral_constant<bool, false>{}, tall);
+        if constexpr (kExact) {
+            k_step_exact(std::integral_constant<bool, true>{}, tall);
+            for (uint32_t step = 1; step < steps; ++step) k_step_exact(std::integral_constant<bool, false>{}, tall);
+        } else {
+            k_step(std::integral_constant<bool, true>{}, tall);
+            for (uint32_t step = 1; step < steps; ++step) k_step(std::integral_constant<bool, false>{}, tall);
+        }
         // first row of this wavefront's row block i
         auto block_row = [&](int i) -> uint32_t { return i < kRowBlocks ? wm * 128u + (uint32_t)i * 16u : 256u + wm * 16u; };
 

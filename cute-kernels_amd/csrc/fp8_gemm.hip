@@ -24,20 +24,20 @@ int launch_gemm(const char* who, int epilogue, const GemmArgs& args, hipStream_t
     const int64_t tiles = ((int64_t)args.R / kTileM + (args.E < args.R ? args.E : args.R)) * ((args.N + cols - 1) / cols);
     const int64_t cus = num_compute_units() > 0 ? num_compute_units() : 256;
     const dim3 grid((uint32_t)(tiles < cus ? tiles : cus)), block(kGemmThreads);
-    const bool gather = args.row_index != nullptr, tall = args.E <= kTallGroups;
+    const bool tall = args.E <= kTallGroups;
     auto run = [&](auto low, auto high) {
         if (tall) hipLaunchKernelGGL(high, grid, block, 0, st, args);
         else hipLaunchKernelGGL(low, grid, block, 0, st, args);
     };
-#define FMA_FP8_RUN(EPI, GATHER) run(fp8_gemm_kernel<EPI, GATHER, false>, fp8_gemm_kernel<EPI, GATHER, true>)
+#define FMA_FP8_RUN(EPI) run(fp8_gemm_kernel<EPI, false>, fp8_gemm_kernel<EPI, true>)
     switch (epilogue) {
-        case EPI_BF16: FMA_FP8_RUN(EPI_BF16, false); break;
-        case EPI_F16: FMA_FP8_RUN(EPI_F16, false); break;
-        case EPI_F32: FMA_FP8_RUN(EPI_F32, false); break;
-        case EPI_GLU: gather ? FMA_FP8_RUN(EPI_GLU, true) : FMA_FP8_RUN(EPI_GLU, false); break;
-        case EPI_GLU_KEEP: gather ? FMA_FP8_RUN(EPI_GLU_KEEP, true) : FMA_FP8_RUN(EPI_GLU_KEEP, false); break;
-        case EPI_GLU_BWD_BF16: FMA_FP8_RUN(EPI_GLU_BWD_BF16, false); break;
-        default: FMA_FP8_RUN(EPI_GLU_BWD_F16, false); break;
+        case EPI_BF16: FMA_FP8_RUN(EPI_BF16); break;
+        case EPI_F16: FMA_FP8_RUN(EPI_F16); break;
+        case EPI_F32: FMA_FP8_RUN(EPI_F32); break;
+        case EPI_GLU: FMA_FP8_RUN(EPI_GLU); break;
+        case EPI_GLU_KEEP: FMA_FP8_RUN(EPI_GLU_KEEP); break;
+        case EPI_GLU_BWD_BF16: FMA_FP8_RUN(EPI_GLU_BWD_BF16); break;
+        default: FMA_FP8_RUN(EPI_GLU_BWD_F16); break;
     }
 #undef FMA_FP8_RUN
     return launch_status(who);
