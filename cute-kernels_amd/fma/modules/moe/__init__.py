@@ -372,8 +372,11 @@ class MoE(nn.Module):
 
     def quantize_experts(self) -> "MoE":
         """Switches the experts' products to 8 bits (fp8_experts) and lays both projections out in 8 bits once, for calls that no backward
-        pass follows: a serving program calls it after loading the weights, and again after changing them (a forward pass on weights that
-        have changed since quantises them in the call, as one without this call does)."""
+        pass follows: a serving program calls it after loading the weights, and again after changing them. A forward pass on weights that
+        have changed since, as far as their version counters tell, quantises them in the call, as one without this call does; changes that
+        no counter sees (through .data, or by a replayed graph) need the call again. A compiled layer quantises in the call."""
+        if any(t.is_inference() for t in (self.c_fc.weight, self.c_proj.weight)):
+            raise ValueError("quantize_experts: parameters that were made in inference mode do not tell when they change")
         self._check_fp8_experts(self.c_fc.weight.dtype)
         self.fp8_experts = True
         with torch.no_grad():
@@ -399,7 +402,7 @@ class MoE(nn.Module):
     ) -> torch.Tensor:
         self._check_fp8_experts(hidden_states.dtype)
         weights = self.c_fc.weight, self.c_proj.weight
-        if self._fp8_weights is not None and not torch.is_grad_enabled():
+        if self._fp8_weights is not None and not torch.is_grad_enabled() and not torch.compiler.is_compiling():
             made_of, blocks = self._fp8_weights
             if all(a[0] is b[0] and a[1:] == b[1:] for a, b in zip(made_of, self._weight_versions())):
                 weights = blocks

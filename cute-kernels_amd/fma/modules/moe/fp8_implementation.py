@@ -1,10 +1,12 @@
 """The expert path of a SwiGLU layer with its products in 8 bits (fma_swiglu_experts_fp8 and its backward, one call per direction)."""
 
 import torch
+from torch.autograd import forward_ad
 
 from ... import _lib
 from ..._ops import hip_op
 from ...ops.fp8 import BLOCK_SIZE, Fp8Blocks, quantize_fp8
+from ...ops.fp8.cuda_implementation import is_scales_dtype, operator_scales
 from ...utils import ensure_contiguous
 
 
@@ -17,7 +19,7 @@ def _check_operands(x, router_weights, selected_experts, weight1, weight1_scales
     assert selected_experts.shape == router_weights.shape == (T, k) and selected_experts.dtype in (torch.int32, torch.int64)
     assert x.dtype == router_weights.dtype and x.dtype in (torch.float16, torch.bfloat16)
     for values, scales in ((weight1, weight1_scales), (weight2, weight2_scales)):
-        assert values.dtype == torch.float8_e4m3fn and scales.dtype == torch.float8_e8m0fnu
+        assert values.dtype == torch.float8_e4m3fn and is_scales_dtype(scales.dtype)
         N, K = values.shape[-2:]
         assert scales.shape == (*values.shape[:-2], -(-N // 128), 4 * -(-K // 512))
     for t in (x, router_weights, selected_experts, weight1, weight1_scales, weight2, weight2_scales):
@@ -121,9 +123,11 @@ class _SwigluExpertsFp8(torch.autograd.Function):
         if keeps:
             buffer = x.new_empty(buffer_bytes(T, selected_experts.size(1), E, H, two_I // 2), dtype=torch.uint8)
         if T:
-            swiglu_experts_fp8_cuda(x, router_weights, selected_experts, *c_fc, *c_proj, output, buffer)
+            operands = c_fc[0], operator_scales(c_fc[1]), c_proj[0], operator_scales(c_proj[1])
+            swiglu_experts_fp8_cuda(x, router_weights, selected_experts, *operands, output, buffer)
         if keeps:
-            ctx.save_for_backward(router_weights, selected_experts, *c_fc_t, *c_proj_t, buffer)
+            operands = c_fc_t[0], operator_scales(c_fc_t[1]), c_proj_t[0], operator_scales(c_proj_t[1])
+            ctx.save_for_backward(router_weights, selected_experts, *operands, buffer)
         return output
 
     @staticmethod
@@ -174,15 +178,18 @@ def swiglu_experts_fp8(
         E, I = c_fc.size(0), c_fc.size(1) // 2
         assert c_fc.shape == (E, 2 * I, H) and c_proj.shape == (E, H, I), "sizes of tokens and projections should agree"
         assert c_fc.dtype == c_proj.dtype == x.dtype, "projections in 16 bits should have the tokens' dtype"
+    assert E > 0, "there should be an expert"
     assert H > 0 and I > 0 and H % 16 == 0 and I % 16 == 0, "hidden and intermediate size should be multiples of 16"
     if not prepared:
         return _SwigluExpertsFp8.apply(x, router_weights, selected_experts, c_fc, c_proj, torch.is_grad_enabled())
-    if torch.is_grad_enabled() and (x.requires_grad or router_weights.requires_grad):
+    tangents = forward_ad._current_level >= 0 and any(forward_ad.unpack_dual(t).tangent is not None for t in (x, router_weights))
+    if tangents or (torch.is_grad_enabled() and (x.requires_grad or router_weights.requires_grad)):
         raise RuntimeError("swiglu_experts_fp8 has no gradients through projections that are in 8 bits already: pass the 16-bit tensors")
     with torch.no_grad():
         x, router_weights, selected_experts = x.contiguous(), router_weights.contiguous(), selected_experts.contiguous()
         output = torch.empty_like(x)
         if x.size(0):
-            operands = [t.contiguous() for t in (*c_fc, *c_proj)]
+            c_fc, c_fc_scales, c_proj, c_proj_scales = (t.contiguous() for t in (*c_fc, *c_proj))
+            operands = c_fc, operator_scales(c_fc_scales), c_proj, operator_scales(c_proj_scales)
             swiglu_experts_fp8_cuda(x, router_weights, selected_experts, *operands, output, None)
         return output

@@ -19,7 +19,9 @@ from .cuda_implementation import (
     grouped_gemm_fp8_cuda,
     grouped_linear_fp8_backward_cuda,
     grouped_linear_fp8_cuda,
+    operator_scales,
     quantize_fp8_cuda,
+    scales_dtype,
 )
 
 BLOCK_SIZE = 128
@@ -42,7 +44,7 @@ def _empty_blocks(shape: tuple[int, ...], block_rows: int, device: torch.device)
     *batch, N, K = shape
     return Fp8Blocks(
         torch.empty(shape, dtype=torch.float8_e4m3fn, device=device),
-        torch.empty(*batch, ceil_divide(N, block_rows), scale_columns(K), dtype=torch.float8_e8m0fnu, device=device),
+        torch.empty(*batch, ceil_divide(N, block_rows), scale_columns(K), dtype=scales_dtype(), device=device),
     )
 
 
@@ -63,6 +65,8 @@ def quantize_fp8(
     blocks = _empty_blocks(shape, block_rows, x.device)
     other = _empty_blocks((*shape[:-2], shape[-1], shape[-2]), block_rows, x.device) if transposed else None
     quantize_fp8_cuda(x, *blocks, *(other or (None, None)), block_rows)
+    if torch.compiler.is_compiling():
+        blocks, other = (b and Fp8Blocks(b.values, b.scales.view(torch.float8_e8m0fnu)) for b in (blocks, other))
     if one_row:
         return Fp8Blocks(blocks.values[0], blocks.scales[0])
     return blocks if other is None else (blocks, other)
@@ -89,7 +93,7 @@ def dequantize_fp8(blocks: Fp8Blocks, dtype: torch.dtype = torch.bfloat16) -> to
         values, scales = values[None], scales[None]
     block_rows = block_rows_of((values, scales))
     output = torch.empty(values.shape, dtype=dtype, device=values.device)
-    dequantize_fp8_cuda(values, scales, output, block_rows)
+    dequantize_fp8_cuda(values, operator_scales(scales), output, block_rows)
     return output[0] if one_row else output
 
 
@@ -127,7 +131,8 @@ def grouped_gemm_fp8(
     else:
         assert E == 1, "several groups need M_array"
     output = torch.empty(R, N, dtype=output_dtype, device=a.device)
-    grouped_gemm_fp8_cuda(a.contiguous(), a_scales.contiguous(), b.contiguous(), b_scales.contiguous(), M_array, output)
+    a_scales, b_scales = operator_scales(a_scales.contiguous()), operator_scales(b_scales.contiguous())
+    grouped_gemm_fp8_cuda(a.contiguous(), a_scales, b.contiguous(), b_scales, M_array, output)
     return output
 
 

@@ -6,6 +6,20 @@ from ... import _lib
 from ..._ops import hip_op
 
 
+def scales_dtype() -> torch.dtype:
+    """float8_e8m0fnu; bytes in a traced function, whose compiler cannot write a tensor of that type by way of an operator"""
+    return torch.uint8 if torch.compiler.is_compiling() else torch.float8_e8m0fnu
+
+
+def operator_scales(scales: torch.Tensor) -> torch.Tensor:
+    """scales as an operator takes them (see scales_dtype)"""
+    return scales.view(torch.uint8) if torch.compiler.is_compiling() and scales.dtype is not torch.uint8 else scales
+
+
+def is_scales_dtype(dtype: torch.dtype) -> bool:
+    return dtype == torch.float8_e8m0fnu or dtype == torch.uint8
+
+
 def _matrices(t: torch.Tensor) -> tuple[int, int, int]:
     """t [.., N, K] as (matrices, N, K)"""
     N, K = t.shape[-2:]
@@ -16,7 +30,7 @@ def _matrices(t: torch.Tensor) -> tuple[int, int, int]:
 
 
 def _check_blocks(values: torch.Tensor, scales: torch.Tensor, N: int, K: int, block_rows: int) -> None:
-    assert values.dtype == torch.float8_e4m3fn and scales.dtype == torch.float8_e8m0fnu
+    assert values.dtype == torch.float8_e4m3fn and is_scales_dtype(scales.dtype)
     assert values.is_contiguous() and scales.is_contiguous()
     assert scales.shape == (*values.shape[:-2], -(-N // block_rows), 4 * -(-K // 512))
 

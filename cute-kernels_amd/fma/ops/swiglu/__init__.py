@@ -10,6 +10,7 @@ import torch
 from ...kernel_backend import KernelBackend, is_hip_kernel_backend
 from ...math import ceil_divide, divide_if_divisible
 from ...utils import ensure_contiguous
+from ..fp8.cuda_implementation import scales_dtype
 from .cuda_implementation import swiglu_backward_cuda, swiglu_forward_cuda, swiglu_fp8_backward_cuda, swiglu_fp8_forward_cuda
 
 _BLOCK_SIZE = 1024  # a launch-shape argument of the reference's stubs; the HIP kernels choose their own
@@ -92,7 +93,7 @@ class _SwigluPackedFp8(torch.autograd.Function):
         output = x.new_empty(*x.shape[:-1], half)
         rows = x.numel() // x.size(-1)
         values = torch.empty(rows, 2, half, dtype=torch.float8_e4m3fn, device=x.device)
-        scales = torch.empty(rows, 2, 4 * ceil_divide(half, 512), dtype=torch.float8_e8m0fnu, device=x.device)
+        scales = torch.empty(rows, 2, 4 * ceil_divide(half, 512), dtype=scales_dtype(), device=x.device)
         swiglu_fp8_forward_cuda(x.view(rows, 2 * half), output.view(rows, half), values, scales)
         ctx.save_for_backward(values, scales)
         return output

@@ -7,6 +7,7 @@ import torch
 
 from ... import _lib
 from ..._ops import hip_op
+from ..fp8.cuda_implementation import is_scales_dtype
 
 
 def _rows_view(t: torch.Tensor) -> tuple[int, int, int] | None:
@@ -89,7 +90,7 @@ def swiglu_backward_cuda(
 def _check_packed_rows(x: torch.Tensor, half: torch.Tensor, values: torch.Tensor, scales: torch.Tensor) -> tuple[int, int]:
     R, I = half.shape
     assert x.shape == (R, 2 * I) and values.shape == (R, 2, I) and scales.shape == (R, 2, 4 * -(-I // 512))
-    assert x.dtype == half.dtype and values.dtype == torch.float8_e4m3fn and scales.dtype == torch.float8_e8m0fnu
+    assert x.dtype == half.dtype and values.dtype == torch.float8_e4m3fn and is_scales_dtype(scales.dtype)
     for t in (x, half, values, scales):
         assert t.is_contiguous()
     return R, I

@@ -180,3 +180,25 @@ def test_refusals_of_the_expert_path():
     assert not moe.fp8_experts and "fp8" not in str(list(moe.state_dict()))
     with pytest.raises(RuntimeError, match="GPU only"):
         quantize_expert_weights(w1, w2)
+
+
+def test_refusals_of_serving_with_tangents_and_without_experts():
+    x, gates, ids = torch.zeros(3, 32).bfloat16(), torch.zeros(3, 2).bfloat16(), torch.zeros(3, 2, dtype=torch.int64)
+    with pytest.raises(AssertionError, match="an expert"):
+        fma.swiglu_experts_fp8(x, gates, ids, torch.zeros(0, 64, 32).bfloat16(), torch.zeros(0, 32, 32).bfloat16())
+
+    def blocks(*shape):
+        scales = torch.full((*shape[:-2], 1, 4), 127, dtype=torch.uint8).view(torch.float8_e8m0fnu)
+        return fma.Fp8Blocks(torch.zeros(shape, dtype=torch.uint8).view(torch.float8_e4m3fn), scales)
+
+    with torch.autograd.forward_ad.dual_level():
+        dual = torch.autograd.forward_ad.make_dual(x, torch.ones_like(x))
+        with pytest.raises(RuntimeError, match="no gradients"):
+            fma.swiglu_experts_fp8(dual, gates, ids, blocks(2, 2, 32, 32), blocks(2, 32, 32))
+
+
+def test_refusal_of_parameters_made_in_inference_mode():
+    with torch.inference_mode():
+        moe = fma.MoE(4, 2, 32, 32, fma.swiglu_packed, True, False, 0.02).to(torch.bfloat16)
+    with pytest.raises(ValueError, match="inference mode"):
+        moe.quantize_experts()

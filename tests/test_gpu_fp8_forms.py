@@ -4,7 +4,10 @@ numbers of rows per group around the choice between the kernels, other streams, 
 import pytest
 import torch
 
-from fma import Fp8Blocks, grouped_gemm_fp8, grouped_linear_fp8, quantize_expert_weights, quantize_fp8, swiglu_experts_fp8
+from fma import (
+    Fp8Blocks, KernelBackend, MoE, dequantize_fp8, grouped_gemm_fp8, grouped_linear_fp8, quantize_expert_weights, quantize_fp8,
+    swiglu_experts_fp8, swiglu_packed, swiglu_packed_fp8,
+)  # fmt: skip
 from gpu_util import DEV
 from oracle import fp8_oracle as O
 from test_gpu_fp8 import _check_product, _operands, _sizes
@@ -175,3 +178,106 @@ def test_two_calls_at_once():
     for runs, exact in zip(got, want):
         for run in runs:
             assert all(torch.equal(a, b) for a, b in zip(run, exact))
+
+
+def test_a_second_backward_reads_what_the_first_read():
+    x, gates, ids, w1, w2, dy = (t.to(DEV) for t in _case(300, 256, 144, 4, 2, torch.bfloat16, seed=7))
+    leaves = [t.requires_grad_() for t in (x, gates, w1, w2)]
+    y = swiglu_experts_fp8(leaves[0], leaves[1], ids, *leaves[2:])
+    first = torch.autograd.grad(y, leaves, dy, retain_graph=True)
+    assert all(torch.equal(a, b) for a, b in zip(first, torch.autograd.grad(y, leaves, dy)))
+
+
+@pytest.mark.parametrize("value", [float("inf"), float("nan")])
+def test_a_training_step_keeps_what_is_not_a_number_to_its_token(value):
+    x, gates, ids, w1, w2, dy = (t.to(DEV) for t in _case(300, 272, 144, 4, 2, torch.bfloat16, seed=8))
+
+    def step(x):
+        leaves = [t.detach().requires_grad_() for t in (x, gates, w1, w2)]
+        y = swiglu_experts_fp8(leaves[0], leaves[1], ids, *leaves[2:])
+        return (y, *torch.autograd.grad(y, leaves, dy))
+
+    fine, bad = step(x), x.clone()
+    bad[17, 3] = value
+    got = step(bad)
+    rest = torch.arange(300, device=DEV) != 17
+    assert got[0][17].isnan().all() and got[1][17].isnan().all() and got[2][17].isnan().all()
+    assert all(torch.equal(a[rest], b[rest]) for a, b in zip(got[:3], fine[:3]))
+    for a, b in zip(got[3:], fine[3:]):
+        for e in range(4):
+            if not (ids[17] == e).any():
+                assert torch.equal(a[e], b[e]), e
+
+
+def test_tokens_of_very_different_sizes():
+    """a scale per token, over sixty powers of two: with every token's result brought to the same size, the norm over all of them is what it
+    is for tokens of one size (a bound per token would not hold: one rounding that falls to the other side of a border is an eighth of one of
+    a token's 144 activations, and the largest may carry most of the token)"""
+    x, gates, ids, w1, w2, _ = _case(300, 256, 144, 4, 2, torch.bfloat16, seed=9)
+    powers = torch.randint(-40, 20, (300, 1), generator=torch.Generator().manual_seed(9)).float()
+    x = (x.float() * torch.exp2(powers)).bfloat16()
+    exact = _oracle(x, gates, ids, w1, w2)[0]
+    leaf = w1.to(DEV).requires_grad_()  # (as a training step, then as a serving one)
+    trained = swiglu_experts_fp8(x.to(DEV), gates.to(DEV), ids.to(DEV), leaf, w2.to(DEV)).detach()
+    with torch.no_grad():
+        served = swiglu_experts_fp8(x.to(DEV), gates.to(DEV), ids.to(DEV), leaf, w2.to(DEV))
+    size = exact.norm(dim=1, keepdim=True)
+    for out in (trained, served):
+        _close(out.cpu().double() / size, exact / size, torch.bfloat16, 1, "y")
+
+
+def _same(got, want):
+    return all(torch.equal(a.contiguous().view(torch.uint8), b.contiguous().view(torch.uint8)) for a, b in zip(got, want, strict=True))
+
+
+def test_compiled_operators():
+    x, gates, ids, w1, w2, dy = (t.to(DEV) for t in _case(60, 128, 144, 8, 2, torch.bfloat16, seed=10))
+    counts, blocks = _sizes([10, 0, 30, 20, 0, 0, 0, 0]), quantize_expert_weights(w1, w2)
+
+    def conversions(x, w):
+        rows, (tiles, turned) = quantize_fp8(x), quantize_fp8(w, 128, transposed=True)
+        return (*rows, *tiles, *turned, dequantize_fp8(rows), dequantize_fp8(turned), grouped_gemm_fp8(rows, turned, counts))
+
+    def serve(x, gates, ids):
+        return (swiglu_experts_fp8(x, gates, ids, *blocks),)
+
+    with torch.no_grad():
+        assert _same(torch.compile(conversions, fullgraph=True)(x, w2), conversions(x, w2))
+        assert _same(torch.compile(serve, fullgraph=True)(x, gates, ids), serve(x, gates, ids))
+
+    def linear(x, w):
+        return grouped_linear_fp8(x, w, counts)
+
+    def experts(x, gates, w1, w2):
+        return swiglu_experts_fp8(x, gates, ids, w1, w2)
+
+    for call, operands in ((swiglu_packed_fp8, [x]), (linear, [x, w1]), (experts, [x, gates, w1, w2])):
+        results = []
+        for f in (call, torch.compile(call, fullgraph=True)):
+            leaves = [t.clone().requires_grad_() for t in operands]
+            y = f(*leaves)
+            results.append((y.detach(), *torch.autograd.grad(y, leaves, torch.ones_like(y))))
+        assert _same(*results), call
+
+
+def test_compiled_layer():
+    torch.manual_seed(0)
+    moe = MoE(8, 2, 128, 144, swiglu_packed, True, False, 0.02).to(torch.bfloat16).to(DEV)
+    moe.fp8_experts = True
+    x = torch.randn(60, 128, device=DEV).bfloat16()
+
+    def run(x):
+        return moe(x, kernel_backend=KernelBackend.cuda)[0]
+
+    compiled = torch.compile(run, fullgraph=True)
+    grads = []
+    for call in (run, compiled):
+        leaf = x.clone().requires_grad_()
+        y = call(leaf)
+        grads.append((y.detach(), *torch.autograd.grad(y.float().pow(2).sum(), [leaf, moe.c_fc.weight, moe.c_proj.weight])))
+    for a, b in zip(*grads):
+        assert float((a - b).float().norm() / a.float().norm()) <= 2.0**-6  # (the traced layer's router is another kernel)
+    moe.quantize_experts()
+    with torch.no_grad():
+        want, got = run(x), torch.compile(run, fullgraph=True)(x)
+    assert float((want - got).float().norm() / want.float().norm()) <= 2.0**-6
