@@ -227,8 +227,16 @@ __global__ __launch_bounds__(kThreads) void quantize_blocks_generic_kernel(const
 
 // ---- back -----------------------------------------------------------------------------------------------------------
 
-// Eight elements a lane, so that a store of a 16-bit type takes whole lines, four times per workgroup with all loads in front. row_shift: 0, or 7 where 128 rows of a matrix of N rows share their
-// scales. Index arithmetic in 32 bits (I32) where the sizes allow it: a 64-bit division costs more than the rest of the kernel.
+// The float16 numbers from 63488 to 65504 become 65536 in 8 bits, which float16 would round to infinity: on the way back they are 65504,
+// 2^-11 away, so that a gradient made from finite tokens stays finite.
+template <typename T>
+__device__ __forceinline__ float in_range(float v) {
+    if constexpr (std::is_same_v<T, f16_t>) return fabsf(v) == 65536.f ? copysignf(65504.f, v) : v;
+    else return v;
+}
+
+// Eight elements a lane, so that a store of a 16-bit type takes whole lines, four times per workgroup with all loads in front. row_shift: 0, or
+// 7 where 128 rows of a matrix of N rows share their scales. Index arithmetic in 32 bits (I32) where the sizes allow it: a 64-bit division costs more than the rest of the kernel.
 // [65536, 1408] bf16: 95 -> 53 us (5.2 TB/s).
 constexpr int kDequantizeUnroll = 4;
 template <typename T, bool I32>
@@ -266,7 +274,7 @@ __global__ __launch_bounds__(kThreads) void dequantize_kernel(const uint8_t* __r
             float g[4];
             unpack4(w[j], g);
 #pragma unroll
-            for (int x = 0; x < 4; ++x) f[4 * j + x] = g[x] * scale[i];
+            for (int x = 0; x < 4; ++x) f[4 * j + x] = in_range<T>(g[x] * scale[i]);
         }
         if constexpr (sizeof(T) == 4) {
             store_floats(out + at[i], f);
@@ -293,7 +301,7 @@ __global__ __launch_bounds__(kThreads) void dequantize_generic_kernel(const uint
         const int64_t e = row / N, s_row = e * scale_rows + ((row - e * N) >> row_shift);
         float g[4];
         unpack4(values[i], g);
-        out[i] = Num<T>::down(g[0] * scale_value(scales[s_row * pitch + k / kBlock]));
+        out[i] = Num<T>::down(in_range<T>(g[0] * scale_value(scales[s_row * pitch + k / kBlock])));
     }
 }
 

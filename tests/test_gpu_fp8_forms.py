@@ -226,6 +226,23 @@ def test_tokens_of_very_different_sizes():
         _close(out.cpu().double() / size, exact / size, torch.bfloat16, 1, "y")
 
 
+@pytest.mark.parametrize("K", [128, 130])
+def test_the_largest_float16_numbers_stay_finite(K):
+    x = torch.tensor([65504.0, -65504.0, 63488.0, 63456.0, -1.0, 0.0]).half()[:, None].expand(6, K).contiguous().to(DEV)
+    back = dequantize_fp8(quantize_fp8(x), torch.float16)
+    assert back.isfinite().all() and bool(((back.double() - x.double()).abs() <= 2.0**-4 * x.double().abs()).all())
+    wide = dequantize_fp8(quantize_fp8(x), torch.float32)
+    assert float(wide[0, 0]) == 65536.0 and float(back[0, 0]) == 65504.0 and float(back[1, K - 1]) == -65504.0
+    x[0, 0] = float("inf")
+    assert dequantize_fp8(quantize_fp8(x), torch.float16)[0, :128].isnan().all()
+    if K % 16 == 0:
+        tokens = torch.full((40, K), 65504.0, device=DEV).half()
+        w = (1e-6 * torch.ones(1, 32, K, device=DEV)).half().requires_grad_()
+        y = grouped_linear_fp8(tokens, w, _sizes([40]))
+        grad = torch.autograd.grad(y, w, torch.full_like(y, 0.015625))[0]
+        assert bool(((grad.float() - 40 * 65504 * 0.015625).abs() <= 40 * 65504 * 0.015625 * 2.0**-10).all())
+
+
 def _same(got, want):
     return all(torch.equal(a.contiguous().view(torch.uint8), b.contiguous().view(torch.uint8)) for a, b in zip(got, want, strict=True))
 
