@@ -16,6 +16,7 @@ namespace {
 using namespace fp8;
 
 constexpr int kThreads = 256;
+constexpr uint32_t kFloat16Scale = 127 + 7;  // 448 * 2^7 = 57344: the largest scale of a block that float16 holds
 
 // The expert of a slot, -1 for an id that names none: such a choice has no row, and takes no part in anything.
 __device__ __forceinline__ bool names_expert(const void* ids, int id_bytes, int64_t slot, uint32_t E) {
@@ -84,13 +85,18 @@ int sum_choices(const void* o, const void* ids, int id_bytes, const int32_t* inv
 
 // ---- the combine's backward, and the rows' gradient in 8 bits beside it ----------------------------------------------
 // One wavefront per (token, choice): do = gate * dy rounded to T and, from the unrounded products, in 8 bits; dgate = <dy, o>. H % 8 == 0.
-template <typename T>
+//
+// SHIFTED (float16): an activation may be past float16's range (its sums are fp32), and the product do^T a8 takes a 16-bit copy of it. A row whose
+// largest block has a scale of 2^(7 + s), s > 0, gives that copy 2^-s of its activations, 57344 at most, and do 2^s of its gradient, which leaves every
+// product what it is: powers of two, written to `shift`. (A do that overflows by that belongs to a product of 2^30 and more.)
+template <typename T, bool SHIFTED>
 __global__ __launch_bounds__(kThreads) void combine_bwd_fp8_kernel(const T* __restrict__ dy, const T* __restrict__ o,
                                                                    const void* __restrict__ ids, int id_bytes,
                                                                    const int32_t* __restrict__ inv, const T* __restrict__ gates,
                                                                    int64_t slots, uint32_t top_k, uint32_t E, uint32_t H, T* __restrict__ d_o,
                                                                    uint8_t* __restrict__ values, uint32_t* __restrict__ scales,
-                                                                   T* __restrict__ d_gates) {
+                                                                   T* __restrict__ d_gates, const uint8_t* __restrict__ a8_s, uint32_t a_blocks,
+                                                               uint32_t a_pitch, uint8_t* __restrict__ shift) {
     const uint32_t lane = threadIdx.x & 63u;
     const int64_t slot = ((int64_t)blockIdx.x * kThreads + threadIdx.x) / 64;
     if (slot >= slots) return;
@@ -101,6 +107,18 @@ __global__ __launch_bounds__(kThreads) void combine_bwd_fp8_kernel(const T* __re
     }
     const float gate = Num<T>::up(gates[slot]);
     const uint32_t quads = (H + 511u) / 512u;
+    float raise = 1.f;
+    if constexpr (SHIFTED) {
+        uint32_t top = 0;
+        for (uint32_t b = lane; b < a_blocks; b += 64u) {
+            const uint32_t byte = a8_s[row * a_pitch + b];
+            top = max_u32(top, byte == 255u ? 0u : byte);  // (a block that is not a number stays that)
+        }
+        top = group_max<64>(top);
+        const uint32_t by = top > kFloat16Scale ? top - kFloat16Scale : 0u;
+        raise = __uint_as_float((127u + by) << 23);
+        if (lane == 0) shift[row] = (uint8_t)by;
+    }
     const T* const from = dy + slot / top_k * H;
     float dot = 0.f;
     for (uint32_t c = 0; c < quads; ++c) {
@@ -119,7 +137,7 @@ __global__ __launch_bounds__(kThreads) void combine_bwd_fp8_kernel(const T* __re
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
                 d[i] = gate * Num<T>::up(v.v[i]);
-                out.v[i] = Num<T>::down(d[i]);
+                out.v[i] = Num<T>::down(SHIFTED ? d[i] * raise : d[i]);
                 m = max_u32(m, magnitude_bits(d[i]));
             }
             if (d_o) *reinterpret_cast<Vec16<T>*>(d_o + row * H + h) = out;
@@ -200,6 +218,7 @@ int64_t index_rows_bytes(int64_t R) { return (R * 4 + 255) & ~(int64_t)255; }
 struct GradBuffers {
     uint8_t *do8, *do8_s, *dh8, *dh8_s;
     void *d_o, *dh, *dx, *a16, *x16;
+    uint8_t* shift;
     int64_t bytes;
 };
 
@@ -220,6 +239,7 @@ GradBuffers lay_out_grad(uint8_t* base, const Shape& s) {
     b.dx = take(s.R * s.H * 2);
     b.a16 = take(s.R * s.I * 2);
     b.x16 = take(s.T * s.H * 2);
+    b.shift = take(s.R);
     b.bytes = at;
     return b;
 }
@@ -351,15 +371,17 @@ int fma_swiglu_experts_fp8_bwd(const void* dy, const void* gates, const void* id
     const dim3 grid((uint32_t)((s.R + 3) / 4)), block(kThreads);
     auto combine_bwd = [&](auto kernel, auto* dy_, auto* o_, auto* gates_, auto* d_o_, auto* d_gates_) {
         hipLaunchKernelGGL(kernel, grid, block, 0, st, dy_, o_, ids, id_bytes, b.inv, gates_, s.R, (uint32_t)top_k, (uint32_t)E, (uint32_t)H, d_o_, needs_h ? g.do8 : nullptr,
-                           (uint32_t*)g.do8_s, d_gates_);
+                           (uint32_t*)g.do8_s, d_gates_, b.a8_s, (uint32_t)((I + kBlock - 1) / kBlock), (uint32_t)scale_pitch(I), g.shift);
     };
     if (dtype == FMA_BF16)
-        combine_bwd(combine_bwd_fp8_kernel<bf16_t>, (const bf16_t*)dy, (const bf16_t*)b.o, (const bf16_t*)gates, (bf16_t*)(dW2 ? g.d_o : nullptr), (bf16_t*)d_gates);
+        combine_bwd(combine_bwd_fp8_kernel<bf16_t, false>, (const bf16_t*)dy, (const bf16_t*)b.o, (const bf16_t*)gates, (bf16_t*)(dW2 ? g.d_o : nullptr), (bf16_t*)d_gates);
     else
-        combine_bwd(combine_bwd_fp8_kernel<f16_t>, (const f16_t*)dy, (const f16_t*)b.o, (const f16_t*)gates, (f16_t*)(dW2 ? g.d_o : nullptr), (f16_t*)d_gates);
+        combine_bwd(dW2 ? combine_bwd_fp8_kernel<f16_t, true> : combine_bwd_fp8_kernel<f16_t, false>, (const f16_t*)dy, (const f16_t*)b.o, (const f16_t*)gates, (f16_t*)(dW2 ? g.d_o : nullptr), (f16_t*)d_gates);
     if (const int rc = launch_status("swiglu_experts_fp8_bwd")) return rc;
     if (dW2) {
-        if (const int rc = fma_dequantize_fp8(b.a8, b.a8_s, g.a16, 1, s.R, I, 1, dtype, stream)) return rc;
+        const int rc_a = dtype == FMA_BF16 ? fma_dequantize_fp8(b.a8, b.a8_s, g.a16, 1, s.R, I, 1, dtype, stream)
+                                           : dequantize_shifted(b.a8, b.a8_s, g.shift, g.a16, s.R, I, st);
+        if (rc_a) return rc_a;
         if (const int rc = fma_grouped_gemm_ragged(g.d_o, g.a16, dW2, b.counts, nullptr, E, /*FMA_VARY_K*/ 1, H, I, 0, 1, 0, 1.0f, dtype, stream)) return rc;
     }
     if (!needs_h) return FMA_OK;

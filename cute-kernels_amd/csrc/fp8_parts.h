@@ -52,6 +52,9 @@ __device__ __forceinline__ void unpack4(uint32_t q, float (&f)[4]) {
     f[3] = hi[1];
 }
 
+// Rows [R, K] in blocks of 1 x 128 as float16, 2^-shift[r] of row r. K a multiple of eight, values aligned to 8 bytes, out to 16.
+int dequantize_shifted(const uint8_t* values, const uint8_t* scales, const uint8_t* shift, void* out, int64_t R, int64_t K, hipStream_t st);
+
 // largest of v over a group of LANES neighbouring lanes
 template <int LANES>
 __device__ __forceinline__ uint32_t group_max(uint32_t v) {

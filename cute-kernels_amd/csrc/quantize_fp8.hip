@@ -237,11 +237,11 @@ __device__ __forceinline__ float in_range(float v) {
 
 // Eight elements a lane, so that a store of a 16-bit type takes whole lines, four times per workgroup with all loads in front. row_shift: 0, or
 // 7 where 128 rows of a matrix of N rows share their scales. Index arithmetic in 32 bits (I32) where the sizes allow it: a 64-bit division costs more than the rest of the kernel.
-// [65536, 1408] bf16: 95 -> 53 us (5.2 TB/s).
+// [65536, 1408] bf16: 95 -> 53 us (5.2 TB/s). SHIFTED: 2^-shift[row] of every row.
 constexpr int kDequantizeUnroll = 4;
-template <typename T, bool I32>
+template <typename T, bool I32, bool SHIFTED>
 __global__ __launch_bounds__(kThreads) void dequantize_kernel(const uint8_t* __restrict__ values, const uint8_t* __restrict__ scales,
-                                                              T* __restrict__ out, int64_t total, uint32_t per_row, int64_t K,
+                                                              const uint8_t* __restrict__ shift, T* __restrict__ out, int64_t total, uint32_t per_row, int64_t K,
                                                               int64_t pitch, int64_t N, int64_t scale_rows, int row_shift) {
     typedef std::conditional_t<I32, uint32_t, int64_t> index;
     const int64_t first = (int64_t)blockIdx.x * (kDequantizeUnroll * kThreads) + threadIdx.x;
@@ -262,6 +262,7 @@ __global__ __launch_bounds__(kThreads) void dequantize_kernel(const uint8_t* __r
             at[i] = (int64_t)row * K + k;
             q[i] = *reinterpret_cast<const uint2*>(values + at[i]);
             scale[i] = scale_value(scales[(int64_t)s_row * pitch + k / kBlock]);
+            if constexpr (SHIFTED) scale[i] *= __uint_as_float((127u - shift[row]) << 23);
         }
     }
 #pragma unroll
@@ -349,10 +350,11 @@ int dequantize(const uint8_t* values, const uint8_t* scales, void* out, int64_t 
         const int64_t total = E * N * (K / 8), per = kDequantizeUnroll * kThreads;
         const dim3 grid((uint32_t)((total + per - 1) / per));
         auto run = [&](auto kernel) {
-            hipLaunchKernelGGL(kernel, grid, dim3(kThreads), 0, st, values, scales, (T*)out, total, (uint32_t)(K / 8), K, pitch, N, scale_rows, shift);
+            hipLaunchKernelGGL(kernel, grid, dim3(kThreads), 0, st, values, scales, nullptr, (T*)out, total, (uint32_t)(K / 8), K, pitch, N, scale_rows,
+                               shift);
         };
-        if (total + per < (1ll << 31)) run(dequantize_kernel<T, true>);
-        else run(dequantize_kernel<T, false>);
+        if (total + per < (1ll << 31)) run(dequantize_kernel<T, true, false>);
+        else run(dequantize_kernel<T, false, false>);
     } else {
         const int64_t total = E * N * K, blocks = (total + kThreads - 1) / kThreads;
         const dim3 grid((uint32_t)(blocks < (1 << 20) ? blocks : (1 << 20)));
@@ -376,6 +378,18 @@ int check_matrix(const char* who, int64_t E, int64_t N, int64_t K, int64_t block
 }
 
 }  // namespace
+
+int fp8::dequantize_shifted(const uint8_t* values, const uint8_t* scales, const uint8_t* shift, void* out, int64_t R, int64_t K, hipStream_t st) {
+    const int64_t total = R * (K / 8), per = kDequantizeUnroll * kThreads;
+    auto run = [&](auto kernel) {
+        hipLaunchKernelGGL(kernel, dim3((uint32_t)((total + per - 1) / per)), dim3(kThreads), 0, st, values, scales, shift, (f16_t*)out, total,
+                           (uint32_t)(K / 8), K, scale_pitch(K), R, R, 0);
+    };
+    if (total + per < (1ll << 31)) run(dequantize_kernel<f16_t, true, true>);
+    else run(dequantize_kernel<f16_t, false, true>);
+    return launch_status("dequantize_fp8");
+}
+
 }  // namespace fmahip
 
 extern "C" {

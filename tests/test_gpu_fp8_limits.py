@@ -6,9 +6,38 @@ import torch
 
 from fma import quantize_expert_weights, swiglu_experts_fp8
 from gpu_util import DEV
-from test_gpu_fp8_experts import _case, _oracle
+from oracle import fp8_oracle as O
+from test_gpu_fp8_experts import _case, _close, _oracle
 
 pytestmark = pytest.mark.gpu
+
+
+@pytest.mark.parametrize("T,k", [(40, 1), (300, 2)])
+def test_activations_past_float16s_range(T, k):
+    """up and gate of some 300 make activations of 90000, which the forward pass takes as they are (its sums are fp32), and so do the gradients"""
+    x, gates, ids, w1, w2, dy = _case(T, 128, 144, 3, k, torch.float16, seed=T)
+    I = 144
+    for column in (3, 140):  # (a column of each of the two blocks)
+        w1[:, column] *= 400
+        w1[:, I + column] *= 400
+        w2[:, :, column] *= 2.0**-10
+    dy = dy * 2.0**-8  # (the weight gradient's elements stay below 65504)
+    y, dx, dg, dw1, dw2 = _oracle(x, gates, ids, w1, w2, dy)
+    assert float(dw2.abs().max()) < 65504 and float(y.abs().max()) < 65504
+    h = O.seen(x) @ O.seen(w1[0, :I], 128).t(), O.seen(x) @ O.seen(w1[0, I:], 128).t()
+    assert float((h[0] * h[1] * torch.sigmoid(h[1])).abs().max()) > 2**17
+    leaves = [t.to(DEV).requires_grad_() for t in (x, gates, w1, w2)]
+    got = swiglu_experts_fp8(leaves[0], leaves[1], ids.to(DEV), *leaves[2:])
+    got.backward(dy.to(DEV))
+    _close(got, y, torch.float16, 1, "y")
+    wide = torch.zeros(I, dtype=torch.bool)
+    wide[[3, 140]] = True
+    both = wide.repeat(2)
+    for what, a, b, links in (("dx", leaves[0].grad, dx, 2), ("dgates", leaves[1].grad, dg, 1), ("dw1 wide", leaves[2].grad[:, both], dw1[:, both], 1),
+                              ("dw1", leaves[2].grad[:, ~both], dw1[:, ~both], 1), ("dw2 wide", leaves[3].grad[:, :, wide], dw2[:, :, wide], 1),
+                              ("dw2", leaves[3].grad[:, :, ~wide], dw2[:, :, ~wide], 1)):  # fmt: skip
+        assert bool(a.isfinite().all()), what
+        _close(a, b, torch.float16, links, what)
 
 
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
