@@ -760,7 +760,7 @@ __global__ __launch_bounds__(kGemmThreads) void fp8_gemm_kernel(const GemmArgs a
                 if (i + kAhead < kBlocks) kept[i % kAhead] = fetch(i + kAhead);
                 float d[2][2][8];  // [half][columns p][x]
                 uint32_t m[2] = {0u, 0u};
-                const float su = scale_value(k.s[0]), sg = scale_value(k.s[1]);
+                const float su = finite_scale_value(k.s[0]), sg = finite_scale_value(k.s[1]);
 #pragma unroll
                 for (int p = 0; p < 2; ++p) {
                     float u[8], g[8];

@@ -6,7 +6,7 @@
 //
 // A block with an infinity or a NaN has the scale byte 255 (NaN) and NaN values: e4m3 has no infinity, and a value that overflowed must
 // not come back as a number. Powers of two because the matrix instruction v_mfma_scale_f32_16x16x128_f8f6f4 applies them to its operands
-// at no cost, and because value * scale is then exact in bf16 and fp32 (in fp16 as far as its exponents reach).
+// at no cost, and because value * scale is then exact in bf16 and fp32 (in fp16 as far as its exponents reach; numbers of 248 * 2^120 and more round up to 2^128).
 //
 // A row of K elements has ceil(K / 128) scale bytes, filled up with 127 (one) to whole dwords: kernels fetch four at a time.
 #pragma once
@@ -36,6 +36,8 @@ __device__ __forceinline__ float scale_inverse(uint32_t byte) {
 __device__ __forceinline__ float scale_value(uint32_t byte) {
     return __uint_as_float(byte == 255u ? 0x7fc00000u : byte << 23);
 }
+// For arithmetic on the values: 2^128, the 8-bit form of the largest numbers, has to stay one, so a scale of 2^120 is one step less (2^-24 of it)
+__device__ __forceinline__ float finite_scale_value(uint32_t byte) { return byte == 247u ? __uint_as_float(0x7b7fffffu) : scale_value(byte); }
 __device__ __forceinline__ uint32_t magnitude_bits(float x) { return __float_as_uint(x) & 0x7fffffffu; }
 __device__ __forceinline__ uint32_t max_u32(uint32_t a, uint32_t b) { return a > b ? a : b; }
 

@@ -227,12 +227,13 @@ __global__ __launch_bounds__(kThreads) void quantize_blocks_generic_kernel(const
 
 // ---- back -----------------------------------------------------------------------------------------------------------
 
-// The float16 numbers from 63488 to 65504 become 65536 in 8 bits, which float16 would round to infinity: on the way back they are 65504,
-// 2^-11 away, so that a gradient made from finite tokens stays finite.
+// A type's largest numbers round up past its range in 8 bits: float16's from 63488 on to 65536, the others' from 248 * 2^120 on to 2^128, which
+// fp32 has as an infinity (no value times its scale is one otherwise, and a block with one is NaN). On the way back they are the type's
+// largest, so that a gradient made from finite tokens stays finite.
 template <typename T>
 __device__ __forceinline__ float in_range(float v) {
     if constexpr (std::is_same_v<T, f16_t>) return fabsf(v) == 65536.f ? copysignf(65504.f, v) : v;
-    else return v;
+    else return fabsf(v) == INFINITY ? copysignf(__uint_as_float(std::is_same_v<T, bf16_t> ? 0x7f7f0000u : 0x7f7fffffu), v) : v;
 }
 
 // Eight elements a lane, so that a store of a 16-bit type takes whole lines, four times per workgroup with all loads in front. row_shift: 0, or

@@ -126,8 +126,8 @@ __global__ __launch_bounds__(kThreads) void swiglu_fp8_bwd_kernel(const uint8_t*
             col[u] = (v - row[u] * vectors) * 8;
             qu[u] = *reinterpret_cast<const uint2*>(values + row[u] * 2 * I + col[u]);
             qg[u] = *reinterpret_cast<const uint2*>(values + row[u] * 2 * I + I + col[u]);
-            su[u] = scale_value(scales[row[u] * 2 * pitch + col[u] / kBlock]);
-            sg[u] = scale_value(scales[row[u] * 2 * pitch + pitch + col[u] / kBlock]);
+            su[u] = finite_scale_value(scales[row[u] * 2 * pitch + col[u] / kBlock]);
+            sg[u] = finite_scale_value(scales[row[u] * 2 * pitch + pitch + col[u] / kBlock]);
             load8(dy + row[u] * I + col[u], d[u]);
         }
     }
@@ -187,8 +187,8 @@ __global__ __launch_bounds__(kThreads) void swiglu_fp8_bwd_generic_kernel(const 
         float u[4], g[4], dg, du;
         unpack4(values[row * 2 * I + c], u);
         unpack4(values[row * 2 * I + I + c], g);
-        const float up = u[0] * scale_value(scales[row * 2 * pitch + c / kBlock]);
-        const float gate = g[0] * scale_value(scales[row * 2 * pitch + pitch + c / kBlock]);
+        const float up = u[0] * finite_scale_value(scales[row * 2 * pitch + c / kBlock]);
+        const float gate = g[0] * finite_scale_value(scales[row * 2 * pitch + pitch + c / kBlock]);
         swiglu_b<T>(gate, up, Num<T>::up(dy[i]), dg, du);
         dx[row * 2 * I + c] = Num<T>::down(du);
         dx[row * 2 * I + I + c] = Num<T>::down(dg);

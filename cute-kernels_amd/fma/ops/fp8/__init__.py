@@ -85,8 +85,8 @@ def block_rows_of(blocks: Fp8Blocks) -> int:
 
 
 def dequantize_fp8(blocks: Fp8Blocks, dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
-    """The numbers that the blocks stand for, rounded to dtype (exact in float32 and bfloat16; in float16 65536, to which its
-    largest numbers round in 8 bits, becomes 65504)."""
+    """The numbers that the blocks stand for, rounded to dtype: exact in float32 and bfloat16. What a dtype's largest numbers round up to in
+    8 bits, 65536 and 2^128 (numbers of 63488 and of 248 * 2^120 and more), becomes its largest number."""
     assert dtype in _FLOATS, f"dequantize_fp8 gives float32, float16 and bfloat16, not {dtype}"
     values, scales = (t.contiguous() for t in blocks)
     one_row = values.dim() == 1

@@ -448,8 +448,8 @@ int64_t fma_fp8_scale_pitch(int64_t K);
  * Any size and alignment; rows of multiples of 16 (8 with 128 x 128 blocks) elements, aligned, take the 16-byte kernels. */
 int fma_quantize_fp8(const void* x, void* values, void* scales, void* values_t, void* scales_t, int64_t E, int64_t N, int64_t K,
                      int64_t block_rows, int dtype, void* stream);
-/* out [E, N, K] = value * scale, rounded to dtype once (exact in fp32 and bf16; 65536, to which float16's largest numbers round in 8 bits,
- * becomes 65504 in FMA_F16). */
+/* out [E, N, K] = value * scale, rounded to dtype once: exact in fp32 and bf16. What a dtype's largest numbers round up to in 8 bits, 65536
+ * and 2^128 (numbers of 63488 and of 248 * 2^120 and more), becomes its largest number. */
 int fma_dequantize_fp8(const void* values, const void* scales, void* out, int64_t E, int64_t N, int64_t K, int64_t block_rows,
                        int dtype, void* stream);
 

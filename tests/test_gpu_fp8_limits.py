@@ -4,9 +4,10 @@ rows, weights laid out anew behind a captured graph, the sums that a few tokens'
 import pytest
 import torch
 
-from fma import quantize_expert_weights, swiglu_experts_fp8
+from fma import dequantize_fp8, grouped_linear_fp8, quantize_expert_weights, quantize_fp8, swiglu_experts_fp8, swiglu_packed_fp8
 from gpu_util import DEV
 from oracle import fp8_oracle as O
+from test_gpu_fp8 import _sizes
 from test_gpu_fp8_experts import _case, _close, _oracle
 
 pytestmark = pytest.mark.gpu
@@ -38,6 +39,64 @@ def test_activations_past_float16s_range(T, k):
                               ("dw2", leaves[3].grad[:, :, ~wide], dw2[:, :, ~wide], 1)):  # fmt: skip
         assert bool(a.isfinite().all()), what
         _close(a, b, torch.float16, links, what)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("K", [128, 130])
+def test_the_largest_numbers_stay_finite(dtype, K):
+    """248 * 2^120 and more is 2^128 in 8 bits, which no 16- or 32-bit number is: it comes back as the type's largest"""
+    most = torch.finfo(dtype).max
+    x = torch.tensor([most, -most, 248 * 2.0**120, 247 * 2.0**120, 240 * 2.0**120, -1.0]).to(dtype)[:, None].expand(6, K).contiguous()
+    blocks = quantize_fp8(x.to(DEV))
+    assert torch.equal(blocks.values[:3, 0].float().cpu(), torch.tensor([256.0, -256.0, 256.0]))  # (248: a tie, to the even one)
+    for rows in (1, 128):
+        back = dequantize_fp8(quantize_fp8(x.to(DEV), rows), dtype).cpu().double()
+        assert back.isfinite().all() and float(back[0, 0]) == most == -float(back[1, K - 1])
+        # half a step of e4m3, relative to the value
+        assert bool(((back - x.double()).abs()[:5] <= 2.0**-4 * x.double().abs()[:5]).all())
+        assert float(back[4, 0]) == 240 * 2.0**120
+    x[0, 0] = float("inf")
+    assert dequantize_fp8(quantize_fp8(x.to(DEV)), dtype)[0, :128].isnan().all()
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("I", [128, 130])
+def test_gradients_at_the_largest_numbers(dtype, I):
+    """a gate of 2^128 in 8 bits lets everything through, and so does its slope"""
+    most = torch.finfo(dtype).max
+    x = torch.zeros(2, 2 * I)
+    x[:, :I] = 2.0**-100  # up
+    x[0, I:], x[1, I:] = most, 1.0
+    leaf = x.to(dtype).to(DEV).requires_grad_()
+    y = swiglu_packed_fp8(leaf)
+    y.backward(torch.full_like(y, 0.5))
+    assert y.isfinite().all() and leaf.grad.isfinite().all()
+    # d up = gate / 2, within half a step of e4m3 and one of the type; d gate = up / 2
+    assert bool(((leaf.grad[0, :I].double().cpu() / (most / 2) - 1).abs() <= 2.0**-4 + torch.finfo(dtype).eps).all())
+    assert bool(((leaf.grad[0, I:].double().cpu() / 2.0**-101 - 1).abs() <= torch.finfo(dtype).eps).all())
+
+
+def test_an_experts_gradient_at_the_largest_pre_activation():
+    """a gate of 248 * 2^120, which is 2^128 where it is kept in 8 bits; every product on the way to the tokens' gradient is a power of two or exact"""
+    x, gates, ids = torch.full((3, 128), 2.0**100).bfloat16(), torch.ones(3, 1).bfloat16(), torch.zeros(3, 1, dtype=torch.int32)
+    w1 = torch.full((1, 256, 128), 2.0**-110)
+    w1[:, 128:, 0::2], w1[:, 128:, 1::2] = 1.875 * 2.0**20, 2.0**21
+    w1, w2, dy = w1.bfloat16(), torch.full((1, 128, 128), 2.0**-120).bfloat16(), torch.full((3, 128), 2.0**20).bfloat16()
+    leaf = x.to(DEV).requires_grad_()
+    y = swiglu_experts_fp8(leaf, gates.to(DEV), ids.to(DEV), w1.to(DEV), w2.to(DEV))
+    y.backward(dy.to(DEV))
+    assert bool((y == 128 * 32).all())  # (31 * 2^120 is 32 * 2^120 in 8 bits)
+    # d up = da gate = 2^-93 2^128, d gate = da up = 2^-93 2^-3; two roundings to the type, one step of the scale
+    exact = 128 * 2.0**35 * w1[0, 0].double() + 128 * 2.0**-96 * w1[0, 128].double()
+    assert bool(((leaf.grad.cpu().double() - exact).abs() <= exact * (torch.finfo(torch.bfloat16).eps + 2.0**-23)).all())
+
+
+def test_weight_gradient_of_the_largest_tokens():
+    most = torch.finfo(torch.bfloat16).max
+    tokens, w = torch.full((40, 128), most, device=DEV).bfloat16(), (1e-36 * torch.ones(1, 32, 128, device=DEV)).bfloat16().requires_grad_()
+    y = grouped_linear_fp8(tokens, w, _sizes([40]))
+    grad = torch.autograd.grad(y, w, torch.full_like(y, 2.0**-20))[0]
+    assert bool(((grad.double() / (40 * most * 2.0**-20) - 1).abs() <= 2.0**-8 + 40 * 2.0**-23).all())
 
 
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
