@@ -53,6 +53,7 @@ def _headers() -> list[str]:
 # the operands have landed. Their kernels must use no scratch memory; the build checks the compiler's resource report.
 NO_SCRATCH_SOURCES = {"grouped_gemm.hip": "grouped_gemm_kernel", "grouped_gemm_ragged.hip": "ragged_gemm_kernel",
                       "grouped_gemm_ragged_tall.hip": "ragged_gemm_kernel",
+                      "fp8_gemm.hip": "fp8_gemm_kernel",
                       "thin_experts.hip": "thin_gemm_kernel|one_token", "decode.hip": "router_logits_kernel", "router.hip": "router_logits"}
 
 

@@ -219,10 +219,10 @@ __global__ __launch_bounds__(kGemmThreads) void fp8_gemm_kernel(const GemmArgs a
 
     // ---- the load stream ----
     const uint32_t lr = lane >> 3, lp = lane & 7u;
-    const uint32_t a_chunk = (lp ^ (((wave * 8u + lr) >> 1) & 7u)) * 16u;
-    const uint32_t b_chunk = (lp ^ ((wave & 3u) * 2u + ((lr >> 1) & 1u))) * 16u;
-    const uint32_t a_lane = (wave * 8u + lr) * args.a_pitch + a_chunk;
-    const uint32_t b_lane = (wave * 8u + lr) * K + b_chunk;
+    uint32_t a_chunk = (lp ^ (((wave * 8u + lr) >> 1) & 7u)) * 16u;
+    uint32_t b_chunk = (lp ^ ((wave & 3u) * 2u + ((lr >> 1) & 1u))) * 16u;
+    uint32_t a_lane = (wave * 8u + lr) * args.a_pitch + a_chunk;
+    uint32_t b_lane = (wave * 8u + lr) * K + b_chunk;
     const uint32_t lds0 = lds_address(s_op);
     const uint32_t lds_x = lds_address(s_x);
     const uint32_t lds_scale = lds_address(reinterpret_cast<const uint8_t*>(s_scale)) + wave * 256u;
@@ -330,13 +330,13 @@ __global__ __launch_bounds__(kGemmThreads) void fp8_gemm_kernel(const GemmArgs a
 
     // ---- fragments ----
     const uint32_t a_key = (r16 >> 1) & 7u, b_key = (r16 >> 2) * 2u + ((r16 >> 1) & 1u);
-    const uint32_t a_off = (wm * 128u + r16) * kBlock + ((q ^ a_key) << 4);
+    uint32_t a_off = (wm * 128u + r16) * kBlock + ((q ^ a_key) << 4);
     const uint32_t b_base = kGlu ? wn * 32u : wn * 64u;
-    const uint32_t b_off = kOperandBytes + (b_base + (r16 >> 2) * 8u + (r16 & 3u)) * kBlock + ((q ^ b_key) << 4);
+    uint32_t b_off = kOperandBytes + (b_base + (r16 >> 2) * 8u + (r16 & 3u)) * kBlock + ((q ^ b_key) << 4);
     // bytes from fragment 0 of B to fragment j
     auto b_step = [](int j) -> uint32_t { return (uint32_t)((kGlu ? (j >> 1) * 128 : (j >> 1) * 32) + (j & 1) * 4) * kBlock; };
     const uint8_t* const sc = reinterpret_cast<const uint8_t*>(s_scale);
-    const uint32_t sa_off = (wm * 128u + r16) * 4u;
+    uint32_t sa_off = (wm * 128u + r16) * 4u;
     const uint32_t sb_off = (256u + (kGlu ? 0u : wn >> 1)) * 4u;
     uint32_t c_stage = 0, c_ks = 0, c_quad = 0;  // the step whose fragments are read
 
@@ -803,6 +803,20 @@ __global__ __launch_bounds__(kGemmThreads) void fp8_gemm_kernel(const GemmArgs a
                 __builtin_amdgcn_sched_barrier(0);
             }
         }
+        }
+        if constexpr (kBwd) {
+            // What the loads and fragments take from the lane, formed anew: kept over this epilogue these registers were spilled, and their reloads
+            // waited for the whole load stream in every K step (64 x 1024 rows, 1408 x 2048: 476 -> 425 us).
+            asm volatile("" : "+v"(here));
+            const uint32_t lr = here >> 3, lp = here & 7u, r16 = here & 15u, q = here >> 4;
+            const uint32_t a_key = (r16 >> 1) & 7u, b_key = (r16 >> 2) * 2u + ((r16 >> 1) & 1u);
+            a_chunk = (lp ^ (((wave * 8u + lr) >> 1) & 7u)) * 16u;
+            b_chunk = (lp ^ ((wave & 3u) * 2u + ((lr >> 1) & 1u))) * 16u;
+            a_lane = (wave * 8u + lr) * args.a_pitch + a_chunk;
+            b_lane = (wave * 8u + lr) * K + b_chunk;
+            a_off = (wm * 128u + r16) * kBlock + ((q ^ a_key) << 4);
+            b_off = kOperandBytes + (b_base + (r16 >> 2) * 8u + (r16 & 3u)) * kBlock + ((q ^ b_key) << 4);
+            sa_off = (wm * 128u + r16) * 4u;
         }
         // The next tile's first fragments once more: 42 registers that these epilogues use meanwhile.
         if constexpr (kGlu || kBwd) first_fragments();

@@ -25,6 +25,10 @@ for every instantiation of ragged_gemm_kernel, that the instruction stream has t
    hardware wants in scalar registers (what the compiler generates around a vector-memory instruction whose descriptor or
    scalar offset it cannot prove to be the same in every lane: each costs a dozen instructions and a branch per use).
 
+The kernels of csrc/fp8_gemm.h count the same way: a K step waits for all but the four loads behind its first barrier, in a tile's first step also
+for all but the stores that an epilogue issues whatever its tile is. Checked are those waits, that there are that many such stores, and that there is no
+scratch access.
+
 For these kernels and those of csrc/grouped_gemm.hip it checks as well that a wavefront reaches every barrier with all of its LDS
 reads returned. Behind a barrier the other wavefronts' loads may fill the stage that was read, and the compiler is free to move a matrix
 instruction, and with it the wait for its fragments, past the barrier: only a wait of its own in front of the barrier keeps the reads there.
@@ -225,6 +229,49 @@ def reads_out_at_barriers(body):
     return len(flagged)
 
 
+# the 8-bit product's epilogues: stores that the first step's wait allows for, and the instruction that makes them (None: fewer are waited for
+# than the counter holds, or all)
+FP8_STORES = {0: (16, "buffer_store_dwordx4"), 1: (16, "buffer_store_dwordx4"), 2: (0, None), 3: (8, "buffer_store_dwordx2"),
+              4: (24, "buffer_store_dwordx2"), 5: (59, None), 6: (59, None)}  # fmt: skip
+FP8_KERNEL = r"_ZN6fmahip3fp815fp8_gemm_kernel"
+FP8_STEP = re.compile(r"\|(O+)(?:w\d+,)*w(\d+),\|(?:w\d+,)*(O*)")
+
+
+def audit_fp8_kernel(name: str, body) -> list:
+    """The problems of one instantiation of fp8_gemm_kernel."""
+    epi, tall = (int(x) for x in re.search(r"fp8_gemm_kernelILi(\d)ELb(\d)E", name).groups())
+    blocks, _ = tokens(body)
+    stores, kind = FP8_STORES[epi]
+    problems = []
+    if any("X" in b for b in blocks):
+        problems.append("scratch access")
+    # (a block may end between a barrier and the loads: blocks without a barrier of their own are put together)
+    steps = FP8_STEP.findall("".join(blocks))
+    waits = sorted(int(w) for _, w, _ in steps)
+    if waits != sorted((4, min(4 + stores, 63))):
+        problems.append(f"steps wait for all but {waits}, expected {sorted((4, min(4 + stores, 63)))}")
+    for first, _, second in steps:
+        if len(first) != 4 or len(second) not in (4, 4 + tall):
+            problems.append(f"{len(first)} and {len(second)} operand loads in a step, expected 4 and 4 (a fifth in a tall tile)")
+    made = sum(line.strip().startswith(kind or "buffer_store") for line in body)
+    if kind and made != stores * (8 + tall) // 8 or made < (stores if kind is None else 0):
+        problems.append(f"{made} stores, the first step's wait allows for {stores}")
+    if reads_out_at_barriers([line.strip() for line in body]):
+        problems.append("barriers with LDS reads outstanding")
+    return [f"fp8 epilogue={epi} tall={tall}: {p}" for p in problems]
+
+
+def audit_fp8(asm_path: str) -> int:
+    problems, seen = [], 0
+    for name, body in kernels(asm_path, FP8_KERNEL):
+        seen += 1
+        problems += audit_fp8_kernel(name, body)
+    for p in problems:
+        print("PROBLEM " + p)
+    print(f"{os.path.basename(asm_path)}: waits and stores of {seen} kernels of 8-bit products, {len(problems)} problems")
+    return len(problems)
+
+
 def audit_barriers(asm_path: str) -> int:
     """Every grouped-GEMM kernel of a listing: no barrier with LDS reads outstanding."""
     problems, seen = 0, 0
@@ -261,6 +308,9 @@ def main() -> int:
         path = os.path.join(tmp, "grouped_gemm.hip.s")
         compile_to_assembly(os.path.join(CSRC, "grouped_gemm.hip"), path)
         problems += audit_barriers(path)
+        path = os.path.join(tmp, "fp8_gemm.hip.s")
+        compile_to_assembly(os.path.join(CSRC, "fp8_gemm.hip"), path)
+        problems += audit_fp8(path)
         path = os.path.join(tmp, "f32.s")
         compile_to_assembly(os.path.join(CSRC, "grouped_gemm_f32.hip"), path)
         problems += audit_f32(path)
