@@ -15,7 +15,7 @@ from torch.autograd import forward_ad
 
 from ...kernel_backend import KernelBackend, is_hip_kernel_backend
 from ...ops.swiglu import swiglu_packed
-from .fp8_implementation import quantize_expert_weights, swiglu_experts_fp8
+from .fp8_implementation import quantize_expert_weights, requantize_expert_weights, swiglu_experts_fp8
 from .cuda_implementation import (
     add_expert_bias,
     build_routing_index,
@@ -374,13 +374,19 @@ class MoE(nn.Module):
         """Switches the experts' products to 8 bits (fp8_experts) and lays both projections out in 8 bits once, for calls that no backward
         pass follows: a serving program calls it after loading the weights, and again after changing them. A forward pass on weights that
         have changed since, as far as their version counters tell, quantises them in the call, as one without this call does; changes that
-        no counter sees (through .data, or by a replayed graph) need the call again. A compiled layer quantises in the call."""
+        no counter sees (through .data, or by a replayed graph) need the call again. A compiled layer quantises in the call. Called again, it
+        writes to the same memory, so that a graph captured before serves the new weights (unless they are on another device since)."""
         if any(t.is_inference() for t in (self.c_fc.weight, self.c_proj.weight)):
             raise ValueError("quantize_experts: parameters that were made in inference mode do not tell when they change")
         self._check_fp8_experts(self.c_fc.weight.dtype)
+        with torch.inference_mode(False), torch.no_grad():  # (a later call writes to what is made here, in whatever mode)
+            weights, blocks = (self.c_fc.weight, self.c_proj.weight), self._fp8_weights and self._fp8_weights[1]
+            if blocks and all(b.values.device == w.device for b, w in zip(blocks, weights)):
+                requantize_expert_weights(*weights, *blocks)
+            else:
+                blocks = quantize_expert_weights(*weights)
+            self._fp8_weights = (self._weight_versions(), blocks)
         self.fp8_experts = True
-        with torch.no_grad():
-            self._fp8_weights = (self._weight_versions(), quantize_expert_weights(self.c_fc.weight, self.c_proj.weight))
         return self
 
     def _weight_versions(self) -> tuple:

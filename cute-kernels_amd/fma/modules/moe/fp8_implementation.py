@@ -6,7 +6,7 @@ from torch.autograd import forward_ad
 from ... import _lib
 from ..._ops import hip_op
 from ...ops.fp8 import BLOCK_SIZE, Fp8Blocks, quantize_fp8
-from ...ops.fp8.cuda_implementation import is_scales_dtype, operator_scales
+from ...ops.fp8.cuda_implementation import is_scales_dtype, operator_scales, quantize_fp8_cuda
 from ...utils import ensure_contiguous
 
 
@@ -100,6 +100,12 @@ def quantize_expert_weights(
         quantize_fp8(weight1.reshape(E, 2, two_I // 2, H), BLOCK_SIZE, transposed),
         quantize_fp8(weight2, BLOCK_SIZE, transposed),
     )
+
+
+def requantize_expert_weights(weight1: torch.Tensor, weight2: torch.Tensor, blocks1: Fp8Blocks, blocks2: Fp8Blocks) -> None:
+    """quantize_expert_weights into the blocks that it has given for weights of the same shapes"""
+    for weight, blocks in ((weight1, blocks1), (weight2, blocks2)):
+        quantize_fp8_cuda(weight.detach().contiguous().view(blocks.values.shape), *blocks, None, None, BLOCK_SIZE)
 
 
 class _SwigluExpertsFp8(torch.autograd.Function):

@@ -4,7 +4,10 @@ rows, weights laid out anew behind a captured graph, the sums that a few tokens'
 import pytest
 import torch
 
-from fma import dequantize_fp8, grouped_linear_fp8, quantize_expert_weights, quantize_fp8, swiglu_experts_fp8, swiglu_packed_fp8
+from fma import (
+    KernelBackend, MoE, dequantize_fp8, grouped_linear_fp8, quantize_expert_weights, quantize_fp8,
+    swiglu_experts_fp8, swiglu_packed, swiglu_packed_fp8,
+)  # fmt: skip
 from gpu_util import DEV
 from oracle import fp8_oracle as O
 from test_gpu_fp8 import _sizes
@@ -97,6 +100,52 @@ def test_weight_gradient_of_the_largest_tokens():
     y = grouped_linear_fp8(tokens, w, _sizes([40]))
     grad = torch.autograd.grad(y, w, torch.full_like(y, 2.0**-20))[0]
     assert bool(((grad.double() / (40 * most * 2.0**-20) - 1).abs() <= 2.0**-8 + 40 * 2.0**-23).all())
+
+
+def test_a_layer_laid_out_anew_behind_a_captured_graph():
+    """quantize_experts() after a change of the weights: a graph captured before it serves the new ones"""
+    torch.manual_seed(0)
+    moe = MoE(8, 2, 128, 144, swiglu_packed, True, False, 0.05).to(torch.bfloat16).to(DEV)
+    moe.quantize_experts()
+    x = torch.randn(12, 128, device=DEV).bfloat16()
+
+    def run():
+        return moe(x, kernel_backend=KernelBackend.cuda)[0]
+
+    with torch.no_grad():
+        side = torch.cuda.Stream()
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side):
+            run()
+        torch.cuda.current_stream().wait_stream(side)
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            captured = run()
+        first = run().clone()
+        for seed in range(3):
+            moe.c_fc.weight.copy_(0.1 * torch.randn(moe.c_fc.weight.shape, generator=torch.Generator().manual_seed(seed)))
+            moe.c_proj.weight.mul_(1.5)
+            before = [t.data_ptr() for b in moe._fp8_weights[1] for t in b]
+            if seed == 1:
+                with torch.inference_mode():  # (serving programs call it there too)
+                    moe.quantize_experts()
+            else:
+                moe.quantize_experts()
+            assert [t.data_ptr() for b in moe._fp8_weights[1] for t in b] == before
+            graph.replay()
+            torch.cuda.synchronize()
+            want = run()
+            assert torch.equal(captured, want) and not torch.equal(captured, first)
+            junk = [torch.full_like(t.view(torch.uint8), 0x7E) for b in moe._fp8_weights[1] for t in b]  # (whatever was freed is overwritten)
+            torch.randn(1 << 20, device=DEV).sum().item()
+            del junk
+        # a copy has blocks of its own
+        import copy
+
+        other = copy.deepcopy(moe).quantize_experts()
+        other.c_proj.weight.mul_(2)
+        other.quantize_experts()
+        assert torch.equal(run(), want)
 
 
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
