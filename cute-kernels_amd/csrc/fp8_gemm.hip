@@ -3,6 +3,12 @@
 #include "fp8_thin.h"
 
 namespace fmahip {
+namespace gemm {
+// grouped_gemm_ragged.hip
+int weight_gradient(const void* dy, const void* x, void* dW, const uint32_t* sizes, int64_t rows, int64_t E, int64_t M, int64_t N, int dtype,
+                    hipStream_t st);
+}  // namespace gemm
+
 namespace fp8 {
 
 int check_gemm(const char* who, int64_t E, int64_t R, int64_t N, int64_t K, int64_t segs) {
@@ -122,7 +128,7 @@ int fma_grouped_linear_fp8_bwd(const void* dy, const void* x_values, const void*
     }
     if (dW) {
         if (const int rc = fma_dequantize_fp8(x_values, x_scales, x16, 1, R, K, 1, dtype, stream)) return rc;
-        return fma_grouped_gemm_ragged(dy, x16, dW, M_arr, nullptr, E, /*FMA_VARY_K*/ 1, N, K, 0, 1, 0, 1.0f, dtype, stream);
+        return gemm::weight_gradient(dy, x16, dW, M_arr, R, E, N, K, dtype, (hipStream_t)stream);
     }
     return FMA_OK;
 }

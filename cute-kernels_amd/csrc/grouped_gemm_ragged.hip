@@ -139,6 +139,24 @@ int launch_ragged_from_arrays(const void* A, const void* B, void* D, const uint3
                              : ragged::launch_plain<ElemF16, true>(args, a_kc, b_kc, st);
 }
 
+// dW_e[M, N] = dy_e^T x_e of `rows` packed rows, to which the sizes are cut: fma_grouped_gemm_ragged (reduction varies, trans_a = 1, trans_b = 0) for
+// callers that cannot answer for sizes in device memory. M and N multiples of eight below 2^23, rows below 2^31; pointers aligned to 16 bytes.
+int weight_gradient(const void* dy, const void* x, void* dW, const uint32_t* sizes, int64_t rows, int64_t E, int64_t M, int64_t N, int dtype,
+                    hipStream_t st) {
+    ragged::Args args{};
+    args.A = (const uint16_t*)dy;
+    args.B = (const uint16_t*)x;
+    args.D = (uint16_t*)dW;
+    args.sizes = sizes;
+    args.E = (uint32_t)E;
+    args.m = (uint32_t)M;
+    args.n = (uint32_t)N;
+    args.alpha = 1.0f;
+    args.k_rows = (uint32_t)rows;
+    return dtype == FMA_BF16 ? ragged::launch_plain<ElemBf16, true>(args, false, false, st)
+                             : ragged::launch_plain<ElemF16, true>(args, false, false, st);
+}
+
 }  // namespace gemm
 }  // namespace fmahip
 

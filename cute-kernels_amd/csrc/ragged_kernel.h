@@ -117,6 +117,8 @@ struct Args {
     // last part can end inside a step or on an odd one); part s of packed row r goes to partial[(s * rows + r) * n ..]
     float* partial;
     uint32_t splits, split_steps, rows;
+    // reduction varies: the reduction rows that there are (below 2^31), to which the sizes are cut; 0: as many as the sizes say
+    uint32_t k_rows;
     // not NULL: the kernel runs only if *taken, which it decides (takes_many_passes) and writes first if pass_bits is not 0;
     // otherwise the streaming kernel behind it computes the product (thin_experts.hip)
     uint32_t* taken;
@@ -360,13 +362,26 @@ __global__ __launch_bounds__(NT) void ragged_gemm_kernel(const Args args) {
                 t = tiles_of(group_m(s_order[e]));  // the group at position e of the tile sequence
             }
             const uint32_t it = wave_inclusive_scan<uint32_t>(t);
-            const uint32_t is = wave_inclusive_scan<uint32_t>(sz);
-            if (e < E) {
-                s_tile_start[e] = carry_t + it - t;
-                s_prefix[e] = carry_s + is - sz;
+            if (VARY_K && args.k_rows) {
+                // (sums that stop at the rows: no two values below 2^31 overflow)
+                const uint32_t most = args.k_rows;
+                sz = sz < most ? sz : most;
+#pragma unroll
+                for (int d = 1; d < 64; d <<= 1) {
+                    const uint32_t below = __shfl_up(sz, d, 64);
+                    if (lane >= (uint32_t)d) sz = sz + below < most ? sz + below : most;
+                }
+                const uint32_t below = __shfl_up(sz, 1, 64), before = lane ? below : 0u;
+                if (e < E) s_prefix[e] = carry_s + before < most ? carry_s + before : most;
+                const uint32_t all = carry_s + __shfl(sz, 63, 64);
+                carry_s = all < most ? all : most;
+            } else {
+                const uint32_t is = wave_inclusive_scan<uint32_t>(sz);
+                if (e < E) s_prefix[e] = carry_s + is - sz;
+                carry_s += __shfl(is, 63, 64);
             }
+            if (e < E) s_tile_start[e] = carry_t + it - t;
             carry_t += __shfl(it, 63, 64);
-            carry_s += __shfl(is, 63, 64);
         }
         if (lane == 0) {
             s_tile_start[E] = carry_t;
@@ -455,6 +470,10 @@ __global__ __launch_bounds__(NT) void ragged_gemm_kernel(const Args args) {
         t.e = e;
         t.Me = group_m(e);
         t.Ke = group_k(e);
+        if (VARY_K && args.k_rows) {
+            const uint32_t left = args.k_rows - uniform(s_prefix[e]);
+            t.Ke = t.Ke < left ? t.Ke : left;
+        }
         const uint32_t tiles_m = row_tiles(t.Me);
         const uint32_t tile_n = (kCanNarrow && narrow && t.Me <= 64u) ? kTileN / 2 : kTileN;
         const uint32_t tiles_n = (n_span + tile_n - 1) / tile_n;

@@ -170,7 +170,8 @@ class _GroupedLinearFp8(torch.autograd.Function):
 
 def grouped_linear_fp8(x: torch.Tensor, weight: torch.Tensor, M_array: torch.Tensor) -> torch.Tensor:
     """y_e = x_e W_e^T for every group e with the product in 8 bits, from 16-bit tensors: x [R, K], rows of the groups back to back, weight
-    [E, N, K], M_array uint32 [E] on the device, summing to R. x is quantised in blocks of 128 along its rows, the weight in 128 x 128 blocks.
+    [E, N, K], M_array uint32 [E] on the device, summing to R (rows past the last group are not written, of the gradient neither; sizes past R
+    are cut to it). x is quantised in blocks of 128 along its rows, the weight in 128 x 128 blocks.
 
     The gradient of x is the 8-bit product of output_grad, quantised along its rows, with the quantised weight; the gradient of the weight
     the 16-bit product of output_grad with the quantised x, which is all of x that is kept. K and N must be multiples of 16."""

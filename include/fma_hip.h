@@ -463,7 +463,8 @@ int fma_grouped_gemm_fp8(const void* A, const void* A_scales, const void* B, con
 /* The product of 16-bit tensors, quantised on the way: y_e = q(x_e) q(W_e)^T, x [R, K], W [E, N, K], y [R, N] of dtype (FMA_BF16 or
  * FMA_F16); x_values and W_values with their scales are written, Wt_values (the transposed copy, for dx) unless it is NULL.
  * Backward: dx = q(dy_e) q(W_e) [R, K] and dW_e = dy_e^T x^_e [E, N, K], x^ the stored values, the second product in 16 bits; each is
- * computed unless NULL. N % 16 == K % 16 == 0 there; R > 0 (dW is not written without rows). */
+ * computed unless NULL. N % 16 == K % 16 == 0 there; R > 0 (dW is not written without rows). As for fma_grouped_gemm_fp8, rows past
+ * the last group (of y and dx) are not written, and rows past R do not exist whatever M_arr says. */
 int fma_grouped_linear_fp8(const void* x, const void* W, void* x_values, void* x_scales, void* W_values, void* W_scales, void* Wt_values,
                            void* Wt_scales, void* y, const uint32_t* M_arr, int64_t E, int64_t R, int64_t N, int64_t K, int dtype,
                            void* stream);

@@ -102,6 +102,25 @@ def test_weight_gradient_of_the_largest_tokens():
     assert bool(((grad.double() / (40 * most * 2.0**-20) - 1).abs() <= 2.0**-8 + 40 * 2.0**-23).all())
 
 
+@pytest.mark.parametrize("counts,clamped", [([30, 4000], [30, 42]), ([2**31 - 1, 2**31 - 1], [72, 0]), ([-1, -1, 5], [72, 0, 0]), ([20, 10, 0], [20, 10, 0]),
+                                            ([72] + [-1] * 200, [72] + [0] * 200)])  # fmt: skip
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+def test_gradients_of_sizes_that_do_not_fit_the_rows(dtype, counts, clamped):
+    """rows past the last one do not exist, whatever the sizes say: output and gradients are those of the sizes cut to the rows"""
+    R, N, K, E = 72, 48, 64, len(counts)
+    g = torch.Generator().manual_seed(E)
+    x, w, dy = (torch.randn(*s, generator=g).to(dtype).to(DEV) for s in ((R, K), (E, N, K), (R, N)))
+    rows = sum(clamped)
+    results = []
+    for sizes in (counts, clamped):
+        a, b = x.detach().requires_grad_(), w.detach().requires_grad_()
+        y = grouped_linear_fp8(a, b, _sizes(sizes))
+        x_grad, w_grad = torch.autograd.grad(y, (a, b), dy)
+        results.append((y[:rows], x_grad[:rows], w_grad))
+    for a, b in zip(*results):
+        assert torch.equal(a, b)
+
+
 def test_a_layer_laid_out_anew_behind_a_captured_graph():
     """quantize_experts() after a change of the weights: a graph captured before it serves the new ones"""
     torch.manual_seed(0)
