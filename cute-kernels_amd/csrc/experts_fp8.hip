@@ -252,6 +252,9 @@ int check_shape(const char* who, const Shape& s, int dtype) {
     FMA_REQUIRE(s.k <= 65536 && s.T <= ((1ll << 31) - 1) / s.k, FMA_ERR_TOO_MANY_ELEMENTS, "%s: more than 2^31 - 1 (token, choice) slots", who);
     FMA_REQUIRE(s.I < (1 << 20) && s.H < (1 << 21) && s.T * s.H < (1ll << 30), FMA_ERR_TOO_MANY_ELEMENTS,
                 "%s: I < 2^20, H < 2^21, T * H < 2^30", who);
+    // (launches of one workgroup per token, of one per four slots, of a thread per 32 elements of the activation)
+    FMA_REQUIRE(s.T <= kMostWorkgroups && (s.R + 3) / 4 <= kMostWorkgroups && s.R < (1ll << 37) / s.I, FMA_ERR_TOO_MANY_ELEMENTS,
+                "%s: T < 2^24, T * top_k < 2^26 - 3, T * top_k * I < 2^37", who);
     if (const int rc = check_gemm(who, s.E, s.R, s.I, s.H, 2)) return rc;
     return check_gemm(who, s.E, s.R, s.H, s.I, 2);
 }

@@ -18,6 +18,8 @@ namespace fp8 {
 
 constexpr int kBlock = 128;
 
+constexpr int64_t kMostWorkgroups = (1 << 24) - 1;  // of 256 threads: a launch has fewer than 2^32 threads
+
 __host__ __device__ constexpr int64_t scale_pitch(int64_t K) { return (K + 511) / 512 * 4; }
 
 typedef __attribute__((ext_vector_type(2))) float f32x2;

@@ -310,13 +310,13 @@ __global__ __launch_bounds__(kThreads) void dequantize_generic_kernel(const uint
 template <typename T>
 int quantize_rows(const void* x, uint8_t* values, uint8_t* scales, int64_t R, int64_t K, hipStream_t st) {
     const int64_t pitch = scale_pitch(K);
-    const bool vec = K % 16 == 0 && aligned16(x) && aligned16(values) && (reinterpret_cast<uintptr_t>(scales) & 3u) == 0;
+    constexpr int kUnroll = sizeof(T) == 4 ? 1 : 2;
+    const int64_t units = R * (pitch / 4), per = (int64_t)kUnroll * (kThreads / 32), grid = (units + per - 1) / per;
+    // (2^27 and more short rows take the kernel whose workgroups make several turns)
+    const bool vec = K % 16 == 0 && aligned16(x) && aligned16(values) && (reinterpret_cast<uintptr_t>(scales) & 3u) == 0 && grid <= kMostWorkgroups;
     if (vec) {
-        constexpr int kUnroll = sizeof(T) == 4 ? 1 : 2;
-        const int64_t total = R * (pitch / 4), per = (int64_t)kUnroll * (kThreads / 32);
-        const dim3 grid((uint32_t)((total + per - 1) / per));
-        hipLaunchKernelGGL((quantize_rows_kernel<T, kUnroll>), grid, dim3(kThreads), 0, st, (const T*)x, values, (uint32_t*)scales, total,
-                           (uint32_t)(pitch / 4), K);
+        hipLaunchKernelGGL((quantize_rows_kernel<T, kUnroll>), dim3((uint32_t)grid), dim3(kThreads), 0, st, (const T*)x, values, (uint32_t*)scales,
+                           units, (uint32_t)(pitch / 4), K);
     } else {
         const int64_t total = R * pitch, blocks = (total + kThreads / 8 - 1) / (kThreads / 8);
         const dim3 grid((uint32_t)(blocks < (1 << 16) ? blocks : (1 << 16)));
@@ -347,9 +347,10 @@ int dequantize(const uint8_t* values, const uint8_t* scales, void* out, int64_t 
                hipStream_t st) {
     const int64_t pitch = scale_pitch(K), scale_rows = (N + block_rows - 1) / block_rows;
     const int shift = block_rows == 1 ? 0 : 7;
-    if (K % 8 == 0 && (reinterpret_cast<uintptr_t>(values) & 7u) == 0 && aligned16(out)) {
-        const int64_t total = E * N * (K / 8), per = kDequantizeUnroll * kThreads;
-        const dim3 grid((uint32_t)((total + per - 1) / per));
+    constexpr int64_t per = kDequantizeUnroll * kThreads;
+    const int64_t total = E * N * (K / 8), workgroups = (total + per - 1) / per;
+    if (K % 8 == 0 && (reinterpret_cast<uintptr_t>(values) & 7u) == 0 && aligned16(out) && workgroups <= kMostWorkgroups) {
+        const dim3 grid((uint32_t)workgroups);
         auto run = [&](auto kernel) {
             hipLaunchKernelGGL(kernel, grid, dim3(kThreads), 0, st, values, scales, nullptr, (T*)out, total, (uint32_t)(K / 8), K, pitch, N, scale_rows,
                                shift);
@@ -357,9 +358,9 @@ int dequantize(const uint8_t* values, const uint8_t* scales, void* out, int64_t 
         if (total + per < (1ll << 31)) run(dequantize_kernel<T, true, false>);
         else run(dequantize_kernel<T, false, false>);
     } else {
-        const int64_t total = E * N * K, blocks = (total + kThreads - 1) / kThreads;
+        const int64_t elements = E * N * K, blocks = (elements + kThreads - 1) / kThreads;
         const dim3 grid((uint32_t)(blocks < (1 << 20) ? blocks : (1 << 20)));
-        hipLaunchKernelGGL(dequantize_generic_kernel<T>, grid, dim3(kThreads), 0, st, values, scales, (T*)out, total, K, pitch, N, scale_rows,
+        hipLaunchKernelGGL(dequantize_generic_kernel<T>, grid, dim3(kThreads), 0, st, values, scales, (T*)out, elements, K, pitch, N, scale_rows,
                            shift);
     }
     return launch_status("dequantize_fp8");
@@ -369,12 +370,12 @@ int check_matrix(const char* who, int64_t E, int64_t N, int64_t K, int64_t block
     FMA_REQUIRE(dtype_bytes(dtype) != 0, FMA_ERR_BAD_DTYPE, "%s: dtype code %d", who, dtype);
     FMA_REQUIRE(E >= 0 && N >= 0 && K >= 1, FMA_ERR_BAD_SIZE, "%s: bad size E=%lld N=%lld K=%lld", who, (long long)E, (long long)N, (long long)K);
     FMA_REQUIRE(block_rows == 1 || block_rows == kBlock, FMA_ERR_BAD_SIZE, "%s: blocks have 1 or 128 rows, not %lld", who, (long long)block_rows);
-    // (64-bit offsets in the kernels; what is limited is the number of workgroups and K / 16)
+    // (64-bit offsets in the kernels; what is limited is K / 16 and the number of units of 512 elements)
     FMA_REQUIRE(K <= (1ll << 31) && N <= (1ll << 40) && E <= (1ll << 31), FMA_ERR_TOO_MANY_ELEMENTS, "%s: K <= 2^31", who);
     const int64_t units = block_rows == 1 ? (K + 511) / 512 : (K + 127) / 128;
     const int64_t rows = block_rows == 1 ? N : (N + 127) / 128;
     FMA_REQUIRE(E == 0 || rows == 0 || units * rows <= ((1ll << 31) - 1) / E, FMA_ERR_TOO_MANY_ELEMENTS,
-                "%s: more than 2^31 - 1 blocks", who);
+                "%s: more than 2^31 - 1 pieces of 512 elements of a row, or blocks of 128 x 128", who);
     return FMA_OK;
 }
 
@@ -404,6 +405,8 @@ int fma_quantize_fp8(const void* x, void* values, void* scales, void* values_t, 
     FMA_REQUIRE(!values_t == !scales_t, FMA_ERR_NULL_POINTER, "quantize_fp8: the transposed copy takes values and scales");
     FMA_REQUIRE(!values_t || block_rows == 128, FMA_ERR_UNSUPPORTED, "quantize_fp8: a transposed copy exists of 128 x 128 blocks only");
     if (E == 0 || N == 0) return FMA_OK;
+    FMA_REQUIRE(block_rows == 1 || E * ((N + 127) / 128) * ((K + 127) / 128) <= kMostWorkgroups, FMA_ERR_TOO_MANY_ELEMENTS,
+                "quantize_fp8: more than 2^24 - 1 blocks of 128 x 128");
     FMA_REQUIRE(x && values && scales, FMA_ERR_NULL_POINTER, "quantize_fp8: x, values or scales is NULL");
     FMA_REQUIRE((reinterpret_cast<uintptr_t>(x) & (uintptr_t)(dtype_bytes(dtype) - 1)) == 0, FMA_ERR_MISALIGNED, "quantize_fp8: x is not aligned to its elements");
     hipStream_t st = (hipStream_t)stream;

@@ -198,11 +198,13 @@ __global__ __launch_bounds__(kThreads) void swiglu_fp8_bwd_generic_kernel(const 
 template <typename T>
 int forward(const void* x, void* y, uint8_t* values, uint8_t* scales, int64_t R, int64_t I, hipStream_t st) {
     const int64_t pitch = scale_pitch(I);
-    if (I % 8 == 0 && aligned16(x) && aligned16(y) && (reinterpret_cast<uintptr_t>(values) & 7u) == 0 && (reinterpret_cast<uintptr_t>(scales) & 3u) == 0) {
-        constexpr int kUnroll = sizeof(T) == 4 ? 1 : 2;
-        const int64_t total = R * (pitch / 4), per = kUnroll * (kThreads / 64);
-        hipLaunchKernelGGL((swiglu_fp8_fwd_kernel<T, kUnroll>), dim3((uint32_t)((total + per - 1) / per)), dim3(kThreads), 0, st, (const T*)x, (T*)y,
-                           values, (uint32_t*)scales, total, (uint32_t)(pitch / 4), I);
+    constexpr int kUnroll = sizeof(T) == 4 ? 1 : 2;
+    const int64_t units = R * (pitch / 4), per = kUnroll * (kThreads / 64), grid = (units + per - 1) / per;
+    // (2^26 and more short rows take the kernel whose workgroups make several turns)
+    if (I % 8 == 0 && aligned16(x) && aligned16(y) && (reinterpret_cast<uintptr_t>(values) & 7u) == 0 && (reinterpret_cast<uintptr_t>(scales) & 3u) == 0 &&
+        grid <= kMostWorkgroups) {
+        hipLaunchKernelGGL((swiglu_fp8_fwd_kernel<T, kUnroll>), dim3((uint32_t)grid), dim3(kThreads), 0, st, (const T*)x, (T*)y, values,
+                           (uint32_t*)scales, units, (uint32_t)(pitch / 4), I);
     } else {
         const int64_t total = R * pitch, blocks = (total + kThreads / 8 - 1) / (kThreads / 8);
         hipLaunchKernelGGL(swiglu_fp8_fwd_generic_kernel<T>, dim3((uint32_t)(blocks < (1 << 16) ? blocks : (1 << 16))), dim3(kThreads), 0, st,
@@ -214,11 +216,11 @@ int forward(const void* x, void* y, uint8_t* values, uint8_t* scales, int64_t R,
 template <typename T>
 int backward(const uint8_t* values, const uint8_t* scales, const void* dy, void* dx, int64_t R, int64_t I, hipStream_t st) {
     const int64_t pitch = scale_pitch(I);
-    if (I % 8 == 0 && aligned16(dy) && aligned16(dx) && (reinterpret_cast<uintptr_t>(values) & 7u) == 0) {
-        constexpr int kUnroll = sizeof(T) == 4 ? 1 : 2;
-        const int64_t total = R * (I / 8), per = kUnroll * kThreads;
-        hipLaunchKernelGGL((swiglu_fp8_bwd_kernel<T, kUnroll>), dim3((uint32_t)((total + per - 1) / per)), dim3(kThreads), 0, st, values, scales,
-                           (const T*)dy, (T*)dx, total, (uint32_t)(I / 8), I, pitch);
+    constexpr int kUnroll = sizeof(T) == 4 ? 1 : 2;
+    const int64_t vectors = R * (I / 8), per = kUnroll * kThreads, grid = (vectors + per - 1) / per;
+    if (I % 8 == 0 && aligned16(dy) && aligned16(dx) && (reinterpret_cast<uintptr_t>(values) & 7u) == 0 && grid <= kMostWorkgroups) {
+        hipLaunchKernelGGL((swiglu_fp8_bwd_kernel<T, kUnroll>), dim3((uint32_t)grid), dim3(kThreads), 0, st, values, scales, (const T*)dy, (T*)dx,
+                           vectors, (uint32_t)(I / 8), I, pitch);
     } else {
         const int64_t total = R * I, blocks = (total + kThreads - 1) / kThreads;
         hipLaunchKernelGGL(swiglu_fp8_bwd_generic_kernel<T>, dim3((uint32_t)(blocks < (1 << 20) ? blocks : (1 << 20))), dim3(kThreads), 0, st, values,

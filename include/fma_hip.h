@@ -445,7 +445,7 @@ int64_t fma_fp8_scale_pitch(int64_t K);
 
 /* x [E, N, K] of dtype -> values [E, N, K], scales [E, N, pitch(K)] (block_rows 1) or [E, ceil(N / 128), pitch(K)] (block_rows 128).
  * With 128 x 128 blocks a transposed copy too, values_t [E, K, N] with scales_t [E, ceil(K / 128), pitch(N)], unless both are NULL.
- * Any size and alignment; rows of multiples of 16 (8 with 128 x 128 blocks) elements, aligned, take the 16-byte kernels. */
+ * Any size (below 2^24 blocks of 128 x 128) and alignment; rows of multiples of 16 (8 with 128 x 128 blocks) elements, aligned, take the 16-byte kernels. */
 int fma_quantize_fp8(const void* x, void* values, void* scales, void* values_t, void* scales_t, int64_t E, int64_t N, int64_t K,
                      int64_t block_rows, int dtype, void* stream);
 /* out [E, N, K] = value * scale, rounded to dtype once: exact in fp32 and bf16. What a dtype's largest numbers round up to in 8 bits, 65536
@@ -484,7 +484,7 @@ int fma_swiglu_fp8_backward(const void* values, const void* scales, const void* 
  * buffer: fma_swiglu_experts_fp8_buffer_bytes, 16-byte aligned, no initialisation; with keep it holds what the backward call reads
  * (tokens, pre-activation and activation in 8 bits, the experts' output, the routing index) and must not be touched in between.
  * The backward takes the transposed copies W1t [E, 2, H, I] and W2t [E, I, H]; dx, d_gates, dW1 [E, 2 I, H], dW2 [E, H, I] of dtype
- * are each computed unless NULL. H % 16 == I % 16 == 0, T * H < 2^30, I < 2^20, 2 * I * H < 2^32, E <= FMA_MAX_GROUPS;
+ * are each computed unless NULL. H % 16 == I % 16 == 0, T < 2^24, T * H < 2^30, T * top_k < 2^26 - 3, I < 2^20, 2 * I * H < 2^32, E <= FMA_MAX_GROUPS;
  * dtype FMA_BF16 or FMA_F16. */
 int64_t fma_swiglu_experts_fp8_buffer_bytes(int64_t T, int64_t top_k, int64_t E, int64_t H, int64_t I, int keep);
 int64_t fma_swiglu_experts_fp8_workspace_bytes(int64_t T, int64_t top_k, int64_t E);

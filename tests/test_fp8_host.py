@@ -202,3 +202,21 @@ def test_refusal_of_parameters_made_in_inference_mode():
         moe = fma.MoE(4, 2, 32, 32, fma.swiglu_packed, True, False, 0.02).to(torch.bfloat16)
     with pytest.raises(ValueError, match="inference mode"):
         moe.quantize_experts()
+
+
+def test_launches_that_would_not_fit_are_refused_up_front(lib):
+    """a launch has fewer than 2^32 threads: sizes that need more are refused before anything is enqueued"""
+    buf, p = _pointer()
+    assert lib.fma_quantize_fp8(p, p, p, None, None, 1 << 24, 1, 128, 128, 2, None) == -5 and "2^24" in _err(lib)
+    assert lib.fma_quantize_fp8(p, p, p, p, p, 1 << 12, 1 << 12, 1 << 14, 128, 2, None) == -5
+
+    def forward(T, k, H=16, I=16):
+        return lib.fma_swiglu_experts_fp8(p, p, p, 4, p, p, p, p, p, T, k, 4, H, I, 0, p, 0, p, 0, 2, None)
+
+    def backward(T, k, H=16, I=16):
+        return lib.fma_swiglu_experts_fp8_bwd(p, p, p, 4, p, p, p, p, p, 0, p, p, p, p, T, k, 4, H, I, p, 0, 2, None)
+
+    for call in (forward, backward):
+        assert call(1 << 24, 1) == -5 and "T < 2^24" in _err(lib)
+        assert call(1 << 22, 16) == -5 and call((1 << 22) - 1, 16) == -7  # (the next refusal: no buffer)
+        assert call((1 << 24) - 1, 1) == -7 and call(1 << 22, 8, I=1 << 13) == -5 and call(1 << 22, 8, I=1 << 10) == -7

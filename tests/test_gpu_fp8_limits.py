@@ -183,3 +183,24 @@ def test_a_few_tokens_hold_few_stray_roundings(dtype, T, H, I, E):
     left = ((got - exact).abs() - torch.finfo(dtype).eps / 2 * exact.abs()).clamp(min=0)
     off = left.norm(dim=1) / exact.norm(dim=1)
     assert int((off > 2.0**-13).sum()) <= 3, (int((off > 2.0**-13).sum()), float(off.max()))
+
+
+def test_conversions_of_very_many_rows():
+    """more rows than one launch of the 16-byte kernels has threads for"""
+    for rows, dtype in ((2**28 + 5, torch.bfloat16), (2**27 + 5, torch.float32)):
+        x = torch.randn(1 << 16, 16, device=DEV).to(dtype).repeat(rows // (1 << 16) + 1, 1)[:rows]
+        values, scales = quantize_fp8(x)
+        for part in (slice(0, 70000), slice(rows - 70000, rows)):
+            few = quantize_fp8(x[part])
+            assert torch.equal(few.values.view(torch.uint8), values[part].view(torch.uint8))
+            assert torch.equal(few.scales.view(torch.uint8), scales[part].view(torch.uint8))
+        del x, values, scales
+    rows = 2**27 + 3
+    x = torch.randn(1 << 16, 16, device=DEV).bfloat16().repeat(rows // (1 << 16) + 1, 1)[:rows].requires_grad_()
+    y = swiglu_packed_fp8(x)
+    y.backward(torch.ones_like(y))
+    for part in (slice(0, 70000), slice(rows - 70000, rows)):
+        few = x.detach()[part].requires_grad_()
+        z = swiglu_packed_fp8(few)
+        z.backward(torch.ones_like(z))
+        assert torch.equal(y[part], z) and torch.equal(x.grad[part], few.grad)
