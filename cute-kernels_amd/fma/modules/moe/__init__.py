@@ -170,6 +170,10 @@ def _is_swiglu_packed(activation_function: Callable) -> bool:
 
 
 class MoE(nn.Module):
+    # (of the class as well: a pickled layer from before they existed has none of its own)
+    fp8_experts = False
+    _fp8_weights: tuple | None = None
+
     def __init__(
         self,
         num_experts: int,
@@ -208,7 +212,7 @@ class MoE(nn.Module):
 
         # the experts' products in 8 bits (swiglu_experts_fp8): a SwiGLU layer without biases in a 16-bit type
         self.fp8_experts = False
-        self._fp8_weights: tuple | None = None  # what quantize_experts() made, and the versions it made it of
+        self._fp8_weights = None  # what quantize_experts() made, and the versions it made it of
 
         self.act = activation_function
         # swiglu_packed as the activation of a GLU layer is computed inside the up-projection's epilogue (a kernel for

@@ -220,3 +220,17 @@ def test_launches_that_would_not_fit_are_refused_up_front(lib):
         assert call(1 << 24, 1) == -5 and "T < 2^24" in _err(lib)
         assert call(1 << 22, 16) == -5 and call((1 << 22) - 1, 16) == -7  # (the next refusal: no buffer)
         assert call((1 << 24) - 1, 1) == -7 and call(1 << 22, 8, I=1 << 13) == -5 and call(1 << 22, 8, I=1 << 10) == -7
+
+
+def test_a_layer_saved_before_it_had_8_bit_experts_still_loads_and_runs():
+    """a pickled module comes back with the attributes that it was saved with"""
+    moe = MoE(4, 2, 32, 32, swiglu_packed, True, False, 0.02).to(torch.bfloat16)
+    for name in ("fp8_experts", "_fp8_weights"):
+        moe.__dict__.pop(name, None)
+    loaded = MoE.__new__(MoE)
+    loaded.__setstate__(moe.__dict__.copy())
+    assert loaded.fp8_experts is False
+    with pytest.raises(RuntimeError, match="GPU only"):
+        loaded(torch.zeros(3, 32).bfloat16(), kernel_backend=fma.KernelBackend.cuda)
+    with pytest.raises(RuntimeError, match="GPU only"):
+        loaded.quantize_experts()
