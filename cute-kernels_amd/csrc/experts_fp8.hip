@@ -18,7 +18,7 @@ using namespace fp8;
 constexpr int kThreads = 256;
 constexpr uint32_t kFloat16Scale = 127 + 7;  // 448 * 2^7 = 57344: the largest scale of a block that float16 holds
 
-// The expert of a slot, -1 for an id that names none: such a choice has no row, and takes no part in anything.
+// Whether a slot's id names an expert: a choice that names none has no row, and takes no part in anything.
 __device__ __forceinline__ bool names_expert(const void* ids, int id_bytes, int64_t slot, uint32_t E) {
     const int64_t id = id_bytes == 8 ? ((const int64_t*)ids)[slot] : (int64_t)((const int32_t*)ids)[slot];
     return (uint64_t)id < E;

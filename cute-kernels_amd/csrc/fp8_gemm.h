@@ -117,7 +117,6 @@ __global__ __launch_bounds__(kGemmThreads) void fp8_gemm_kernel(const GemmArgs a
     __shared__ __attribute__((aligned(256))) uint32_t s_scale[2 * kScaleWords];
     __shared__ __attribute__((aligned(16))) uint32_t s_max[kMaxima ? kMaxima * kMostRows * 4 : 4];
     __shared__ __attribute__((aligned(1024))) uint8_t s_x[TALL ? 2 * 32 * kBlock : 16];  // rows 256 .. 287 of A, per stage
-    __shared__ uint32_t s_height;
     __shared__ __attribute__((aligned(1024))) uint8_t s_out[EPI == EPI_BF16 || EPI == EPI_F16 ? kWaves * 2048 : 16];
     __shared__ uint32_t s_tiles[kMostGroups + 1];  // row tiles of the groups before
     __shared__ uint32_t s_first[kMostGroups + 1];  // first row of the group
@@ -170,7 +169,6 @@ __global__ __launch_bounds__(kGemmThreads) void fp8_gemm_kernel(const GemmArgs a
         if (lane == 0) {
             s_tiles[E] = tiles;
             s_first[E] = rows;
-            s_height = height;
         }
     }
     __syncthreads();

@@ -344,6 +344,9 @@ int launch(const char* who, ThinArgs a, hipStream_t st) {
     const uint32_t per = OUT == OUT_GLU ? 16u : 32u;
     a.col_blocks = (a.N + per - 1) / per;
     const int64_t groups = a.E < a.R ? a.E : a.R, cus = num_compute_units() > 0 ? num_compute_units() : 256;
+    // Passes of 32 rows where groups of more than 16, which passes of 16 stream their weights twice for, are to be expected: their 25 registers more
+    // cost otherwise. 16 / 32, us, at 4, 8, 10, 16 rows a group on average: 8 x 4096 x 14336 83, 88, 105, 130 / 92, 95, 101, 111; 8 x 2048 x
+    // 8192 31, 32, 41, 54 / 34, 35, 36, 40; 8 x 28672 x 4096 163, 167, 187, 237 / 161, 165, 174, 202; 64 x 2816 x 2048 64, 69, 73, 101 / 64, 67, 71, 83.
     const bool wide = (int64_t)a.R > 8 * groups;
     // parts of the reduction, of two blocks at least, until there are 32 wavefronts per compute unit, two rounds (12: 8 x 4 rows, 28672 x 4096,
     // 179 -> 169 us; 64: 64 x 16 rows, 2816 x 2048, 84 -> 96)
