@@ -18,7 +18,8 @@
 //  * The instruction's sums: eight neighbouring products are aligned to the largest of them and cut below 2^-13 of it before they are added
 //    to the fp32 sum (measured; the unscaled 8-bit instructions do the same), 2^-16 of a sum of random terms, root mean square. A result
 //    that leaves in 16 bits loses nothing by that, and where a result becomes e4m3 the next product's many terms average the roundings that
-//    fall to the other side (0.003 of the result instead of 0.0017). The pre-activation of a training pass, of which gradients are made
+//    fall to the other side (0.003 of the result instead of 0.0017; exact sums for a prefill's activation: 4096 tokens, hidden 2048, I 1408, E 64,
+//    k 8, 356 -> 504 us, hidden 4096, I 14336, E 8, k 2, 1286 -> 1900). The pre-activation of a training pass, of which gradients are made
 //    element by element, takes the bfloat16 instruction instead (k_step_exact).
 //  * GLU: the tile holds 128 "up" and 128 "gate" columns; the activation, 128 columns or one block, is quantised from the fp32 sums: the
 //    largest magnitude of a row goes from wavefront to wavefront through LDS. With KEEP the pre-activation is kept in 8 bits too.

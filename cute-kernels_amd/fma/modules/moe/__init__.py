@@ -210,7 +210,10 @@ class MoE(nn.Module):
         # the activation's backward inside the second projection's input-gradient GEMM (see _runs_swiglu_experts_as_one_node)
         self.fuse_swiglu_backward = True
 
-        # the experts' products in 8 bits (swiglu_experts_fp8): a SwiGLU layer without biases in a 16-bit type
+        # The experts' products in 8 bits (swiglu_experts_fp8): a SwiGLU layer without biases in a 16-bit type. 16 / 8 bits, us: hidden 2048, I 1408,
+        # E 64, k 8, prepared weights, 1 token 34 / 38 (called eagerly 36 / 80), 16 tokens 174 / 124, 4096 tokens 560 / 366; training steps of 8192 and
+        # 32768 tokens 3438 / 3471, 12250 / 11835; hidden 4096, I 1536, E 128, k 8, 1 token 64 / 62, 4096 tokens 1398 / 823, a training step
+        # of 8192 tokens 7578 / 8436, which keeps 3362 MB instead of 1211 (8-bit copies of the weights among them).
         self.fp8_experts = False
         self._fp8_weights = None  # what quantize_experts() made, and the versions it made it of
 
@@ -376,7 +379,8 @@ class MoE(nn.Module):
 
     def quantize_experts(self) -> "MoE":
         """Switches the experts' products to 8 bits (fp8_experts) and lays both projections out in 8 bits once, for calls that no backward
-        pass follows: a serving program calls it after loading the weights, and again after changing them. A forward pass on weights that
+        pass follows: a serving program of more than a token or two at a time (see __init__) calls it after loading the weights, and again
+        after changing them. A forward pass on weights that
         have changed since, as far as their version counters tell, quantises them in the call, as one without this call does; changes that
         no counter sees (through .data, or by a replayed graph) need the call again. A compiled layer quantises in the call. Called again, it
         writes to the same memory, so that a graph captured before serves the new weights (unless they are on another device since)."""
