@@ -117,7 +117,7 @@ struct Args {
     // last part can end inside a step or on an odd one); part s of packed row r goes to partial[(s * rows + r) * n ..]
     float* partial;
     uint32_t splits, split_steps, rows;
-    // reduction varies: the reduction rows that there are (below 2^31), to which the sizes are cut; 0: as many as the sizes say
+    // weight gradients of packed rows (kCutK): the rows that there are (below 2^31), to which the sizes are cut; 0: as many as the sizes say
     uint32_t k_rows;
     // not NULL: the kernel runs only if *taken, which it decides (takes_many_passes) and writes first if pass_bits is not 0;
     // otherwise the streaming kernel behind it computes the product (thin_experts.hip)
@@ -169,6 +169,8 @@ __global__ __launch_bounds__(NT) void ragged_gemm_kernel(const Args args) {
     // GATHER: the rows of A are picked through row_index (forward); kGatherK: the reduction rows of B are (weight gradient)
     constexpr bool GATHER = GATHER_ANY && !VARY_K;
     constexpr bool kGatherK = GATHER_ANY && VARY_K;
+    // (in the layouts with a contiguous reduction the look-up of the prefix would bring waits for all loads into the K loop)
+    constexpr bool kCutK = VARY_K && !A_KC && !B_KC && !GATHER_ANY;
     // kGlu: a forward SwiGLU epilogue (the tile holds 128 "up" and 128 "gate" columns of the product)
     constexpr bool kGlu = EPI == EPI_SWIGLU || EPI == EPI_SWIGLU_ACT;
     static_assert(!kGlu || (A_KC && B_KC && !VARY_K), "the SwiGLU epilogue exists for the NT layout only");
@@ -362,7 +364,7 @@ __global__ __launch_bounds__(NT) void ragged_gemm_kernel(const Args args) {
                 t = tiles_of(group_m(s_order[e]));  // the group at position e of the tile sequence
             }
             const uint32_t it = wave_inclusive_scan<uint32_t>(t);
-            if (VARY_K && args.k_rows) {
+            if (kCutK && args.k_rows) {
                 // (sums that stop at the rows: no two values below 2^31 overflow)
                 const uint32_t most = args.k_rows;
                 sz = sz < most ? sz : most;
@@ -470,7 +472,7 @@ __global__ __launch_bounds__(NT) void ragged_gemm_kernel(const Args args) {
         t.e = e;
         t.Me = group_m(e);
         t.Ke = group_k(e);
-        if (VARY_K && args.k_rows) {
+        if (kCutK && args.k_rows) {
             const uint32_t left = args.k_rows - uniform(s_prefix[e]);
             t.Ke = t.Ke < left ? t.Ke : left;
         }
