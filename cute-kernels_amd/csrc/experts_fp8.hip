@@ -7,7 +7,7 @@
 // with q the block format of fp8_parts.h. The tokens are quantised once and gathered inside the first product, the activation is quantised
 // in that product's epilogue. What a training step keeps is in 8 bits (tokens, pre-activation, activation; the experts' output, which the
 // gates' gradient reads, in 16). The weight gradients are products in 16 bits: of the unrounded gradients' 16-bit form and the 8-bit
-// activations, which are exact in bf16 (in fp16 as far as its exponents reach).
+// activations, which are exact in bf16 (in fp16 as far as its exponents reach; a row past its range shares a power of two with its gradient).
 #include "fp8_gemm_launch.h"
 #include "fp8_thin.h"
 
