@@ -210,7 +210,8 @@ def _plain_clip(s):
         norm = torch.stack([g.float().square().sum() for g in grads]).sum().sqrt()
     else:
         norm = torch.stack([g.abs().max() for g in grads]).max().float()
-    torch._foreach_mul_(grads, torch.clamp(bound / (norm + 1e-6), max=1.0))
+    # (a factor of one dimension: one without any would be rounded to the gradients' type before the product)
+    s["bucket"].mul_(torch.clamp(bound / (norm + 1e-6), max=1.0).view(1))
     return dict(norm=norm, grads=s["bucket"])
 
 
