@@ -1,0 +1,323 @@
+// The norm of many tensors together, and scaling them down to a bound:
+//
+//   norm = sqrt(sum over all elements of all tensors of g^2)   or   max |g|
+//   g   *= min(1, max_norm / (norm + 1e-6))
+//
+// HBM-bound: one pass reads every element, a second reads and writes it. Squares are added in 64 bits from the first one on: in 32 bits
+// a gradient of 2^64 or of 2^-75 would already be lost in its square. Tensors come as a table in the kernel's arguments (no table in
+// device memory that a captured graph or a second call would have to share), cut into chunks of 16384 elements.
+#include "common.h"
+
+#include <stdlib.h>
+
+#include <algorithm>
+
+namespace fmahip {
+namespace {
+
+constexpr int kThreads = 256;
+constexpr int kWaves = kThreads / kWave;
+constexpr int kChunk = 16384;   // elements; a multiple of every 16-byte vector, so that all chunks of a tensor are aligned alike
+constexpr int kTable = 160;     // tensors per launch: 3.4 KB of kernel arguments
+constexpr int kPerCU = 8;       // workgroups per compute unit
+
+struct Table {
+    void* ptr[kTable];
+    int64_t numel[kTable];
+    uint32_t first[kTable + 1];  // chunks in front of each tensor
+    uint8_t dtype[kTable];
+    int32_t count;
+};
+
+struct Chunk {
+    void* ptr;
+    int32_t n;
+    int32_t dtype;
+};
+
+__device__ __forceinline__ Chunk find_chunk(const Table& t, uint32_t c) {
+    int low = 0, high = t.count - 1;
+    while (low < high) {
+        const int mid = (low + high + 1) / 2;
+        if (t.first[mid] <= c) low = mid;
+        else high = mid - 1;
+    }
+    const int64_t begin = (int64_t)(c - t.first[low]) * kChunk, rest = t.numel[low] - begin;
+    const int dtype = t.dtype[low];
+    Chunk out;
+    out.ptr = (char*)t.ptr[low] + begin * (dtype == FMA_F32 ? 4 : 2);
+    out.n = (int32_t)(rest < kChunk ? rest : kChunk);
+    out.dtype = dtype;
+    return out;
+}
+
+// elements in front of the first 16-byte boundary
+template <typename T>
+__device__ __forceinline__ int head_of(const T* p, int n) {
+    const int head = (int)((16 - ((uintptr_t)p & 15)) & 15) / (int)sizeof(T);
+    return head < n ? head : n;
+}
+
+// sum of squares, or the largest magnitude's bits (as those of a float: their order is that of the numbers, with NaN on top)
+template <bool MAX>
+struct Accumulator {
+    double sum = 0.0;
+    __device__ __forceinline__ void add(float x) { sum = __builtin_fma((double)x, (double)x, sum); }
+    __device__ __forceinline__ void join(uint64_t bits) { sum += __builtin_bit_cast(double, bits); }
+    __device__ __forceinline__ uint64_t bits() const { return __builtin_bit_cast(uint64_t, sum); }
+};
+template <>
+struct Accumulator<true> {
+    uint32_t most = 0;
+    __device__ __forceinline__ void add(float x) { most = max(most, __float_as_uint(x) & 0x7fffffffu); }
+    __device__ __forceinline__ void join(uint64_t bits) { most = max(most, (uint32_t)bits); }
+    __device__ __forceinline__ uint64_t bits() const { return most; }
+};
+
+template <bool MAX, int WAVES>
+__device__ __forceinline__ void join_workgroup(Accumulator<MAX>& acc) {
+    __shared__ uint64_t s_part[WAVES];
+#pragma unroll
+    for (int d = kWave / 2; d > 0; d >>= 1) acc.join(__shfl_xor(acc.bits(), d, kWave));
+    if ((threadIdx.x & (kWave - 1)) == 0) s_part[threadIdx.x / kWave] = acc.bits();
+    __syncthreads();
+    acc = Accumulator<MAX>();
+#pragma unroll
+    for (int w = 0; w < WAVES; ++w) acc.join(s_part[w]);
+}
+
+template <typename T, bool MAX>
+__device__ __forceinline__ void add_chunk(Accumulator<MAX>& acc, const T* p, int n) {
+    constexpr int V = Vec16<T>::N;
+    const int head = head_of(p, n);
+    if ((int)threadIdx.x < head) acc.add(Num<T>::up(p[threadIdx.x]));
+    p += head;
+    n -= head;
+    const int nvec = n / V;
+    const Vec16<T>* const v = (const Vec16<T>*)p;
+    for (int i = threadIdx.x; i < nvec; i += kThreads) {
+        const Vec16<T> x = v[i];
+#pragma unroll
+        for (int e = 0; e < V; ++e) acc.add(Num<T>::up(x.v[e]));
+    }
+    const int tail = nvec * V + (int)threadIdx.x;
+    if (tail < n) acc.add(Num<T>::up(p[tail]));
+}
+
+template <bool MAX>
+__global__ __launch_bounds__(kThreads) void grad_norm_kernel(const Table t, uint64_t* __restrict__ partial) {
+    Accumulator<MAX> acc;
+    for (uint32_t c = blockIdx.x; c < t.first[t.count]; c += gridDim.x) {
+        const Chunk k = find_chunk(t, c);
+        if (k.dtype == FMA_F32) add_chunk(acc, (const float*)k.ptr, k.n);
+        else if (k.dtype == FMA_F16) add_chunk(acc, (const f16_t*)k.ptr, k.n);
+        else add_chunk(acc, (const bf16_t*)k.ptr, k.n);
+    }
+    join_workgroup<MAX, kWaves>(acc);
+    if (threadIdx.x == 0) partial[blockIdx.x] = acc.bits();
+}
+
+// the partial results in a fixed order; the norm in 64 bits for the scaling that follows, and in 32 for the caller
+constexpr int kJoinThreads = 1024;
+template <bool MAX>
+__global__ __launch_bounds__(kJoinThreads) void grad_norm_join_kernel(const uint64_t* __restrict__ partial, int64_t count,
+                                                                      double* __restrict__ norm64, float* __restrict__ norm) {
+    Accumulator<MAX> acc;
+    for (int64_t i = threadIdx.x; i < count; i += kJoinThreads) acc.join(partial[i]);
+    join_workgroup<MAX, kJoinThreads / kWave>(acc);
+    if (threadIdx.x == 0) {
+        double n;
+        if constexpr (MAX) n = (double)__uint_as_float(acc.most);
+        else n = sqrt(acc.sum);
+        *norm64 = n;
+        *norm = (float)n;
+    }
+}
+
+template <typename T>
+__device__ __forceinline__ void scale_chunk(T* p, int n, float factor) {
+    constexpr int V = Vec16<T>::N;
+    const int head = head_of(p, n);
+    if ((int)threadIdx.x < head) p[threadIdx.x] = Num<T>::down(Num<T>::up(p[threadIdx.x]) * factor);
+    p += head;
+    n -= head;
+    const int nvec = n / V;
+    Vec16<T>* const v = (Vec16<T>*)p;
+    for (int i = threadIdx.x; i < nvec; i += kThreads) {
+        Vec16<T> x = v[i];
+#pragma unroll
+        for (int e = 0; e < V; ++e) x.v[e] = Num<T>::down(Num<T>::up(x.v[e]) * factor);
+        v[i] = x;
+    }
+    const int tail = nvec * V + (int)threadIdx.x;
+    if (tail < n) p[tail] = Num<T>::down(Num<T>::up(p[tail]) * factor);
+}
+
+// a factor of one leaves the tensors alone: nothing is read or written then. A NaN goes through.
+__global__ __launch_bounds__(kThreads) void scale_grads_kernel(const Table t, const double* __restrict__ norm64,
+                                                               const float* __restrict__ norm, double max_norm) {
+    const double ratio = max_norm / ((norm64 ? *norm64 : (double)*norm) + 1e-6);
+    if (ratio >= 1.0) return;
+    const float factor = (float)ratio;
+    for (uint32_t c = blockIdx.x; c < t.first[t.count]; c += gridDim.x) {
+        const Chunk k = find_chunk(t, c);
+        if (k.dtype == FMA_F32) scale_chunk((float*)k.ptr, k.n, factor);
+        else if (k.dtype == FMA_F16) scale_chunk((f16_t*)k.ptr, k.n, factor);
+        else scale_chunk((bf16_t*)k.ptr, k.n, factor);
+    }
+}
+
+int64_t most_workgroups() { return (num_compute_units() > 0 ? num_compute_units() : 256) * (int64_t)kPerCU; }
+
+// Tables of the tensors that have elements, in order, and what `launch` makes of each; stops at the first that fails.
+template <typename F>
+int for_each_table(void* const* tensors, const int64_t* sizes, const int32_t* dtypes, int64_t count, F launch) {
+    Table t;
+    int64_t i = 0;
+    while (i < count) {
+        t.count = 0;
+        t.first[0] = 0;
+        for (; i < count && t.count < kTable; ++i) {
+            if (sizes[i] == 0) continue;
+            const int64_t chunks = (sizes[i] + kChunk - 1) / kChunk;  // 2^23 at the most, of all tensors of a table below 2^31
+            t.ptr[t.count] = tensors[i];
+            t.numel[t.count] = sizes[i];
+            t.dtype[t.count] = (uint8_t)dtypes[i];
+            t.first[t.count + 1] = t.first[t.count] + (uint32_t)chunks;
+            ++t.count;
+        }
+        if (t.count > 0) {
+            const int rc = launch(t);
+            if (rc) return rc;
+        }
+    }
+    return FMA_OK;
+}
+
+int check_tensors(const char* what, void* const* tensors, const int64_t* sizes, const int32_t* dtypes, int64_t count) {
+    FMA_REQUIRE(count >= 0 && count <= FMA_MAX_GRAD_TENSORS, FMA_ERR_BAD_SIZE, "%s: bad number of tensors %lld", what, (long long)count);
+    if (count == 0) return FMA_OK;
+    FMA_REQUIRE(tensors && sizes && dtypes, FMA_ERR_NULL_POINTER, "%s: NULL pointer", what);
+    for (int64_t i = 0; i < count; ++i) {
+        const int bytes = dtype_bytes(dtypes[i]);
+        FMA_REQUIRE(bytes != 0, FMA_ERR_BAD_DTYPE, "%s: unknown dtype code %d of tensor %lld", what, (int)dtypes[i], (long long)i);
+        FMA_REQUIRE(sizes[i] >= 0 && sizes[i] <= FMA_MAX_GRAD_ELEMENTS, FMA_ERR_BAD_SIZE, "%s: bad size %lld of tensor %lld", what,
+                    (long long)sizes[i], (long long)i);
+        FMA_REQUIRE(sizes[i] == 0 || tensors[i], FMA_ERR_NULL_POINTER, "%s: tensor %lld is NULL", what, (long long)i);
+        FMA_REQUIRE(((uintptr_t)tensors[i] & (uintptr_t)(bytes - 1)) == 0, FMA_ERR_MISALIGNED,
+                    "%s: tensor %lld is not aligned to its elements", what, (long long)i);
+    }
+    return FMA_OK;
+}
+
+// No element may be scaled twice, least of all by two workgroups at once.
+int check_disjoint(const char* what, void* const* tensors, const int64_t* sizes, const int32_t* dtypes, int64_t count) {
+    struct Range {
+        uintptr_t begin, end;
+    };
+    Range* const r = (Range*)malloc((size_t)(count > 0 ? count : 1) * sizeof(Range));
+    FMA_REQUIRE(r, FMA_ERR_BAD_SIZE, "%s: no host memory for %lld tensors", what, (long long)count);
+    int64_t n = 0;
+    for (int64_t i = 0; i < count; ++i)
+        if (sizes[i] > 0) {
+            r[n].begin = (uintptr_t)tensors[i];
+            r[n++].end = (uintptr_t)tensors[i] + (uintptr_t)sizes[i] * (uintptr_t)dtype_bytes(dtypes[i]);
+        }
+    std::sort(r, r + n, [](const Range& a, const Range& b) { return a.begin < b.begin; });
+    bool apart = true;
+    for (int64_t i = 1; i < n; ++i) apart = apart && r[i - 1].end <= r[i].begin;
+    free(r);
+    FMA_REQUIRE(apart, FMA_ERR_UNSUPPORTED, "%s: two tensors share memory", what);
+    return FMA_OK;
+}
+
+int launch_norm(void* const* tensors, const int64_t* sizes, const int32_t* dtypes, int64_t count, int infinity, float* norm, double* norm64,
+                hipStream_t st) {
+    uint64_t* const partial = (uint64_t*)(norm64 + 1);
+    const int64_t most = most_workgroups();
+    int64_t parts = 0;
+    int rc = for_each_table(tensors, sizes, dtypes, count, [&](const Table& t) {
+        const int64_t chunks = t.first[t.count], grid = chunks < most ? chunks : most;
+        if (infinity) hipLaunchKernelGGL(grad_norm_kernel<true>, dim3((uint32_t)grid), dim3(kThreads), 0, st, t, partial + parts);
+        else hipLaunchKernelGGL(grad_norm_kernel<false>, dim3((uint32_t)grid), dim3(kThreads), 0, st, t, partial + parts);
+        parts += grid;
+        return launch_status("grad_norm");
+    });
+    if (rc) return rc;
+    if (infinity) hipLaunchKernelGGL(grad_norm_join_kernel<true>, dim3(1), dim3(kJoinThreads), 0, st, partial, parts, norm64, norm);
+    else hipLaunchKernelGGL(grad_norm_join_kernel<false>, dim3(1), dim3(kJoinThreads), 0, st, partial, parts, norm64, norm);
+    return launch_status("grad_norm (join)");
+}
+
+int launch_scale(void* const* tensors, const int64_t* sizes, const int32_t* dtypes, int64_t count, const double* norm64, const float* norm,
+                 double max_norm, hipStream_t st) {
+    const int64_t most = most_workgroups();
+    return for_each_table(tensors, sizes, dtypes, count, [&](const Table& t) {
+        const int64_t chunks = t.first[t.count], grid = chunks < most ? chunks : most;
+        hipLaunchKernelGGL(scale_grads_kernel, dim3((uint32_t)grid), dim3(kThreads), 0, st, t, norm64, norm, max_norm);
+        return launch_status("scale_grads");
+    });
+}
+
+int check_workspace(const char* what, const void* workspace, int64_t bytes, int64_t count) {
+    FMA_REQUIRE(workspace, FMA_ERR_NULL_POINTER, "%s: NULL workspace", what);
+    const int64_t need = fma_grad_norm_workspace_bytes(count);
+    FMA_REQUIRE(bytes >= need, FMA_ERR_WORKSPACE_TOO_SMALL, "%s: workspace of %lld bytes, %lld needed", what, (long long)bytes,
+                (long long)need);
+    FMA_REQUIRE(((uintptr_t)workspace & 7u) == 0, FMA_ERR_MISALIGNED, "%s: workspace must be 8-byte aligned", what);
+    return FMA_OK;
+}
+
+int check_bound(const char* what, double max_norm) {
+    FMA_REQUIRE(max_norm >= 0.0, FMA_ERR_BAD_SIZE, "%s: max_norm must not be negative or NaN", what);
+    return FMA_OK;
+}
+
+}  // namespace
+}  // namespace fmahip
+
+extern "C" {
+
+int64_t fma_grad_norm_workspace_bytes(int64_t count) {
+    if (count < 0 || count > FMA_MAX_GRAD_TENSORS) return 0;
+    // the norm in 64 bits, and a partial result per workgroup of every launch
+    return 8 + 8 * fmahip::most_workgroups() * ((count + fmahip::kTable - 1) / fmahip::kTable);
+}
+
+int fma_grad_norm(void* const* tensors, const int64_t* sizes, const int32_t* dtypes, int64_t count, int infinity, float* norm,
+                  void* workspace, int64_t workspace_bytes, void* stream) {
+    using namespace fmahip;
+    int rc = check_tensors("grad_norm", tensors, sizes, dtypes, count);
+    if (rc) return rc;
+    FMA_REQUIRE(norm, FMA_ERR_NULL_POINTER, "grad_norm: norm is NULL");
+    rc = check_workspace("grad_norm", workspace, workspace_bytes, count);
+    if (rc) return rc;
+    return launch_norm(tensors, sizes, dtypes, count, infinity, norm, (double*)workspace, (hipStream_t)stream);
+}
+
+int fma_scale_grads(void* const* tensors, const int64_t* sizes, const int32_t* dtypes, int64_t count, const float* norm, double max_norm,
+                    void* stream) {
+    using namespace fmahip;
+    int rc = check_tensors("scale_grads", tensors, sizes, dtypes, count);
+    if (!rc) rc = check_bound("scale_grads", max_norm);
+    if (!rc) rc = check_disjoint("scale_grads", tensors, sizes, dtypes, count);
+    if (rc) return rc;
+    FMA_REQUIRE(norm, FMA_ERR_NULL_POINTER, "scale_grads: norm is NULL");
+    return launch_scale(tensors, sizes, dtypes, count, nullptr, norm, max_norm, (hipStream_t)stream);
+}
+
+int fma_clip_grad_norm(void* const* tensors, const int64_t* sizes, const int32_t* dtypes, int64_t count, int infinity, double max_norm,
+                       float* norm, void* workspace, int64_t workspace_bytes, void* stream) {
+    using namespace fmahip;
+    int rc = check_tensors("clip_grad_norm", tensors, sizes, dtypes, count);
+    if (!rc) rc = check_bound("clip_grad_norm", max_norm);
+    if (!rc) rc = check_disjoint("clip_grad_norm", tensors, sizes, dtypes, count);
+    if (rc) return rc;
+    FMA_REQUIRE(norm, FMA_ERR_NULL_POINTER, "clip_grad_norm: norm is NULL");
+    rc = check_workspace("clip_grad_norm", workspace, workspace_bytes, count);
+    if (!rc) rc = launch_norm(tensors, sizes, dtypes, count, infinity, norm, (double*)workspace, (hipStream_t)stream);
+    if (!rc) rc = launch_scale(tensors, sizes, dtypes, count, (const double*)workspace, nullptr, max_norm, (hipStream_t)stream);
+    return rc;
+}
+
+}  // extern "C"

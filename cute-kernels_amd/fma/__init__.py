@@ -6,9 +6,12 @@ from .math import ceil_divide, divide_if_divisible
 from .modules import MoE, quantize_expert_weights, swiglu_experts_fp8
 from .ops import (
     Fp8Blocks,
+    clip_grad_norm_,
+    clip_grads_with_norm_,
     continuous_count,
     dequantize_fp8,
     fused_residual_add_rmsnorm,
+    get_total_norm,
     grouped_gemm,
     grouped_gemm_fp8,
     grouped_linear_fp8,

@@ -27,6 +27,7 @@ _p = ctypes.c_void_p
 _i64 = ctypes.c_int64
 _i32 = ctypes.c_int
 _f32 = ctypes.c_float
+_f64 = ctypes.c_double
 
 # name -> (restype, argtypes); one entry per declaration of include/fma_hip.h
 SIGNATURES = {
@@ -93,6 +94,10 @@ SIGNATURES = {
     "fma_swiglu_experts_fp8": (_i32, [_p] * 3 + [_i32] + [_p] * 5 + [_i64] * 5 + [_i32, _p, _i64, _p, _i64, _i32, _p]),
     "fma_swiglu_experts_fp8_bwd_workspace_bytes": (_i64, [_i64] * 4),
     "fma_swiglu_experts_fp8_bwd": (_i32, [_p] * 3 + [_i32] + [_p] * 5 + [_i64] + [_p] * 4 + [_i64] * 5 + [_p, _i64, _i32, _p]),
+    "fma_grad_norm_workspace_bytes": (_i64, [_i64]),
+    "fma_grad_norm": (_i32, [_p] * 3 + [_i64, _i32, _p, _p, _i64, _p]),
+    "fma_scale_grads": (_i32, [_p] * 3 + [_i64, _p, _f64, _p]),
+    "fma_clip_grad_norm": (_i32, [_p] * 3 + [_i64, _i32, _f64, _p, _p, _i64, _p]),
 }
 
 _lib = None

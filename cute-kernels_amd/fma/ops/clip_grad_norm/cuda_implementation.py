@@ -1,0 +1,97 @@
+"""Calls of fma_grad_norm, fma_scale_grads and fma_clip_grad_norm of libfma_hip.so. They take lists of tensors that may be a few hundred, and
+are no operators of the dispatcher, which would look at each of them twice more."""
+
+from array import array
+
+import torch
+from torch._C import _increment_version
+
+from ... import _lib
+
+_TENSORS = (torch.Tensor, torch.nn.Parameter)
+
+
+def _is_dense(t: torch.Tensor) -> bool:
+    """whether the elements fill one piece of memory, in whatever order"""
+    if t.is_contiguous():
+        return True
+    return t.permute(sorted(range(t.dim()), key=t.stride, reverse=True)).is_contiguous()
+
+
+class _Table:
+    """What the library needs to know of the tensors. Those with gaps between their elements come as copies; `copied` says which of what."""
+
+    def __init__(self, tensors: list[torch.Tensor], written: bool) -> None:
+        first = tensors[0]
+        self.device = device = first.device
+        self.copied = []
+        for i, t in enumerate(tensors):
+            if type(t) not in _TENSORS or t.layout is not torch.strided:
+                raise TypeError(f"dense tensors are taken, not {type(t).__name__} of layout {t.layout}")
+            if t.device != device:
+                raise RuntimeError(f"all tensors should be on one device: got {device} and {t.device}")
+            if not t.is_contiguous() and not _is_dense(t):
+                if written and torch._debug_has_internal_overlap(t) == 1:
+                    raise RuntimeError("a gradient has elements that share memory: make it contiguous first")
+                if not self.copied:
+                    tensors = list(tensors)
+                tensors[i] = t.contiguous()
+                self.copied.append((t, tensors[i]))
+        _lib.require_gpu(first)
+        self.tensors = tensors  # (holds the copies)
+        self._pointers = array("Q", [t.data_ptr() for t in tensors])
+        self._sizes = array("q", [t.numel() for t in tensors])
+        self._dtypes = array("i", [_lib.dtype_code(t.dtype) for t in tensors])
+        self.arguments = *(a.buffer_info()[0] for a in (self._pointers, self._sizes, self._dtypes)), len(tensors)
+
+
+@torch.no_grad()
+def grad_norm_cuda(tensors: list[torch.Tensor], infinity: bool) -> torch.Tensor:
+    if not tensors:
+        return torch.tensor(0.0)
+    table, lib = _Table(tensors, False), _lib.load()
+    with _lib.on_device(table.device):
+        norm = torch.empty((), dtype=torch.float32, device=table.device)
+        nbytes = lib.fma_grad_norm_workspace_bytes(len(tensors))
+        workspace = torch.empty(nbytes, dtype=torch.uint8, device=table.device)
+        rc = lib.fma_grad_norm(
+            *table.arguments, infinity, norm.data_ptr(), workspace.data_ptr(), nbytes, _lib.current_stream(table.device)
+        )
+    _lib.check(rc, "get_total_norm")
+    return norm
+
+
+def _written(table: _Table, grads: list[torch.Tensor]) -> None:
+    for t, copy in table.copied:
+        t.copy_(copy)
+    _increment_version(grads)
+
+
+@torch.no_grad()
+def scale_grads_cuda(grads: list[torch.Tensor], max_norm: float, norm: torch.Tensor) -> None:
+    if not grads:
+        return
+    table, lib = _Table(grads, True), _lib.load()
+    assert norm.numel() == 1, "total_norm should be a scalar"
+    norm = norm.to(device=table.device, dtype=torch.float32)
+    with _lib.on_device(table.device):
+        rc = lib.fma_scale_grads(*table.arguments, norm.data_ptr(), max_norm, _lib.current_stream(table.device))
+    _lib.check(rc, "clip_grads_with_norm_")
+    _written(table, grads)
+
+
+@torch.no_grad()
+def clip_grad_norm_cuda(grads: list[torch.Tensor], infinity: bool, max_norm: float) -> torch.Tensor:
+    if not grads:
+        return torch.tensor(0.0)
+    table, lib = _Table(grads, True), _lib.load()
+    with _lib.on_device(table.device):
+        norm = torch.empty((), dtype=torch.float32, device=table.device)
+        nbytes = lib.fma_grad_norm_workspace_bytes(len(grads))
+        workspace = torch.empty(nbytes, dtype=torch.uint8, device=table.device)
+        rc = lib.fma_clip_grad_norm(
+            *table.arguments, infinity, max_norm, norm.data_ptr(), workspace.data_ptr(), nbytes, _lib.current_stream(table.device)
+        )
+    _lib.check(rc, "clip_grad_norm_")
+    _written(table, grads)
+    return norm

@@ -48,6 +48,9 @@ extern "C" {
 #define FMA_MAX_DECODE_EXPERTS 256
 /* longest row of the normalisation kernels (the reference's MAX_TRITON_BLOCK_SIZE, fma/constants.py:17) */
 #define FMA_MAX_NORM_HIDDEN 65536
+/* tensors of one gradient norm, and elements of each */
+#define FMA_MAX_GRAD_TENSORS (1 << 20)
+#define FMA_MAX_GRAD_ELEMENTS (1ll << 37)
 
 /* ---- library ---------------------------------------------------------------------------- */
 
@@ -497,6 +500,22 @@ int fma_swiglu_experts_fp8_bwd(const void* dy, const void* gates, const void* id
                                const void* W2t, const void* W2t_scales, const void* buffer, int64_t buffer_bytes, void* dx, void* d_gates,
                                void* dW1, void* dW2, int64_t T, int64_t top_k, int64_t E, int64_t H, int64_t I, void* workspace,
                                int64_t workspace_bytes, int dtype, void* stream);
+
+/* ---- norm and clipping of gradients ------------------------------------------------------------- */
+
+/* The norm of `count` tensors together, sqrt of the sum of all squares or (infinity != 0) the largest magnitude, to *norm (device).
+ * tensors, sizes (elements) and dtypes (FMA_F32 / FMA_F16 / FMA_BF16) are HOST arrays, read before the call returns; every tensor is dense
+ * device memory, aligned to its elements. Sums are kept in 64 bits, in an order that depends on the sizes alone. A NaN anywhere makes the norm
+ * NaN. No tensors, or none with elements: 0. workspace: 8-byte aligned, no initialisation. No counterpart in the reference. */
+int64_t fma_grad_norm_workspace_bytes(int64_t count);
+int fma_grad_norm(void* const* tensors, const int64_t* sizes, const int32_t* dtypes, int64_t count, int infinity, float* norm,
+                  void* workspace, int64_t workspace_bytes, void* stream);
+/* Every element times min(1, max_norm / (*norm + 1e-6)), rounded to its type once; with a factor of one nothing is touched. The tensors
+ * must not overlap. fma_clip_grad_norm is fma_grad_norm and this with the norm as it is in 64 bits. */
+int fma_scale_grads(void* const* tensors, const int64_t* sizes, const int32_t* dtypes, int64_t count, const float* norm, double max_norm,
+                    void* stream);
+int fma_clip_grad_norm(void* const* tensors, const int64_t* sizes, const int32_t* dtypes, int64_t count, int infinity, double max_norm,
+                       float* norm, void* workspace, int64_t workspace_bytes, void* stream);
 
 #ifdef __cplusplus
 }
