@@ -16,6 +16,7 @@ from .ops import (
     grouped_gemm_fp8,
     grouped_linear_fp8,
     quantize_fp8,
+    router_loss,
     swiglu,
     swiglu_packed,
     swiglu_packed_fp8,

@@ -94,6 +94,9 @@ SIGNATURES = {
     "fma_swiglu_experts_fp8": (_i32, [_p] * 3 + [_i32] + [_p] * 5 + [_i64] * 5 + [_i32, _p, _i64, _p, _i64, _i32, _p]),
     "fma_swiglu_experts_fp8_bwd_workspace_bytes": (_i64, [_i64] * 4),
     "fma_swiglu_experts_fp8_bwd": (_i32, [_p] * 3 + [_i32] + [_p] * 5 + [_i64] + [_p] * 4 + [_i64] * 5 + [_p, _i64, _i32, _p]),
+    "fma_router_loss_workspace_bytes": (_i64, [_i64] * 2),
+    "fma_router_loss": (_i32, [_p] * 2 + [_i64] * 3 + [_p] * 5 + [_i64, _i32, _p]),
+    "fma_router_loss_bwd": (_i32, [_p] * 2 + [_i64] * 2 + [_p] * 4 + [_i32, _p]),
     "fma_grad_norm_workspace_bytes": (_i64, [_i64]),
     "fma_grad_norm": (_i32, [_p] * 3 + [_i64, _i32, _p, _p, _i64, _p]),
     "fma_scale_grads": (_i32, [_p] * 3 + [_i64, _p, _f64, _p]),

@@ -14,6 +14,7 @@ import torch.nn.functional as F
 from torch.autograd import forward_ad
 
 from ...kernel_backend import KernelBackend, is_hip_kernel_backend
+from ...ops.router_loss import router_loss
 from ...ops.swiglu import swiglu_packed
 from .fp8_implementation import quantize_expert_weights, requantize_expert_weights, swiglu_experts_fp8
 from .cuda_implementation import (
@@ -275,6 +276,13 @@ class MoE(nn.Module):
         hidden_states = hidden_states.view(original_shape)
 
         return hidden_states, router_logits
+
+    def router_loss(
+        self, router_logits: torch.Tensor, mask: torch.Tensor | None = None
+    ) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+        """router_loss of the logits that forward returned: balance loss, z loss and tokens per expert. mask: False for tokens that do not
+        count (padding), in the shape of the tokens that forward took."""
+        return router_loss(router_logits, self.top_k, mask)
 
     def _router_is_fusable(self, hidden_states: torch.Tensor, gate_weight: torch.Tensor | None = None) -> bool:
         # the last three lines are the size limits of fma_router_topk (32-bit offsets into logits and choices): larger

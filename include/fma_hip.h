@@ -501,6 +501,21 @@ int fma_swiglu_experts_fp8_bwd(const void* dy, const void* gates, const void* id
                                void* dW1, void* dW2, int64_t T, int64_t top_k, int64_t E, int64_t H, int64_t I, void* workspace,
                                int64_t workspace_bytes, int dtype, void* stream);
 
+/* ---- losses on the router's logits ---------------------------------------------------------------- */
+
+/* logits [T, E] of dtype (any alignment to its elements), mask: a byte per token or NULL; tokens whose byte is 0 are not looked at. With
+ * p_t = softmax(logits_t), N tokens counted and c_e those among whose top_k largest logits expert e is (equal logits: the lowest expert
+ * first, NaN above everything):
+ *   balance = E / (top_k N^2) sum_e c_e sum_t p_te,   z = 1 / N sum_t logsumexp(logits_t)^2,   counts[e] = c_e
+ * balance, z: one float; counts: E uint32; table: E + 1 floats for the backward call. Without tokens all are 0. T < 2^31, E <= FMA_MAX_GROUPS.
+ * workspace: 8-byte aligned, no initialisation. Sums over tokens have a fixed order. No counterpart in the reference.
+ * Backward: logits_grad [T, E] (0 in rows that are not counted) for the gradients *balance_grad and *z_grad (device; NULL: 0). */
+int64_t fma_router_loss_workspace_bytes(int64_t T, int64_t E);
+int fma_router_loss(const void* logits, const uint8_t* mask, int64_t T, int64_t E, int64_t top_k, float* balance, float* z, uint32_t* counts,
+                    float* table, void* workspace, int64_t workspace_bytes, int dtype, void* stream);
+int fma_router_loss_bwd(const void* logits, const uint8_t* mask, int64_t T, int64_t E, const float* table, const float* balance_grad,
+                        const float* z_grad, void* logits_grad, int dtype, void* stream);
+
 /* ---- norm and clipping of gradients ------------------------------------------------------------- */
 
 /* The norm of `count` tensors together, sqrt of the sum of all squares or (infinity != 0) the largest magnitude, to *norm (device).
