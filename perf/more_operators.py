@@ -236,7 +236,8 @@ def _own(s):
             with torch.no_grad():
                 normed, stream = fma.fused_sandwich_rmsnorm(*(s[n] for n in names[:4]), EPS, s["gate"], s["multiplier"])
             return dict(normed=normed, stream=stream)
-        t = {n: _leaf(s[n]) for n in names}
+        # in float32 the leaves are the state's tensors, as in the plain form: gradients add up over passes, as in a program that accumulates them
+        t = {n: s[n].requires_grad_() if s["x"].dtype is torch.float32 and s[n] is not None else _leaf(s[n]) for n in names}
         normed, stream = fma.fused_sandwich_rmsnorm(*(t[n] for n in names[:4]), EPS, t["gate"], s["multiplier"])
         torch.autograd.backward([normed, stream], s["grads"])
         grads = {n + "_grad": t[n].grad for n in names if t[n] is not None}
