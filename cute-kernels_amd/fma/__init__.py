@@ -11,6 +11,7 @@ from .ops import (
     continuous_count,
     dequantize_fp8,
     fused_residual_add_rmsnorm,
+    fused_sandwich_rmsnorm,
     get_total_norm,
     grouped_gemm,
     grouped_gemm_fp8,

@@ -97,6 +97,9 @@ SIGNATURES = {
     "fma_router_loss_workspace_bytes": (_i64, [_i64] * 2),
     "fma_router_loss": (_i32, [_p] * 2 + [_i64] * 3 + [_p] * 5 + [_i64, _i32, _p]),
     "fma_router_loss_bwd": (_i32, [_p] * 2 + [_i64] * 2 + [_p] * 4 + [_i32, _p]),
+    "fma_sandwich_rmsnorm_fwd": (_i32, [_p] * 5 + [_i64] * 2 + [_p] * 3 + [_i64] * 2 + [_f32] * 2 + [_i32, _p]),
+    "fma_sandwich_rmsnorm_bwd_workspace_bytes": (_i64, [_i64] * 4),
+    "fma_sandwich_rmsnorm_bwd": (_i32, [_p] * 5 + [_i64] * 2 + [_p] * 8 + [_i64] * 2 + [_f32, _p, _i64, _i32, _p]),
     "fma_grad_norm_workspace_bytes": (_i64, [_i64]),
     "fma_grad_norm": (_i32, [_p] * 3 + [_i64, _i32, _p, _p, _i64, _p]),
     "fma_scale_grads": (_i32, [_p] * 3 + [_i64, _p, _f64, _p]),

@@ -1,0 +1,109 @@
+"""`fused_sandwich_rmsnorm`: what a transformer block with a norm on either side does at its end, in one pass over the rows:
+
+    stream = residual + multiplier * gate * rms_norm(x) * post_weight
+    output = rms_norm(stream) * weight                                    the next block's input
+
+The reference has no counterpart; its fused_residual_add_rmsnorm (fma/ops/fused_residual_add_rmsnorm/__init__.py) is the block's end without
+the norm behind it."""
+
+import torch
+from torch.autograd.function import once_differentiable
+
+from ...kernel_backend import KernelBackend, is_hip_kernel_backend
+from .cuda_implementation import fused_sandwich_rmsnorm_backward_cuda, fused_sandwich_rmsnorm_forward_cuda
+
+_FLOATS = (torch.float32, torch.float16, torch.bfloat16)
+
+
+def gate_rows(gate: torch.Tensor, x: torch.Tensor) -> int:
+    """How many rows the gate has; each serves the same number of neighbouring rows of x. Raises AssertionError for any other gate."""
+    shape = (1,) * (x.dim() - gate.dim()) + tuple(gate.shape)
+    fits = gate.dim() <= x.dim() and shape[-1] in (1, x.size(-1))
+    # from the left: dimensions of x, then ones
+    rows, shared = 1, False
+    for n, m in zip(shape[:-1], x.shape[:-1]) if fits else ():
+        fits = fits and n in (1, m) and not (shared and n > 1)
+        shared = shared or n != m
+        rows *= n
+    assert fits, (
+        f"a gate of shape {tuple(gate.shape)} does not fit x of shape {tuple(x.shape)}: its leading dimensions should be those of x up to some "
+        "point and 1 from there on, its last one 1 or that of x"
+    )
+    return rows
+
+
+class _FusedSandwichRMSNorm(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, residual, post_weight, weight, gate, eps, multiplier, grad_enabled):
+        x, residual = x.contiguous(), residual.contiguous()
+        post_weight, weight, gate = (t if t is None else t.contiguous() for t in (post_weight, weight, gate))
+        output, stream = torch.empty_like(x), torch.empty_like(x)
+        keep = grad_enabled and any(ctx.needs_input_grad)
+        rows = x.numel() // x.size(-1)
+        stats = x.new_empty(2, rows, dtype=torch.float32) if keep else None  # 1 / rms of every row of x and of the stream
+        fused_sandwich_rmsnorm_forward_cuda(
+            x, residual, post_weight, weight, gate, output, stream, stats, 0 if gate is None else gate_rows(gate, x), eps, multiplier
+        )
+        if keep:
+            ctx.save_for_backward(x, stream, post_weight, weight, gate, stats)
+            ctx.multiplier = multiplier
+        ctx.set_materialize_grads(False)
+        return output, stream
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, output_grad, stream_grad):
+        if output_grad is None and stream_grad is None:
+            return (None,) * 8
+        x, stream, post_weight, weight, gate, stats = ctx.saved_tensors
+        output_grad, stream_grad = (t if t is None else t.contiguous() for t in (output_grad, stream_grad))
+        x_grad, residual_grad = torch.empty_like(x), torch.empty_like(x)
+        needs = ctx.needs_input_grad[2:5]
+        # (without rows the sums over them are zero)
+        new = torch.empty_like if x.numel() else torch.zeros_like
+        post_weight_grad, weight_grad, gate_grad = (new(t) if n else None for t, n in zip((post_weight, weight, gate), needs))
+        if x.numel():
+            fused_sandwich_rmsnorm_backward_cuda(
+                x, stream, post_weight, weight, gate, output_grad, stream_grad, stats, x_grad, residual_grad, post_weight_grad, weight_grad,
+                gate_grad, 0 if gate is None else gate_rows(gate, x), ctx.multiplier,
+            )  # fmt: skip
+        return x_grad, residual_grad, post_weight_grad, weight_grad, gate_grad, None, None, None
+
+
+def fused_sandwich_rmsnorm(
+    x: torch.Tensor,
+    residual: torch.Tensor,
+    post_weight: torch.Tensor | None,
+    weight: torch.Tensor | None,
+    eps: float | None,
+    gate: torch.Tensor | None = None,
+    multiplier: float | None = None,
+    kernel_backend: KernelBackend = KernelBackend.triton,
+) -> tuple[torch.Tensor, torch.Tensor]:
+    """Returns (the next block's normalised input, the updated residual stream), both shaped and typed like x.
+
+    x: the block's output; residual: the stream of the same shape; float32, float16 or bfloat16, rows along the last dimension, at most 65536
+    long. post_weight, weight: 1-D scales of the norm behind the block and of the one before the next, or None. eps: added to both mean
+    squares; None takes the dtype's machine epsilon. gate: multiplies the normed output; of x's dtype and, from the left, of x's dimensions up
+    to some point and 1 from there on, the last one 1 or x's (dimensions of 1 may be left out in front): a scale per element (x's shape), per
+    channel ([H]), per token ([.., 1]), per sequence and channel ([batch, 1, H]), or a single number. multiplier: the residual scale; None means 1.
+    Arithmetic is in float32 with one rounding per output, the second norm is taken of the unrounded stream, and the backward
+    pass (once; no second derivatives) starts from the rounded one. kernel_backend: `triton` (the default) and `cuda` both run the HIP
+    kernels; anything else raises ValueError.
+    """
+    if not is_hip_kernel_backend(kernel_backend):
+        raise ValueError(f"unexpected kernel_backend ({kernel_backend})")
+    assert x.dtype in _FLOATS, f"fused_sandwich_rmsnorm takes float32, float16 and bfloat16, not {x.dtype}"
+    assert x.dim() >= 1 and x.size(-1) > 0, "x should have rows of one element at least"
+    assert residual.shape == x.shape and residual.dtype == x.dtype, "x and residual should be of one shape and dtype"
+    for name, w in (("post_weight", post_weight), ("weight", weight)):
+        assert w is None or (w.shape == x.shape[-1:] and w.dtype == x.dtype), f"{name} should be 1-D, of x's row length and dtype"
+    if gate is not None:
+        assert gate.dtype == x.dtype, "gate should have x's dtype"
+        gate_rows(gate, x)
+    for t in (residual, post_weight, weight, gate):
+        assert t is None or t.device == x.device, "all tensors should be on one device"
+    eps = torch.finfo(x.dtype).eps if eps is None else float(eps)
+    return _FusedSandwichRMSNorm.apply(
+        x, residual, post_weight, weight, gate, eps, 1.0 if multiplier is None else float(multiplier), torch.is_grad_enabled()
+    )

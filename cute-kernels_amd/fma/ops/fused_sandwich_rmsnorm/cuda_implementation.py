@@ -1,0 +1,66 @@
+"""Custom ops over fma_sandwich_rmsnorm_fwd and fma_sandwich_rmsnorm_bwd of libfma_hip.so."""
+
+import torch
+
+from ... import _lib
+from ..._ops import hip_op
+
+
+def _check(x: torch.Tensor, like_x: tuple, post_weight, weight, gate, gate_rows: int, stats) -> tuple[int, int, int]:
+    B, H = x.numel() // x.size(-1), x.size(-1)
+    for t in like_x:
+        assert t is None or (t.shape == x.shape and t.dtype == x.dtype and t.is_contiguous() and t.device == x.device)
+    for t in (post_weight, weight):
+        assert t is None or (t.shape == (H,) and t.dtype == x.dtype and t.is_contiguous() and t.device == x.device)
+    gate_width = 0
+    if gate is not None:
+        assert gate.dtype == x.dtype and gate.is_contiguous() and gate.device == x.device
+        gate_width = gate.size(-1) if gate.dim() else 1
+        assert gate.numel() == gate_rows * gate_width and gate_width in (1, H)
+    assert stats is None or (stats.shape == (2, B) and stats.dtype == torch.float32 and stats.is_contiguous() and stats.device == x.device)
+    return B, H, gate_width
+
+
+@hip_op("fused_sandwich_rmsnorm_forward_cuda", mutates_args={"output", "stream", "stats"})
+def fused_sandwich_rmsnorm_forward_cuda(
+    x: torch.Tensor, residual: torch.Tensor, post_weight: torch.Tensor | None, weight: torch.Tensor | None, gate: torch.Tensor | None,
+    output: torch.Tensor, stream: torch.Tensor, stats: torch.Tensor | None, gate_rows: int, eps: float, multiplier: float,
+) -> None:  # fmt: skip
+    _lib.require_gpu(x, residual, post_weight, weight, gate, output, stream, stats)
+    B, H, gate_width = _check(x, (x, residual, output, stream), post_weight, weight, gate, gate_rows, stats)
+    if B == 0:
+        return
+    with _lib.on_device(x.device):
+        rc = _lib.load().fma_sandwich_rmsnorm_fwd(
+            x.data_ptr(), residual.data_ptr(), _lib.ptr(post_weight), _lib.ptr(weight), _lib.ptr(gate), gate_rows, gate_width,
+            output.data_ptr(), stream.data_ptr(), _lib.ptr(stats), B, H, eps, multiplier, _lib.dtype_code(x.dtype),
+            _lib.current_stream(x.device),
+        )  # fmt: skip
+    _lib.check(rc, "fused_sandwich_rmsnorm_forward_cuda")
+
+
+@hip_op("fused_sandwich_rmsnorm_backward_cuda", mutates_args={"x_grad", "residual_grad", "post_weight_grad", "weight_grad", "gate_grad"})
+def fused_sandwich_rmsnorm_backward_cuda(
+    x: torch.Tensor, stream: torch.Tensor, post_weight: torch.Tensor | None, weight: torch.Tensor | None, gate: torch.Tensor | None,
+    output_grad: torch.Tensor | None, stream_grad: torch.Tensor | None, stats: torch.Tensor, x_grad: torch.Tensor,
+    residual_grad: torch.Tensor, post_weight_grad: torch.Tensor | None, weight_grad: torch.Tensor | None, gate_grad: torch.Tensor | None,
+    gate_rows: int, multiplier: float,
+) -> None:  # fmt: skip
+    _lib.require_gpu(
+        x, stream, post_weight, weight, gate, output_grad, stream_grad, stats, x_grad, residual_grad, post_weight_grad, weight_grad, gate_grad
+    )
+    like_x = (x, stream, output_grad, stream_grad, x_grad, residual_grad)
+    B, H, gate_width = _check(x, like_x, post_weight, weight, gate, gate_rows, stats)
+    for grad, t in ((post_weight_grad, post_weight), (weight_grad, weight), (gate_grad, gate)):
+        assert grad is None or (grad.shape == t.shape and grad.dtype == x.dtype and grad.is_contiguous() and grad.device == x.device)
+    lib = _lib.load()
+    with _lib.on_device(x.device):
+        nbytes = lib.fma_sandwich_rmsnorm_bwd_workspace_bytes(B, H, gate_rows, gate_width)
+        workspace = torch.empty(nbytes, dtype=torch.uint8, device=x.device)
+        rc = lib.fma_sandwich_rmsnorm_bwd(
+            x.data_ptr(), stream.data_ptr(), _lib.ptr(post_weight), _lib.ptr(weight), _lib.ptr(gate), gate_rows, gate_width,
+            _lib.ptr(output_grad), _lib.ptr(stream_grad), stats.data_ptr(), x_grad.data_ptr(), residual_grad.data_ptr(), _lib.ptr(gate_grad),
+            _lib.ptr(post_weight_grad), _lib.ptr(weight_grad), B, H, multiplier, workspace.data_ptr(), nbytes, _lib.dtype_code(x.dtype),
+            _lib.current_stream(x.device),
+        )  # fmt: skip
+    _lib.check(rc, "fused_sandwich_rmsnorm_backward_cuda")
