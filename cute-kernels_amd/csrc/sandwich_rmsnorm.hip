@@ -22,7 +22,17 @@ namespace {
 
 constexpr int kThreads = 256;
 constexpr int kWaves = kThreads / kWave;
-constexpr int kBwdPerCU = 2;
+// Threads of the forward pass per compute unit, each with its share of a row and of the next one. us with 512 to 1024 / 2048, bf16:
+// [16384, 4096] 87 / 94, [16384, 2048] 48 / 56, [8188, 2880] with a full gate 41 / 52; a workgroup per row, which ends with it, 110, 60 and 63.
+constexpr int kFwdThreadsPerCU = 1024;
+// teams of a workgroup: those of one wavefront meet at no barrier, four of them make a workgroup
+constexpr int teams_of(int team) { return team == kWave ? 4 : 1; }
+// Teams of the backward pass per compute unit, each with a row in its registers and one on the way: 512 threads. More of them add partial sums
+// and gain no rate (us with a third / half / all of 1536 threads, bf16: [16384, 4096] 133 / 145 / 145, [16384, 2048] 78 / 73 / 81,
+// [8188, 2880] 53 / 58 / 66, [32768, 512] 40 / 45 / -), and at least two rows for each ([300, 4096] 13.5 / 11.9 / 12.9 us with one / two / four,
+// [1021, 2048] 14.6 / 15.1 / 13.6).
+constexpr int workers_per_cu(int team) { return team < 512 ? 512 / team : 1; }
+constexpr int kBwdMinRows = 2;
 
 // how rows of x share a row of the gate; decides what is summed for its gradient
 enum Mode {
@@ -48,14 +58,17 @@ Shape shape_of(int64_t B, int64_t H, int64_t gate_rows, int64_t gate_width) {
     return s;
 }
 
-// The workgroups of the backward pass: `parts` for each of `groups` of neighbouring rows (one group unless the gate has several rows that
-// serve several rows each), or, with more groups than workgroups are wanted, whole groups for each.
+// The workers of the backward pass: `parts` for each of `groups` of neighbouring rows (one group unless the gate has several rows that
+// serve several rows each), or, with more groups than workers are wanted, whole groups for each.
 struct Split {
-    int64_t groups, rows, parts, workgroups;
+    int64_t groups, rows, parts, workers;
+    int64_t sums;  // rows of partial sums: workgroups
 };
-Split split_of(const Shape& s) {
-    const int64_t cus = num_compute_units() > 0 ? num_compute_units() : 256, want = cus * kBwdPerCU;
-    Split p{1, s.B, 1, 1};
+Split split_of(const Shape& s, int team, int teams) {
+    const int64_t cus = num_compute_units() > 0 ? num_compute_units() : 256;
+    int64_t want = cus * workers_per_cu(team);
+    if (want > s.B / kBwdMinRows) want = s.B / kBwdMinRows > 0 ? s.B / kBwdMinRows : 1;
+    Split p{1, s.B, 1, 1, 1};
     if (s.mode == kGroup) {
         p.groups = s.B / s.R;
         p.rows = s.R;
@@ -63,25 +76,31 @@ Split split_of(const Shape& s) {
     p.parts = want / p.groups;
     if (p.parts > p.rows) p.parts = p.rows;
     if (p.parts < 1) p.parts = 1;
-    p.workgroups = p.parts > 1 || p.groups <= want ? p.groups * p.parts : want;
+    p.workers = p.parts > 1 || p.groups <= want ? p.groups * p.parts : want;
+    p.sums = (p.workers + teams - 1) / teams;
     return p;
 }
 
-// the workspace: partial sums [workgroups, H] for dw, dw_post and (kGroup) dgate, one number per row (kScalar)
+// the workspace: partial sums [sums, H] for dw and dw_post, [workers, H] for dgate (kGroup), one number per row (kScalar)
 struct Partial {
     float *w, *wp, *gate, *rows;
 };
 Partial partial_of(void* workspace, const Shape& s, const Split& p) {
-    const int64_t n = p.workgroups * s.H;
     Partial part;
     part.w = (float*)workspace;
-    part.wp = part.w + n;
-    part.gate = part.wp + n;
-    part.rows = part.wp + n;
+    part.wp = part.w + p.sums * s.H;
+    part.gate = part.rows = part.wp + p.sums * s.H;  // (never both)
     return part;
 }
+// enough for every type and alignment
 int64_t workspace_bytes_of(const Shape& s) {
-    return 4 * (split_of(s).workgroups * s.H * (s.mode == kGroup ? 3 : 2) + (s.mode == kScalar ? s.B : 0));
+    int64_t most = 0;
+    for (int team : {64, 256, 1024}) {
+        const Split p = split_of(s, team, teams_of(team));
+        const int64_t n = p.sums * s.H * 2 + (s.mode == kGroup ? p.workers * s.H : 0) + (s.mode == kScalar ? s.B : 0);
+        most = n > most ? n : most;
+    }
+    return 4 * most;
 }
 
 __device__ __forceinline__ float inverse_rms(float sum_of_squares, float inv_H, float eps) {
@@ -127,6 +146,8 @@ __device__ __forceinline__ float at(const T* p, int64_t i) {
     return p ? Num<T>::up(p[i]) : 1.0f;
 }
 
+__device__ __forceinline__ int64_t gate_row(const Shape& s, int64_t row) { return (uint32_t)row / (uint32_t)s.R; }  // (both below 2^31)
+
 // ---- any H, any alignment: element by element -----------------------------------------------------------------------------
 
 template <typename T>
@@ -136,7 +157,7 @@ __global__ __launch_bounds__(kThreads) void sandwich_fwd_generic_kernel(const Fw
     const int64_t H = k.s.H;
     for (int64_t row = blockIdx.x; row < k.s.B; row += gridDim.x) {
         const int64_t base = row * H;
-        const T* const gate = k.gate ? k.gate + row / k.s.R * (k.s.mode == kScalar ? 1 : H) : nullptr;
+        const T* const gate = k.gate ? k.gate + gate_row(k.s, row) * (k.s.mode == kScalar ? 1 : H) : nullptr;
         const bool scalar = k.s.mode == kScalar;
         auto stream = [&](int64_t h, float inv_x) {
             const float n = Num<T>::up(k.x[base + h]) * inv_x * at(k.post_weight, h);
@@ -186,7 +207,7 @@ __global__ __launch_bounds__(kThreads) void sandwich_bwd_generic_kernel(const Bw
         for (int64_t i = part; i < k.p.rows; i += k.p.parts) {
             const int64_t row = group * k.p.rows + i, base = row * H;
             const bool scalar = k.s.mode == kScalar;
-            const T* const gate = k.gate ? k.gate + row / k.s.R * (scalar ? 1 : H) : nullptr;
+            const T* const gate = k.gate ? k.gate + gate_row(k.s, row) * (scalar ? 1 : H) : nullptr;
             const float inv_x = k.stats[row], inv_r = k.stats[k.s.B + row];
             float dot = 0.f;
             if (k.d_out)
@@ -229,6 +250,389 @@ __global__ __launch_bounds__(kThreads) void sandwich_bwd_generic_kernel(const Bw
     }
 }
 
+// ---- rows of whole 16-byte vectors: a row in the registers of its team of threads -----------------------------------------------
+//
+// A team of TEAM threads per row, VPT vectors per thread, the next row requested before this one is worked on. All accesses of the loops are
+// buffer instructions, whose range check stands for every condition: past the row's end, behind the last row, where a tensor is absent
+// (num_records 0), loads give zeros and stores go nowhere. A branch around a load or a store would make the compiler wait for everything
+// that is outstanding, the next row included, since it cannot count what lies behind.
+
+template <int CTRL>
+__device__ __forceinline__ float dpp_add(float v) {
+    return v + __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, v), CTRL, 0xf, 0xf, false));
+}
+// the sum over a wavefront, in all lanes: 16 lanes by data-parallel moves, the four rows of 16 through scalar registers
+__device__ __forceinline__ float wave_total(float v) {
+    v = dpp_add<0xb1>(v);
+    v = dpp_add<0x4e>(v);
+    v = dpp_add<0x141>(v);
+    v = dpp_add<0x140>(v);
+    auto lane = [&](int i) { return __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, v), i)); };
+    return (lane(0) + lane(16)) + (lane(32) + lane(48));
+}
+template <int TEAM>
+__device__ __forceinline__ float team_sum(float v, float (*slots)[TEAM / kWave], int& parity) {
+    v = wave_total(v);
+    if constexpr (TEAM > kWave) {
+        float* const slot = slots[parity];
+        parity ^= 1;
+        if ((threadIdx.x & (kWave - 1)) == 0) slot[threadIdx.x / kWave] = v;
+        __syncthreads();
+        v = 0.f;
+#pragma unroll
+        for (int w = 0; w < TEAM / kWave; ++w) v += slot[w];
+    }
+    return v;
+}
+
+// Sixteen bytes of a row as they are in memory. They stay that way in the registers and are widened where they are used: as an array of
+// 16-bit elements the compiler would hold each of them in a register of its own.
+typedef __attribute__((ext_vector_type(4))) uint32_t Raw;
+
+template <typename T>
+struct Wide;
+template <>
+struct Wide<float> {
+    static constexpr int N = 4;
+    static constexpr uint32_t kOnes = 0x3f800000u;
+    static __device__ __forceinline__ float up(const Raw& r, int e) { return __uint_as_float(r[e]); }
+    static __device__ __forceinline__ Raw down(const float (&f)[N]) {
+        return Raw{__float_as_uint(f[0]), __float_as_uint(f[1]), __float_as_uint(f[2]), __float_as_uint(f[3])};
+    }
+};
+template <>
+struct Wide<bf16_t> {
+    static constexpr int N = 8;
+    static constexpr uint32_t kOnes = 0x3f803f80u;
+    typedef __attribute__((ext_vector_type(2))) float f32x2;
+    typedef __attribute__((ext_vector_type(2))) __bf16 bf16x2;
+    static __device__ __forceinline__ float up(const Raw& r, int e) {
+        return __uint_as_float(e & 1 ? r[e / 2] & 0xffff0000u : r[e / 2] << 16);
+    }
+    static __device__ __forceinline__ uint32_t pair(float a, float b) {
+        return __builtin_bit_cast(uint32_t, __builtin_convertvector((f32x2{a, b}), bf16x2));
+    }
+    static __device__ __forceinline__ Raw down(const float (&f)[N]) {
+        return Raw{pair(f[0], f[1]), pair(f[2], f[3]), pair(f[4], f[5]), pair(f[6], f[7])};
+    }
+};
+template <>
+struct Wide<f16_t> {
+    static constexpr int N = 8;
+    static constexpr uint32_t kOnes = 0x3c003c00u;
+    typedef __attribute__((ext_vector_type(2))) _Float16 f16x2;
+    static __device__ __forceinline__ float up(const Raw& r, int e) {
+        const uint32_t two = r[e / 2];  // (a bit cast of the vector's element itself takes the vector's first one)
+        return (float)__builtin_bit_cast(f16x2, two)[e & 1];
+    }
+    static __device__ __forceinline__ uint32_t pair(float a, float b) { return __builtin_bit_cast(uint32_t, (f16x2{(_Float16)a, (_Float16)b})); }
+    static __device__ __forceinline__ Raw down(const float (&f)[N]) {
+        return Raw{pair(f[0], f[1]), pair(f[2], f[3]), pair(f[4], f[5]), pair(f[6], f[7])};
+    }
+};
+
+constexpr int kStream = 2;                // cache policy: non-temporal
+constexpr uint32_t kNowhere = 0x7fffffffu;  // an offset past every buffer
+
+// `bytes` at p; nothing where p is NULL. p and bytes are the same in all lanes.
+__device__ __forceinline__ __amdgpu_buffer_rsrc_t buffer_of(const void* p, uint32_t bytes) {
+    return __builtin_amdgcn_make_buffer_rsrc(const_cast<void*>(p), 0, p ? (int)bytes : 0, 0x00020000);
+}
+template <int TEAM, int VPT, int POLICY>
+__device__ __forceinline__ void load_row(Raw (&to)[VPT], __amdgpu_buffer_rsrc_t row, int tid) {
+#pragma unroll
+    for (int i = 0; i < VPT; ++i) to[i] = __builtin_amdgcn_raw_buffer_load_b128(row, (tid + i * TEAM) * 16, 0, POLICY);
+}
+template <typename T>
+__device__ __forceinline__ void store_row(__amdgpu_buffer_rsrc_t row, int v, const float (&f)[Wide<T>::N]) {
+    __builtin_amdgcn_raw_buffer_store_b128(Wide<T>::down(f), row, v * 16, 0, kStream);
+}
+__device__ __forceinline__ float load_float(__amdgpu_buffer_rsrc_t b, uint32_t offset) {
+    return __uint_as_float(__builtin_amdgcn_raw_buffer_load_b32(b, (int)offset, 0, 0));
+}
+__device__ __forceinline__ void store_float(__amdgpu_buffer_rsrc_t b, uint32_t offset, float v) {
+    __builtin_amdgcn_raw_buffer_store_b32(__float_as_uint(v), b, (int)offset, 0, 0);
+}
+template <typename T>
+__device__ __forceinline__ float load_element(__amdgpu_buffer_rsrc_t b) {
+    if constexpr (sizeof(T) == 4) return load_float(b, 0);
+    else return Num<T>::up(__builtin_bit_cast(T, (uint16_t)__builtin_amdgcn_raw_buffer_load_b16(b, 0, 0, 0)));
+}
+template <typename T>
+__device__ __forceinline__ void store_element(__amdgpu_buffer_rsrc_t b, uint32_t offset, float v) {
+    if constexpr (sizeof(T) == 4) store_float(b, offset, v);
+    else __builtin_amdgcn_raw_buffer_store_b16(__builtin_bit_cast(uint16_t, Num<T>::down(v)), b, (int)offset, 0, 0);
+}
+
+// a thread's share of a weight, kept over all rows: ones where there is none
+template <typename T, int TEAM, int VPT>
+__device__ __forceinline__ void load_weight(Raw (&to)[VPT], const T* p, uint32_t bytes, int tid) {
+    load_row<TEAM, VPT, 0>(to, buffer_of(p, bytes), tid);
+    if (!p) {
+#pragma unroll
+        for (int i = 0; i < VPT; ++i) to[i] = Wide<T>::kOnes;
+    }
+}
+// Keeps the compiler from widening once and holding the wide values over a barrier
+template <int VPT>
+__device__ __forceinline__ void stay_packed(Raw (&a)[VPT]) {
+#pragma unroll
+    for (int i = 0; i < VPT; ++i) asm volatile("" : "+v"(a[i]));
+}
+
+// index of a team, the same in all of its lanes and known to be
+template <int TEAM>
+__device__ __forceinline__ int64_t team_index() {
+    if constexpr (teams_of(TEAM) == 1) return blockIdx.x;
+    else return (int64_t)blockIdx.x * teams_of(TEAM) + __builtin_amdgcn_readfirstlane((int)(threadIdx.x / TEAM));
+}
+
+template <typename T, int TEAM, int VPT, Mode MODE>
+__global__ __launch_bounds__(TEAM * teams_of(TEAM)) void sandwich_fwd_kernel(const FwdArgs<T> k) {
+    constexpr int N = Wide<T>::N;
+    constexpr bool kVector = MODE == kFull || MODE == kGroup;
+    __shared__ float s_red[2][TEAM / kWave];
+    int parity = 0;
+    const int tid = threadIdx.x % TEAM;
+    const int64_t H = k.s.H, step = (int64_t)gridDim.x * teams_of(TEAM);
+    const uint32_t bytes = (uint32_t)(H * (int64_t)sizeof(T)), first_lane = tid == 0 ? 0u : kNowhere;
+    Raw wp[VPT], w[VPT];
+    load_weight<T, TEAM, VPT>(wp, k.post_weight, bytes, tid);
+    load_weight<T, TEAM, VPT>(w, k.weight, bytes, tid);
+    struct Row {
+        Raw x[VPT], r[VPT], gate[VPT];
+        float scalar;
+    } now, next;
+    auto fetch = [&](Row& to, int64_t row) {
+        const uint32_t n = row < k.s.B ? bytes : 0u;
+        load_row<TEAM, VPT, kStream>(to.x, buffer_of(k.x + row * H, n), tid);
+        load_row<TEAM, VPT, kStream>(to.r, buffer_of(k.residual + row * H, n), tid);
+        if constexpr (MODE == kFull) load_row<TEAM, VPT, kStream>(to.gate, buffer_of(k.gate + row * H, n), tid);
+        if constexpr (MODE == kGroup) load_row<TEAM, VPT, 0>(to.gate, buffer_of(k.gate + gate_row(k.s, row) * H, n), tid);
+        if constexpr (MODE == kScalar) to.scalar = load_element<T>(buffer_of(k.gate + gate_row(k.s, row), n ? (uint32_t)sizeof(T) : 0u));
+    };
+    int64_t row = team_index<TEAM>();
+    fetch(now, row);
+    for (; row < k.s.B; row += step) {
+        const int64_t base = row * H;
+        fetch(next, row + step);
+        float ss = 0.f;
+#pragma unroll
+        for (int i = 0; i < VPT; ++i)
+#pragma unroll
+            for (int e = 0; e < N; ++e) {
+                const float v = Wide<T>::up(now.x[i], e);
+                ss += v * v;
+            }
+        const float inv_x = inverse_rms(team_sum<TEAM>(ss, s_red, parity), k.inv_H, k.eps);
+        const float a = MODE == kScalar ? k.a * now.scalar : k.a;
+        const __amdgpu_buffer_rsrc_t to_stream = buffer_of(k.stream + base, bytes), to_out = buffer_of(k.out + base, bytes);
+        float f[VPT][N];
+        ss = 0.f;
+#pragma unroll
+        for (int i = 0; i < VPT; ++i) {
+            const int v = tid + i * TEAM;
+#pragma unroll
+            for (int e = 0; e < N; ++e) {
+                float n = Wide<T>::up(now.x[i], e) * inv_x * Wide<T>::up(wp[i], e);
+                if constexpr (kVector) n *= Wide<T>::up(now.gate[i], e);
+                f[i][e] = Wide<T>::up(now.r[i], e) + a * n;
+                ss += f[i][e] * f[i][e];
+            }
+            store_row<T>(to_stream, v, f[i]);
+        }
+        const float inv_r = inverse_rms(team_sum<TEAM>(ss, s_red, parity), k.inv_H, k.eps);
+#pragma unroll
+        for (int i = 0; i < VPT; ++i) {
+            float o[N];
+#pragma unroll
+            for (int e = 0; e < N; ++e) o[e] = f[i][e] * inv_r * Wide<T>::up(w[i], e);
+            store_row<T>(to_out, tid + i * TEAM, o);
+        }
+        store_float(buffer_of(k.stats ? k.stats + row : nullptr, 4), first_lane, inv_x);
+        store_float(buffer_of(k.stats ? k.stats + k.s.B + row : nullptr, 4), first_lane, inv_r);
+        now = next;
+    }
+}
+
+template <typename T, int TEAM, int VPT, Mode MODE>
+__global__ __launch_bounds__(TEAM * teams_of(TEAM)) void sandwich_bwd_kernel(const BwdArgs<T> k) {
+    constexpr int N = Wide<T>::N, kTeams = teams_of(TEAM);
+    constexpr bool kAhead = TEAM * VPT <= 1024;  // (two vectors for each of 1024 threads leave no registers for a second row)
+    constexpr bool kVector = MODE == kFull || MODE == kGroup || MODE == kChannel;
+    __shared__ float s_red[2][TEAM / kWave];
+    int parity = 0;
+    const int tid = threadIdx.x % TEAM;
+    const int64_t H = k.s.H, worker = team_index<TEAM>();
+    const uint32_t bytes = (uint32_t)(H * (int64_t)sizeof(T)), first_lane = tid == 0 ? 0u : kNowhere;
+    Raw wp[VPT], w[VPT], channel[VPT];
+    load_weight<T, TEAM, VPT>(wp, k.post_weight, bytes, tid);
+    load_weight<T, TEAM, VPT>(w, k.weight, bytes, tid);
+    if constexpr (MODE == kChannel) load_row<TEAM, VPT, 0>(channel, buffer_of(k.gate, bytes), tid);
+    float sw[VPT][N], swp[VPT][N], sg[VPT][N];
+#pragma unroll
+    for (int i = 0; i < VPT; ++i)
+#pragma unroll
+        for (int e = 0; e < N; ++e) sw[i][e] = swp[i][e] = sg[i][e] = 0.f;
+
+    struct Row {
+        Raw x[VPT], r[VPT], dy[VPT], dr[VPT], gate[VPT];
+        float inv_x, inv_r, scalar;
+    } now, next;
+    auto fetch = [&](Row& to, int64_t row, bool in) {
+        const int64_t base = row * H;
+        const uint32_t n = in ? bytes : 0u, one = in ? 4u : 0u;
+        load_row<TEAM, VPT, kStream>(to.x, buffer_of(k.x + base, n), tid);
+        load_row<TEAM, VPT, kStream>(to.r, buffer_of(k.stream + base, n), tid);
+        load_row<TEAM, VPT, kStream>(to.dy, buffer_of(k.d_out ? k.d_out + base : nullptr, n), tid);
+        load_row<TEAM, VPT, kStream>(to.dr, buffer_of(k.d_stream ? k.d_stream + base : nullptr, n), tid);
+        if constexpr (MODE == kFull) load_row<TEAM, VPT, kStream>(to.gate, buffer_of(k.gate + base, n), tid);
+        if constexpr (MODE == kGroup) load_row<TEAM, VPT, 0>(to.gate, buffer_of(k.gate + gate_row(k.s, row) * H, n), tid);
+        if constexpr (MODE == kScalar) to.scalar = load_element<T>(buffer_of(k.gate + gate_row(k.s, row), in ? (uint32_t)sizeof(T) : 0u));
+        to.inv_x = load_float(buffer_of(k.stats + row, one), 0);
+        to.inv_r = load_float(buffer_of(k.stats + k.s.B + row, one), 0);
+    };
+    // the rows of a group `parts` apart, then the next group: rows in flight at the same time are neighbours in memory
+    const int64_t part = worker % k.p.parts, groups = k.p.workers / k.p.parts;
+    int64_t group = worker / k.p.parts, place = part;
+    bool more = worker < k.p.workers;
+    if constexpr (kAhead) fetch(now, group * k.p.rows + place, more);
+    while (more) {
+        const int64_t row = group * k.p.rows + place, base = row * H;
+        int64_t next_group = group, next_place = place + k.p.parts;
+        if (next_place >= k.p.rows) {
+            next_place = part;
+            next_group += groups;
+        }
+        more = next_group < k.p.groups;
+        if constexpr (kAhead) fetch(next, next_group * k.p.rows + next_place, more);
+        else fetch(now, row, true);
+
+        float dot = 0.f;
+#pragma unroll
+        for (int i = 0; i < VPT; ++i)
+#pragma unroll
+            for (int e = 0; e < N; ++e) dot += Wide<T>::up(now.dy[i], e) * Wide<T>::up(w[i], e) * Wide<T>::up(now.r[i], e);
+        const float c_r = team_sum<TEAM>(dot, s_red, parity) * now.inv_r * k.inv_H;
+        auto d_stream = [&](int i, int e, float dy, float rh) {
+            return Wide<T>::up(now.dr[i], e) + now.inv_r * (dy * Wide<T>::up(w[i], e) - rh * c_r);
+        };
+        auto gate = [&](int i, int e) {
+            if constexpr (MODE == kChannel) return Wide<T>::up(channel[i], e);
+            else return Wide<T>::up(now.gate[i], e);
+        };
+        auto stay = [&] {
+            stay_packed(now.x);
+            stay_packed(now.r);
+            stay_packed(now.dy);
+            stay_packed(now.dr);
+            stay_packed(w);
+            stay_packed(wp);
+            if constexpr (MODE == kChannel) stay_packed(channel);
+            else if constexpr (kVector) stay_packed(now.gate);
+        };
+        stay();
+        const float a = MODE == kScalar ? k.a * now.scalar : k.a;
+        const __amdgpu_buffer_rsrc_t to_residual = buffer_of(k.d_residual + base, bytes), to_x = buffer_of(k.dx + base, bytes);
+        dot = 0.f;
+#pragma unroll
+        for (int i = 0; i < VPT; ++i) {
+            float o[N];
+#pragma unroll
+            for (int e = 0; e < N; ++e) {
+                const float dy = Wide<T>::up(now.dy[i], e), rh = Wide<T>::up(now.r[i], e) * now.inv_r, dr = d_stream(i, e, dy, rh);
+                sw[i][e] += dy * rh;
+                float u = dr * Wide<T>::up(wp[i], e);
+                if constexpr (kVector) u *= gate(i, e);
+                dot += u * Wide<T>::up(now.x[i], e);
+                o[e] = dr;
+            }
+            store_row<T>(to_residual, tid + i * TEAM, o);
+        }
+        dot = team_sum<TEAM>(dot, s_red, parity) * now.inv_x;
+        if constexpr (MODE == kScalar) {
+            const bool own = k.d_gate && k.s.R == 1;  // the row's number is the gate's gradient, or one of those it sums
+            store_element<T>(buffer_of(own ? k.d_gate + row : nullptr, sizeof(T)), first_lane, k.a * dot);
+            store_float(buffer_of(own || !k.d_gate ? nullptr : k.part.rows + row, 4), first_lane, k.a * dot);
+        }
+        const float c_x = a * dot * k.inv_H;
+        stay();
+#pragma unroll
+        for (int i = 0; i < VPT; ++i) {
+            float o[N], og[N];
+#pragma unroll
+            for (int e = 0; e < N; ++e) {
+                const float xh = Wide<T>::up(now.x[i], e) * now.inv_x, p = Wide<T>::up(wp[i], e);
+                // (formed once more: kept over the barrier it would take a register per element)
+                const float dr = d_stream(i, e, Wide<T>::up(now.dy[i], e), Wide<T>::up(now.r[i], e) * now.inv_r);
+                const float dz = a * dr;  // (kScalar: a with the row's gate in it)
+                float gated = dz;
+                if constexpr (kVector) gated *= gate(i, e);
+                o[e] = now.inv_x * (gated * p - xh * c_x);
+                og[e] = dz * p * xh;
+                swp[i][e] += (MODE == kChannel ? dz : gated) * xh;
+                if constexpr (MODE == kGroup) sg[i][e] += dz * xh;
+            }
+            store_row<T>(to_x, tid + i * TEAM, o);
+            if constexpr (MODE == kFull) store_row<T>(buffer_of(k.d_gate ? k.d_gate + base : nullptr, bytes), tid + i * TEAM, og);
+        }
+        if constexpr (MODE == kGroup)
+            if (!more || next_group != group) {  // the group's sum is whole here, or this team's part of it
+                const __amdgpu_buffer_rsrc_t to_gate = buffer_of(k.d_gate && k.p.parts == 1 ? k.d_gate + group * H : nullptr, bytes);
+                const __amdgpu_buffer_rsrc_t to_part =
+                    buffer_of(k.d_gate && k.p.parts > 1 ? k.part.gate + worker * H : nullptr, (uint32_t)(H * 4));
+#pragma unroll
+                for (int i = 0; i < VPT; ++i) {
+                    const int v = tid + i * TEAM;
+                    float o[N];
+#pragma unroll
+                    for (int e = 0; e < N; ++e) {
+                        o[e] = sg[i][e] * Wide<T>::up(wp[i], e);
+                        store_float(to_part, (uint32_t)(v * N + e) * 4, sg[i][e]);
+                        sg[i][e] = 0.f;
+                    }
+                    store_row<T>(to_gate, v, o);
+                }
+            }
+        if constexpr (kAhead) now = next;
+        group = next_group;
+        place = next_place;
+    }
+    // the partial sums of a workgroup's teams together, in order
+    const __amdgpu_buffer_rsrc_t to_w = buffer_of(k.sums_w ? k.part.w + (int64_t)blockIdx.x * H : nullptr, (uint32_t)(H * 4));
+    const __amdgpu_buffer_rsrc_t to_wp = buffer_of(k.sums_wp ? k.part.wp + (int64_t)blockIdx.x * H : nullptr, (uint32_t)(H * 4));
+    if constexpr (kTeams == 1) {
+#pragma unroll
+        for (int i = 0; i < VPT; ++i)
+#pragma unroll
+            for (int e = 0; e < N; e += 4) {
+                auto four = [&](const float (&f)[N]) {
+                    return Raw{__float_as_uint(f[e]), __float_as_uint(f[e + 1]), __float_as_uint(f[e + 2]), __float_as_uint(f[e + 3])};
+                };
+                __builtin_amdgcn_raw_buffer_store_b128(four(sw[i]), to_w, ((tid + i * TEAM) * N + e) * 4, 0, 0);
+                __builtin_amdgcn_raw_buffer_store_b128(four(swp[i]), to_wp, ((tid + i * TEAM) * N + e) * 4, 0, 0);
+            }
+    } else {
+        __shared__ float s_sum[kTeams][TEAM * VPT * N];
+        auto join = [&](const float (&f)[VPT][N], __amdgpu_buffer_rsrc_t to) {
+            __syncthreads();
+#pragma unroll
+            for (int i = 0; i < VPT; ++i)
+#pragma unroll
+                for (int e = 0; e < N; ++e) s_sum[threadIdx.x / TEAM][(tid + i * TEAM) * N + e] = f[i][e];
+            __syncthreads();
+            for (int c = threadIdx.x; c < TEAM * VPT * N; c += TEAM * kTeams) {
+                float t = 0.f;
+#pragma unroll
+                for (int j = 0; j < kTeams; ++j) t += s_sum[j][c];
+                store_float(to, (uint32_t)c * 4, t);
+            }
+        };
+        join(sw, to_w);
+        join(swp, to_wp);
+    }
+}
+
 // ---- sums over rows -----------------------------------------------------------------------------------------------------------
 
 template <typename T>
@@ -240,11 +644,11 @@ struct ReduceArgs {
     Split p;
 };
 
-// A workgroup owns 32 columns; its 8 groups of 32 threads each add every 8th row in 64 bits, and the 8 results are added in order.
+// A workgroup owns 32 columns; its 32 groups of 32 threads each add every 32nd row in 64 bits, and the 32 results are added in order.
 // blockIdx.y: 0 dw, 1 dw_post (and with kChannel dgate, which is the same sum), 2 .. the rows of dgate (kGroup).
-constexpr int kReduceCols = 32, kReduceGroups = kThreads / kReduceCols;
+constexpr int kReduceThreads = 1024, kReduceCols = 32, kReduceGroups = kReduceThreads / kReduceCols;
 template <typename T>
-__global__ __launch_bounds__(kThreads) void sandwich_reduce_kernel(const ReduceArgs<T> k) {
+__global__ __launch_bounds__(kReduceThreads) void sandwich_reduce_kernel(const ReduceArgs<T> k) {
     __shared__ double s_acc[kReduceGroups][kReduceCols];
     const int col = threadIdx.x % kReduceCols, group = threadIdx.x / kReduceCols;
     const int64_t H = k.s.H, h = (int64_t)blockIdx.x * kReduceCols + col;
@@ -252,7 +656,7 @@ __global__ __launch_bounds__(kThreads) void sandwich_reduce_kernel(const ReduceA
     const bool channel = k.s.mode == kChannel;
     if (what == 0 ? !k.d_weight : what == 1 ? !(k.d_post_weight || (channel && k.d_gate)) : !k.d_gate) return;
     const float* p = what == 0 ? k.part.w : what == 1 ? k.part.wp : k.part.gate + (int64_t)(what - 2) * k.p.parts * H;
-    const int64_t rows = what < 2 ? k.p.workgroups : k.p.parts;
+    const int64_t rows = what < 2 ? k.p.sums : k.p.parts;
     double acc = 0.0;
     if (h < H) {
         int64_t g = group;
@@ -299,27 +703,90 @@ __global__ __launch_bounds__(kThreads) void sandwich_reduce_scalar_kernel(const 
 
 // ---- launch -------------------------------------------------------------------------------------------------------------------
 
+template <int TEAM, int VPT>
+struct Team {
+    static constexpr int team = TEAM, vpt = VPT;
+};
+// calls `launch` with the team of a row of nvec vectors, as a type; false: no team holds it
+template <typename F>
+bool with_team(int64_t nvec, F launch) {
+    if (nvec <= 64) launch(Team<64, 1>());
+    else if (nvec <= 128) launch(Team<64, 2>());
+    else if (nvec <= 256) launch(Team<256, 1>());
+    else if (nvec <= 384) launch(Team<384, 1>());
+    else if (nvec <= 512) launch(Team<512, 1>());
+    else if (nvec <= 768) launch(Team<768, 1>());
+    else if (nvec <= 1024) launch(Team<1024, 1>());
+    else if (nvec <= 2048) launch(Team<1024, 2>());
+    else return false;
+    return true;
+}
+// vectors of a row, or more than any team holds if rows are no whole vectors
+template <typename T>
+int64_t vectors_of(int64_t H, std::initializer_list<const void*> pointers) {
+    bool fine = H * (int64_t)sizeof(T) % 16 == 0;
+    for (const void* p : pointers) fine = fine && aligned16(p);
+    return fine ? H * (int64_t)sizeof(T) / 16 : INT64_MAX;
+}
+template <Mode MODE>
+using As = std::integral_constant<Mode, MODE>;
+
 template <typename T>
 int launch_fwd(const FwdArgs<T>& k, hipStream_t st) {
-    const int64_t cus = num_compute_units() > 0 ? num_compute_units() : 256, most = cus * 16;
-    const dim3 grid((uint32_t)(k.s.B < most ? k.s.B : most));
-    hipLaunchKernelGGL(sandwich_fwd_generic_kernel<T>, grid, dim3(kThreads), 0, st, k);
+    const int64_t cus = num_compute_units() > 0 ? num_compute_units() : 256;
+    const int64_t nvec = vectors_of<T>(k.s.H, {k.x, k.residual, k.post_weight, k.weight, k.s.mode == kScalar ? nullptr : k.gate, k.out, k.stream});
+    const bool held = with_team(nvec, [&](auto t) {
+        constexpr int TEAM = decltype(t)::team, VPT = decltype(t)::vpt;
+        constexpr int kTeams = teams_of(TEAM);
+        const int64_t want = (k.s.B + kTeams - 1) / kTeams, most = cus * (kFwdThreadsPerCU / (TEAM * kTeams));
+        auto launch = [&](auto mode) {
+            hipLaunchKernelGGL((sandwich_fwd_kernel<T, TEAM, VPT, decltype(mode)::value>), dim3((uint32_t)(want < most ? want : most)),
+                               dim3(TEAM * kTeams), 0, st, k);
+        };
+        switch (k.s.mode) {
+            case kNoGate: launch(As<kNoGate>()); break;
+            case kFull: launch(As<kFull>()); break;
+            case kScalar: launch(As<kScalar>()); break;
+            default: launch(As<kGroup>()); break;
+        }
+    });
+    const int64_t most = cus * 16;
+    if (!held)
+        hipLaunchKernelGGL(sandwich_fwd_generic_kernel<T>, dim3((uint32_t)(k.s.B < most ? k.s.B : most)), dim3(kThreads), 0, st, k);
     return launch_status("sandwich_rmsnorm_fwd");
 }
 
 template <typename T>
-int launch_bwd(const BwdArgs<T>& k, T* d_weight, T* d_post_weight, hipStream_t st) {
-    if (k.s.B > 0) {
-        hipLaunchKernelGGL(sandwich_bwd_generic_kernel<T>, dim3((uint32_t)k.p.workgroups), dim3(kThreads), 0, st, k);
-        const int rc = launch_status("sandwich_rmsnorm_bwd");
-        if (rc) return rc;
-    }
+int launch_bwd(BwdArgs<T> k, T* d_weight, T* d_post_weight, void* workspace, hipStream_t st) {
+    k.p = split_of(k.s, kThreads, 1);  // of the element-wise kernel
+    k.part = partial_of(workspace, k.s, k.p);
+    const int64_t nvec = vectors_of<T>(k.s.H, {k.x, k.stream, k.post_weight, k.weight, k.s.mode == kScalar ? nullptr : k.gate, k.d_out, k.d_stream, k.dx,
+                                               k.d_residual, k.s.mode == kScalar ? nullptr : k.d_gate});
+    const bool held = with_team(nvec, [&](auto t) {
+        constexpr int TEAM = decltype(t)::team, VPT = decltype(t)::vpt;
+        k.p = split_of(k.s, TEAM, teams_of(TEAM));
+        k.part = partial_of(workspace, k.s, k.p);
+        auto launch = [&](auto mode) {
+            hipLaunchKernelGGL((sandwich_bwd_kernel<T, TEAM, VPT, decltype(mode)::value>), dim3((uint32_t)k.p.sums), dim3(TEAM * teams_of(TEAM)), 0,
+                               st, k);
+        };
+        switch (k.s.mode) {
+            case kNoGate: launch(As<kNoGate>()); break;
+            case kFull: launch(As<kFull>()); break;
+            case kChannel: launch(As<kChannel>()); break;
+            case kScalar: launch(As<kScalar>()); break;
+            default: launch(As<kGroup>()); break;
+        }
+    });
+    if (!held) hipLaunchKernelGGL(sandwich_bwd_generic_kernel<T>, dim3((uint32_t)k.p.workers), dim3(kThreads), 0, st, k);
+    int rc = launch_status("sandwich_rmsnorm_bwd");
+    if (rc) return rc;
     const ReduceArgs<T> r{k.part, k.post_weight, k.gate, d_weight, d_post_weight, k.d_gate, k.s, k.p};
     const int64_t groups = k.s.mode == kGroup && k.d_gate && k.p.parts > 1 ? k.p.groups : 0;
     if (d_weight || d_post_weight || (k.s.mode == kChannel && k.d_gate) || groups) {
         hipLaunchKernelGGL(sandwich_reduce_kernel<T>, dim3((uint32_t)((k.s.H + kReduceCols - 1) / kReduceCols), (uint32_t)(2 + groups)),
-                           dim3(kThreads), 0, st, r);
-        const int rc = launch_status("sandwich_rmsnorm_bwd (sums)");
+                           dim3(kReduceThreads), 0, st, r);
+        rc = launch_status("sandwich_rmsnorm_bwd (sums)");
         if (rc) return rc;
     }
     if (k.s.mode == kScalar && k.d_gate && k.s.R > 1) {
@@ -362,11 +829,10 @@ template <typename T>
 int backward(const void* x, const void* stream, const void* post_weight, const void* weight, const void* gate, const void* d_out,
              const void* d_stream, const float* stats, void* dx, void* d_residual, void* d_gate, void* d_post_weight, void* d_weight,
              const Shape& s, float a, void* workspace, hipStream_t st) {
-    const Split p = split_of(s);
     const BwdArgs<T> k{(const T*)x, (const T*)stream, (const T*)post_weight, (const T*)weight, (const T*)gate, (const T*)d_out, (const T*)d_stream,
-                       stats, (T*)dx, (T*)d_residual, (T*)d_gate, partial_of(workspace, s, p), s, p, 1.0f / (float)s.H, a, d_weight != nullptr,
+                       stats, (T*)dx, (T*)d_residual, (T*)d_gate, Partial{}, s, Split{}, 1.0f / (float)s.H, a, d_weight != nullptr,
                        d_post_weight != nullptr || (s.mode == kChannel && d_gate)};
-    return launch_bwd<T>(k, (T*)d_weight, (T*)d_post_weight, st);
+    return launch_bwd<T>(k, (T*)d_weight, (T*)d_post_weight, workspace, st);
 }
 
 }  // namespace
