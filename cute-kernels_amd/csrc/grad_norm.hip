@@ -5,21 +5,27 @@
 //
 // HBM-bound: one pass reads every element, a second reads and writes it. Squares are added in 64 bits from the first one on: in 32 bits
 // a gradient of 2^64 or of 2^-75 would already be lost in its square. Tensors come as a table in the kernel's arguments (no table in
-// device memory that a captured graph or a second call would have to share), cut into chunks of 16384 elements.
+// device memory that a captured graph or a second call would have to share), cut into chunks.
 #include "common.h"
 
 #include <stdlib.h>
 
 #include <algorithm>
+#include <type_traits>
 
 namespace fmahip {
 namespace {
 
 constexpr int kThreads = 256;
 constexpr int kWaves = kThreads / kWave;
-constexpr int kChunk = 16384;   // elements; a multiple of every 16-byte vector, so that all chunks of a tensor are aligned alike
-constexpr int kTable = 160;     // tensors per launch: 3.4 KB of kernel arguments
-constexpr int kPerCU = 8;       // workgroups per compute unit
+// Elements of a chunk; multiples of every 16-byte vector, so that all chunks of a tensor are aligned alike
+constexpr int kNormChunk = 16384, kScaleChunk = 8192;
+constexpr int kTable = 160;         // tensors per launch: 3.4 KB of kernel arguments
+constexpr int kNormPerCU = 8;       // workgroups per compute unit; the scaling has one for every chunk
+constexpr int64_t kMostGrid = 1 << 22;
+// Bytes of all tensors from which on they are read and written as a stream (non-temporal), and not left in the caches for the second pass. us of
+// norm and scaling, streamed / not: 68 MB 42 / 38, 151 MB 79 / 93, 302 MB 149 / 178, 2.2 GB 1061 / 1202.
+constexpr int64_t kStreamBytes = 128ll << 20;
 
 struct Table {
     void* ptr[kTable];
@@ -35,18 +41,23 @@ struct Chunk {
     int32_t dtype;
 };
 
-__device__ __forceinline__ Chunk find_chunk(const Table& t, uint32_t c) {
-    int low = 0, high = t.count - 1;
-    while (low < high) {
-        const int mid = (low + high + 1) / 2;
-        if (t.first[mid] <= c) low = mid;
-        else high = mid - 1;
+// chunk c, of tensor `at` or one behind it; `at` follows
+template <int CHUNK>
+__device__ __forceinline__ Chunk find_chunk(const Table& t, uint32_t c, int& at) {
+    if (t.first[at + 1] <= c) {
+        int low = at + 1, high = t.count - 1;
+        while (low < high) {
+            const int mid = (low + high + 1) / 2;
+            if (t.first[mid] <= c) low = mid;
+            else high = mid - 1;
+        }
+        at = low;
     }
-    const int64_t begin = (int64_t)(c - t.first[low]) * kChunk, rest = t.numel[low] - begin;
-    const int dtype = t.dtype[low];
+    const int64_t begin = (int64_t)(c - t.first[at]) * CHUNK, rest = t.numel[at] - begin;
+    const int dtype = t.dtype[at];
     Chunk out;
-    out.ptr = (char*)t.ptr[low] + begin * (dtype == FMA_F32 ? 4 : 2);
-    out.n = (int32_t)(rest < kChunk ? rest : kChunk);
+    out.ptr = (char*)t.ptr[at] + begin * (dtype == FMA_F32 ? 4 : 2);
+    out.n = (int32_t)(rest < CHUNK ? rest : CHUNK);
     out.dtype = dtype;
     return out;
 }
@@ -86,32 +97,55 @@ __device__ __forceinline__ void join_workgroup(Accumulator<MAX>& acc) {
     for (int w = 0; w < WAVES; ++w) acc.join(s_part[w]);
 }
 
-template <typename T, bool MAX>
-__device__ __forceinline__ void add_chunk(Accumulator<MAX>& acc, const T* p, int n) {
+// The elements of a chunk: those in front of the first 16-byte boundary and behind the last one go to `one`, the vectors between them to
+// `many`, UNROLL neighbouring groups of 256 vectors at a time, and one by one what is left of them.
+template <int UNROLL, typename T, typename ONE, typename MANY>
+__device__ __forceinline__ void over_chunk(T* p, int n, ONE one, MANY many) {
     constexpr int V = Vec16<T>::N;
     const int head = head_of(p, n);
-    if ((int)threadIdx.x < head) acc.add(Num<T>::up(p[threadIdx.x]));
+    if ((int)threadIdx.x < head) one(p + threadIdx.x);
     p += head;
     n -= head;
     const int nvec = n / V;
-    const Vec16<T>* const v = (const Vec16<T>*)p;
-    for (int i = threadIdx.x; i < nvec; i += kThreads) {
-        const Vec16<T> x = v[i];
-#pragma unroll
-        for (int e = 0; e < V; ++e) acc.add(Num<T>::up(x.v[e]));
-    }
+    Vec16<T>* const v = (Vec16<T>*)p;
+    int i = threadIdx.x;
+    for (; i + (UNROLL - 1) * kThreads < nvec; i += UNROLL * kThreads) many(v + i, std::integral_constant<int, UNROLL>());
+    for (; i < nvec; i += kThreads) many(v + i, std::integral_constant<int, 1>());
     const int tail = nvec * V + (int)threadIdx.x;
-    if (tail < n) acc.add(Num<T>::up(p[tail]));
+    if (tail < n) one(p + tail);
 }
 
-template <bool MAX>
+template <bool STREAM, typename V>
+__device__ __forceinline__ V load(const V* p) {
+    if constexpr (STREAM) return load_streaming16(p);
+    else return *p;
+}
+
+template <bool STREAM, typename T, bool MAX>
+__device__ __forceinline__ void add_chunk(Accumulator<MAX>& acc, T* p, int n) {
+    over_chunk<8>(
+        p, n, [&](const T* x) { acc.add(Num<T>::up(*x)); },
+        [&](const Vec16<T>* v, auto times) {
+            constexpr int U = decltype(times)::value;
+            Vec16<T> x[U];
+#pragma unroll
+            for (int u = 0; u < U; ++u) x[u] = load<STREAM>(v + u * kThreads);
+#pragma unroll
+            for (int u = 0; u < U; ++u)
+#pragma unroll
+                for (int e = 0; e < Vec16<T>::N; ++e) acc.add(Num<T>::up(x[u].v[e]));
+        });
+}
+
+template <bool MAX, bool STREAM>
 __global__ __launch_bounds__(kThreads) void grad_norm_kernel(const Table t, uint64_t* __restrict__ partial) {
     Accumulator<MAX> acc;
+    int at = 0;
     for (uint32_t c = blockIdx.x; c < t.first[t.count]; c += gridDim.x) {
-        const Chunk k = find_chunk(t, c);
-        if (k.dtype == FMA_F32) add_chunk(acc, (const float*)k.ptr, k.n);
-        else if (k.dtype == FMA_F16) add_chunk(acc, (const f16_t*)k.ptr, k.n);
-        else add_chunk(acc, (const bf16_t*)k.ptr, k.n);
+        const Chunk k = find_chunk<kNormChunk>(t, c, at);
+        if (k.dtype == FMA_F32) add_chunk<STREAM>(acc, (float*)k.ptr, k.n);
+        else if (k.dtype == FMA_F16) add_chunk<STREAM>(acc, (f16_t*)k.ptr, k.n);
+        else add_chunk<STREAM>(acc, (bf16_t*)k.ptr, k.n);
     }
     join_workgroup<MAX, kWaves>(acc);
     if (threadIdx.x == 0) partial[blockIdx.x] = acc.bits();
@@ -134,44 +168,52 @@ __global__ __launch_bounds__(kJoinThreads) void grad_norm_join_kernel(const uint
     }
 }
 
-template <typename T>
+template <bool STREAM, typename T>
 __device__ __forceinline__ void scale_chunk(T* p, int n, float factor) {
-    constexpr int V = Vec16<T>::N;
-    const int head = head_of(p, n);
-    if ((int)threadIdx.x < head) p[threadIdx.x] = Num<T>::down(Num<T>::up(p[threadIdx.x]) * factor);
-    p += head;
-    n -= head;
-    const int nvec = n / V;
-    Vec16<T>* const v = (Vec16<T>*)p;
-    for (int i = threadIdx.x; i < nvec; i += kThreads) {
-        Vec16<T> x = v[i];
+    over_chunk<4>(
+        p, n, [&](T* x) { *x = Num<T>::down(Num<T>::up(*x) * factor); },
+        [&](Vec16<T>* v, auto times) {
+            constexpr int U = decltype(times)::value;
+            Vec16<T> x[U];
 #pragma unroll
-        for (int e = 0; e < V; ++e) x.v[e] = Num<T>::down(Num<T>::up(x.v[e]) * factor);
-        v[i] = x;
-    }
-    const int tail = nvec * V + (int)threadIdx.x;
-    if (tail < n) p[tail] = Num<T>::down(Num<T>::up(p[tail]) * factor);
+            for (int u = 0; u < U; ++u) x[u] = load<STREAM>(v + u * kThreads);
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+#pragma unroll
+                for (int e = 0; e < Vec16<T>::N; ++e) x[u].v[e] = Num<T>::down(Num<T>::up(x[u].v[e]) * factor);
+                if constexpr (STREAM) store_streaming16(v + u * kThreads, x[u]);
+                else v[u * kThreads] = x[u];
+            }
+        });
 }
 
 // a factor of one leaves the tensors alone: nothing is read or written then. A NaN goes through.
+template <bool STREAM>
 __global__ __launch_bounds__(kThreads) void scale_grads_kernel(const Table t, const double* __restrict__ norm64,
                                                                const float* __restrict__ norm, double max_norm) {
     const double ratio = max_norm / ((norm64 ? *norm64 : (double)*norm) + 1e-6);
     if (ratio >= 1.0) return;
     const float factor = (float)ratio;
+    int at = 0;
     for (uint32_t c = blockIdx.x; c < t.first[t.count]; c += gridDim.x) {
-        const Chunk k = find_chunk(t, c);
-        if (k.dtype == FMA_F32) scale_chunk((float*)k.ptr, k.n, factor);
-        else if (k.dtype == FMA_F16) scale_chunk((f16_t*)k.ptr, k.n, factor);
-        else scale_chunk((bf16_t*)k.ptr, k.n, factor);
+        const Chunk k = find_chunk<kScaleChunk>(t, c, at);
+        if (k.dtype == FMA_F32) scale_chunk<STREAM>((float*)k.ptr, k.n, factor);
+        else if (k.dtype == FMA_F16) scale_chunk<STREAM>((f16_t*)k.ptr, k.n, factor);
+        else scale_chunk<STREAM>((bf16_t*)k.ptr, k.n, factor);
     }
 }
 
-int64_t most_workgroups() { return (num_compute_units() > 0 ? num_compute_units() : 256) * (int64_t)kPerCU; }
+int64_t most_workgroups() { return (num_compute_units() > 0 ? num_compute_units() : 256) * (int64_t)kNormPerCU; }
+
+bool streams(const int64_t* sizes, const int32_t* dtypes, int64_t count) {
+    int64_t bytes = 0;
+    for (int64_t i = 0; i < count && bytes <= kStreamBytes; ++i) bytes += sizes[i] * dtype_bytes(dtypes[i]);
+    return bytes > kStreamBytes;
+}
 
 // Tables of the tensors that have elements, in order, and what `launch` makes of each; stops at the first that fails.
 template <typename F>
-int for_each_table(void* const* tensors, const int64_t* sizes, const int32_t* dtypes, int64_t count, F launch) {
+int for_each_table(void* const* tensors, const int64_t* sizes, const int32_t* dtypes, int64_t count, int chunk, F launch) {
     Table t;
     int64_t i = 0;
     while (i < count) {
@@ -179,7 +221,7 @@ int for_each_table(void* const* tensors, const int64_t* sizes, const int32_t* dt
         t.first[0] = 0;
         for (; i < count && t.count < kTable; ++i) {
             if (sizes[i] == 0) continue;
-            const int64_t chunks = (sizes[i] + kChunk - 1) / kChunk;  // 2^23 at the most, of all tensors of a table below 2^31
+            const int64_t chunks = (sizes[i] + chunk - 1) / chunk;  // 2^24 at the most, of all tensors of a table below 2^32
             t.ptr[t.count] = tensors[i];
             t.numel[t.count] = sizes[i];
             t.dtype[t.count] = (uint8_t)dtypes[i];
@@ -223,7 +265,8 @@ int check_disjoint(const char* what, void* const* tensors, const int64_t* sizes,
             r[n].begin = (uintptr_t)tensors[i];
             r[n++].end = (uintptr_t)tensors[i] + (uintptr_t)sizes[i] * (uintptr_t)dtype_bytes(dtypes[i]);
         }
-    std::sort(r, r + n, [](const Range& a, const Range& b) { return a.begin < b.begin; });
+    const auto before = [](const Range& a, const Range& b) { return a.begin < b.begin; };
+    if (!std::is_sorted(r, r + n, before)) std::sort(r, r + n, before);  // (those of a bucket are)
     bool apart = true;
     for (int64_t i = 1; i < n; ++i) apart = apart && r[i - 1].end <= r[i].begin;
     free(r);
@@ -236,10 +279,12 @@ int launch_norm(void* const* tensors, const int64_t* sizes, const int32_t* dtype
     uint64_t* const partial = (uint64_t*)(norm64 + 1);
     const int64_t most = most_workgroups();
     int64_t parts = 0;
-    int rc = for_each_table(tensors, sizes, dtypes, count, [&](const Table& t) {
+    const bool stream = streams(sizes, dtypes, count);
+    int rc = for_each_table(tensors, sizes, dtypes, count, kNormChunk, [&](const Table& t) {
         const int64_t chunks = t.first[t.count], grid = chunks < most ? chunks : most;
-        if (infinity) hipLaunchKernelGGL(grad_norm_kernel<true>, dim3((uint32_t)grid), dim3(kThreads), 0, st, t, partial + parts);
-        else hipLaunchKernelGGL(grad_norm_kernel<false>, dim3((uint32_t)grid), dim3(kThreads), 0, st, t, partial + parts);
+        const auto kernel = infinity ? (stream ? grad_norm_kernel<true, true> : grad_norm_kernel<true, false>)
+                                     : (stream ? grad_norm_kernel<false, true> : grad_norm_kernel<false, false>);
+        hipLaunchKernelGGL(kernel, dim3((uint32_t)grid), dim3(kThreads), 0, st, t, partial + parts);
         parts += grid;
         return launch_status("grad_norm");
     });
@@ -251,10 +296,10 @@ int launch_norm(void* const* tensors, const int64_t* sizes, const int32_t* dtype
 
 int launch_scale(void* const* tensors, const int64_t* sizes, const int32_t* dtypes, int64_t count, const double* norm64, const float* norm,
                  double max_norm, hipStream_t st) {
-    const int64_t most = most_workgroups();
-    return for_each_table(tensors, sizes, dtypes, count, [&](const Table& t) {
-        const int64_t chunks = t.first[t.count], grid = chunks < most ? chunks : most;
-        hipLaunchKernelGGL(scale_grads_kernel, dim3((uint32_t)grid), dim3(kThreads), 0, st, t, norm64, norm, max_norm);
+    const auto kernel = streams(sizes, dtypes, count) ? scale_grads_kernel<true> : scale_grads_kernel<false>;
+    return for_each_table(tensors, sizes, dtypes, count, kScaleChunk, [&](const Table& t) {
+        const int64_t chunks = t.first[t.count], grid = chunks < kMostGrid ? chunks : kMostGrid;
+        hipLaunchKernelGGL(kernel, dim3((uint32_t)grid), dim3(kThreads), 0, st, t, norm64, norm, max_norm);
         return launch_status("scale_grads");
     });
 }

@@ -8,15 +8,20 @@
 // a wavefront takes 64 / L tokens at a time and a lane meets the same experts in every token: sums over tokens stay in its registers until
 // the workgroup ends. Partial sums go to a workspace and are joined in a fixed order in 64 bits: the same bits on every run.
 //
-// The k-th largest logit is found by its bits from the top down (the largest threshold that k logits reach); the search ends where exactly
-// k do. Only if logits equal to the k-th stay on both sides of the line are places among them counted.
 #include "common.h"
+
+#include <type_traits>
 
 namespace fmahip {
 namespace {
 
-constexpr int kFwdThreads = 1024, kFwdWaves = kFwdThreads / kWave;
+// threads of a workgroup of the forward pass: half of them where each holds 16 logits and would not have the registers
+constexpr int fwd_threads(int values) { return values > 8 ? 512 : 1024; }
 constexpr int kBwdThreads = 256;
+// Choices up to which their threshold is found from the largest logit down (see count_largest). Both kernels of the forward pass, us from
+// the top / by bisection: 131072 tokens of 256 experts in fp32, 2, 4 and 8 choices 51 / 83, 65 / 89, 93 / 89, in bf16 6 choices 79 / 86; 16384 of
+// 1024, 8 choices 73 / 65; 200000 of 32 (bf16), 4 and 8 choices 21 / 26, 26 / 30; 65536 of 64, 8 choices 19.0 / 19.2; 262144 of 8, 3 choices 16 / 19.
+constexpr uint32_t few_choices(int lanes) { return lanes <= 8 ? 8 : 6; }
 
 template <int CTRL>
 __device__ __forceinline__ uint32_t dpp(uint32_t v) {
@@ -24,6 +29,10 @@ __device__ __forceinline__ uint32_t dpp(uint32_t v) {
 }
 struct Max {
     static __device__ __forceinline__ float of(float a, float b) { return fmaxf(a, b); }
+    static __device__ __forceinline__ uint32_t of(uint32_t a, uint32_t b) { return a > b ? a : b; }
+};
+struct Min {
+    static __device__ __forceinline__ uint32_t of(uint32_t a, uint32_t b) { return a < b ? a : b; }
 };
 struct Sum {
     static __device__ __forceinline__ float of(float a, float b) { return a + b; }
@@ -38,135 +47,213 @@ __device__ __forceinline__ V over_token(V v) {
     if constexpr (L >= 4) v = OP::of(v, from(dpp<0x4e>(as(v))));    // the other pair of the quad
     if constexpr (L >= 8) v = OP::of(v, from(dpp<0x141>(as(v))));   // the mirrored half row: the other quad
     if constexpr (L >= 16) v = OP::of(v, from(dpp<0x140>(as(v))));  // the mirrored row: its other half
-    if constexpr (L >= 32) v = OP::of(v, from((uint32_t)__shfl_xor((int)as(v), 16, kWave)));
-    if constexpr (L >= 64) v = OP::of(v, from((uint32_t)__shfl_xor((int)as(v), 32, kWave)));
+    if constexpr (L >= 32) {                                        // odd rows of 16 lanes and even ones
+        const auto r = __builtin_amdgcn_permlane16_swap(as(v), as(v), false, false);
+        v = OP::of(from((uint32_t)r[0]), from((uint32_t)r[1]));
+    }
+    if constexpr (L >= 64) {  // the halves of the wavefront
+        const auto r = __builtin_amdgcn_permlane32_swap(as(v), as(v), false, false);
+        v = OP::of(from((uint32_t)r[0]), from((uint32_t)r[1]));
+    }
     return v;
 }
 
-// Unsigned numbers in the order of the logits: NaN on top, -0 equal to +0; every key is above 0, which stands for "no logit here".
-template <typename T>
-struct Keys;
-template <>
-struct Keys<float> {
-    static constexpr uint32_t kTop = 1u << 31;
-    static __device__ __forceinline__ uint32_t of(float x) {
-        uint32_t b = __float_as_uint(x);
-        if (x != x) return 0xffffffffu;
-        b = b == 0x80000000u ? 0u : b;
-        return b & 0x80000000u ? ~b : b | 0x80000000u;
+// the sum over a wavefront's tokens: of the lanes that are the same one of their tokens
+template <int L, typename V>
+__device__ __forceinline__ V over_tokens(V v) {
+    auto as = [](V x) { return __builtin_bit_cast(uint32_t, x); };
+    auto from = [](uint32_t x) { return __builtin_bit_cast(V, x); };
+    if constexpr (L <= 8) v += from(dpp<0x128>(as(v)));  // rows of 16 lanes turned by eight, four, two and one
+    if constexpr (L <= 4) v += from(dpp<0x124>(as(v)));
+    if constexpr (L <= 2) v += from(dpp<0x122>(as(v)));
+    if constexpr (L <= 1) v += from(dpp<0x121>(as(v)));
+    if constexpr (L <= 16) {
+        const auto r = __builtin_amdgcn_permlane16_swap(as(v), as(v), false, false);
+        v = from((uint32_t)r[0]) + from((uint32_t)r[1]);
     }
-};
-template <typename T>
-struct Keys16 {
-    static constexpr uint32_t kTop = 1u << 15;
-    static __device__ __forceinline__ uint32_t of(T x) {
-        uint32_t b = __builtin_bit_cast(uint16_t, x);
-        const float f = Num<T>::up(x);
-        if (f != f) return 0xffffu;
-        b = b == 0x8000u ? 0u : b;
-        return b & 0x8000u ? ~b & 0xffffu : b | 0x8000u;
+    if constexpr (L <= 32) {
+        const auto r = __builtin_amdgcn_permlane32_swap(as(v), as(v), false, false);
+        v = from((uint32_t)r[0]) + from((uint32_t)r[1]);
     }
-};
-template <>
-struct Keys<bf16_t> : Keys16<bf16_t> {};
-template <>
-struct Keys<f16_t> : Keys16<f16_t> {};
-
-template <typename T>
-__device__ __forceinline__ float exp_for(float x) {
-    if constexpr (sizeof(T) == 4) return expf(x);
-    else return __expf(x);  // logits of 16 bits are far coarser than its error
+    return v;
 }
 
-// the logits of a lane: columns j * NV .. of one row; -infinity past its end
-template <typename T, int NV, bool VEC>
-__device__ __forceinline__ void load_logits(const T* __restrict__ row, int first, int E, T (&x)[NV]) {
-    if constexpr (VEC) {  // rows are whole 16-byte vectors
-        constexpr int V = Vec16<T>::N;
+// A lane's logits as they are in memory, and widened. What is past a row's end is not fetched (a buffer's range check) and stands as -infinity:
+// it adds nothing to a sum, and of equal logits the choice takes the ones further left, of which there are enough.
+constexpr uint32_t kNowhere = 0x7fffffffu;
+template <typename T, int NV>
+struct Logits {
+    static constexpr int kWords = NV * (int)sizeof(T) / 4;
+    uint32_t word[kWords];
+    __device__ __forceinline__ float up(int i) const {
+        if constexpr (sizeof(T) == 4) {
+            return __uint_as_float(word[i]);
+        } else {
+            const uint16_t bits = (uint16_t)(i & 1 ? word[i / 2] >> 16 : word[i / 2]);
+            return Num<T>::up(__builtin_bit_cast(T, bits));
+        }
+    }
+    // Zeros for a token that does not count, whatever was there; else -infinity behind the `in` logits that there are
+    template <bool VEC>
+    __device__ __forceinline__ void settle(bool counted, int in) {
+        constexpr uint32_t kInf = sizeof(T) == 4 ? 0xff800000u : std::is_same<T, bf16_t>::value ? 0xff80u : 0xfc00u;
 #pragma unroll
-        for (int i = 0; i < NV / V; ++i)
-            if (first + i * V < E) {
-                const Vec16<T> v = *(const Vec16<T>*)(row + first + i * V);
+        for (int j = 0; j < kWords; ++j) {
+            if constexpr (sizeof(T) == 4) word[j] = j < in ? word[j] : kInf;
+            else if constexpr (VEC) word[j] = 2 * j < in ? word[j] : kInf << 16 | kInf;
+            else word[j] = (2 * j < in ? word[j] & 0xffffu : kInf) | (2 * j + 1 < in ? word[j] & 0xffff0000u : kInf << 16);
+            word[j] = counted ? word[j] : 0u;
+        }
+    }
+    // offset: of the lane's first logit, in bytes; `in`: how many of its logits there are
+    template <bool VEC>
+    __device__ __forceinline__ void load(__amdgpu_buffer_rsrc_t from, uint32_t offset, int in) {
+        if constexpr (VEC) {  // rows are whole 16-byte vectors
+            constexpr int V = Vec16<T>::N;
 #pragma unroll
-                for (int e = 0; e < V; ++e) x[i * V + e] = v.v[e];
+            for (int v = 0; v < NV / V; ++v) {
+                const auto four = __builtin_amdgcn_raw_buffer_load_b128(from, (int)(v * V < in ? offset + v * 16 : kNowhere), 0, 0);
+#pragma unroll
+                for (int j = 0; j < 4; ++j) word[v * 4 + j] = four[j];
             }
-    } else {
+        } else if constexpr (sizeof(T) == 4) {
 #pragma unroll
-        for (int i = 0; i < NV; ++i)
-            if (first + i < E) x[i] = row[first + i];
+            for (int i = 0; i < NV; ++i) word[i] = __builtin_amdgcn_raw_buffer_load_b32(from, (int)(i < in ? offset + i * 4 : kNowhere), 0, 0);
+        } else {
+            uint32_t one[NV];
+#pragma unroll
+            for (int i = 0; i < NV; ++i) one[i] = (uint16_t)__builtin_amdgcn_raw_buffer_load_b16(from, (int)(i < in ? offset + i * 2 : kNowhere), 0, 0);
+#pragma unroll
+            for (int i = 0; i < NV; i += 2) word[i / 2] = one[i] | one[i + 1] << 16;
+        }
     }
+};
+
+// `tokens` rows of logits from p on (as many as a workgroup takes at a time, and no more than `left`) as a buffer
+template <typename T>
+__device__ __forceinline__ __amdgpu_buffer_rsrc_t rows_at(const T* p, int64_t left, int tokens, int E) {
+    const uint32_t rows = left > 0 ? (uint32_t)(left < tokens ? left : tokens) : 0u;
+    return __builtin_amdgcn_make_buffer_rsrc(const_cast<T*>(p), 0, (int)(rows * (uint32_t)E * (uint32_t)sizeof(T)), 0x00020000);
 }
 
-// softmax of a token: p (0 past its end) and, in all its lanes, the log of the sum
+// A token's largest logit, the exponentials of its logits against it, their sum: exp and log of the hardware, whose errors
+// (two units, and that of an argument rounded in float32) are those of the subtraction in front of them.
 template <typename T, int L, int NV>
-__device__ __forceinline__ float softmax_token(const T (&x)[NV], int first, int E, float (&p)[NV]) {
-    float top = -__builtin_inff();
+__device__ __forceinline__ void softmax_token(const Logits<T, NV>& x, float (&e)[NV], float& top, float& sum) {
+    top = -__builtin_inff();
 #pragma unroll
-    for (int i = 0; i < NV; ++i)
-        if (first + i < E) top = fmaxf(top, Num<T>::up(x[i]));
+    for (int i = 0; i < NV; ++i) top = fmaxf(top, x.up(i));
     top = over_token<L, Max>(top);
-    float sum = 0.f;
+    sum = 0.f;
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
-        p[i] = first + i < E ? exp_for<T>(Num<T>::up(x[i]) - top) : 0.f;
-        sum += p[i];
+        e[i] = __expf(x.up(i) - top);
+        sum += e[i];
     }
     sum = over_token<L, Sum>(sum);
-    const float inv = 1.0f / sum;
-#pragma unroll
-    for (int i = 0; i < NV; ++i) p[i] *= inv;
-    return top + logf(sum);
 }
 
-// bit i of the result: whether logit i of this lane is among the token's k largest
-template <typename T, int L, int NV>
-__device__ __forceinline__ uint32_t choose(const T (&x)[NV], int first, int E, uint32_t k, bool counted) {
-    uint32_t key[NV];
+// Unsigned numbers in the order of the logits: NaN on top if it is looked for, -0 equal to +0, consecutive numbers for consecutive values of the
+// type; every key is above 0.
+template <typename T>
+struct Keys {
+    static constexpr int kDrop = 0;
+};
+template <>
+struct Keys<bf16_t> {
+    static constexpr int kDrop = 16;
+};
+template <>
+struct Keys<f16_t> {
+    static constexpr int kDrop = 13;
+};
+template <typename T, bool NANS>
+__device__ __forceinline__ uint32_t key_of(float x) {
+    const uint32_t b = __float_as_uint(x + 0.0f);
+    uint32_t key = b ^ ((uint32_t)((int32_t)b >> 31) | 0x80000000u);
+    if constexpr (NANS) key = x != x ? 0xffffffffu : key;
+    return key >> Keys<T>::kDrop;
+}
+
+// Adds one to count[i] of the token's k largest logits. Their threshold, the largest that k logits reach, is found from the largest logit down,
+// one value after the other, where k is small, and otherwise by bisection of the keys between the smallest of the lanes' largest (where k lanes
+// have logits) and the largest, which ends where exactly k reach the middle. Only where equal logits are left on both sides of the line are
+// places among them counted.
+template <typename T, int L, int NV, bool NANS>
+__device__ __forceinline__ void count_largest(const Logits<T, NV>& x, int in, bool enough_lanes, uint32_t k, bool counted, uint32_t (&count)[NV]) {
+    uint32_t key[NV], most = 0;
 #pragma unroll
-    for (int i = 0; i < NV; ++i) key[i] = first + i < E ? Keys<T>::of(x[i]) : 0u;
-    auto reach = [&](uint32_t threshold) {
+    for (int i = 0; i < NV; ++i) {
+        key[i] = key_of<T, NANS>(x.up(i));
+        most = Max::of(most, key[i]);
+    }
+    auto reach = [&](uint32_t line) {
         uint32_t n = 0;
 #pragma unroll
-        for (int i = 0; i < NV; ++i) n += key[i] >= threshold ? 1u : 0u;
+        for (int i = 0; i < NV; ++i) n += key[i] >= line ? 1u : 0u;
         return over_token<L, Sum>(n);
     };
-    uint32_t threshold = 0;
-    bool open = counted;
-    for (uint32_t bit = Keys<T>::kTop; bit != 0 && __any(open); bit >>= 1) {
-        const uint32_t n = reach(threshold | bit);
-        if (open && n >= k) threshold |= bit;
-        open = open && n != k;
+    uint32_t low, high = over_token<L, Max>(most);
+    bool exact = !counted;
+    if (k <= few_choices(L)) {
+        low = high;
+        uint32_t n = reach(low);
+        while (__any(!exact && n < k)) {
+            uint32_t below = 0;
+#pragma unroll
+            for (int i = 0; i < NV; ++i) below = Max::of(below, key[i] < low ? key[i] : 0u);
+            below = over_token<L, Max>(below);
+            if (n < k) {
+                low = below;
+                n = reach(below);
+            }
+        }
+        exact = exact || n == k;
+    } else {
+        uint32_t least = most;
+        if (!enough_lanes) {
+#pragma unroll
+            for (int i = 0; i < NV; ++i) least = Min::of(least, key[i]);
+        }
+        low = over_token<L, Min>(in > 0 ? least : 0xffffffffu);
+        while (__any(!exact && low < high)) {
+            const uint32_t mid = low + (high - low + 1) / 2, n = reach(mid);
+            if (!exact && low < high) {
+                if (n >= k) low = mid;
+                else high = mid - 1;
+                exact = n == k;
+            }
+        }
     }
-    uint32_t chosen = 0;
+    if (!__any(!exact)) {
+        const uint32_t line = counted ? low : 0xffffffffu;  // (no logit of such a token, which are all zeros then, reaches it)
 #pragma unroll
-    for (int i = 0; i < NV; ++i) chosen |= (key[i] >= threshold && key[i] != 0 ? 1u : 0u) << i;
-    if (__any(open)) {  // more than k reach it: those above, and of the equal ones the first
-        uint32_t above = 0, equal = 0;
-#pragma unroll
-        for (int i = 0; i < NV; ++i) {
-            above |= (key[i] > threshold ? 1u : 0u) << i;
-            equal |= (key[i] == threshold ? 1u : 0u) << i;
-        }
-        const uint32_t mine = __popc(equal), lane = threadIdx.x & (L - 1);
-        uint32_t before = mine;  // inclusive sum over the lanes of the token
-#pragma unroll
-        for (int d = 1; d < L; d <<= 1) {
-            const uint32_t v = (uint32_t)__shfl_up((int)before, d, L);
-            before += (int)lane >= d ? v : 0u;
-        }
-        before -= mine;
-        uint32_t left = k - over_token<L, Sum>((uint32_t)__popc(above));
-        left = left > before ? left - before : 0u;  // of this lane's
-        uint32_t first_ones = 0;
-#pragma unroll
-        for (int i = 0; i < NV; ++i) {
-            const uint32_t take = (equal >> i & 1u) & (left > 0 ? 1u : 0u);
-            first_ones |= take << i;
-            left -= take;
-        }
-        if (open) chosen = above | first_ones;
+        for (int i = 0; i < NV; ++i) count[i] += key[i] >= line ? 1u : 0u;
+        return;
     }
-    return counted ? chosen : 0u;
+    // k or more reach it: those above, and of the equal ones the first
+    uint32_t above = 0, equal = 0;
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+        above |= (key[i] > low ? 1u : 0u) << i;
+        equal |= (key[i] == low ? 1u : 0u) << i;
+    }
+    const uint32_t mine = __popc(equal), lane = threadIdx.x & (L - 1);
+    uint32_t before = mine;  // inclusive sum over the lanes of the token
+#pragma unroll
+    for (int d = 1; d < L; d <<= 1) {
+        const uint32_t v = (uint32_t)__shfl_up((int)before, d, L);
+        before += lane >= (uint32_t)d ? v : 0u;
+    }
+    before -= mine;
+    uint32_t left = k - over_token<L, Sum>((uint32_t)__popc(above));
+    left = left > before ? left - before : 0u;  // of this lane's
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+        const uint32_t take = equal >> i & (left > 0 ? 1u : 0u);
+        left -= take;
+        count[i] += counted ? (above >> i & 1u) | take : 0u;
+    }
 }
 
 struct Partial {
@@ -177,14 +264,17 @@ struct Partial {
 };
 
 template <typename T, int L, int NV, bool VEC>
-__global__ __launch_bounds__(kFwdThreads) void router_loss_kernel(const T* __restrict__ logits, const uint8_t* __restrict__ mask, int64_t T_,
+__global__ __launch_bounds__(fwd_threads(NV)) void router_loss_kernel(const T* __restrict__ logits, const uint8_t* __restrict__ mask, int64_t T_,
                                                                   int E, uint32_t k, Partial part) {
-    constexpr int kTokens = kFwdThreads / L;  // of a workgroup at a time
+    constexpr int kFwdThreads = fwd_threads(NV), kFwdWaves = kFwdThreads / kWave, kTokens = kFwdThreads / L;  // tokens of a workgroup at a time
     __shared__ float s_p[kFwdWaves][L * NV];
     __shared__ uint32_t s_c[kFwdWaves][L * NV];
     __shared__ double s_z[kFwdWaves];
     __shared__ uint32_t s_n[kFwdWaves];
-    const int lane = threadIdx.x & (L - 1), first = lane * NV;
+    const int lane = threadIdx.x & (L - 1), first = lane * NV, token = threadIdx.x / L;
+    const int in = E - first < 0 ? 0 : E - first < NV ? E - first : NV;
+    const bool enough_lanes = (uint32_t)((E + NV - 1) / NV) >= k;
+    const uint32_t offset = (uint32_t)(token * E + first) * (uint32_t)sizeof(T);
     float psum[NV];
     uint32_t count[NV];
 #pragma unroll
@@ -194,33 +284,45 @@ __global__ __launch_bounds__(kFwdThreads) void router_loss_kernel(const T* __res
     }
     double zsum = 0.0;
     uint32_t n = 0;
+    auto fetch = [&](Logits<T, NV>& x, uint32_t& use, int64_t base) {
+        x.template load<VEC>(rows_at(logits + base * E, T_ - base, kTokens, E), offset, in);
+        const int64_t left = T_ - base;
+        const uint32_t tokens = left > 0 ? (uint32_t)(left < kTokens ? left : kTokens) : 0u;
+        if (mask) use = (uint8_t)__builtin_amdgcn_raw_buffer_load_b8(
+                      __builtin_amdgcn_make_buffer_rsrc(const_cast<uint8_t*>(mask) + base, 0, (int)tokens, 0x00020000), token, 0, 0);
+        else use = (uint32_t)token < tokens ? 1u : 0u;
+    };
+    Logits<T, NV> x, next;
+    uint32_t use, next_use;
+    int64_t base = (int64_t)blockIdx.x * kTokens;
+    const int64_t step = (int64_t)gridDim.x * kTokens;
+    fetch(x, use, base);
     // (all lanes of a wavefront stay in the loop: they look at each other's values)
-    for (int64_t base = (int64_t)blockIdx.x * kTokens; base < T_; base += (int64_t)gridDim.x * kTokens) {
-        const int64_t t = base + threadIdx.x / L;
-        const bool counted = t < T_ && (!mask || mask[t] != 0);
-        T x[NV] = {};
-        if (counted) load_logits<T, NV, VEC>(logits + t * E, first, E, x);
-        float p[NV];
-        const float lse = softmax_token<T, L, NV>(x, first, E, p);
-        const uint32_t chosen = choose<T, L, NV>(x, first, E, k, counted);
+    for (; base < T_; base += step) {
+        fetch(next, next_use, base + step);  // the next tokens, before these are worked on
+        const bool counted = use != 0;
+        x.template settle<VEC>(counted, in);
+        float e[NV], top, sum;
+        softmax_token<T, L, NV>(x, e, top, sum);
+        const float inv = counted ? __builtin_amdgcn_rcpf(sum) : 0.f, lse = counted ? top + __logf(sum) : 0.f;
 #pragma unroll
-        for (int i = 0; i < NV; ++i) {
-            psum[i] += counted ? p[i] : 0.f;
-            count[i] += chosen >> i & 1u;
-        }
-        if (counted && lane == 0) {
-            zsum += (double)lse * (double)lse;
-            ++n;
-        }
+        for (int i = 0; i < NV; ++i) psum[i] += e[i] * inv;
+        zsum = __builtin_fma((double)lse, (double)lse, zsum);
+        n += counted ? 1u : 0u;
+        if (__any(lse != lse)) count_largest<T, L, NV, true>(x, in, enough_lanes, k, counted, count);
+        else count_largest<T, L, NV, false>(x, in, enough_lanes, k, counted, count);
+        x = next;
+        use = next_use;
+    }
+    if (lane != 0) {  // (the lanes of a token have the same)
+        zsum = 0.0;
+        n = 0;
     }
     const int wave = threadIdx.x / kWave;
 #pragma unroll
-    for (int d = L; d < kWave; d <<= 1) {
-#pragma unroll
-        for (int i = 0; i < NV; ++i) {
-            psum[i] += __shfl_xor(psum[i], d, kWave);
-            count[i] += (uint32_t)__shfl_xor((int)count[i], d, kWave);
-        }
+    for (int i = 0; i < NV; ++i) {
+        psum[i] = over_tokens<L>(psum[i]);
+        count[i] = over_tokens<L>(count[i]);
     }
 #pragma unroll
     for (int d = 1; d < kWave; d <<= 1) {
@@ -263,67 +365,86 @@ __global__ __launch_bounds__(kFwdThreads) void router_loss_kernel(const T* __res
 }
 
 // table: E f_e of every expert, then 1 / N, for the backward pass
-constexpr int kJoinThreads = 1024;
+constexpr int kJoinThreads = 1024, kJoinWaves = kJoinThreads / kWave;
+struct Total {
+    double a, b;
+};
+// over the workgroup, in a fixed order; every thread gets both
+__device__ __forceinline__ Total join_total(double a, double b, double (*slots)[2]) {
+#pragma unroll
+    for (int d = 1; d < kWave; d <<= 1) {
+        a += __shfl_xor(a, d, kWave);
+        b += __shfl_xor(b, d, kWave);
+    }
+    if ((threadIdx.x & (kWave - 1)) == 0) {
+        slots[threadIdx.x / kWave][0] = a;
+        slots[threadIdx.x / kWave][1] = b;
+    }
+    __syncthreads();
+    Total t{0.0, 0.0};
+#pragma unroll
+    for (int w = 0; w < kJoinWaves; ++w) {
+        t.a += slots[w][0];
+        t.b += slots[w][1];
+    }
+    return t;
+}
+
 __global__ __launch_bounds__(kJoinThreads) void router_loss_join_kernel(Partial part, int G, int E, uint32_t k, float* __restrict__ balance,
                                                                         float* __restrict__ z, uint32_t* __restrict__ counts,
                                                                         float* __restrict__ table) {
     __shared__ double s_sum[kJoinThreads];
-    __shared__ uint64_t s_count[kJoinThreads];
+    __shared__ uint32_t s_count[kJoinThreads];
+    __shared__ double s_total[2][kJoinWaves][2];
     const int tid = threadIdx.x;
-    auto total = [&](double v) {  // over the workgroup, in a fixed order
-        s_sum[tid] = v;
-        __syncthreads();
-        for (int d = kJoinThreads / 2; d > 0; d >>= 1) {
-            if (tid < d) s_sum[tid] += s_sum[tid + d];
-            __syncthreads();
-        }
-        const double t = s_sum[0];
-        __syncthreads();
-        return t;
-    };
-    double zsum = 0.0, tokens = 0.0;
-    for (int g = tid; g < G; g += kJoinThreads) {
-        zsum += part.z[g];
-        tokens += (double)part.n[g];
-    }
-    zsum = total(zsum);
-    tokens = total(tokens);
-    const double inv_n = tokens > 0.0 ? 1.0 / tokens : 0.0;
-    // a power of two of columns at a time, the other threads share the rows
+    // a power of two of columns, the other threads share the rows; eight rows of a thread on the way at a time
     int cols = 1;
-    while (cols < E && cols < kJoinThreads) cols <<= 1;
-    const int rows = kJoinThreads / cols, col = tid % cols, row = tid / cols;
+    while (cols < E) cols <<= 1;
+    const int rows = kJoinThreads / cols, col = tid & (cols - 1), row = tid / cols;
     double p = 0.0;
-    uint64_t c = 0;
+    uint32_t c = 0;
     if (col < E)
-        for (int g = row; g < G; g += rows) {
-            p += (double)part.p[(int64_t)g * E + col];
-            c += part.c[(int64_t)g * E + col];
+        for (int g = row; g < G; g += 8 * rows) {
+            float pv[8];
+            uint32_t cv[8];
+#pragma unroll
+            for (int u = 0; u < 8; ++u) {
+                const int at = g + u * rows < G ? g + u * rows : g;
+                pv[u] = part.p[(int64_t)at * E + col];
+                cv[u] = part.c[(int64_t)at * E + col];
+            }
+#pragma unroll
+            for (int u = 0; u < 8; ++u)
+                if (g + u * rows < G) {
+                    p += (double)pv[u];
+                    c += cv[u];
+                }
         }
+    double zsum = 0.0, tokens = 0.0;
+    if (tid < G) {  // (G is at most the number of compute units)
+        zsum = part.z[tid];
+        tokens = (double)part.n[tid];
+    }
+    const Total all = join_total(zsum, tokens, s_total[0]);
+    const double inv_n = all.b > 0.0 ? 1.0 / all.b : 0.0;
     s_sum[tid] = p;
     s_count[tid] = c;
     __syncthreads();
-    for (int d = rows / 2; d > 0; d >>= 1) {
-        if (row < d) {
-            s_sum[tid] += s_sum[tid + d * cols];
-            s_count[tid] += s_count[tid + d * cols];
-        }
-        __syncthreads();
-    }
-    p = s_sum[tid];
-    c = s_count[tid];
-    __syncthreads();
     double term = 0.0;
-    if (row == 0 && col < E) {
+    if (tid < cols && tid < E) {
+        for (int r = 1; r < rows; ++r) {
+            p += s_sum[tid + r * cols];
+            c += s_count[tid + r * cols];
+        }
         const double f = (double)c * inv_n / (double)k;
         term = f * p;
-        counts[col] = (uint32_t)c;
-        table[col] = (float)((double)E * f);
+        counts[tid] = c;
+        table[tid] = (float)((double)E * f);
     }
-    term = total(term);
+    const Total loss = join_total(term, 0.0, s_total[1]);
     if (tid == 0) {
-        *balance = (float)((double)E * inv_n * term);
-        *z = (float)(zsum * inv_n);
+        *balance = (float)((double)E * inv_n * loss.a);
+        *z = (float)(all.a * inv_n);
         table[E] = (float)inv_n;
     }
 }
@@ -334,41 +455,49 @@ __global__ __launch_bounds__(kBwdThreads) void router_loss_bwd_kernel(const T* _
                                                                       const float* __restrict__ balance_grad,
                                                                       const float* __restrict__ z_grad, T* __restrict__ grad) {
     constexpr int kTokens = kBwdThreads / L;
-    const int first = (threadIdx.x & (L - 1)) * NV;
+    const int first = (threadIdx.x & (L - 1)) * NV, token = threadIdx.x / L;
+    const int in = E - first < 0 ? 0 : E - first < NV ? E - first : NV;
+    const uint32_t offset = (uint32_t)(token * E + first) * (uint32_t)sizeof(T);
     const float inv_n = table[E];
     const float gb = balance_grad ? *balance_grad * inv_n : 0.f, gz = z_grad ? 2.0f * *z_grad * inv_n : 0.f;
     float f[NV];
 #pragma unroll
-    for (int i = 0; i < NV; ++i) f[i] = first + i < E ? table[first + i] : 0.f;
+    for (int i = 0; i < NV; ++i) f[i] = i < in ? table[first + i] : 0.f;
     for (int64_t base = (int64_t)blockIdx.x * kTokens; base < T_; base += (int64_t)gridDim.x * kTokens) {
-        const int64_t t = base + threadIdx.x / L;
-        const bool in = t < T_, counted = in && (!mask || mask[t] != 0);
-        T x[NV] = {};
-        if (counted) load_logits<T, NV, VEC>(logits + t * E, first, E, x);
-        float p[NV];
-        const float lse = softmax_token<T, L, NV>(x, first, E, p);
+        Logits<T, NV> x;
+        x.template load<VEC>(rows_at(logits + base * E, T_ - base, kTokens, E), offset, in);
+        const bool counted = base + token < T_ && (!mask || mask[base + token] != 0);
+        x.template settle<VEC>(counted, in);
+        float e[NV], top, sum;
+        softmax_token<T, L, NV>(x, e, top, sum);
+        const float inv = counted ? __builtin_amdgcn_rcpf(sum) : 0.f, lse = top + __logf(sum);
         float dot = 0.f;
 #pragma unroll
-        for (int i = 0; i < NV; ++i) dot += f[i] * p[i];
-        dot = over_token<L, Sum>(dot);
+        for (int i = 0; i < NV; ++i) {
+            e[i] *= inv;
+            dot += f[i] * e[i];
+        }
+        const float shift = gz * lse - gb * over_token<L, Sum>(dot);
 #pragma unroll
-        for (int i = 0; i < NV; ++i) x[i] = Num<T>::down(counted ? p[i] * (gb * (f[i] - dot) + gz * lse) : 0.f);
-        if (!in) continue;
-        T* const to = grad + t * E + first;
+        for (int i = 0; i < NV; ++i) e[i] = counted ? e[i] * (gb * f[i] + shift) : 0.f;
+        const __amdgpu_buffer_rsrc_t to = rows_at(grad + base * E, T_ - base, kTokens, E);
         if constexpr (VEC) {
             constexpr int V = Vec16<T>::N;
 #pragma unroll
-            for (int i = 0; i < NV / V; ++i)
-                if (first + i * V < E) {
-                    Vec16<T> v;
+            for (int v = 0; v < NV / V; ++v) {
+                Vec16<T> o;
 #pragma unroll
-                    for (int e = 0; e < V; ++e) v.v[e] = x[i * V + e];
-                    *(Vec16<T>*)(to + i * V) = v;
-                }
+                for (int i = 0; i < V; ++i) o.v[i] = Num<T>::down(e[v * V + i]);
+                typedef __attribute__((ext_vector_type(4))) uint32_t u32x4;
+                __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4, o), to, (int)(v * V < in ? offset + v * 16 : kNowhere), 0, 0);
+            }
         } else {
 #pragma unroll
-            for (int i = 0; i < NV; ++i)
-                if (first + i < E) to[i] = x[i];
+            for (int i = 0; i < NV; ++i) {
+                const uint32_t at = i < in ? offset + (uint32_t)(i * sizeof(T)) : kNowhere;
+                if constexpr (sizeof(T) == 4) __builtin_amdgcn_raw_buffer_store_b32(__float_as_uint(e[i]), to, (int)at, 0, 0);
+                else __builtin_amdgcn_raw_buffer_store_b16(__builtin_bit_cast(uint16_t, Num<T>::down(e[i])), to, (int)at, 0, 0);
+            }
         }
     }
 }
@@ -385,7 +514,7 @@ int lanes_per_token(int64_t E) {
 
 // workgroups of the forward pass: rows of the workspace
 int64_t forward_workgroups(int64_t T, int64_t E) {
-    const int64_t tokens = kFwdThreads / lanes_per_token(E), want = (T + tokens - 1) / tokens, most = compute_units();
+    const int64_t tokens = fwd_threads(E > 512 ? 16 : 8) / lanes_per_token(E), want = (T + tokens - 1) / tokens, most = compute_units();
     return want < 1 ? 1 : want < most ? want : most;
 }
 
@@ -430,7 +559,7 @@ int launch_fwd(const void* logits, const uint8_t* mask, int64_t T_, int64_t E, i
     const Partial part = partial_of(workspace, G, E);
     with_shape(E, whole_vectors<T>(logits, nullptr, E), [&](auto lanes, auto values, auto vec) {
         hipLaunchKernelGGL((router_loss_kernel<T, decltype(lanes)::value, decltype(values)::value, decltype(vec)::value>), dim3((uint32_t)G),
-                           dim3(kFwdThreads), 0, st, (const T*)logits, mask, T_, (int)E, (uint32_t)k, part);
+                           dim3(fwd_threads(decltype(values)::value)), 0, st, (const T*)logits, mask, T_, (int)E, (uint32_t)k, part);
         return 0;
     });
     const int rc = launch_status("router_loss");

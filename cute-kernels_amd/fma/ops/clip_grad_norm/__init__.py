@@ -19,7 +19,7 @@ def _gradients(parameters: torch.Tensor | Iterable[torch.Tensor]) -> list[torch.
     """a parameter that comes twice (a tied one) has one gradient"""
     if isinstance(parameters, torch.Tensor):
         parameters = (parameters,)
-    return [grad for grad in [p.grad for p in dict.fromkeys(parameters)] if grad is not None]
+    return [grad for grad in [p.grad for p in {id(p): p for p in parameters}.values()] if grad is not None]
 
 
 def _is_infinity_norm(norm_type: float) -> bool:

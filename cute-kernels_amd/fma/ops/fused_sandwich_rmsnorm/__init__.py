@@ -34,19 +34,16 @@ def gate_rows(gate: torch.Tensor, x: torch.Tensor) -> int:
 
 class _FusedSandwichRMSNorm(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, x, residual, post_weight, weight, gate, eps, multiplier, grad_enabled):
-        x, residual = x.contiguous(), residual.contiguous()
-        post_weight, weight, gate = (t if t is None else t.contiguous() for t in (post_weight, weight, gate))
+    def forward(ctx, x, residual, post_weight, weight, gate, rows_of_gate, eps, multiplier, grad_enabled):
+        x, residual, post_weight, weight, gate = [t if t is None else t.contiguous() for t in (x, residual, post_weight, weight, gate)]
         output, stream = torch.empty_like(x), torch.empty_like(x)
         keep = grad_enabled and any(ctx.needs_input_grad)
-        rows = x.numel() // x.size(-1)
-        stats = x.new_empty(2, rows, dtype=torch.float32) if keep else None  # 1 / rms of every row of x and of the stream
-        fused_sandwich_rmsnorm_forward_cuda(
-            x, residual, post_weight, weight, gate, output, stream, stats, 0 if gate is None else gate_rows(gate, x), eps, multiplier
-        )
+        # 1 / rms of every row of x and of the stream
+        stats = torch.empty(2, x.numel() // x.size(-1), dtype=torch.float32, device=x.device) if keep else None
+        fused_sandwich_rmsnorm_forward_cuda(x, residual, post_weight, weight, gate, output, stream, stats, rows_of_gate, eps, multiplier)
         if keep:
             ctx.save_for_backward(x, stream, post_weight, weight, gate, stats)
-            ctx.multiplier = multiplier
+            ctx.rows_of_gate, ctx.multiplier = rows_of_gate, multiplier
         ctx.set_materialize_grads(False)
         return output, stream
 
@@ -54,20 +51,20 @@ class _FusedSandwichRMSNorm(torch.autograd.Function):
     @once_differentiable
     def backward(ctx, output_grad, stream_grad):
         if output_grad is None and stream_grad is None:
-            return (None,) * 8
+            return (None,) * 9
         x, stream, post_weight, weight, gate, stats = ctx.saved_tensors
-        output_grad, stream_grad = (t if t is None else t.contiguous() for t in (output_grad, stream_grad))
+        output_grad, stream_grad = [t if t is None else t.contiguous() for t in (output_grad, stream_grad)]
         x_grad, residual_grad = torch.empty_like(x), torch.empty_like(x)
-        needs = ctx.needs_input_grad[2:5]
+        rows = x.numel()
         # (without rows the sums over them are zero)
-        new = torch.empty_like if x.numel() else torch.zeros_like
-        post_weight_grad, weight_grad, gate_grad = (new(t) if n else None for t, n in zip((post_weight, weight, gate), needs))
-        if x.numel():
+        new = torch.empty_like if rows else torch.zeros_like
+        post_weight_grad, weight_grad, gate_grad = [new(t) if n else None for t, n in zip((post_weight, weight, gate), ctx.needs_input_grad[2:5])]
+        if rows:
             fused_sandwich_rmsnorm_backward_cuda(
                 x, stream, post_weight, weight, gate, output_grad, stream_grad, stats, x_grad, residual_grad, post_weight_grad, weight_grad,
-                gate_grad, 0 if gate is None else gate_rows(gate, x), ctx.multiplier,
+                gate_grad, ctx.rows_of_gate, ctx.multiplier,
             )  # fmt: skip
-        return x_grad, residual_grad, post_weight_grad, weight_grad, gate_grad, None, None, None
+        return x_grad, residual_grad, post_weight_grad, weight_grad, gate_grad, None, None, None, None
 
 
 def fused_sandwich_rmsnorm(
@@ -95,15 +92,12 @@ def fused_sandwich_rmsnorm(
         raise ValueError(f"unexpected kernel_backend ({kernel_backend})")
     assert x.dtype in _FLOATS, f"fused_sandwich_rmsnorm takes float32, float16 and bfloat16, not {x.dtype}"
     assert x.dim() >= 1 and x.size(-1) > 0, "x should have rows of one element at least"
-    assert residual.shape == x.shape and residual.dtype == x.dtype, "x and residual should be of one shape and dtype"
-    for name, w in (("post_weight", post_weight), ("weight", weight)):
-        assert w is None or (w.shape == x.shape[-1:] and w.dtype == x.dtype), f"{name} should be 1-D, of x's row length and dtype"
+    rows = 0
     if gate is not None:
         assert gate.dtype == x.dtype, "gate should have x's dtype"
-        gate_rows(gate, x)
-    for t in (residual, post_weight, weight, gate):
-        assert t is None or t.device == x.device, "all tensors should be on one device"
+        rows = gate_rows(gate, x)
+    # (the operator looks at the other tensors)
     eps = torch.finfo(x.dtype).eps if eps is None else float(eps)
     return _FusedSandwichRMSNorm.apply(
-        x, residual, post_weight, weight, gate, eps, 1.0 if multiplier is None else float(multiplier), torch.is_grad_enabled()
+        x, residual, post_weight, weight, gate, rows, eps, 1.0 if multiplier is None else float(multiplier), torch.is_grad_enabled()
     )

@@ -14,10 +14,10 @@ MAX_EXPERTS = 1024
 class _RouterLoss(torch.autograd.Function):
     @staticmethod
     def forward(ctx, logits: torch.Tensor, top_k: int, mask: torch.Tensor | None) -> tuple[torch.Tensor, ...]:
-        E = logits.size(1)
-        balance, z = logits.new_empty((), dtype=torch.float32), logits.new_empty((), dtype=torch.float32)
-        counts = torch.empty(E, dtype=torch.uint32, device=logits.device)
-        table = logits.new_empty(E + 1, dtype=torch.float32)  # what the backward needs to know of all tokens
+        E, device = logits.size(1), logits.device
+        balance, z = [torch.empty((), dtype=torch.float32, device=device) for _ in range(2)]
+        counts = torch.empty(E, dtype=torch.uint32, device=device)
+        table = torch.empty(E + 1, dtype=torch.float32, device=device)  # what the backward needs to know of all tokens
         router_loss_cuda(logits, mask, top_k, balance, z, counts, table)
         ctx.save_for_backward(logits, mask, table)
         ctx.mark_non_differentiable(counts)
@@ -60,12 +60,11 @@ def router_loss(
     *tokens, E = router_logits.shape
     assert 1 <= E <= MAX_EXPERTS, f"there should be 1 to {MAX_EXPERTS} experts, not {E}"
     assert 1 <= num_experts_per_tok <= E, f"num_experts_per_tok should be in [1, {E}], not {num_experts_per_tok}"
-    logits = router_logits.reshape(-1, E).contiguous()
+    logits = (router_logits if len(tokens) == 1 else router_logits.reshape(-1, E)).contiguous()
     if mask is not None:
         assert mask.dtype == torch.bool, "mask should be bool"
         assert mask.shape == tuple(tokens) or (len(tokens) == 1 and mask.numel() == tokens[0]), (
             f"a mask of shape {tuple(mask.shape)} does not fit logits of shape {tuple(router_logits.shape)}"
         )
-        assert mask.device == logits.device, "mask and router_logits should be on one device"
         mask = mask.reshape(-1).contiguous()
     return _RouterLoss.apply(logits, num_experts_per_tok, mask)
