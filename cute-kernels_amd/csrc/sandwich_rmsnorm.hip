@@ -148,7 +148,7 @@ __device__ __forceinline__ float at(const T* p, int64_t i) {
 
 __device__ __forceinline__ int64_t gate_row(const Shape& s, int64_t row) { return (uint32_t)row / (uint32_t)s.R; }  // (both below 2^31)
 
-// ---- any H, any alignment: element by element -----------------------------------------------------------------------------
+// ---- rows that no team holds: element by element, inputs read again from the caches ---------------------------------------------
 
 template <typename T>
 __global__ __launch_bounds__(kThreads) void sandwich_fwd_generic_kernel(const FwdArgs<T> k) {
@@ -250,12 +250,14 @@ __global__ __launch_bounds__(kThreads) void sandwich_bwd_generic_kernel(const Bw
     }
 }
 
-// ---- rows of whole 16-byte vectors: a row in the registers of its team of threads -----------------------------------------------
+// ---- a row in the registers of its team of threads ------------------------------------------------------------------------------
 //
-// A team of TEAM threads per row, VPT vectors per thread, the next row requested before this one is worked on. All accesses of the loops are
-// buffer instructions, whose range check stands for every condition: past the row's end, behind the last row, where a tensor is absent
-// (num_records 0), loads give zeros and stores go nowhere. A branch around a load or a store would make the compiler wait for everything
-// that is outstanding, the next row included, since it cannot count what lies behind.
+// A team of TEAM threads per row, VPT vectors of 16 bytes per thread, the next row requested before this one is worked on. All accesses of
+// the loops are buffer instructions, whose range check stands for every condition: past the row's end (each dword of an access by itself),
+// behind the last row, where a tensor is absent (num_records 0), loads give zeros and stores go nowhere. A branch around a load or a store
+// would make the compiler wait for everything that is outstanding, the next row included, since it cannot count what lies behind.
+// Rows that start on a dword boundary are accessed 16 bytes at a time; those of an odd number of 16-bit elements, or off such a boundary,
+// element by element (ELEM), in the same places.
 
 template <int CTRL>
 __device__ __forceinline__ float dpp_add(float v) {
@@ -338,14 +340,35 @@ constexpr uint32_t kNowhere = 0x7fffffffu;  // an offset past every buffer
 __device__ __forceinline__ __amdgpu_buffer_rsrc_t buffer_of(const void* p, uint32_t bytes) {
     return __builtin_amdgcn_make_buffer_rsrc(const_cast<void*>(p), 0, p ? (int)bytes : 0, 0x00020000);
 }
-template <int TEAM, int VPT, int POLICY>
+template <bool ELEM, int TEAM, int VPT, int POLICY>
 __device__ __forceinline__ void load_row(Raw (&to)[VPT], __amdgpu_buffer_rsrc_t row, int tid) {
 #pragma unroll
-    for (int i = 0; i < VPT; ++i) to[i] = __builtin_amdgcn_raw_buffer_load_b128(row, (tid + i * TEAM) * 16, 0, POLICY);
+    for (int i = 0; i < VPT; ++i) {
+        const int at = (tid + i * TEAM) * 16;
+        if constexpr (ELEM) {
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                const uint32_t low = (uint16_t)__builtin_amdgcn_raw_buffer_load_b16(row, at + 4 * j, 0, 0);
+                to[i][j] = low | (uint32_t)(uint16_t)__builtin_amdgcn_raw_buffer_load_b16(row, at + 4 * j + 2, 0, 0) << 16;
+            }
+        } else {
+            to[i] = __builtin_amdgcn_raw_buffer_load_b128(row, at, 0, POLICY);
+        }
+    }
 }
-template <typename T>
+template <bool ELEM, typename T>
 __device__ __forceinline__ void store_row(__amdgpu_buffer_rsrc_t row, int v, const float (&f)[Wide<T>::N]) {
-    __builtin_amdgcn_raw_buffer_store_b128(Wide<T>::down(f), row, v * 16, 0, kStream);
+    const Raw r = Wide<T>::down(f);
+    if constexpr (ELEM) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            const uint32_t two = r[j];
+            __builtin_amdgcn_raw_buffer_store_b16((uint16_t)two, row, v * 16 + 4 * j, 0, 0);
+            __builtin_amdgcn_raw_buffer_store_b16((uint16_t)(two >> 16), row, v * 16 + 4 * j + 2, 0, 0);
+        }
+    } else {
+        __builtin_amdgcn_raw_buffer_store_b128(r, row, v * 16, 0, kStream);
+    }
 }
 __device__ __forceinline__ float load_float(__amdgpu_buffer_rsrc_t b, uint32_t offset) {
     return __uint_as_float(__builtin_amdgcn_raw_buffer_load_b32(b, (int)offset, 0, 0));
@@ -365,9 +388,9 @@ __device__ __forceinline__ void store_element(__amdgpu_buffer_rsrc_t b, uint32_t
 }
 
 // a thread's share of a weight, kept over all rows: ones where there is none
-template <typename T, int TEAM, int VPT>
+template <bool ELEM, typename T, int TEAM, int VPT>
 __device__ __forceinline__ void load_weight(Raw (&to)[VPT], const T* p, uint32_t bytes, int tid) {
-    load_row<TEAM, VPT, 0>(to, buffer_of(p, bytes), tid);
+    load_row<ELEM, TEAM, VPT, 0>(to, buffer_of(p, bytes), tid);
     if (!p) {
 #pragma unroll
         for (int i = 0; i < VPT; ++i) to[i] = Wide<T>::kOnes;
@@ -387,7 +410,7 @@ __device__ __forceinline__ int64_t team_index() {
     else return (int64_t)blockIdx.x * teams_of(TEAM) + __builtin_amdgcn_readfirstlane((int)(threadIdx.x / TEAM));
 }
 
-template <typename T, int TEAM, int VPT, Mode MODE>
+template <typename T, bool ELEM, int TEAM, int VPT, Mode MODE>
 __global__ __launch_bounds__(TEAM * teams_of(TEAM)) void sandwich_fwd_kernel(const FwdArgs<T> k) {
     constexpr int N = Wide<T>::N;
     constexpr bool kVector = MODE == kFull || MODE == kGroup;
@@ -397,18 +420,18 @@ __global__ __launch_bounds__(TEAM * teams_of(TEAM)) void sandwich_fwd_kernel(con
     const int64_t H = k.s.H, step = (int64_t)gridDim.x * teams_of(TEAM);
     const uint32_t bytes = (uint32_t)(H * (int64_t)sizeof(T)), first_lane = tid == 0 ? 0u : kNowhere;
     Raw wp[VPT], w[VPT];
-    load_weight<T, TEAM, VPT>(wp, k.post_weight, bytes, tid);
-    load_weight<T, TEAM, VPT>(w, k.weight, bytes, tid);
+    load_weight<ELEM, T, TEAM, VPT>(wp, k.post_weight, bytes, tid);
+    load_weight<ELEM, T, TEAM, VPT>(w, k.weight, bytes, tid);
     struct Row {
         Raw x[VPT], r[VPT], gate[VPT];
         float scalar;
     } now, next;
     auto fetch = [&](Row& to, int64_t row) {
         const uint32_t n = row < k.s.B ? bytes : 0u;
-        load_row<TEAM, VPT, kStream>(to.x, buffer_of(k.x + row * H, n), tid);
-        load_row<TEAM, VPT, kStream>(to.r, buffer_of(k.residual + row * H, n), tid);
-        if constexpr (MODE == kFull) load_row<TEAM, VPT, kStream>(to.gate, buffer_of(k.gate + row * H, n), tid);
-        if constexpr (MODE == kGroup) load_row<TEAM, VPT, 0>(to.gate, buffer_of(k.gate + gate_row(k.s, row) * H, n), tid);
+        load_row<ELEM, TEAM, VPT, kStream>(to.x, buffer_of(k.x + row * H, n), tid);
+        load_row<ELEM, TEAM, VPT, kStream>(to.r, buffer_of(k.residual + row * H, n), tid);
+        if constexpr (MODE == kFull) load_row<ELEM, TEAM, VPT, kStream>(to.gate, buffer_of(k.gate + row * H, n), tid);
+        if constexpr (MODE == kGroup) load_row<ELEM, TEAM, VPT, 0>(to.gate, buffer_of(k.gate + gate_row(k.s, row) * H, n), tid);
         if constexpr (MODE == kScalar) to.scalar = load_element<T>(buffer_of(k.gate + gate_row(k.s, row), n ? (uint32_t)sizeof(T) : 0u));
     };
     int64_t row = team_index<TEAM>();
@@ -439,7 +462,7 @@ __global__ __launch_bounds__(TEAM * teams_of(TEAM)) void sandwich_fwd_kernel(con
                 f[i][e] = Wide<T>::up(now.r[i], e) + a * n;
                 ss += f[i][e] * f[i][e];
             }
-            store_row<T>(to_stream, v, f[i]);
+            store_row<ELEM, T>(to_stream, v, f[i]);
         }
         const float inv_r = inverse_rms(team_sum<TEAM>(ss, s_red, parity), k.inv_H, k.eps);
 #pragma unroll
@@ -447,7 +470,7 @@ __global__ __launch_bounds__(TEAM * teams_of(TEAM)) void sandwich_fwd_kernel(con
             float o[N];
 #pragma unroll
             for (int e = 0; e < N; ++e) o[e] = f[i][e] * inv_r * Wide<T>::up(w[i], e);
-            store_row<T>(to_out, tid + i * TEAM, o);
+            store_row<ELEM, T>(to_out, tid + i * TEAM, o);
         }
         store_float(buffer_of(k.stats ? k.stats + row : nullptr, 4), first_lane, inv_x);
         store_float(buffer_of(k.stats ? k.stats + k.s.B + row : nullptr, 4), first_lane, inv_r);
@@ -455,7 +478,7 @@ __global__ __launch_bounds__(TEAM * teams_of(TEAM)) void sandwich_fwd_kernel(con
     }
 }
 
-template <typename T, int TEAM, int VPT, Mode MODE>
+template <typename T, bool ELEM, int TEAM, int VPT, Mode MODE>
 __global__ __launch_bounds__(TEAM * teams_of(TEAM)) void sandwich_bwd_kernel(const BwdArgs<T> k) {
     constexpr int N = Wide<T>::N, kTeams = teams_of(TEAM);
     constexpr bool kAhead = TEAM * VPT <= 1024;  // (two vectors for each of 1024 threads leave no registers for a second row)
@@ -466,9 +489,9 @@ __global__ __launch_bounds__(TEAM * teams_of(TEAM)) void sandwich_bwd_kernel(con
     const int64_t H = k.s.H, worker = team_index<TEAM>();
     const uint32_t bytes = (uint32_t)(H * (int64_t)sizeof(T)), first_lane = tid == 0 ? 0u : kNowhere;
     Raw wp[VPT], w[VPT], channel[VPT];
-    load_weight<T, TEAM, VPT>(wp, k.post_weight, bytes, tid);
-    load_weight<T, TEAM, VPT>(w, k.weight, bytes, tid);
-    if constexpr (MODE == kChannel) load_row<TEAM, VPT, 0>(channel, buffer_of(k.gate, bytes), tid);
+    load_weight<ELEM, T, TEAM, VPT>(wp, k.post_weight, bytes, tid);
+    load_weight<ELEM, T, TEAM, VPT>(w, k.weight, bytes, tid);
+    if constexpr (MODE == kChannel) load_row<ELEM, TEAM, VPT, 0>(channel, buffer_of(k.gate, bytes), tid);
     float sw[VPT][N], swp[VPT][N], sg[VPT][N];
 #pragma unroll
     for (int i = 0; i < VPT; ++i)
@@ -482,12 +505,12 @@ __global__ __launch_bounds__(TEAM * teams_of(TEAM)) void sandwich_bwd_kernel(con
     auto fetch = [&](Row& to, int64_t row, bool in) {
         const int64_t base = row * H;
         const uint32_t n = in ? bytes : 0u, one = in ? 4u : 0u;
-        load_row<TEAM, VPT, kStream>(to.x, buffer_of(k.x + base, n), tid);
-        load_row<TEAM, VPT, kStream>(to.r, buffer_of(k.stream + base, n), tid);
-        load_row<TEAM, VPT, kStream>(to.dy, buffer_of(k.d_out ? k.d_out + base : nullptr, n), tid);
-        load_row<TEAM, VPT, kStream>(to.dr, buffer_of(k.d_stream ? k.d_stream + base : nullptr, n), tid);
-        if constexpr (MODE == kFull) load_row<TEAM, VPT, kStream>(to.gate, buffer_of(k.gate + base, n), tid);
-        if constexpr (MODE == kGroup) load_row<TEAM, VPT, 0>(to.gate, buffer_of(k.gate + gate_row(k.s, row) * H, n), tid);
+        load_row<ELEM, TEAM, VPT, kStream>(to.x, buffer_of(k.x + base, n), tid);
+        load_row<ELEM, TEAM, VPT, kStream>(to.r, buffer_of(k.stream + base, n), tid);
+        load_row<ELEM, TEAM, VPT, kStream>(to.dy, buffer_of(k.d_out ? k.d_out + base : nullptr, n), tid);
+        load_row<ELEM, TEAM, VPT, kStream>(to.dr, buffer_of(k.d_stream ? k.d_stream + base : nullptr, n), tid);
+        if constexpr (MODE == kFull) load_row<ELEM, TEAM, VPT, kStream>(to.gate, buffer_of(k.gate + base, n), tid);
+        if constexpr (MODE == kGroup) load_row<ELEM, TEAM, VPT, 0>(to.gate, buffer_of(k.gate + gate_row(k.s, row) * H, n), tid);
         if constexpr (MODE == kScalar) to.scalar = load_element<T>(buffer_of(k.gate + gate_row(k.s, row), in ? (uint32_t)sizeof(T) : 0u));
         to.inv_x = load_float(buffer_of(k.stats + row, one), 0);
         to.inv_r = load_float(buffer_of(k.stats + k.s.B + row, one), 0);
@@ -547,7 +570,7 @@ __global__ __launch_bounds__(TEAM * teams_of(TEAM)) void sandwich_bwd_kernel(con
                 dot += u * Wide<T>::up(now.x[i], e);
                 o[e] = dr;
             }
-            store_row<T>(to_residual, tid + i * TEAM, o);
+            store_row<ELEM, T>(to_residual, tid + i * TEAM, o);
         }
         dot = team_sum<TEAM>(dot, s_red, parity) * now.inv_x;
         if constexpr (MODE == kScalar) {
@@ -573,8 +596,8 @@ __global__ __launch_bounds__(TEAM * teams_of(TEAM)) void sandwich_bwd_kernel(con
                 swp[i][e] += (MODE == kChannel ? dz : gated) * xh;
                 if constexpr (MODE == kGroup) sg[i][e] += dz * xh;
             }
-            store_row<T>(to_x, tid + i * TEAM, o);
-            if constexpr (MODE == kFull) store_row<T>(buffer_of(k.d_gate ? k.d_gate + base : nullptr, bytes), tid + i * TEAM, og);
+            store_row<ELEM, T>(to_x, tid + i * TEAM, o);
+            if constexpr (MODE == kFull) store_row<ELEM, T>(buffer_of(k.d_gate ? k.d_gate + base : nullptr, bytes), tid + i * TEAM, og);
         }
         if constexpr (MODE == kGroup)
             if (!more || next_group != group) {  // the group's sum is whole here, or this team's part of it
@@ -591,7 +614,7 @@ __global__ __launch_bounds__(TEAM * teams_of(TEAM)) void sandwich_bwd_kernel(con
                         store_float(to_part, (uint32_t)(v * N + e) * 4, sg[i][e]);
                         sg[i][e] = 0.f;
                     }
-                    store_row<T>(to_gate, v, o);
+                    store_row<ELEM, T>(to_gate, v, o);
                 }
             }
         if constexpr (kAhead) now = next;
@@ -703,13 +726,24 @@ __global__ __launch_bounds__(kThreads) void sandwich_reduce_scalar_kernel(const 
 
 // ---- launch -------------------------------------------------------------------------------------------------------------------
 
-template <int TEAM, int VPT>
+template <int TEAM, int VPT, bool ELEM = false>
 struct Team {
     static constexpr int team = TEAM, vpt = VPT;
+    static constexpr bool elem = ELEM;
 };
-// calls `launch` with the team of a row of nvec vectors, as a type; false: no team holds it
-template <typename F>
-bool with_team(int64_t nvec, F launch) {
+// calls `launch` with the team of a row of nvec vectors, the last of which may not be full, as a type; false: no team holds it
+template <typename T, typename F>
+bool with_team(int64_t nvec, bool dwords, F launch) {
+    if (nvec > 2048) return false;
+    if constexpr (sizeof(T) == 2)
+        if (!dwords) {
+            if (nvec <= 128) launch(Team<64, 2, true>());
+            else if (nvec <= 256) launch(Team<256, 1, true>());
+            else if (nvec <= 512) launch(Team<512, 1, true>());
+            else if (nvec <= 1024) launch(Team<1024, 1, true>());
+            else launch(Team<1024, 2, true>());
+            return true;
+        }
     if (nvec <= 64) launch(Team<64, 1>());
     else if (nvec <= 128) launch(Team<64, 2>());
     else if (nvec <= 256) launch(Team<256, 1>());
@@ -717,16 +751,19 @@ bool with_team(int64_t nvec, F launch) {
     else if (nvec <= 512) launch(Team<512, 1>());
     else if (nvec <= 768) launch(Team<768, 1>());
     else if (nvec <= 1024) launch(Team<1024, 1>());
-    else if (nvec <= 2048) launch(Team<1024, 2>());
-    else return false;
+    else launch(Team<1024, 2>());
     return true;
 }
-// vectors of a row, or more than any team holds if rows are no whole vectors
 template <typename T>
-int64_t vectors_of(int64_t H, std::initializer_list<const void*> pointers) {
-    bool fine = H * (int64_t)sizeof(T) % 16 == 0;
-    for (const void* p : pointers) fine = fine && aligned16(p);
-    return fine ? H * (int64_t)sizeof(T) / 16 : INT64_MAX;
+int64_t vectors_of(int64_t H) {
+    return (H * (int64_t)sizeof(T) + 15) / 16;
+}
+// whether all rows start on a dword boundary
+template <typename T>
+bool dwords_of(int64_t H, std::initializer_list<const void*> pointers) {
+    bool fine = H * (int64_t)sizeof(T) % 4 == 0;
+    for (const void* p : pointers) fine = fine && ((uintptr_t)p & 3u) == 0;
+    return fine;
 }
 template <Mode MODE>
 using As = std::integral_constant<Mode, MODE>;
@@ -734,13 +771,13 @@ using As = std::integral_constant<Mode, MODE>;
 template <typename T>
 int launch_fwd(const FwdArgs<T>& k, hipStream_t st) {
     const int64_t cus = num_compute_units() > 0 ? num_compute_units() : 256;
-    const int64_t nvec = vectors_of<T>(k.s.H, {k.x, k.residual, k.post_weight, k.weight, k.s.mode == kScalar ? nullptr : k.gate, k.out, k.stream});
-    const bool held = with_team(nvec, [&](auto t) {
+    const bool dwords = dwords_of<T>(k.s.H, {k.x, k.residual, k.post_weight, k.weight, k.s.mode == kScalar ? nullptr : k.gate, k.out, k.stream});
+    const bool held = with_team<T>(vectors_of<T>(k.s.H), dwords, [&](auto t) {
         constexpr int TEAM = decltype(t)::team, VPT = decltype(t)::vpt;
         constexpr int kTeams = teams_of(TEAM);
         const int64_t want = (k.s.B + kTeams - 1) / kTeams, most = cus * (kFwdThreadsPerCU / (TEAM * kTeams));
         auto launch = [&](auto mode) {
-            hipLaunchKernelGGL((sandwich_fwd_kernel<T, TEAM, VPT, decltype(mode)::value>), dim3((uint32_t)(want < most ? want : most)),
+            hipLaunchKernelGGL((sandwich_fwd_kernel<T, decltype(t)::elem, TEAM, VPT, decltype(mode)::value>), dim3((uint32_t)(want < most ? want : most)),
                                dim3(TEAM * kTeams), 0, st, k);
         };
         switch (k.s.mode) {
@@ -760,14 +797,14 @@ template <typename T>
 int launch_bwd(BwdArgs<T> k, T* d_weight, T* d_post_weight, void* workspace, hipStream_t st) {
     k.p = split_of(k.s, kThreads, 1);  // of the element-wise kernel
     k.part = partial_of(workspace, k.s, k.p);
-    const int64_t nvec = vectors_of<T>(k.s.H, {k.x, k.stream, k.post_weight, k.weight, k.s.mode == kScalar ? nullptr : k.gate, k.d_out, k.d_stream, k.dx,
-                                               k.d_residual, k.s.mode == kScalar ? nullptr : k.d_gate});
-    const bool held = with_team(nvec, [&](auto t) {
+    const bool dwords = dwords_of<T>(k.s.H, {k.x, k.stream, k.post_weight, k.weight, k.s.mode == kScalar ? nullptr : k.gate, k.d_out, k.d_stream, k.dx,
+                                             k.d_residual, k.s.mode == kScalar ? nullptr : k.d_gate});
+    const bool held = with_team<T>(vectors_of<T>(k.s.H), dwords, [&](auto t) {
         constexpr int TEAM = decltype(t)::team, VPT = decltype(t)::vpt;
         k.p = split_of(k.s, TEAM, teams_of(TEAM));
         k.part = partial_of(workspace, k.s, k.p);
         auto launch = [&](auto mode) {
-            hipLaunchKernelGGL((sandwich_bwd_kernel<T, TEAM, VPT, decltype(mode)::value>), dim3((uint32_t)k.p.sums), dim3(TEAM * teams_of(TEAM)), 0,
+            hipLaunchKernelGGL((sandwich_bwd_kernel<T, decltype(t)::elem, TEAM, VPT, decltype(mode)::value>), dim3((uint32_t)k.p.sums), dim3(TEAM * teams_of(TEAM)), 0,
                                st, k);
         };
         switch (k.s.mode) {

@@ -37,7 +37,11 @@ class _Table:
         self.tensors = tensors  # (holds the copies)
         self._pointers = array("Q", [t.data_ptr() for t in tensors])
         self._sizes = array("q", [t.numel() for t in tensors])
-        self._dtypes = array("i", [_lib.dtype_code(d) for d in [t.dtype for t in tensors]])
+        codes = {d: _lib.dtype_code(d) for d in {t.dtype for t in tensors}}
+        if len(codes) == 1:
+            self._dtypes = array("i", codes.values()) * len(tensors)
+        else:
+            self._dtypes = array("i", [codes[t.dtype] for t in tensors])
         self.arguments = *(a.buffer_info()[0] for a in (self._pointers, self._sizes, self._dtypes)), len(tensors)
 
     def _dense(self, t: torch.Tensor, written: bool) -> torch.Tensor:
