@@ -92,10 +92,11 @@ Partial partial_of(void* workspace, const Shape& s, const Split& p) {
     part.gate = part.rows = part.wp + p.sums * s.H;  // (never both)
     return part;
 }
-// enough for every type and alignment
+// enough for every type and alignment (teams of a wavefront hold rows of up to 1024 elements)
 int64_t workspace_bytes_of(const Shape& s) {
     int64_t most = 0;
     for (int team : {64, 256, 1024}) {
+        if (team == 64 && s.H > 1024) continue;
         const Split p = split_of(s, team, teams_of(team));
         const int64_t n = p.sums * s.H * 2 + (s.mode == kGroup ? p.workers * s.H : 0) + (s.mode == kScalar ? s.B : 0);
         most = n > most ? n : most;

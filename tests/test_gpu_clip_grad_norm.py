@@ -261,3 +261,20 @@ def test_compiled_function_breaks_its_graph_here():
     got = torch.compile(step)(torch.ones((), device=DEV))
     _check_norm(got, want)
     _check_scaled(grads, before, want, 0.5)
+
+
+def test_long_tensors():
+    """elements past 2^31, and a set that is read and written as a stream"""
+    n = 2**31 + 16384 + 5
+    g = torch.zeros(n, dtype=torch.bfloat16, device=DEV)
+    places = torch.tensor([0, 1, 2**31 - 1, 2**31, 2**31 + 16383, n - 1], device=DEV)
+    g[places] = torch.arange(1.0, 7.0, device=DEV).bfloat16()
+    small = torch.full((3,), 2.0, device=DEV)
+    norm = fma.clip_grad_norm_(_parameters([small, g]), 0.5)
+    want = math.sqrt(91.0 + 12.0)
+    _check_norm(norm, want)
+    factor = 0.5 / (want + 1e-6)
+    for got, exact in ((g[places].double(), torch.arange(1.0, 7.0, device=DEV).double() * factor), (small.double(), small.new_full((3,), 2.0).double() * factor)):
+        assert bool(((got - exact).abs() <= exact * 2.0**-8 * 1.001).all())
+    assert int(torch.count_nonzero(g)) == 6
+    _check_norm(fma.get_total_norm([g], math.inf), float(g[n - 1].double()))

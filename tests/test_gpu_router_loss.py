@@ -299,6 +299,33 @@ def test_compiled_matches_eager():
     assert all(torch.equal(a, b) for a, b in zip(*out))
 
 
+def test_long_tensors():
+    """logits past 2^31: the counts of the whole are those of its parts, the last tokens' gradients theirs alone"""
+    E, k = 256, 8
+    T = 2**31 // E + 5000
+    logits = torch.zeros(T, E, dtype=torch.bfloat16, device=DEV)
+    logits[:, 0] = 1.0
+    logits[-3000:] = _logits(3000, E, torch.bfloat16)
+    mask = torch.zeros(T, dtype=torch.bool, device=DEV)
+    mask[-3000:] = True
+    _check(logits[-3000:], k, None, 0.7, -0.3, tuple(v if i < 3 else v[-3000:] for i, v in enumerate(_run(logits, k, mask, 0.7, -0.3))))
+    counts = fma.router_loss(logits, k)[2].view(torch.int32).long()
+    assert torch.equal(counts, sum(fma.router_loss(part, k)[2].view(torch.int32).long() for part in logits.split(T // 3)))
+
+
+def test_a_second_pass_through_the_same_node():
+    leaf = _logits(300, 40, torch.bfloat16).requires_grad_()
+    balance, z, _ = fma.router_loss(leaf, 3)
+    (balance + z).backward(retain_graph=True)
+    first, leaf.grad = leaf.grad, None
+    (balance + z).backward()
+    assert torch.equal(first, leaf.grad)
+    with torch.no_grad():
+        leaf.add_(1)
+    with pytest.raises(RuntimeError):  # changed since, or freed by now
+        (balance + z).backward()
+
+
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
 def test_losses_of_the_layers_logits(dtype):
     """the counts are those of the experts that the layer ran, and the losses' gradients reach the gate and the tokens"""

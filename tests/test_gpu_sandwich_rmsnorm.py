@@ -99,7 +99,7 @@ def _exact(t, grads, a, eps=_EPS):
     if t["post_weight"] is not None:
         want["d_post_weight"] = summed(s * gate, es * gate.abs() + 2 * _U * (s * gate).abs(), (H,))
     if t["gate"] is not None:
-        want["d_gate"] = summed(s * wp, es * wp.abs() + 2 * _U * (s * wp).abs(), t["gate"].shape, t["gate"].shape[-1] != H)
+        want["d_gate"] = summed(s * wp, es * wp.abs() + 2 * _U * (s * wp).abs(), t["gate"].shape, t["gate"].shape[-1:] != (H,))
     return want
 
 
@@ -134,7 +134,7 @@ def test_against_fp64(H, gate, dtype):
 # more rows than workgroups, sequences of one row, more sequences than workgroups, one long sequence, a single row
 @pytest.mark.parametrize("dtype", _DTYPES)
 @pytest.mark.parametrize("gate", _GATES)
-@pytest.mark.parametrize("shape", [(1, 1, 96), (1, 1, 4096), (1, 3001, 64), (5, 1023, 48), (3001, 1, 40), (1501, 2, 72), (700, 3, 1024), (2, 1100, 2048), (2, 600, 4096), (1, 1200, 1001)])
+@pytest.mark.parametrize("shape", [(1, 1, 96), (1, 1, 4096), (1, 3001, 64), (5, 1023, 48), (3001, 1, 40), (1501, 2, 72), (700, 3, 1024), (2, 1100, 2048), (2, 600, 4096), (1, 1200, 1001), (2500, 2, 72), (600, 2, 17000)])
 def test_many_rows(shape, gate, dtype):
     _check(shape, _DTYPES[dtype], gate)
 
@@ -146,6 +146,29 @@ def test_many_rows(shape, gate, dtype):
 def test_parts_left_out(H, dtype, use, weights):
     for gate in ("none", "channel", "token"):
         _check((2, 50, H), _DTYPES[dtype], gate, weights, use=use)
+
+
+def test_a_gate_without_dimensions():
+    t, grads = _inputs((2, 30, 96), torch.float32)
+    t["gate"] = torch.tensor(0.7, device=DEV)
+    _compare(_run(t, grads, 1.0), _exact(t, grads, 1.0))
+
+
+def test_the_same_tensor_twice():
+    """the block's output is its stream, and one scale serves both norms: each use adds to the gradient"""
+    t, grads = _inputs((2, 30, 256), torch.bfloat16)
+    t["residual"], t["weight"] = t["x"], t["post_weight"]
+    want = _exact(t, grads, 1.0)
+    x, w = t["x"].detach().requires_grad_(), t["weight"].detach().requires_grad_()
+    out, stream = fma.fused_sandwich_rmsnorm(x, x, w, w, _EPS)
+    torch.autograd.backward([out, stream], [d.expand_as(out) for d in grads], retain_graph=True)
+    first = x.grad.clone(), w.grad.clone()
+    for (a, b), grad in zip((("d_x", "d_residual"), ("d_weight", "d_post_weight")), first):
+        value, bound = want[a][0] + want[b][0], want[a][1] + want[b][1]
+        assert bool(((grad.double() - value).abs() <= bound + 2.0**-8 * value.abs() * 1.01).all())  # (and the sum of the two rounded)
+    x.grad = w.grad = None
+    torch.autograd.backward([out, stream], grads)  # a second time through the same node
+    assert torch.equal(x.grad, first[0]) and torch.equal(w.grad, first[1])
 
 
 @pytest.mark.parametrize("H", [60, 2048, 20000])
@@ -341,6 +364,20 @@ def test_compiled_matches_eager():
         eager = _run(t, grads, 0.5)
         compiled = _run(t, grads, 0.5, function=torch.compile(fma.fused_sandwich_rmsnorm, fullgraph=True))
         assert all(torch.equal(eager[n], compiled[n]) for n in eager)
+    with torch.no_grad():
+        outputs = torch.compile(fma.fused_sandwich_rmsnorm, fullgraph=True)(t["x"], t["residual"], t["post_weight"], t["weight"], _EPS, t["gate"], 0.5)
+    assert torch.equal(outputs[0], eager["out"]) and torch.equal(outputs[1], eager["stream"])
+
+
+def test_transforms_are_not_passed_over():
+    """forward mode and functorch, which have no rule for this operator, raise; also without grad mode"""
+    t, _ = _inputs((2, 3, 64), torch.float32)
+    call = lambda x: fma.fused_sandwich_rmsnorm(x, t["residual"], None, None, _EPS)[0]  # noqa: E731
+    with torch.no_grad(), pytest.raises(RuntimeError):
+        with torch.autograd.forward_ad.dual_level():
+            call(torch.autograd.forward_ad.make_dual(t["x"], torch.ones_like(t["x"])))
+    with torch.no_grad(), pytest.raises(RuntimeError):
+        torch.func.grad(lambda x: call(x).sum())(t["x"])
 
 
 def test_long_tensors():
