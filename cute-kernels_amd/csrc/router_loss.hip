@@ -18,14 +18,10 @@ namespace {
 // threads of a workgroup of the forward pass: half of them where each holds 16 logits and would not have the registers
 constexpr int fwd_threads(int values) { return values > 8 ? 512 : 1024; }
 constexpr int kBwdThreads = 256;
-// Choices up to which their threshold is found from the largest logit down (see count_largest). Both kernels of the forward pass, us from
-// the top / by bisection: 131072 tokens of 256 experts in fp32, 2, 4 and 8 choices 51 / 83, 65 / 89, 93 / 89, in bf16 6 choices 79 / 86; 16384 of
-// 1024, 8 choices 73 / 65; 200000 of 32 (bf16), 4 and 8 choices 21 / 26, 26 / 30; 65536 of 64, 8 choices 19.0 / 19.2; 262144 of 8, 3 choices 16 / 19.
-constexpr uint32_t few_choices(int lanes) { return lanes <= 8 ? 8 : 6; }
 
 template <int CTRL>
 __device__ __forceinline__ uint32_t dpp(uint32_t v) {
-    return (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, CTRL, 0xf, 0xf, false);
+    return (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, CTRL, 0xf, 0xf, true);
 }
 struct Max {
     static __device__ __forceinline__ float of(float a, float b) { return fmaxf(a, b); }
@@ -175,58 +171,94 @@ __device__ __forceinline__ uint32_t key_of(float x) {
     return key >> Keys<T>::kDrop;
 }
 
-// Adds one to count[i] of the token's k largest logits. Their threshold, the largest that k logits reach, is found from the largest logit down,
-// one value after the other, where k is small, and otherwise by bisection of the keys between the smallest of the lanes' largest (where k lanes
-// have logits) and the largest, which ends where exactly k reach the middle. Only where equal logits are left on both sides of the line are
-// places among them counted.
-template <typename T, int L, int NV, bool NANS>
-__device__ __forceinline__ void count_largest(const Logits<T, NV>& x, int in, bool enough_lanes, uint32_t k, bool counted, uint32_t (&count)[NV]) {
-    uint32_t key[NV], most = 0;
+// The k-th largest of a token's keys, k <= P: every lane sorts groups of P of its own downwards by comparators and keeps the P largest of two groups at
+// a time, max(a_i, b_(P-1-i)), which one more pass of comparators sorts; lanes then do the same with each other's. No step depends on the values,
+// and log2(L) of them go from lane to lane. For 8 of 256 that is 15 operations a logit, where a bisection takes 2 for each of its 20 to 25 steps (both
+// kernels of the forward pass, us against bisection: 131072 tokens of 256 experts, 8 choices, fp32 57 / 79, bf16 59 / 79; 16384 of 1024, fp32 60 / 69;
+// 65536 of 64, 6 choices, 15 / 17; 200000 of 32, 8 choices, 19 / 26). For 16 choices it was no faster (79 / 76).
+__device__ __forceinline__ void order(uint32_t& larger, uint32_t& smaller) {
+    const uint32_t a = larger, b = smaller;
+    larger = Max::of(a, b);
+    smaller = Min::of(a, b);
+}
+template <int P, int L, int NV>
+__device__ __forceinline__ uint32_t kth_largest(const uint32_t (&key)[NV], uint32_t k) {
+    uint32_t v[NV];
 #pragma unroll
-    for (int i = 0; i < NV; ++i) {
-        key[i] = key_of<T, NANS>(x.up(i));
-        most = Max::of(most, key[i]);
-    }
-    auto reach = [&](uint32_t line) {
-        uint32_t n = 0;
+    for (int i = 0; i < NV; ++i) v[i] = key[i];
+    // two sorted runs of n to one of 2 n, by Batcher's odd-even merge
 #pragma unroll
-        for (int i = 0; i < NV; ++i) n += key[i] >= line ? 1u : 0u;
-        return over_token<L, Sum>(n);
+    for (int n = 1; n < P; n *= 2)
+#pragma unroll
+        for (int run = 0; run < NV; run += 2 * n) {
+#pragma unroll
+            for (int i = 0; i < n; ++i) order(v[run + i], v[run + n + i]);
+#pragma unroll
+            for (int q = n / 2; q > 0; q /= 2)
+#pragma unroll
+                for (int j = q; j < 2 * n - q; j += 2 * q)
+#pragma unroll
+                    for (int i = 0; i < q; ++i) order(v[run + j + i], v[run + j + q + i]);
+        }
+    // P values that rise to their largest and fall again, or the other way round
+    auto settle = [&](int at) {
+#pragma unroll
+        for (int d = P / 2; d > 0; d /= 2)
+#pragma unroll
+            for (int i = 0; i < P; ++i)
+                if (!(i & d)) order(v[at + i], v[at + i + d]);
     };
-    uint32_t low, high = over_token<L, Max>(most);
-    bool exact = !counted;
-    if (k <= few_choices(L)) {
-        low = high;
-        uint32_t n = reach(low);
-        while (__any(!exact && n < k)) {
-            uint32_t below = 0;
 #pragma unroll
-            for (int i = 0; i < NV; ++i) below = Max::of(below, key[i] < low ? key[i] : 0u);
-            below = over_token<L, Max>(below);
-            if (n < k) {
-                low = below;
-                n = reach(below);
-            }
-        }
-        exact = exact || n == k;
-    } else {
-        uint32_t least = most;
-        if (!enough_lanes) {
+    for (int n = P; n < NV; n *= 2)
 #pragma unroll
-            for (int i = 0; i < NV; ++i) least = Min::of(least, key[i]);
+        for (int at = 0; at < NV; at += 2 * n) {
+#pragma unroll
+            for (int i = 0; i < P; ++i) v[at + i] = Max::of(v[at + i], v[at + n + P - 1 - i]);
+            settle(at);
         }
-        low = over_token<L, Min>(in > 0 ? least : 0xffffffffu);
-        while (__any(!exact && low < high)) {
-            const uint32_t mid = low + (high - low + 1) / 2, n = reach(mid);
-            if (!exact && low < high) {
-                if (n >= k) low = mid;
-                else high = mid - 1;
-                exact = n == k;
-            }
-        }
-    }
+    auto join = [&](auto other) {
+        uint32_t w[P];
+#pragma unroll
+        for (int i = 0; i < P; ++i) w[i] = other(v[i], v[P - 1 - i]);
+#pragma unroll
+        for (int i = 0; i < P; ++i) v[i] = w[i];
+        settle(0);
+    };
+    if constexpr (L >= 2) join([&](uint32_t a, uint32_t b) { return Max::of(a, dpp<0xb1>(b)); });
+    if constexpr (L >= 4) join([&](uint32_t a, uint32_t b) { return Max::of(a, dpp<0x4e>(b)); });
+    if constexpr (L >= 8) join([&](uint32_t a, uint32_t b) { return Max::of(a, dpp<0x141>(b)); });
+    if constexpr (L >= 16) join([&](uint32_t a, uint32_t b) { return Max::of(a, dpp<0x140>(b)); });
+    if constexpr (L >= 32)
+        join([&](uint32_t a, uint32_t b) {
+            const auto p = __builtin_amdgcn_permlane16_swap(a, a, false, false), q = __builtin_amdgcn_permlane16_swap(b, b, false, false);
+            return Max::of((uint32_t)p[0], (uint32_t)q[1]);
+        });
+    if constexpr (L >= 64)
+        join([&](uint32_t a, uint32_t b) {
+            const auto p = __builtin_amdgcn_permlane32_swap(a, a, false, false), q = __builtin_amdgcn_permlane32_swap(b, b, false, false);
+            return Max::of((uint32_t)p[0], (uint32_t)q[1]);
+        });
+    uint32_t line = v[0];
+#pragma unroll
+    for (int i = 1; i < P; ++i) line = (uint32_t)i < k ? v[i] : line;
+    return line;
+}
+
+// how many of a token's logits reach `line`
+template <int L, int NV>
+__device__ __forceinline__ uint32_t reach(const uint32_t (&key)[NV], uint32_t line) {
+    uint32_t n = 0;
+#pragma unroll
+    for (int i = 0; i < NV; ++i) n += key[i] >= line ? 1u : 0u;
+    return over_token<L, Sum>(n);
+}
+
+// Adds one to count[i] of the token's k largest logits, where `low` is the k-th largest, or (`exact`) exactly k reach it. Only where equal logits are
+// left on both sides of the line are places among them counted.
+template <int L, int NV>
+__device__ __forceinline__ void count_from(const uint32_t (&key)[NV], uint32_t low, uint32_t k, bool exact, bool counted, uint32_t (&count)[NV]) {
     if (!__any(!exact)) {
-        const uint32_t line = counted ? low : 0xffffffffu;  // (no logit of such a token, which are all zeros then, reaches it)
+        const uint32_t line = counted ? low : 0xffffffffu;
 #pragma unroll
         for (int i = 0; i < NV; ++i) count[i] += key[i] >= line ? 1u : 0u;
         return;
@@ -254,6 +286,55 @@ __device__ __forceinline__ void count_largest(const Logits<T, NV>& x, int in, bo
         left -= take;
         count[i] += counted ? (above >> i & 1u) | take : 0u;
     }
+}
+
+// by the k-th largest logit itself, k <= P; no logit is a NaN
+template <int P, typename T, int L, int NV>
+__device__ __forceinline__ void count_sorted(const Logits<T, NV>& x, uint32_t k, bool counted, uint32_t (&count)[NV]) {
+    uint32_t key[NV];
+#pragma unroll
+    for (int i = 0; i < NV; ++i) key[i] = key_of<T, false>(x.up(i));
+    const uint32_t line = kth_largest<P, L, NV>(key, k);
+    const bool exact = !counted || reach<L, NV>(key, line) == k;
+    count_from<L, NV>(key, line, k, exact, counted, count);
+}
+
+// By bisection of the keys between the smallest of the lanes' largest (where k lanes have logits) and the largest, which ends where exactly k reach
+// the middle.
+template <typename T, int L, int NV, bool NANS>
+__device__ __forceinline__ void count_bisected(const Logits<T, NV>& x, int in, bool enough_lanes, uint32_t k, bool counted, uint32_t (&count)[NV]) {
+    uint32_t key[NV], most = 0;
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+        key[i] = key_of<T, NANS>(x.up(i));
+        most = Max::of(most, key[i]);
+    }
+    uint32_t least = most;
+    if (!enough_lanes) {
+#pragma unroll
+        for (int i = 0; i < NV; ++i) least = Min::of(least, key[i]);
+    }
+    uint32_t low = over_token<L, Min>(in > 0 ? least : 0xffffffffu), high = over_token<L, Max>(most);
+    bool exact = !counted;
+    while (__any(!exact && low < high)) {
+        const uint32_t mid = low + (high - low + 1) / 2, n = reach<L, NV>(key, mid);
+        if (!exact && low < high) {
+            if (n >= k) low = mid;
+            else high = mid - 1;
+            exact = n == k;
+        }
+    }
+    count_from<L, NV>(key, low, k, exact, counted, count);
+}
+
+template <typename T, int L, int NV>
+__device__ __forceinline__ void count_largest(const Logits<T, NV>& x, int in, bool enough_lanes, uint32_t k, bool nans, bool counted,
+                                              uint32_t (&count)[NV]) {
+    if (nans) count_bisected<T, L, NV, true>(x, in, enough_lanes, k, counted, count);
+    else if (k <= 2) count_sorted<2, T, L, NV>(x, k, counted, count);
+    else if (k <= 4) count_sorted<4, T, L, NV>(x, k, counted, count);
+    else if (k <= 8) count_sorted<8, T, L, NV>(x, k, counted, count);
+    else count_bisected<T, L, NV, false>(x, in, enough_lanes, k, counted, count);
 }
 
 struct Partial {
@@ -309,8 +390,7 @@ __global__ __launch_bounds__(fwd_threads(NV)) void router_loss_kernel(const T* _
         for (int i = 0; i < NV; ++i) psum[i] += e[i] * inv;
         zsum = __builtin_fma((double)lse, (double)lse, zsum);
         n += counted ? 1u : 0u;
-        if (__any(lse != lse)) count_largest<T, L, NV, true>(x, in, enough_lanes, k, counted, count);
-        else count_largest<T, L, NV, false>(x, in, enough_lanes, k, counted, count);
+        count_largest<T, L, NV>(x, in, enough_lanes, k, __any(lse != lse), counted, count);
         x = next;
         use = next_use;
     }
@@ -506,10 +586,10 @@ __global__ __launch_bounds__(kBwdThreads) void router_loss_bwd_kernel(const T* _
 
 int64_t compute_units() { return num_compute_units() > 0 ? num_compute_units() : 256; }
 
-// Logits per lane: 16 where eight would take more than a wavefront, and in the forward pass from 32 lanes on, whose sums and maxima then need
-// no step across rows of 16 lanes (131072 tokens of 256 experts, 8 choices, fp32: forward 79 us against 88, backward 76 against 57; of 128 and fewer
-// experts it is no faster: 48 against 45).
-int values_per_lane(int64_t E, bool forward) { return E > (forward ? 128 : 512) ? 16 : 8; }
+// Logits per lane: 16 where eight would take more than a wavefront, and in the forward pass from 33 on, whose sorting and sums then need one step
+// less between lanes (8 choices, both kernels of the forward pass, us against eight a lane: 131072 tokens of 256 experts, fp32 57 / 69; of 128, bf16
+// 33 / 35; of 64, fp32 20 / 21. The backward pass of the first: 76 / 57).
+int values_per_lane(int64_t E, bool forward) { return E > (forward ? 32 : 512) ? 16 : 8; }
 int lanes_per_token(int64_t E, bool forward) {
     int L = 1;
     while ((int64_t)L * values_per_lane(E, forward) < E) L <<= 1;
@@ -534,6 +614,8 @@ void with_shape(int64_t E, bool vec, F launch) {
     const int L = lanes_per_token(E, FORWARD);
     if (values_per_lane(E, FORWARD) == 16) {
         if constexpr (FORWARD) {
+            if (L == 4) return as(Int<4>(), Int<16>());
+            if (L == 8) return as(Int<8>(), Int<16>());
             if (L == 16) return as(Int<16>(), Int<16>());
             if (L == 32) return as(Int<32>(), Int<16>());
         }
@@ -541,13 +623,13 @@ void with_shape(int64_t E, bool vec, F launch) {
     }
     if (L == 1) return as(Int<1>(), Int<8>());
     if (L == 2) return as(Int<2>(), Int<8>());
-    if (L == 4) return as(Int<4>(), Int<8>());
-    if (L == 8) return as(Int<8>(), Int<8>());
     if constexpr (!FORWARD) {
+        if (L == 8) return as(Int<8>(), Int<8>());
+        if (L == 16) return as(Int<16>(), Int<8>());
         if (L == 32) return as(Int<32>(), Int<8>());
         if (L == 64) return as(Int<64>(), Int<8>());
     }
-    return as(Int<16>(), Int<8>());
+    return as(Int<4>(), Int<8>());
 }
 
 template <typename T>
