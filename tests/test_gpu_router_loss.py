@@ -341,3 +341,33 @@ def test_losses_of_the_layers_logits(dtype):
         assert torch.equal(torch.bincount(selected[mask].reshape(-1), minlength=16), counts.view(torch.int32).long())
     (y.float().square().mean() + 0.01 * balance + 0.001 * z).backward()
     assert moe.gate.weight.grad.abs().max() > 0 and torch.isfinite(moe.gate.weight.grad).all() and torch.isfinite(x.grad).all()
+
+
+@pytest.mark.parametrize("dtype", _DTYPES)
+@pytest.mark.parametrize("E", [5, 8, 11, 32, 33, 64, 100, 160, 256, 300, 512, 700, 1024])
+def test_every_small_number_of_choices(E, dtype):
+    """1 to 17 choices: those around every power of two, of different logits, of few values, and of rows with as good as nothing but -infinity"""
+    distinct = torch.stack([torch.randperm(E, generator=torch.Generator().manual_seed(i)) for i in range(65)]).to(DEV)
+    distinct = ((distinct - E // 2).float() / 64).to(_DTYPES[dtype])  # (exact in every type up to 1024 experts: eleven bits, or rounded to equal ones)
+    few = _logits(65, E, torch.float32).round().to(_DTYPES[dtype])
+    rare = distinct.clone()
+    rare[:, 3:] = -float("inf")
+    for k in range(1, min(E, 17) + 1):
+        for logits in (distinct, few):
+            _check(logits, k)
+        counts = fma.router_loss(rare, k)[2].view(torch.int32).long()
+        chosen = torch.sort(rare.double(), dim=1, descending=True, stable=True).indices[:, :k]
+        assert torch.equal(counts, torch.bincount(chosen.reshape(-1), minlength=E))
+
+
+@pytest.mark.parametrize("dtype", _DTYPES)
+@pytest.mark.parametrize("E", [8, 60, 256, 1024])
+def test_choices_beside_a_nan(E, dtype):
+    """a wavefront with one token that holds a NaN: the NaN comes first, and the other tokens choose as they do without it"""
+    logits = _logits(200, E, _DTYPES[dtype])
+    logits[77, E - 1] = float("nan")
+    for k in (1, 2, 3, 8):
+        order = logits.double()
+        order[77, E - 1] = 1e9
+        chosen = torch.sort(order, dim=1, descending=True, stable=True).indices[:, :k]
+        assert torch.equal(fma.router_loss(logits, k)[2].view(torch.int32).long(), torch.bincount(chosen.reshape(-1), minlength=E))
