@@ -62,7 +62,8 @@ def clip_grad_norm_(
     parameters: torch.Tensor | Iterable[torch.Tensor], max_norm: float, norm_type: float = 2.0, error_if_nonfinite: bool = False
 ) -> torch.Tensor:
     """Clips the gradients of the parameters to max_norm in place and returns their norm from before: get_total_norm and
-    clip_grads_with_norm_ as one call. Parameters without a gradient are passed over; gradients that share memory are refused (RuntimeError).
+    clip_grads_with_norm_ as one call. Parameters without a gradient are passed over. Gradients that share memory are refused (RuntimeError)
+    if they are dense or one strided view; different views that overlap are scaled once, and count twice in the norm.
     With error_if_nonfinite an infinite or NaN norm raises RuntimeError before anything is scaled. Not traced: a compiled function that calls
     it breaks its graph here."""
     infinity, max_norm = _is_infinity_norm(norm_type), _check_bound(max_norm)

@@ -31,7 +31,7 @@ class _Table:
         if len({t.get_device() for t in tensors}) > 1:
             raise RuntimeError("all tensors should be on one device: got " + ", ".join(sorted({str(t.device) for t in tensors})))
         _lib.require_gpu(tensors[0])
-        self.copied = []
+        self.copied, self.views = [], set()
         if not all([t.is_contiguous() for t in tensors]):
             tensors = [self._dense(t, written) for t in tensors]
         self.tensors = tensors  # (holds the copies)
@@ -49,6 +49,11 @@ class _Table:
             return t
         if written and torch._debug_has_internal_overlap(t) == 1:
             raise RuntimeError("a gradient has elements that share memory: make it contiguous first")
+        if written:
+            view = t.data_ptr(), t.shape, t.stride()
+            if view in self.views:
+                raise RuntimeError("two gradients share memory")
+            self.views.add(view)
         copy = t.contiguous()
         self.copied.append((t, copy))
         return copy

@@ -278,3 +278,18 @@ def test_long_tensors():
         assert bool(((got - exact).abs() <= exact * 2.0**-8 * 1.001).all())
     assert int(torch.count_nonzero(g)) == 6
     _check_norm(fma.get_total_norm([g], math.inf), float(g[n - 1].double()))
+
+
+def test_strided_gradients_that_share_memory():
+    """one view twice is refused; views that lie between each other are clipped as ever"""
+    base = torch.randn(40, 30, device=DEV)
+    same = _parameters([base[:, ::2], base[:, ::2]])
+    before = base.clone()
+    with pytest.raises(RuntimeError, match="share memory"):
+        fma.clip_grad_norm_(same, 1e-3)
+    with pytest.raises(RuntimeError, match="share memory"):
+        fma.clip_grads_with_norm_(same, 1e-3, torch.tensor(1.0, device=DEV))
+    assert torch.equal(base, before)
+    norm = fma.clip_grad_norm_(_parameters([base[:, ::2], base[:, 1::2]]), 1e-3)
+    _check_norm(norm, float(before.double().norm()))
+    _check_scaled([base], [before], float(before.double().norm()), 1e-3)
