@@ -174,7 +174,7 @@ __device__ __forceinline__ uint32_t key_of(float x) {
 // The k-th largest of a token's keys, k <= P: every lane sorts groups of P of its own downwards by comparators and keeps the P largest of two groups at
 // a time, max(a_i, b_(P-1-i)), which one more pass of comparators sorts; lanes then do the same with each other's. No step depends on the values,
 // and log2(L) of them go from lane to lane. For 8 of 256 that is 15 operations a logit, where a bisection takes 2 for each of its 20 to 25 steps (both
-// kernels of the forward pass, us against bisection: 131072 tokens of 256 experts, 8 choices, fp32 57 / 79, bf16 59 / 79; 16384 of 1024, fp32 60 / 69;
+// kernels of the forward pass, us against bisection: 131072 tokens of 256 experts, 8 choices, fp32 55 / 77, bf16 57 / 77; 16384 of 1024, fp32 60 / 69;
 // 65536 of 64, 6 choices, 15 / 17; 200000 of 32, 8 choices, 19 / 26). For 16 choices it was no faster (79 / 76).
 __device__ __forceinline__ void order(uint32_t& larger, uint32_t& smaller) {
     const uint32_t a = larger, b = smaller;
@@ -342,6 +342,7 @@ struct Partial {
     uint32_t* c;   // [G, E]
     double* z;     // [G]
     uint32_t* n;   // [G]
+    double* term;  // what each workgroup of the join contributes to the balance
 };
 
 template <typename T, int L, int NV, bool VEC>
@@ -444,7 +445,8 @@ __global__ __launch_bounds__(fwd_threads(NV)) void router_loss_kernel(const T* _
     }
 }
 
-// table: E f_e of every expert, then 1 / N, for the backward pass
+// A workgroup joins the columns of `cols` experts (a power of two). One that has them all also forms the losses; of several each leaves its part of
+// the balance to router_loss_finish_kernel. table: E f_e of every expert, then 1 / N, for the backward pass.
 constexpr int kJoinThreads = 1024, kJoinWaves = kJoinThreads / kWave;
 struct Total {
     double a, b;
@@ -470,17 +472,14 @@ __device__ __forceinline__ Total join_total(double a, double b, double (*slots)[
     return t;
 }
 
-__global__ __launch_bounds__(kJoinThreads) void router_loss_join_kernel(Partial part, int G, int E, uint32_t k, float* __restrict__ balance,
+__global__ __launch_bounds__(kJoinThreads) void router_loss_join_kernel(Partial part, int G, int E, int cols, uint32_t k, float* __restrict__ balance,
                                                                         float* __restrict__ z, uint32_t* __restrict__ counts,
                                                                         float* __restrict__ table) {
     __shared__ double s_sum[kJoinThreads];
     __shared__ uint32_t s_count[kJoinThreads];
     __shared__ double s_total[2][kJoinWaves][2];
-    const int tid = threadIdx.x;
-    // a power of two of columns, the other threads share the rows; eight rows of a thread on the way at a time
-    int cols = 1;
-    while (cols < E) cols <<= 1;
-    const int rows = kJoinThreads / cols, col = tid & (cols - 1), row = tid / cols;
+    // the threads of a column share its rows; eight rows of a thread on the way at a time
+    const int tid = threadIdx.x, rows = kJoinThreads / cols, col = blockIdx.x * cols + (tid & (cols - 1)), row = tid / cols;
     double p = 0.0;
     uint32_t c = 0;
     if (col < E)
@@ -511,22 +510,43 @@ __global__ __launch_bounds__(kJoinThreads) void router_loss_join_kernel(Partial 
     s_count[tid] = c;
     __syncthreads();
     double term = 0.0;
-    if (tid < cols && tid < E) {
+    if (tid < cols && col < E) {
         for (int r = 1; r < rows; ++r) {
             p += s_sum[tid + r * cols];
             c += s_count[tid + r * cols];
         }
         const double f = (double)c * inv_n / (double)k;
         term = f * p;
-        counts[tid] = c;
-        table[tid] = (float)((double)E * f);
+        counts[col] = c;
+        table[col] = (float)((double)E * f);
     }
     const Total loss = join_total(term, 0.0, s_total[1]);
-    if (tid == 0) {
-        *balance = (float)((double)E * inv_n * loss.a);
-        *z = (float)(all.a * inv_n);
-        table[E] = (float)inv_n;
+    if (tid != 0) return;
+    part.term[blockIdx.x] = (double)E * inv_n * loss.a;
+    if (gridDim.x > 1) return;
+    *balance = (float)part.term[0];
+    *z = (float)(all.a * inv_n);
+    table[E] = (float)inv_n;
+}
+
+__global__ __launch_bounds__(kWave) void router_loss_finish_kernel(Partial part, int G, int E, int joins, float* __restrict__ balance,
+                                                                   float* __restrict__ z, float* __restrict__ table) {
+    double loss = (int)threadIdx.x < joins ? part.term[threadIdx.x] : 0.0, zsum = 0.0, tokens = 0.0;
+    for (int g = threadIdx.x; g < G; g += kWave) {
+        zsum += part.z[g];
+        tokens += (double)part.n[g];
     }
+#pragma unroll
+    for (int d = 1; d < kWave; d <<= 1) {
+        loss += __shfl_xor(loss, d, kWave);
+        zsum += __shfl_xor(zsum, d, kWave);
+        tokens += __shfl_xor(tokens, d, kWave);
+    }
+    if (threadIdx.x != 0) return;
+    const double inv_n = tokens > 0.0 ? 1.0 / tokens : 0.0;
+    *balance = (float)loss;
+    *z = (float)(zsum * inv_n);
+    table[E] = (float)inv_n;
 }
 
 template <typename T, int L, int NV, bool VEC>
@@ -637,10 +657,22 @@ bool whole_vectors(const void* p, const void* q, int64_t E) {
     return aligned16(p) && aligned16(q) && E * (int64_t)sizeof(T) % 16 == 0;
 }
 
+// Columns that a workgroup joins: all, or 16 (64 bytes of each row) where a single one would have more than a compute unit's loads bring in some
+// microseconds, against one launch more (all of the forward pass, us one / several: 1024 experts, 256 rows 60 / 39.5, 128 rows 24.9 / 15.8; 512, 256 rows
+// 34 / 26; 256, 256 rows 55.2 / 54.5; 128, 256 rows 16.9 / 19.1; 256, 64 rows 11.9 / 15.6).
+constexpr int kJoinColumns = 16, kMostJoins = FMA_MAX_GROUPS / kJoinColumns;
+static_assert(kMostJoins <= kWave, "router_loss_finish_kernel has a lane for each");
+int join_columns(int64_t G, int64_t E) {
+    int cols = 1;
+    while (cols < E) cols <<= 1;
+    return cols > kJoinColumns && G * cols > 64 * kJoinThreads ? kJoinColumns : cols;
+}
+
 Partial partial_of(void* workspace, int64_t G, int64_t E) {
     Partial part;
     part.z = (double*)workspace;
-    part.p = (float*)(part.z + G);
+    part.term = part.z + G;
+    part.p = (float*)(part.term + kMostJoins);
     part.c = (uint32_t*)(part.p + G * E);
     part.n = part.c + G * E;
     return part;
@@ -657,7 +689,10 @@ int launch_fwd(const void* logits, const uint8_t* mask, int64_t T_, int64_t E, i
     });
     const int rc = launch_status("router_loss");
     if (rc) return rc;
-    hipLaunchKernelGGL(router_loss_join_kernel, dim3(1), dim3(kJoinThreads), 0, st, part, (int)G, (int)E, (uint32_t)k, balance, z, counts, table);
+    const int cols = join_columns(G, E), joins = ((int)E + cols - 1) / cols;
+    hipLaunchKernelGGL(router_loss_join_kernel, dim3((uint32_t)joins), dim3(kJoinThreads), 0, st, part, (int)G, (int)E, cols, (uint32_t)k, balance, z,
+                       counts, table);
+    if (joins > 1) hipLaunchKernelGGL(router_loss_finish_kernel, dim3(1), dim3(kWave), 0, st, part, (int)G, (int)E, joins, balance, z, table);
     return launch_status("router_loss (join)");
 }
 
@@ -688,7 +723,7 @@ extern "C" {
 
 int64_t fma_router_loss_workspace_bytes(int64_t T, int64_t E) {
     if (T < 0 || E < 1 || E > FMA_MAX_GROUPS) return 0;
-    return fmahip::forward_workgroups(T, E) * (8 + 4 + 8 * E);
+    return fmahip::forward_workgroups(T, E) * (8 + 4 + 8 * E) + 8 * fmahip::kMostJoins;
 }
 
 int fma_router_loss(const void* logits, const uint8_t* mask, int64_t T, int64_t E, int64_t top_k, float* balance, float* z, uint32_t* counts,
