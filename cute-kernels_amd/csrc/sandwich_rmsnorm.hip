@@ -4,7 +4,7 @@
 //   r   = residual + a gate n       (stored rounded; a: the residual scale)
 //   out = r inv_r w                 inv_r = 1 / sqrt(mean(r^2) + eps), from the unrounded r
 //
-// with x^ = x inv_x, r^ = r inv_r (from the stored r), g = dout w:
+// with x^ = x inv_x, r^ = r inv_r, g = dout w:
 //
 //   dr = dr_in + inv_r (g - r^ mean(g r^))                      dresidual = dr
 //   dgate = a dr w_post x^, summed over the rows that share it  u = a dr gate w_post
@@ -132,7 +132,7 @@ struct FwdArgs {
 
 template <typename T>
 struct BwdArgs {
-    const T *x, *stream, *post_weight, *weight, *gate, *d_out, *d_stream;
+    const T *x, *residual, *post_weight, *weight, *gate, *d_out, *d_stream;
     const float* stats;
     T *dx, *d_residual, *d_gate;
     Partial part;
@@ -210,14 +210,18 @@ __global__ __launch_bounds__(kThreads) void sandwich_bwd_generic_kernel(const Bw
             const bool scalar = k.s.mode == kScalar;
             const T* const gate = k.gate ? k.gate + gate_row(k.s, row) * (scalar ? 1 : H) : nullptr;
             const float inv_x = k.stats[row], inv_r = k.stats[k.s.B + row];
+            auto normed = [&](int64_t h) {  // r^
+                const float n = Num<T>::up(k.x[base + h]) * inv_x * at(k.post_weight, h);
+                return (Num<T>::up(k.residual[base + h]) + k.a * (n * at(gate, scalar ? 0 : h))) * inv_r;
+            };
             float dot = 0.f;
             if (k.d_out)
                 for (int64_t h = threadIdx.x; h < H; h += kThreads)
-                    dot += Num<T>::up(k.d_out[base + h]) * at(k.weight, h) * Num<T>::up(k.stream[base + h]);
-            const float c_r = workgroup_sum(dot, s_red, parity) * inv_r * k.inv_H;
+                    dot += Num<T>::up(k.d_out[base + h]) * at(k.weight, h) * normed(h);
+            const float c_r = workgroup_sum(dot, s_red, parity) * k.inv_H;
             auto d_stream = [&](int64_t h) {
                 float d = k.d_stream ? Num<T>::up(k.d_stream[base + h]) : 0.f;
-                if (k.d_out) d += inv_r * (Num<T>::up(k.d_out[base + h]) * at(k.weight, h) - Num<T>::up(k.stream[base + h]) * inv_r * c_r);
+                if (k.d_out) d += inv_r * (Num<T>::up(k.d_out[base + h]) * at(k.weight, h) - normed(h) * c_r);
                 return d;
             };
             dot = 0.f;
@@ -241,7 +245,7 @@ __global__ __launch_bounds__(kThreads) void sandwich_bwd_generic_kernel(const Bw
                 k.d_residual[base + h] = Num<T>::down(dr);
                 k.dx[base + h] = Num<T>::down(inv_x * (dz * g * p - x * c_x));
                 if (k.s.mode == kFull && k.d_gate) k.d_gate[base + h] = Num<T>::down(dz * p * x);
-                if (w) w[h] += k.d_out ? Num<T>::up(k.d_out[base + h]) * (Num<T>::up(k.stream[base + h]) * inv_r) : 0.f;
+                if (w) w[h] += k.d_out ? Num<T>::up(k.d_out[base + h]) * normed(h) : 0.f;
                 if (wp) wp[h] += k.s.mode == kChannel ? dz * x : dz * g * x;
                 if (sg) sg[h] += dz * x;
             }
@@ -483,6 +487,7 @@ template <typename T, bool ELEM, int TEAM, int VPT, Mode MODE>
 __global__ __launch_bounds__(TEAM * teams_of(TEAM)) void sandwich_bwd_kernel(const BwdArgs<T> k) {
     constexpr int N = Wide<T>::N, kTeams = teams_of(TEAM);
     constexpr bool kAhead = TEAM * VPT <= 1024;  // (two vectors for each of 1024 threads leave no registers for a second row)
+    constexpr bool kKeep = kAhead;  // (nor for what is formed on the way, which they form again)
     constexpr bool kVector = MODE == kFull || MODE == kGroup || MODE == kChannel;
     __shared__ float s_red[2][TEAM / kWave];
     int parity = 0;
@@ -507,7 +512,7 @@ __global__ __launch_bounds__(TEAM * teams_of(TEAM)) void sandwich_bwd_kernel(con
         const int64_t base = row * H;
         const uint32_t n = in ? bytes : 0u, one = in ? 4u : 0u;
         load_row<ELEM, TEAM, VPT, kStream>(to.x, buffer_of(k.x + base, n), tid);
-        load_row<ELEM, TEAM, VPT, kStream>(to.r, buffer_of(k.stream + base, n), tid);
+        load_row<ELEM, TEAM, VPT, kStream>(to.r, buffer_of(k.residual + base, n), tid);
         load_row<ELEM, TEAM, VPT, kStream>(to.dy, buffer_of(k.d_out ? k.d_out + base : nullptr, n), tid);
         load_row<ELEM, TEAM, VPT, kStream>(to.dr, buffer_of(k.d_stream ? k.d_stream + base : nullptr, n), tid);
         if constexpr (MODE == kFull) load_row<ELEM, TEAM, VPT, kStream>(to.gate, buffer_of(k.gate + base, n), tid);
@@ -532,31 +537,51 @@ __global__ __launch_bounds__(TEAM * teams_of(TEAM)) void sandwich_bwd_kernel(con
         if constexpr (kAhead) fetch(next, next_group * k.p.rows + next_place, more);
         else fetch(now, row, true);
 
-        float dot = 0.f;
-#pragma unroll
-        for (int i = 0; i < VPT; ++i)
-#pragma unroll
-            for (int e = 0; e < N; ++e) dot += Wide<T>::up(now.dy[i], e) * Wide<T>::up(w[i], e) * Wide<T>::up(now.r[i], e);
-        const float c_r = team_sum<TEAM>(dot, s_red, parity) * now.inv_r * k.inv_H;
-        auto d_stream = [&](int i, int e, float dy, float rh) {
-            return Wide<T>::up(now.dr[i], e) + now.inv_r * (dy * Wide<T>::up(w[i], e) - rh * c_r);
-        };
         auto gate = [&](int i, int e) {
             if constexpr (MODE == kChannel) return Wide<T>::up(channel[i], e);
             else return Wide<T>::up(now.gate[i], e);
         };
-        auto stay = [&] {
+        const float a = MODE == kScalar ? k.a * now.scalar : k.a;
+        // r^, from the stream as it was before its rounding
+        const float x_share = a * now.inv_x * now.inv_r;
+        auto form = [&](int i, int e) {
+            float n = Wide<T>::up(now.x[i], e) * Wide<T>::up(wp[i], e);
+            if constexpr (kVector) n *= gate(i, e);
+            return Wide<T>::up(now.r[i], e) * now.inv_r + n * x_share;
+        };
+        float kept[VPT][N];  // a number per element over the barriers: first r^, then dr
+        if constexpr (kKeep) {
+#pragma unroll
+            for (int i = 0; i < VPT; ++i)
+#pragma unroll
+                for (int e = 0; e < N; ++e) kept[i][e] = form(i, e);
+        }
+        auto normed = [&](int i, int e) {
+            if constexpr (kKeep) return kept[i][e];
+            else return form(i, e);
+        };
+        float dot = 0.f;
+#pragma unroll
+        for (int i = 0; i < VPT; ++i)
+#pragma unroll
+            for (int e = 0; e < N; ++e) dot += Wide<T>::up(now.dy[i], e) * Wide<T>::up(w[i], e) * normed(i, e);
+        const float c_r = team_sum<TEAM>(dot, s_red, parity) * k.inv_H;
+        auto d_stream = [&](int i, int e, float dy, float rh) {
+            return Wide<T>::up(now.dr[i], e) + now.inv_r * (dy * Wide<T>::up(w[i], e) - rh * c_r);
+        };
+        auto stay = [&](bool formed) {
             stay_packed(now.x);
-            stay_packed(now.r);
-            stay_packed(now.dy);
-            stay_packed(now.dr);
-            stay_packed(w);
+            if constexpr (!kKeep) stay_packed(now.r);
+            if (!kKeep || !formed) {
+                stay_packed(now.dy);
+                stay_packed(now.dr);
+                stay_packed(w);
+            }
             stay_packed(wp);
             if constexpr (MODE == kChannel) stay_packed(channel);
             else if constexpr (kVector) stay_packed(now.gate);
         };
-        stay();
-        const float a = MODE == kScalar ? k.a * now.scalar : k.a;
+        stay(false);
         const __amdgpu_buffer_rsrc_t to_residual = buffer_of(k.d_residual + base, bytes), to_x = buffer_of(k.dx + base, bytes);
         dot = 0.f;
 #pragma unroll
@@ -564,12 +589,13 @@ __global__ __launch_bounds__(TEAM * teams_of(TEAM)) void sandwich_bwd_kernel(con
             float o[N];
 #pragma unroll
             for (int e = 0; e < N; ++e) {
-                const float dy = Wide<T>::up(now.dy[i], e), rh = Wide<T>::up(now.r[i], e) * now.inv_r, dr = d_stream(i, e, dy, rh);
+                const float dy = Wide<T>::up(now.dy[i], e), rh = normed(i, e), dr = d_stream(i, e, dy, rh);
                 sw[i][e] += dy * rh;
                 float u = dr * Wide<T>::up(wp[i], e);
                 if constexpr (kVector) u *= gate(i, e);
                 dot += u * Wide<T>::up(now.x[i], e);
                 o[e] = dr;
+                if constexpr (kKeep) kept[i][e] = dr;
             }
             store_row<ELEM, T>(to_residual, tid + i * TEAM, o);
         }
@@ -580,15 +606,16 @@ __global__ __launch_bounds__(TEAM * teams_of(TEAM)) void sandwich_bwd_kernel(con
             store_float(buffer_of(own || !k.d_gate ? nullptr : k.part.rows + row, 4), first_lane, k.a * dot);
         }
         const float c_x = a * dot * k.inv_H;
-        stay();
+        stay(true);
 #pragma unroll
         for (int i = 0; i < VPT; ++i) {
             float o[N], og[N];
 #pragma unroll
             for (int e = 0; e < N; ++e) {
                 const float xh = Wide<T>::up(now.x[i], e) * now.inv_x, p = Wide<T>::up(wp[i], e);
-                // (formed once more: kept over the barrier it would take a register per element)
-                const float dr = d_stream(i, e, Wide<T>::up(now.dy[i], e), Wide<T>::up(now.r[i], e) * now.inv_r);
+                float dr;
+                if constexpr (kKeep) dr = kept[i][e];
+                else dr = d_stream(i, e, Wide<T>::up(now.dy[i], e), normed(i, e));
                 const float dz = a * dr;  // (kScalar: a with the row's gate in it)
                 float gated = dz;
                 if constexpr (kVector) gated *= gate(i, e);
@@ -798,7 +825,7 @@ template <typename T>
 int launch_bwd(BwdArgs<T> k, T* d_weight, T* d_post_weight, void* workspace, hipStream_t st) {
     k.p = split_of(k.s, kThreads, 1);  // of the element-wise kernel
     k.part = partial_of(workspace, k.s, k.p);
-    const bool dwords = dwords_of<T>(k.s.H, {k.x, k.stream, k.post_weight, k.weight, k.s.mode == kScalar ? nullptr : k.gate, k.d_out, k.d_stream, k.dx,
+    const bool dwords = dwords_of<T>(k.s.H, {k.x, k.residual, k.post_weight, k.weight, k.s.mode == kScalar ? nullptr : k.gate, k.d_out, k.d_stream, k.dx,
                                              k.d_residual, k.s.mode == kScalar ? nullptr : k.d_gate});
     const bool held = with_team<T>(vectors_of<T>(k.s.H), dwords, [&](auto t) {
         constexpr int TEAM = decltype(t)::team, VPT = decltype(t)::vpt;
@@ -901,7 +928,7 @@ int64_t fma_sandwich_rmsnorm_bwd_workspace_bytes(int64_t B, int64_t H, int64_t g
     return fmahip::workspace_bytes_of(fmahip::shape_of(B, H, gate_rows, gate_width));
 }
 
-int fma_sandwich_rmsnorm_bwd(const void* x, const void* stream_out, const void* post_weight, const void* weight, const void* gate,
+int fma_sandwich_rmsnorm_bwd(const void* x, const void* residual, const void* post_weight, const void* weight, const void* gate,
                              int64_t gate_rows, int64_t gate_width, const void* out_grad, const void* stream_grad, const float* stats,
                              void* x_grad, void* residual_grad, void* gate_grad, void* post_weight_grad, void* weight_grad, int64_t B, int64_t H,
                              float multiplier, void* workspace, int64_t workspace_bytes, int dtype, void* stream) {
@@ -911,8 +938,8 @@ int fma_sandwich_rmsnorm_bwd(const void* x, const void* stream_out, const void* 
     FMA_REQUIRE((gate || !gate_grad) && (post_weight || !post_weight_grad) && (weight || !weight_grad), FMA_ERR_NULL_POINTER,
                 "sandwich_rmsnorm_bwd: a gradient without its input");
     FMA_REQUIRE(B > 0, FMA_ERR_BAD_SIZE, "sandwich_rmsnorm_bwd: no rows");
-    FMA_REQUIRE(x && stream_out && stats && x_grad && residual_grad, FMA_ERR_NULL_POINTER, "sandwich_rmsnorm_bwd: NULL pointer");
-    FMA_REQUIRE(aligned_to_elements({x, stream_out, post_weight, weight, gate, out_grad, stream_grad, x_grad, residual_grad, gate_grad,
+    FMA_REQUIRE(x && residual && stats && x_grad && residual_grad, FMA_ERR_NULL_POINTER, "sandwich_rmsnorm_bwd: NULL pointer");
+    FMA_REQUIRE(aligned_to_elements({x, residual, post_weight, weight, gate, out_grad, stream_grad, x_grad, residual_grad, gate_grad,
                                      post_weight_grad, weight_grad}, dtype),
                 FMA_ERR_MISALIGNED, "sandwich_rmsnorm_bwd: tensors must be aligned to their elements");
     const Shape s = shape_of(B, H, gate ? gate_rows : 0, gate_width);
@@ -924,13 +951,13 @@ int fma_sandwich_rmsnorm_bwd(const void* x, const void* stream_out, const void* 
     hipStream_t st = (hipStream_t)stream;
     switch (dtype) {
         case FMA_F32:
-            return backward<float>(x, stream_out, post_weight, weight, gate, out_grad, stream_grad, stats, x_grad, residual_grad, gate_grad,
+            return backward<float>(x, residual, post_weight, weight, gate, out_grad, stream_grad, stats, x_grad, residual_grad, gate_grad,
                                    post_weight_grad, weight_grad, s, multiplier, workspace, st);
         case FMA_F16:
-            return backward<f16_t>(x, stream_out, post_weight, weight, gate, out_grad, stream_grad, stats, x_grad, residual_grad, gate_grad,
+            return backward<f16_t>(x, residual, post_weight, weight, gate, out_grad, stream_grad, stats, x_grad, residual_grad, gate_grad,
                                    post_weight_grad, weight_grad, s, multiplier, workspace, st);
         default:
-            return backward<bf16_t>(x, stream_out, post_weight, weight, gate, out_grad, stream_grad, stats, x_grad, residual_grad, gate_grad,
+            return backward<bf16_t>(x, residual, post_weight, weight, gate, out_grad, stream_grad, stats, x_grad, residual_grad, gate_grad,
                                     post_weight_grad, weight_grad, s, multiplier, workspace, st);
     }
 }

@@ -40,7 +40,7 @@ def _forward(x, residual, post_weight, weight, gate, rows_of_gate, eps, multipli
     # 1 / rms of every row of x and of the stream
     stats = torch.empty(2, x.numel() // x.size(-1), dtype=torch.float32, device=x.device) if keep else None
     fused_sandwich_rmsnorm_forward_cuda(x, residual, post_weight, weight, gate, output, stream, stats, rows_of_gate, eps, multiplier)
-    return (output, stream), (x, stream, post_weight, weight, gate, stats) if keep else None
+    return (output, stream), (x, residual, post_weight, weight, gate, stats) if keep else None
 
 
 class _FusedSandwichRMSNorm(torch.autograd.Function):
@@ -59,7 +59,7 @@ class _FusedSandwichRMSNorm(torch.autograd.Function):
     def backward(ctx, output_grad, stream_grad):
         if output_grad is None and stream_grad is None:
             return (None,) * 9
-        x, stream, post_weight, weight, gate, stats = ctx.saved_tensors
+        x, residual, post_weight, weight, gate, stats = ctx.saved_tensors
         output_grad, stream_grad = [t if t is None else t.contiguous() for t in (output_grad, stream_grad)]
         x_grad, residual_grad = torch.empty_like(x), torch.empty_like(x)
         rows = x.numel()
@@ -68,7 +68,7 @@ class _FusedSandwichRMSNorm(torch.autograd.Function):
         post_weight_grad, weight_grad, gate_grad = [new(t) if n else None for t, n in zip((post_weight, weight, gate), ctx.needs_input_grad[2:5])]
         if rows:
             fused_sandwich_rmsnorm_backward_cuda(
-                x, stream, post_weight, weight, gate, output_grad, stream_grad, stats, x_grad, residual_grad, post_weight_grad, weight_grad,
+                x, residual, post_weight, weight, gate, output_grad, stream_grad, stats, x_grad, residual_grad, post_weight_grad, weight_grad,
                 gate_grad, ctx.rows_of_gate, ctx.multiplier,
             )  # fmt: skip
         return x_grad, residual_grad, post_weight_grad, weight_grad, gate_grad, None, None, None, None
@@ -91,8 +91,8 @@ def fused_sandwich_rmsnorm(
     squares; None takes the dtype's machine epsilon. gate: multiplies the normed output; of x's dtype and, from the left, of x's dimensions up
     to some point and 1 from there on, the last one 1 or x's (dimensions of 1 may be left out in front): a scale per element (x's shape), per
     channel ([H]), per token ([.., 1]), per sequence and channel ([batch, 1, H]), or a single number. multiplier: the residual scale; None means 1.
-    Arithmetic is in float32 with one rounding per output, the second norm is taken of the unrounded stream, and the backward
-    pass (once; no second derivatives) starts from the rounded one. kernel_backend: `triton` (the default) and `cuda` both run the HIP
+    Arithmetic is in float32 with one rounding per output; the second norm is taken of the unrounded stream, in the backward pass too (once; no
+    second derivatives), which keeps x, residual, gate, the scales and two numbers per row. kernel_backend: `triton` (the default) and `cuda` both run the HIP
     kernels; anything else raises ValueError.
     """
     if not is_hip_kernel_backend(kernel_backend):

@@ -47,12 +47,12 @@ def fused_sandwich_rmsnorm_forward_cuda(
 
 @hip_op("fused_sandwich_rmsnorm_backward_cuda", mutates_args={"x_grad", "residual_grad", "post_weight_grad", "weight_grad", "gate_grad"})
 def fused_sandwich_rmsnorm_backward_cuda(
-    x: torch.Tensor, stream: torch.Tensor, post_weight: torch.Tensor | None, weight: torch.Tensor | None, gate: torch.Tensor | None,
+    x: torch.Tensor, residual: torch.Tensor, post_weight: torch.Tensor | None, weight: torch.Tensor | None, gate: torch.Tensor | None,
     output_grad: torch.Tensor | None, stream_grad: torch.Tensor | None, stats: torch.Tensor, x_grad: torch.Tensor,
     residual_grad: torch.Tensor, post_weight_grad: torch.Tensor | None, weight_grad: torch.Tensor | None, gate_grad: torch.Tensor | None,
     gate_rows: int, multiplier: float,
 ) -> None:  # fmt: skip
-    B, H, gate_width = _check(x, (stream, output_grad, stream_grad, x_grad, residual_grad), post_weight, weight, gate, gate_rows, stats)
+    B, H, gate_width = _check(x, (residual, output_grad, stream_grad, x_grad, residual_grad), post_weight, weight, gate, gate_rows, stats)
     for grad, t in ((post_weight_grad, post_weight), (weight_grad, weight), (gate_grad, gate)):
         assert grad is None or (grad.shape == t.shape and grad.dtype is x.dtype and grad.is_contiguous() and grad.get_device() == x.get_device())
     _lib.require_gpu(x)  # (and with it the others)
@@ -61,7 +61,7 @@ def fused_sandwich_rmsnorm_backward_cuda(
         nbytes = lib.fma_sandwich_rmsnorm_bwd_workspace_bytes(B, H, gate_rows, gate_width)
         workspace = torch.empty(nbytes, dtype=torch.uint8, device=x.device)
         rc = lib.fma_sandwich_rmsnorm_bwd(
-            x.data_ptr(), stream.data_ptr(), _lib.ptr(post_weight), _lib.ptr(weight), _lib.ptr(gate), gate_rows, gate_width,
+            x.data_ptr(), residual.data_ptr(), _lib.ptr(post_weight), _lib.ptr(weight), _lib.ptr(gate), gate_rows, gate_width,
             _lib.ptr(output_grad), _lib.ptr(stream_grad), stats.data_ptr(), x_grad.data_ptr(), residual_grad.data_ptr(), _lib.ptr(gate_grad),
             _lib.ptr(post_weight_grad), _lib.ptr(weight_grad), B, H, multiplier, workspace.data_ptr(), nbytes, _lib.dtype_code(x.dtype),
             _lib.current_stream(x.device),

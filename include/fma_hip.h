@@ -523,13 +523,13 @@ int fma_router_loss_bwd(const void* logits, const uint8_t* mask, int64_t T, int6
  * gate_width H or 1 and gate_rows a divisor of B: row i serves the B / gate_rows rows of x from i * B / gate_rows on. stats: 2 * B floats for
  * the backward call (1 / rms of x, then of the stream) or NULL. fp32 arithmetic, one rounding each; out is formed from the unrounded stream.
  * B < 2^31, H <= FMA_MAX_NORM_HIDDEN. No counterpart in the reference (its fused_residual_add_rmsnorm is the case without the first norm).
- * Backward (B > 0): out_grad and stream_grad may each be NULL (zero); gate_grad, post_weight_grad and weight_grad, shaped and typed like what
+ * Backward (B > 0), from the forward call's inputs and stats (the stream is formed again, unrounded): out_grad and stream_grad may each be NULL (zero); gate_grad, post_weight_grad and weight_grad, shaped and typed like what
  * they belong to, are computed unless NULL. workspace: 16-byte aligned, no initialisation. Sums over rows have a fixed order. */
 int fma_sandwich_rmsnorm_fwd(const void* x, const void* residual, const void* post_weight, const void* weight, const void* gate,
                              int64_t gate_rows, int64_t gate_width, void* out, void* stream_out, float* stats, int64_t B, int64_t H, float eps,
                              float multiplier, int dtype, void* stream);
 int64_t fma_sandwich_rmsnorm_bwd_workspace_bytes(int64_t B, int64_t H, int64_t gate_rows, int64_t gate_width);
-int fma_sandwich_rmsnorm_bwd(const void* x, const void* stream_out, const void* post_weight, const void* weight, const void* gate,
+int fma_sandwich_rmsnorm_bwd(const void* x, const void* residual, const void* post_weight, const void* weight, const void* gate,
                              int64_t gate_rows, int64_t gate_width, const void* out_grad, const void* stream_grad, const float* stats,
                              void* x_grad, void* residual_grad, void* gate_grad, void* post_weight_grad, void* weight_grad, int64_t B, int64_t H,
                              float multiplier, void* workspace, int64_t workspace_bytes, int dtype, void* stream);

@@ -2,8 +2,8 @@
 
 Bounds, with u = 2^-24 and h half a step of the type. A mean over a row is off by n u of its terms' magnitudes, n = max(H / 256, 64) + 24 (a
 thread adds at most that many one after the other, then threads and wavefronts join), an inverse root by half of that and three roundings.
-Errors are carried through the formulas to first order, each product or sum adding one rounding of its terms; what the backward pass starts
-from is the stream rounded to the type (h of each element). A sum over rows adds at most B / 256 + 40 roundings of its terms in 32 bits."""
+Errors are carried through the formulas to first order, each product or sum adding one rounding of its terms; the backward pass starts from the
+stream as it was before its rounding to the type. A sum over rows adds at most B / 256 + 40 roundings of its terms in 32 bits."""
 
 import pytest
 import torch
@@ -71,8 +71,7 @@ def _exact(t, grads, a, eps=_EPS):
     out = r * inv_r * w
     want = dict(out=rounded(out, w.abs() * inv_r * (er + r.abs() * (rel_r + 4 * _U))), stream=rounded(r, er))
 
-    # backward; er: of the stored stream
-    er = er + h * r.abs() + (_TINY[dtype] if h > _U else 0.0)
+    # backward
     rh, erh = r * inv_r, inv_r * er + (r * inv_r).abs() * (rel_r + 2 * _U)
     g = dy * w
     m = mean(g * rh)
@@ -271,11 +270,19 @@ def test_no_grad_gives_the_same_and_only_the_asked_gradients_are_made():
         out, _ = fma.fused_sandwich_rmsnorm(leaf, t["residual"], None, None, _EPS)
         (grad,) = torch.autograd.grad(out.sum(), leaf, create_graph=True)
         grad.sum().backward()
-    # a stream that is changed in place afterwards is noticed
-    leaf = t["x"].detach().requires_grad_()
-    out, stream = fma.fused_sandwich_rmsnorm(leaf, t["residual"], None, None, _EPS)
+    # a residual that is changed in place afterwards is noticed; the stream is not needed again and may be
+    leaf, residual = t["x"].detach().requires_grad_(), t["residual"].clone()
+    out, stream = fma.fused_sandwich_rmsnorm(leaf, residual, t["post_weight"], t["weight"], _EPS, t["gate"], 1.0)
+    (stream + 0).backward(grads[1], retain_graph=True)
     with torch.no_grad():
-        stream.add_(1)
+        stream.mul_(0)
+    out.backward(grads[0])
+    parts = [_run(t, g, 1.0)["d_x"] for g in ((grads[0], None), (None, grads[1]))]
+    assert torch.equal(leaf.grad, parts[0] + parts[1])
+    leaf = t["x"].detach().requires_grad_()
+    out, stream = fma.fused_sandwich_rmsnorm(leaf, residual, None, None, _EPS)
+    with torch.no_grad():
+        residual.add_(1)
     with pytest.raises(RuntimeError, match="modified by an inplace operation"):
         out.sum().backward()
 
