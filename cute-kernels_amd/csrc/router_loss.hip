@@ -132,6 +132,18 @@ __device__ __forceinline__ __amdgpu_buffer_rsrc_t rows_at(const T* p, int64_t le
     return __builtin_amdgcn_make_buffer_rsrc(const_cast<T*>(p), 0, (int)(rows * (uint32_t)E * (uint32_t)sizeof(T)), 0x00020000);
 }
 
+// the logits of a workgroup's tokens from `base` on, and whether they count (those behind the last one do not)
+template <typename T, int NV, bool VEC>
+__device__ __forceinline__ void fetch_token(Logits<T, NV>& x, uint32_t& use, const T* logits, const uint8_t* mask, int64_t base, int64_t T_,
+                                            int group, int E, uint32_t offset, int token, int in) {
+    x.template load<VEC>(rows_at(logits + base * E, T_ - base, group, E), offset, in);
+    const int64_t left = T_ - base;
+    const uint32_t tokens = left > 0 ? (uint32_t)(left < group ? left : group) : 0u;
+    if (mask) use = (uint8_t)__builtin_amdgcn_raw_buffer_load_b8(
+                  __builtin_amdgcn_make_buffer_rsrc(const_cast<uint8_t*>(mask) + base, 0, (int)tokens, 0x00020000), token, 0, 0);
+    else use = (uint32_t)token < tokens ? 1u : 0u;
+}
+
 // A token's largest logit, the exponentials of its logits against it, their sum: exp and log of the hardware, whose errors
 // (two units, and that of an argument rounded in float32) are those of the subtraction in front of them.
 template <typename T, int L, int NV>
@@ -367,12 +379,7 @@ __global__ __launch_bounds__(fwd_threads(NV)) void router_loss_kernel(const T* _
     double zsum = 0.0;
     uint32_t n = 0;
     auto fetch = [&](Logits<T, NV>& x, uint32_t& use, int64_t base) {
-        x.template load<VEC>(rows_at(logits + base * E, T_ - base, kTokens, E), offset, in);
-        const int64_t left = T_ - base;
-        const uint32_t tokens = left > 0 ? (uint32_t)(left < kTokens ? left : kTokens) : 0u;
-        if (mask) use = (uint8_t)__builtin_amdgcn_raw_buffer_load_b8(
-                      __builtin_amdgcn_make_buffer_rsrc(const_cast<uint8_t*>(mask) + base, 0, (int)tokens, 0x00020000), token, 0, 0);
-        else use = (uint32_t)token < tokens ? 1u : 0u;
+        fetch_token<T, NV, VEC>(x, use, logits, mask, base, T_, kTokens, E, offset, token, in);
     };
     Logits<T, NV> x, next;
     uint32_t use, next_use;
@@ -558,15 +565,26 @@ __global__ __launch_bounds__(kBwdThreads) void router_loss_bwd_kernel(const T* _
     const int first = (threadIdx.x & (L - 1)) * NV, token = threadIdx.x / L;
     const int in = E - first < 0 ? 0 : E - first < NV ? E - first : NV;
     const uint32_t offset = (uint32_t)(token * E + first) * (uint32_t)sizeof(T);
+    Logits<T, NV> x;
+    uint32_t use;
+    int64_t base = (int64_t)blockIdx.x * kTokens;
+    // the first token's logits and the table's entries under way together (no branch between them); zeros behind the table's end
+    fetch_token<T, NV, VEC>(x, use, logits, mask, base, T_, kTokens, E, offset, token, in);
+    float f[NV];
+    const __amdgpu_buffer_rsrc_t entries = __builtin_amdgcn_make_buffer_rsrc(const_cast<float*>(table), 0, E * 4, 0x00020000);
+#pragma unroll
+    for (int i = 0; i < NV; i += 4) {
+        const auto four = __builtin_amdgcn_raw_buffer_load_b128(entries, (first + i) * 4, 0, 0);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            const uint32_t one = four[j];
+            f[i + j] = __uint_as_float(one);
+        }
+    }
     const float inv_n = table[E];
     const float gb = balance_grad ? *balance_grad * inv_n : 0.f, gz = z_grad ? 2.0f * *z_grad * inv_n : 0.f;
-    float f[NV];
-#pragma unroll
-    for (int i = 0; i < NV; ++i) f[i] = i < in ? table[first + i] : 0.f;
-    for (int64_t base = (int64_t)blockIdx.x * kTokens; base < T_; base += (int64_t)gridDim.x * kTokens) {
-        Logits<T, NV> x;
-        x.template load<VEC>(rows_at(logits + base * E, T_ - base, kTokens, E), offset, in);
-        const bool counted = base + token < T_ && (!mask || mask[base + token] != 0);
+    for (; base < T_; base += (int64_t)gridDim.x * kTokens) {
+        const bool counted = use != 0;
         x.template settle<VEC>(counted, in);
         float e[NV], top, sum;
         softmax_token<T, L, NV>(x, e, top, sum);
@@ -599,6 +617,7 @@ __global__ __launch_bounds__(kBwdThreads) void router_loss_bwd_kernel(const T* _
                 else __builtin_amdgcn_raw_buffer_store_b16(__builtin_bit_cast(uint16_t, Num<T>::down(e[i])), to, (int)at, 0, 0);
             }
         }
+        fetch_token<T, NV, VEC>(x, use, logits, mask, base + (int64_t)gridDim.x * kTokens, T_, kTokens, E, offset, token, in);
     }
 }
 
