@@ -137,6 +137,7 @@ __device__ __forceinline__ void add_chunk(Accumulator<MAX>& acc, T* p, int n) {
         });
 }
 
+// 2.2 GB of bf16: 323 us, 6.9 TB/s; 18.9 MB in 120 tensors: 7.8 us, most of it launch and latency
 template <bool MAX, bool STREAM>
 __global__ __launch_bounds__(kThreads) void grad_norm_kernel(const Table t, uint64_t* __restrict__ partial) {
     Accumulator<MAX> acc;
@@ -187,7 +188,9 @@ __device__ __forceinline__ void scale_chunk(T* p, int n, float factor) {
         });
 }
 
-// a factor of one leaves the tensors alone: nothing is read or written then. A NaN goes through.
+// A factor of one leaves the tensors alone: nothing is read or written then. A NaN goes through. A workgroup per chunk, which ends with it, keeps more
+// loads and stores in flight than workgroups that stay: 2.2 GB of bf16 722 us, 6.1 TB/s (a copy of that size: 4.8, an elementwise product in place 5.9);
+// 18.9 MB in 120 tensors 12 us.
 template <bool STREAM>
 __global__ __launch_bounds__(kThreads) void scale_grads_kernel(const Table t, const double* __restrict__ norm64,
                                                                const float* __restrict__ norm, double max_norm) {
