@@ -169,10 +169,23 @@ __global__ __launch_bounds__(kJoinThreads) void grad_norm_join_kernel(const uint
     }
 }
 
+// What elements are multiplied by: digits * 2^power. The power is 0 unless the factor lies below float32's normal numbers, where it would have
+// few bits or be 0 while the products (2^125 times 2^-135) are ordinary numbers: the digits are then in [1/2, 1), and the power, which is
+// applied to the product, rounds only what is itself below the normal numbers. (Against a product alone: 723 / 725 us for 2.2 GB of bf16,
+// 9.1 / 9.1 for 18.9 MB of fp32.)
+struct Factor {
+    float digits;
+    int power;
+    __device__ __forceinline__ explicit Factor(double f) : digits((float)f), power(0) {
+        if (fabs(f) < 0x1p-126) digits = (float)frexp(f, &power);
+    }
+    __device__ __forceinline__ float times(float x) const { return ldexpf(x * digits, power); }
+};
+
 template <bool STREAM, typename T>
-__device__ __forceinline__ void scale_chunk(T* p, int n, float factor) {
+__device__ __forceinline__ void scale_chunk(T* p, int n, const Factor& factor) {
     over_chunk<4>(
-        p, n, [&](T* x) { *x = Num<T>::down(Num<T>::up(*x) * factor); },
+        p, n, [&](T* x) { *x = Num<T>::down(factor.times(Num<T>::up(*x))); },
         [&](Vec16<T>* v, auto times) {
             constexpr int U = decltype(times)::value;
             Vec16<T> x[U];
@@ -181,7 +194,7 @@ __device__ __forceinline__ void scale_chunk(T* p, int n, float factor) {
 #pragma unroll
             for (int u = 0; u < U; ++u) {
 #pragma unroll
-                for (int e = 0; e < Vec16<T>::N; ++e) x[u].v[e] = Num<T>::down(Num<T>::up(x[u].v[e]) * factor);
+                for (int e = 0; e < Vec16<T>::N; ++e) x[u].v[e] = Num<T>::down(factor.times(Num<T>::up(x[u].v[e])));
                 if constexpr (STREAM) store_streaming16(v + u * kThreads, x[u]);
                 else v[u * kThreads] = x[u];
             }
@@ -196,7 +209,7 @@ __global__ __launch_bounds__(kThreads) void scale_grads_kernel(const Table t, co
                                                                const float* __restrict__ norm, double max_norm) {
     const double ratio = max_norm / ((norm64 ? *norm64 : (double)*norm) + 1e-6);
     if (ratio >= 1.0) return;
-    const float factor = (float)ratio;
+    const Factor factor(ratio);
     int at = 0;
     for (uint32_t c = blockIdx.x; c < t.first[t.count]; c += gridDim.x) {
         const Chunk k = find_chunk<kScaleChunk>(t, c, at);

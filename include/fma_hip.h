@@ -543,8 +543,9 @@ int fma_sandwich_rmsnorm_bwd(const void* x, const void* residual, const void* po
 int64_t fma_grad_norm_workspace_bytes(int64_t count);
 int fma_grad_norm(void* const* tensors, const int64_t* sizes, const int32_t* dtypes, int64_t count, int infinity, float* norm,
                   void* workspace, int64_t workspace_bytes, void* stream);
-/* Every element times min(1, max_norm / (*norm + 1e-6)), rounded to its type once; with a factor of one nothing is touched. The tensors
- * must not overlap. fma_clip_grad_norm is fma_grad_norm and this with the norm as it is in 64 bits. */
+/* Every element times min(1, max_norm / (*norm + 1e-6)); with a factor of one nothing is touched. The factor is formed in 64 bits, its digits
+ * and the product are rounded to float32 (below float32's normal numbers too, the factor keeps all its digits), the product then to the
+ * tensor's type. The tensors must not overlap. fma_clip_grad_norm is fma_grad_norm and this with the norm as it is in 64 bits. */
 int fma_scale_grads(void* const* tensors, const int64_t* sizes, const int32_t* dtypes, int64_t count, const float* norm, double max_norm,
                     void* stream);
 int fma_clip_grad_norm(void* const* tensors, const int64_t* sizes, const int32_t* dtypes, int64_t count, int infinity, double max_norm,

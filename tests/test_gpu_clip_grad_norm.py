@@ -293,3 +293,25 @@ def test_strided_gradients_that_share_memory():
     norm = fma.clip_grad_norm_(_parameters([base[:, ::2], base[:, 1::2]]), 1e-3)
     _check_norm(norm, float(before.double().norm()))
     _check_scaled([base], [before], float(before.double().norm()), 1e-3)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("magnitude,max_norm", [(2.0**125, 0.37), (2.0**125, 1e-6), (2.0**125, 1e-30), (2.0**125, 1.5e-37), (1e10, 1e-33), (1e-2, 1.5e-37)])
+def test_factors_below_float32s_normal_numbers(magnitude, max_norm, dtype):
+    """The factor lies where float32 has few bits or none, the results do not (or only just). The factor's leading digits are rounded once, as
+    ever; scaling by a power of two rounds only a result that is itself below the normal numbers, by half of float32's smallest."""
+    g = torch.Generator(device=DEV).manual_seed(5)
+    before = (magnitude * (1.0 + 0.9 * torch.rand(1 << 20, generator=g, device=DEV)) * (1 - 2 * (torch.rand(1 << 20, generator=g, device=DEV) < 0.5))).to(dtype)
+    norm = _norm64([before], 2.0)
+    calls = [(norm, lambda p: fma.clip_grad_norm_(p, max_norm))]
+    if norm < 2.0**127:
+        given = torch.tensor(norm, device=DEV)
+        calls.append((float(given.double()), lambda p: fma.clip_grads_with_norm_(p, max_norm, given)))
+    for norm, call in calls:
+        (p,) = _parameters([before.clone()])
+        call([p])
+        factor = max_norm / (norm + 1e-6)
+        assert 0.0 < factor < 2.0**-126
+        want = before.double() * factor
+        bound = want.abs() * (torch.finfo(dtype).eps / 2 + 3 * 2.0**-24) * (1 + 2.0**-20) + _TINY[dtype] + 2.0**-150
+        assert bool(((p.grad.double() - want).abs() <= bound).all()) and bool(p.grad.any())
