@@ -334,6 +334,18 @@ int check_bound(const char* what, double max_norm) {
     return FMA_OK;
 }
 
+int check_scale(void* const* tensors, const int64_t* sizes, const int32_t* dtypes, int64_t count, const void* norm, size_t norm_bytes,
+                double max_norm) {
+    int rc = check_tensors("scale_grads", tensors, sizes, dtypes, count);
+    if (!rc) rc = check_bound("scale_grads", max_norm);
+    if (!rc) rc = check_disjoint("scale_grads", tensors, sizes, dtypes, count);
+    if (rc) return rc;
+    FMA_REQUIRE(norm, FMA_ERR_NULL_POINTER, "scale_grads: norm is NULL");
+    FMA_REQUIRE(((uintptr_t)norm & (norm_bytes - 1)) == 0, FMA_ERR_MISALIGNED, "scale_grads: norm is not aligned to its %d bytes",
+                (int)norm_bytes);
+    return FMA_OK;
+}
+
 }  // namespace
 }  // namespace fmahip
 
@@ -359,12 +371,15 @@ int fma_grad_norm(void* const* tensors, const int64_t* sizes, const int32_t* dty
 int fma_scale_grads(void* const* tensors, const int64_t* sizes, const int32_t* dtypes, int64_t count, const float* norm, double max_norm,
                     void* stream) {
     using namespace fmahip;
-    int rc = check_tensors("scale_grads", tensors, sizes, dtypes, count);
-    if (!rc) rc = check_bound("scale_grads", max_norm);
-    if (!rc) rc = check_disjoint("scale_grads", tensors, sizes, dtypes, count);
-    if (rc) return rc;
-    FMA_REQUIRE(norm, FMA_ERR_NULL_POINTER, "scale_grads: norm is NULL");
-    return launch_scale(tensors, sizes, dtypes, count, nullptr, norm, max_norm, (hipStream_t)stream);
+    const int rc = check_scale(tensors, sizes, dtypes, count, norm, sizeof(*norm), max_norm);
+    return rc ? rc : launch_scale(tensors, sizes, dtypes, count, nullptr, norm, max_norm, (hipStream_t)stream);
+}
+
+int fma_scale_grads_norm64(void* const* tensors, const int64_t* sizes, const int32_t* dtypes, int64_t count, const double* norm,
+                           double max_norm, void* stream) {
+    using namespace fmahip;
+    const int rc = check_scale(tensors, sizes, dtypes, count, norm, sizeof(*norm), max_norm);
+    return rc ? rc : launch_scale(tensors, sizes, dtypes, count, norm, nullptr, max_norm, (hipStream_t)stream);
 }
 
 int fma_clip_grad_norm(void* const* tensors, const int64_t* sizes, const int32_t* dtypes, int64_t count, int infinity, double max_norm,

@@ -103,6 +103,7 @@ SIGNATURES = {
     "fma_grad_norm_workspace_bytes": (_i64, [_i64]),
     "fma_grad_norm": (_i32, [_p] * 3 + [_i64, _i32, _p, _p, _i64, _p]),
     "fma_scale_grads": (_i32, [_p] * 3 + [_i64, _p, _f64, _p]),
+    "fma_scale_grads_norm64": (_i32, [_p] * 3 + [_i64, _p, _f64, _p]),
     "fma_clip_grad_norm": (_i32, [_p] * 3 + [_i64, _i32, _f64, _p, _p, _i64, _p]),
 }
 

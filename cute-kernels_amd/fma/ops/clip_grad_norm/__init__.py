@@ -54,7 +54,8 @@ def get_total_norm(
 
 
 def clip_grads_with_norm_(parameters: torch.Tensor | Iterable[torch.Tensor], max_norm: float, total_norm: torch.Tensor) -> None:
-    """Multiplies the parameters' gradients, in place, by min(1, max_norm / (total_norm + 1e-6)). With a factor of one they are not touched."""
+    """Multiplies the parameters' gradients, in place, by min(1, max_norm / (total_norm + 1e-6)), which is formed in 64 bits from the total_norm
+    as it is given. With a factor of one they are not touched."""
     scale_grads_cuda(_gradients(parameters), _check_bound(max_norm), total_norm)
 
 

@@ -1,4 +1,4 @@
-"""Calls of fma_grad_norm, fma_scale_grads and fma_clip_grad_norm of libfma_hip.so. They take lists of tensors that may be a few hundred, and
+"""Calls of fma_grad_norm, fma_scale_grads (and its form for 64-bit norms) and fma_clip_grad_norm of libfma_hip.so. They take lists of tensors that may be a few hundred, and
 are no operators of the dispatcher, which would look at each of them twice more."""
 
 from array import array
@@ -87,9 +87,11 @@ def scale_grads_cuda(grads: list[torch.Tensor], max_norm: float, norm: torch.Ten
         return
     table, lib = _Table(grads, True), _lib.load()
     assert norm.numel() == 1, "total_norm should be a scalar"
-    norm = norm.to(device=table.device, dtype=torch.float32)
+    # (every type but float32 as 64 bits, which hold it)
+    dtype, scale = (torch.float32, lib.fma_scale_grads) if norm.dtype is torch.float32 else (torch.float64, lib.fma_scale_grads_norm64)
+    norm = norm.to(device=table.device, dtype=dtype)
     with _lib.on_device(table.device):
-        rc = lib.fma_scale_grads(*table.arguments, norm.data_ptr(), max_norm, _lib.current_stream(table.device))
+        rc = scale(*table.arguments, norm.data_ptr(), max_norm, _lib.current_stream(table.device))
     _lib.check(rc, "clip_grads_with_norm_")
     _written(table, grads)
 

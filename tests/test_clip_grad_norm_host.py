@@ -89,3 +89,14 @@ def test_dense_layouts():
         assert _is_dense(dense)
     for gaps in (t[:, ::2], t[..., 1:], t[0, 0, 0].expand(3), t.transpose(0, 2)[:, 1:]):
         assert not _is_dense(gaps)
+
+
+def test_scaling_by_a_norm_in_64_bits_refuses_the_same(lib):
+    p = 1 << 20  # never read, as above
+    scale = lambda *a, norm=p, max_norm=1.0: lib.fma_scale_grads_norm64(*_arrays(*a), norm, max_norm, None)  # noqa: E731
+    assert scale([p], [8], [7]) == -2 and scale([p], [-1], [0]) == -3 and scale([None], [8], [0]) == -1
+    assert scale([p], [8], [0], max_norm=-1.0) == -3 and scale([p], [8], [0], max_norm=math.nan) == -3
+    assert scale([p, p + 28], [8, 8], [0, 0]) == -8
+    assert scale([p], [8], [0], norm=None) == -1
+    assert scale([p], [8], [0], norm=p + 4) == -6 and "aligned" in lib.fma_last_error_string().decode()
+    assert lib.fma_scale_grads(*_arrays([p], [8], [0]), p + 2, 1.0, None) == -6

@@ -315,3 +315,24 @@ def test_factors_below_float32s_normal_numbers(magnitude, max_norm, dtype):
         want = before.double() * factor
         bound = want.abs() * (torch.finfo(dtype).eps / 2 + 3 * 2.0**-24) * (1 + 2.0**-20) + _TINY[dtype] + 2.0**-150
         assert bool(((p.grad.double() - want).abs() <= bound).all()) and bool(p.grad.any())
+
+
+@pytest.mark.parametrize("where", ["cpu", "cuda"])
+def test_a_total_norm_in_64_bits(where):
+    """Scaling goes by its 64 bits: the factor is rounded to float32, the norm is not. Expected bits: factor and product in IEEE arithmetic."""
+    (before,) = _draw([(5003,)], torch.float32)
+    for i in range(24):
+        norm, max_norm = 3.0 + 1e-8 * (i + 1) / 7, 0.1 + 0.013 * i
+        (p,) = _parameters([before.clone()])
+        fma.clip_grads_with_norm_([p], max_norm, torch.tensor(norm, dtype=torch.float64, device=where))
+        factor = torch.tensor(max_norm / (norm + 1e-6), dtype=torch.float64).float().to(DEV)
+        assert torch.equal(p.grad, before * factor)
+    large = torch.full((77,), 1e30, device=DEV)
+    (p,) = _parameters([large.clone()])
+    fma.clip_grads_with_norm_([p], 1.0, torch.tensor(1e40, dtype=torch.float64, device=where))
+    want = large.double() * (1.0 / (1e40 + 1e-6))
+    assert bool(((p.grad.double() - want).abs() <= want * 3 * 2.0**-24).all())
+    whole = torch.tensor(2**24 + 3, device=where)  # a whole number that float32 does not hold: there it is one more
+    (p,) = _parameters([torch.ones(3, device=DEV)])
+    fma.clip_grads_with_norm_([p], float(2**24 + 3) + 1e-6, whole)
+    assert torch.equal(p.grad, torch.ones(3, device=DEV))
