@@ -45,9 +45,12 @@ def get_total_norm(
     tensors: torch.Tensor | Iterable[torch.Tensor], norm_type: float = 2.0, error_if_nonfinite: bool = False
 ) -> torch.Tensor:
     """The norm (norm_type 2 or inf) of all elements of the tensors (float32, float16, bfloat16, on one GPU): a float32 scalar there. A tensor
-    that comes twice counts twice. error_if_nonfinite waits for the result."""
+    that comes twice counts twice. error_if_nonfinite waits for the result and raises RuntimeError unless it is finite as float32."""
     infinity = _is_infinity_norm(norm_type)
-    norm = grad_norm_cuda([tensors] if isinstance(tensors, torch.Tensor) else list(tensors), infinity)
+    tensors = [tensors] if isinstance(tensors, torch.Tensor) else list(tensors)
+    if not tensors:
+        return torch.tensor(0.0)
+    norm, _ = grad_norm_cuda(tensors, infinity)
     if error_if_nonfinite:
         _require_finite(norm)
     return norm
@@ -65,13 +68,15 @@ def clip_grad_norm_(
     """Clips the gradients of the parameters to max_norm in place and returns their norm from before: get_total_norm and
     clip_grads_with_norm_ as one call. Parameters without a gradient are passed over. Gradients that share memory are refused (RuntimeError)
     if they are dense or one strided view; different views that overlap are scaled once, and count twice in the norm.
-    With error_if_nonfinite an infinite or NaN norm raises RuntimeError before anything is scaled. Not traced: a compiled function that calls
-    it breaks its graph here."""
+    The gradients are scaled by the norm in 64 bits; one past float32's range comes back as infinity. With error_if_nonfinite a norm that is
+    infinite or NaN in 64 bits raises RuntimeError before anything is scaled; the call waits for it and changes no bit otherwise. Not
+    traced: a compiled function that calls it breaks its graph here."""
     infinity, max_norm = _is_infinity_norm(norm_type), _check_bound(max_norm)
     grads = _gradients(parameters)
-    if error_if_nonfinite:
-        norm = grad_norm_cuda(grads, infinity)
-        _require_finite(norm)
-        scale_grads_cuda(grads, max_norm, norm)
+    if error_if_nonfinite and grads:
+        norm, workspace = grad_norm_cuda(grads, infinity)
+        norm64 = workspace[:8].view(torch.float64)  # what the call without the check scales by, too
+        _require_finite(norm64)
+        scale_grads_cuda(grads, max_norm, norm64)
         return norm
     return clip_grad_norm_cuda(grads, infinity, max_norm)

@@ -60,9 +60,8 @@ class _Table:
 
 
 @torch.no_grad()
-def grad_norm_cuda(tensors: list[torch.Tensor], infinity: bool) -> torch.Tensor:
-    if not tensors:
-        return torch.tensor(0.0)
+def grad_norm_cuda(tensors: list[torch.Tensor], infinity: bool) -> tuple[torch.Tensor, torch.Tensor]:
+    """the norm, and the workspace, whose first 8 bytes are the norm in 64 bits"""
     table, lib = _Table(tensors, False), _lib.load()
     with _lib.on_device(table.device):
         norm = torch.empty((), dtype=torch.float32, device=table.device)
@@ -72,7 +71,7 @@ def grad_norm_cuda(tensors: list[torch.Tensor], infinity: bool) -> torch.Tensor:
             *table.arguments, infinity, norm.data_ptr(), workspace.data_ptr(), nbytes, _lib.current_stream(table.device)
         )
     _lib.check(rc, "get_total_norm")
-    return norm
+    return norm, workspace
 
 
 def _written(table: _Table, grads: list[torch.Tensor]) -> None:

@@ -539,7 +539,8 @@ int fma_sandwich_rmsnorm_bwd(const void* x, const void* residual, const void* po
 /* The norm of `count` tensors together, sqrt of the sum of all squares or (infinity != 0) the largest magnitude, to *norm (device).
  * tensors, sizes (elements) and dtypes (FMA_F32 / FMA_F16 / FMA_BF16) are HOST arrays, read before the call returns; every tensor is dense
  * device memory, aligned to its elements. Sums are kept in 64 bits, in an order that depends on the sizes alone. A NaN anywhere makes the norm
- * NaN. No tensors, or none with elements: 0. workspace: 8-byte aligned, no initialisation. No counterpart in the reference. */
+ * NaN. No tensors, or none with elements: 0. workspace: 8-byte aligned, no initialisation; its first 8 bytes are the norm in 64 bits
+ * afterwards. No counterpart in the reference. */
 int64_t fma_grad_norm_workspace_bytes(int64_t count);
 int fma_grad_norm(void* const* tensors, const int64_t* sizes, const int32_t* dtypes, int64_t count, int infinity, float* norm,
                   void* workspace, int64_t workspace_bytes, void* stream);

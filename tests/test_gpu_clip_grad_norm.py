@@ -336,3 +336,28 @@ def test_a_total_norm_in_64_bits(where):
     (p,) = _parameters([torch.ones(3, device=DEV)])
     fma.clip_grads_with_norm_([p], float(2**24 + 3) + 1e-6, whole)
     assert torch.equal(p.grad, torch.ones(3, device=DEV))
+
+
+@pytest.mark.parametrize("dtype", _DTYPES)
+def test_the_check_for_finite_norms_changes_no_bit(dtype):
+    """error_if_nonfinite adds a look at the norm, and scales by the same one"""
+    before = _draw([(1001, 37), (5,), (4099,)], _DTYPES[dtype])
+    for i in range(1, 25):
+        ends = []
+        for check in (False, True):
+            grads = [b.clone() for b in before]
+            norm = fma.clip_grad_norm_(_parameters(grads), 0.01 * i, error_if_nonfinite=check)
+            ends.append([norm] + grads)
+        assert all(torch.equal(a, b) for a, b in zip(*ends))
+
+
+def test_a_finite_norm_that_float32_does_not_hold_is_finite():
+    before = torch.full((1 << 20,), 2.0**125, device=DEV).bfloat16()  # norm 2^135
+    ends = []
+    for check in (False, True):
+        g = before.clone()
+        assert float(fma.clip_grad_norm_(_parameters([g]), 3.0, error_if_nonfinite=check)) == math.inf
+        ends.append(g)
+    assert torch.equal(*ends) and torch.equal(ends[0], torch.full_like(before, 1.5 * 2.0**-9))
+    with pytest.raises(RuntimeError, match="finite"):  # what is returned here is not
+        fma.get_total_norm([before], error_if_nonfinite=True)
