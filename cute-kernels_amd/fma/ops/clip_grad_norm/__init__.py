@@ -5,7 +5,11 @@
     clip_grads_with_norm_(parameters, max_norm, norm)      scaling by a norm that is known, e.g. one that was reduced over ranks
 
 Norms are those of the elements on this device, as one long vector: 2-norm or largest magnitude. The squares are added in 64 bits and the
-result is float32, whatever the tensors' types (which may differ). The reference has no counterpart."""
+result is float32, whatever the tensors' types (which may differ). The reference has no counterpart.
+
+What differs from torch.nn.utils: other norms than 2 and infinity raise ValueError, other types and subclasses of tensors TypeError, tensors on
+several devices RuntimeError, and so do most gradients to be scaled that share memory (clip_grad_norm_ says which); a norm has float32, not
+the gradients' type; a parameter that comes twice has one gradient; the tensors always go together, so `foreach` is taken and changes nothing."""
 
 import math
 from typing import Iterable
@@ -42,7 +46,7 @@ def _require_finite(norm: torch.Tensor) -> None:
 
 
 def get_total_norm(
-    tensors: torch.Tensor | Iterable[torch.Tensor], norm_type: float = 2.0, error_if_nonfinite: bool = False
+    tensors: torch.Tensor | Iterable[torch.Tensor], norm_type: float = 2.0, error_if_nonfinite: bool = False, foreach: bool | None = None
 ) -> torch.Tensor:
     """The norm (norm_type 2 or inf) of all elements of the tensors (float32, float16, bfloat16, on one GPU): a float32 scalar there. A tensor
     that comes twice counts twice. error_if_nonfinite waits for the result and raises RuntimeError unless it is finite as float32."""
@@ -56,14 +60,20 @@ def get_total_norm(
     return norm
 
 
-def clip_grads_with_norm_(parameters: torch.Tensor | Iterable[torch.Tensor], max_norm: float, total_norm: torch.Tensor) -> None:
+def clip_grads_with_norm_(
+    parameters: torch.Tensor | Iterable[torch.Tensor], max_norm: float, total_norm: torch.Tensor, foreach: bool | None = None
+) -> None:
     """Multiplies the parameters' gradients, in place, by min(1, max_norm / (total_norm + 1e-6)), which is formed in 64 bits from the total_norm
     as it is given. With a factor of one they are not touched."""
     scale_grads_cuda(_gradients(parameters), _check_bound(max_norm), total_norm)
 
 
 def clip_grad_norm_(
-    parameters: torch.Tensor | Iterable[torch.Tensor], max_norm: float, norm_type: float = 2.0, error_if_nonfinite: bool = False
+    parameters: torch.Tensor | Iterable[torch.Tensor],
+    max_norm: float,
+    norm_type: float = 2.0,
+    error_if_nonfinite: bool = False,
+    foreach: bool | None = None,
 ) -> torch.Tensor:
     """Clips the gradients of the parameters to max_norm in place and returns their norm from before: get_total_norm and
     clip_grads_with_norm_ as one call. Parameters without a gradient are passed over. Gradients that share memory are refused (RuntimeError)

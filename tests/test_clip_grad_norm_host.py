@@ -1,6 +1,7 @@
 """The host side of the gradient norm and of clipping: what is refused, and what needs no GPU. Runs on the CPU."""
 
 import ctypes
+import inspect
 import math
 
 import pytest
@@ -100,3 +101,14 @@ def test_scaling_by_a_norm_in_64_bits_refuses_the_same(lib):
     assert scale([p], [8], [0], norm=None) == -1
     assert scale([p], [8], [0], norm=p + 4) == -6 and "aligned" in lib.fma_last_error_string().decode()
     assert lib.fma_scale_grads(*_arrays([p], [8], [0]), p + 2, 1.0, None) == -6
+
+
+def test_names_and_arguments_are_those_of_the_host_library():
+    """a call of torch.nn.utils works here as it stands"""
+    for name in ("clip_grad_norm_", "get_total_norm", "clip_grads_with_norm_"):
+        ours, theirs = (inspect.signature(getattr(module, name)).parameters for module in (fma, torch.nn.utils))
+        assert [(p.name, p.default) for p in ours.values()] == [(p.name, p.default) for p in theirs.values()], name
+    p = torch.nn.Parameter(torch.ones(3))
+    for foreach in (None, False, True):
+        assert fma.clip_grad_norm_([p], 1.0, 2.0, False, foreach) == 0.0 and fma.get_total_norm([], foreach=foreach) == 0.0
+        assert fma.clip_grads_with_norm_([p], 1.0, torch.ones(()), foreach) is None
