@@ -361,3 +361,35 @@ def test_a_finite_norm_that_float32_does_not_hold_is_finite():
     assert torch.equal(*ends) and torch.equal(ends[0], torch.full_like(before, 1.5 * 2.0**-9))
     with pytest.raises(RuntimeError, match="finite"):  # what is returned here is not
         fma.get_total_norm([before], error_if_nonfinite=True)
+
+
+def test_tensors_in_another_order():
+    """the norm is within its bound whatever the order, and each tensor is scaled by the same factor"""
+    grads = _draw([(700, 33), (1,), (70001,)], torch.bfloat16) + _draw([(129,), (5000,)], torch.float32, 1) + _draw([(77, 7)], torch.float16, 2)
+    want = _norm64(grads, 2.0)
+    for order in ((5, 4, 3, 2, 1, 0), (2, 0, 5, 1, 4, 3), (3, 5, 0, 4, 2, 1)):
+        some = [grads[i].clone() for i in order]
+        before = [g.clone() for g in some]
+        _check_norm(fma.get_total_norm(some), want)
+        _check_norm(fma.clip_grad_norm_(_parameters(some), 0.5 * want), want)
+        _check_scaled(some, before, want, 0.5 * want)
+
+
+@pytest.mark.parametrize("bad", [math.nan, math.inf, -math.inf])
+def test_nothing_is_written_where_the_norm_is_refused(bad):
+    grads = _draw([(100,), (20000,)], torch.bfloat16)
+    grads[1][17777] = bad
+    before, versions = [g.clone() for g in grads], [g._version for g in grads]
+    with pytest.raises(RuntimeError, match="finite"):
+        fma.clip_grad_norm_(_parameters(grads), 1e-3, error_if_nonfinite=True)
+    assert all(torch.equal(g.view(torch.int16), b.view(torch.int16)) for g, b in zip(grads, before))
+    assert [g._version for g in grads] == versions
+
+
+def test_a_dense_gradient_and_a_view_into_it():
+    """views that differ and overlap: every element is scaled once, and counts as often as it is named in the norm"""
+    base = torch.randn(40, 30, generator=torch.Generator(device=DEV).manual_seed(2), device=DEV)
+    before = base.clone()
+    norm = math.sqrt(float(before.double().square().sum()) + float(before[:, ::2].double().square().sum()))
+    _check_norm(fma.clip_grad_norm_(_parameters([base, base[:, ::2]]), 0.5 * norm), norm)
+    _check_scaled([base], [before], norm, 0.5 * norm)

@@ -404,3 +404,13 @@ def test_long_tensors():
     want = _exact(t, grads, 1.0)
     _compare(dict(out=out.detach()[rows][None], stream=stream.detach()[rows][None], d_x=x.grad[rows][None], d_weight=weight.grad),
              {n: want[n] for n in ("out", "stream", "d_x", "d_weight")})
+
+
+@pytest.mark.parametrize("H", [64, 1001, 4096])
+def test_rows_of_zeros_in_fp16(H):
+    """1 / sqrt(eps) = 316 times the upstream gradient, whose largest values here are below 65504 / 316 = 207"""
+    t, grads = _inputs((2, 9, H), torch.float16, "sequence", seed=1)
+    t["x"][0] = 0
+    want = _exact(t, grads, 1.0)
+    assert all(float(value.abs().max()) < 6e4 for value, _ in want.values())
+    _compare(_run(t, grads, 1.0), want)
