@@ -268,8 +268,9 @@ int check_tensors(const char* what, void* const* tensors, const int64_t* sizes, 
     return FMA_OK;
 }
 
-// No element may be scaled twice, least of all by two workgroups at once.
-int check_disjoint(const char* what, void* const* tensors, const int64_t* sizes, const int32_t* dtypes, int64_t count) {
+// No element may be scaled twice, least of all by two workgroups at once, nor the norm that all of them read.
+int check_disjoint(const char* what, void* const* tensors, const int64_t* sizes, const int32_t* dtypes, int64_t count, const void* norm,
+                   size_t norm_bytes) {
     struct Range {
         uintptr_t begin, end;
     };
@@ -283,10 +284,13 @@ int check_disjoint(const char* what, void* const* tensors, const int64_t* sizes,
         }
     const auto before = [](const Range& a, const Range& b) { return a.begin < b.begin; };
     if (!std::is_sorted(r, r + n, before)) std::sort(r, r + n, before);  // (those of a bucket are)
-    bool apart = true;
+    bool apart = true, outside = true;
     for (int64_t i = 1; i < n; ++i) apart = apart && r[i - 1].end <= r[i].begin;
+    const uintptr_t at = (uintptr_t)norm;
+    for (int64_t i = 0; i < n; ++i) outside = outside && (r[i].end <= at || at + norm_bytes <= r[i].begin);
     free(r);
     FMA_REQUIRE(apart, FMA_ERR_UNSUPPORTED, "%s: two tensors share memory", what);
+    FMA_REQUIRE(outside, FMA_ERR_UNSUPPORTED, "%s: the norm shares memory with a tensor", what);
     return FMA_OK;
 }
 
@@ -338,12 +342,11 @@ int check_scale(void* const* tensors, const int64_t* sizes, const int32_t* dtype
                 double max_norm) {
     int rc = check_tensors("scale_grads", tensors, sizes, dtypes, count);
     if (!rc) rc = check_bound("scale_grads", max_norm);
-    if (!rc) rc = check_disjoint("scale_grads", tensors, sizes, dtypes, count);
     if (rc) return rc;
     FMA_REQUIRE(norm, FMA_ERR_NULL_POINTER, "scale_grads: norm is NULL");
     FMA_REQUIRE(((uintptr_t)norm & (norm_bytes - 1)) == 0, FMA_ERR_MISALIGNED, "scale_grads: norm is not aligned to its %d bytes",
                 (int)norm_bytes);
-    return FMA_OK;
+    return check_disjoint("scale_grads", tensors, sizes, dtypes, count, norm, norm_bytes);
 }
 
 }  // namespace
@@ -387,9 +390,10 @@ int fma_clip_grad_norm(void* const* tensors, const int64_t* sizes, const int32_t
     using namespace fmahip;
     int rc = check_tensors("clip_grad_norm", tensors, sizes, dtypes, count);
     if (!rc) rc = check_bound("clip_grad_norm", max_norm);
-    if (!rc) rc = check_disjoint("clip_grad_norm", tensors, sizes, dtypes, count);
     if (rc) return rc;
     FMA_REQUIRE(norm, FMA_ERR_NULL_POINTER, "clip_grad_norm: norm is NULL");
+    rc = check_disjoint("clip_grad_norm", tensors, sizes, dtypes, count, norm, sizeof(*norm));
+    if (rc) return rc;
     rc = check_workspace("clip_grad_norm", workspace, workspace_bytes, count);
     if (!rc) rc = launch_norm(tensors, sizes, dtypes, count, infinity, norm, (double*)workspace, (hipStream_t)stream);
     if (!rc) rc = launch_scale(tensors, sizes, dtypes, count, (const double*)workspace, nullptr, max_norm, (hipStream_t)stream);

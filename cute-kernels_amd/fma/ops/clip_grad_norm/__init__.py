@@ -64,7 +64,8 @@ def clip_grads_with_norm_(
     parameters: torch.Tensor | Iterable[torch.Tensor], max_norm: float, total_norm: torch.Tensor, foreach: bool | None = None
 ) -> None:
     """Multiplies the parameters' gradients, in place, by min(1, max_norm / (total_norm + 1e-6)), which is formed in 64 bits from the total_norm
-    as it is given. With a factor of one they are not touched."""
+    as it is given. With a factor of one they are not touched. A total_norm that is itself an element of such a gradient is refused
+    (RuntimeError) if the gradient is dense."""
     scale_grads_cuda(_gradients(parameters), _check_bound(max_norm), total_norm)
 
 

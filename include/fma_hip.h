@@ -546,7 +546,7 @@ int fma_grad_norm(void* const* tensors, const int64_t* sizes, const int32_t* dty
                   void* workspace, int64_t workspace_bytes, void* stream);
 /* Every element times min(1, max_norm / (*norm + 1e-6)); with a factor of one nothing is touched. The factor is formed in 64 bits, its digits
  * and the product are rounded to float32 (below float32's normal numbers too, the factor keeps all its digits), the product then to the
- * tensor's type. The tensors must not overlap. fma_scale_grads_norm64 is the same by a norm in 64 bits (8-byte aligned), and
+ * tensor's type. The tensors must not overlap, neither each other nor the norm. fma_scale_grads_norm64 is the same by a norm in 64 bits (8-byte aligned), and
  * fma_clip_grad_norm fma_grad_norm and this with the norm as it is in 64 bits. */
 int fma_scale_grads(void* const* tensors, const int64_t* sizes, const int32_t* dtypes, int64_t count, const float* norm, double max_norm,
                     void* stream);

@@ -112,3 +112,14 @@ def test_names_and_arguments_are_those_of_the_host_library():
     for foreach in (None, False, True):
         assert fma.clip_grad_norm_([p], 1.0, 2.0, False, foreach) == 0.0 and fma.get_total_norm([], foreach=foreach) == 0.0
         assert fma.clip_grads_with_norm_([p], 1.0, torch.ones(()), foreach) is None
+
+
+def test_a_norm_inside_a_tensor_is_refused(lib):
+    """every workgroup reads it while others write"""
+    p = 1 << 20  # never read, as above
+    for scale, aligned in ((lib.fma_scale_grads, 4), (lib.fma_scale_grads_norm64, 8)):
+        for at in (p, p + 16, p + 64 - aligned):
+            assert scale(*_arrays([p], [16], [0]), at, 1.0, None) == -8 and "norm" in lib.fma_last_error_string().decode()
+            assert scale(*_arrays([p + 4096, p, p - 4096], [16, 16, 16], [0, 0, 0]), at, 1.0, None) == -8
+        assert scale(*_arrays([p + 4], [16], [0]), p + 4 - 4 * (aligned == 8), 1.0, None) == -8
+    assert lib.fma_clip_grad_norm(*_arrays([p], [16], [0]), 0, 1.0, p + 8, p + 4096, 1 << 20, None) == -8

@@ -393,3 +393,22 @@ def test_a_dense_gradient_and_a_view_into_it():
     norm = math.sqrt(float(before.double().square().sum()) + float(before[:, ::2].double().square().sum()))
     _check_norm(fma.clip_grad_norm_(_parameters([base, base[:, ::2]]), 0.5 * norm), norm)
     _check_scaled([base], [before], norm, 0.5 * norm)
+
+
+def test_a_norm_that_is_an_element_of_a_gradient():
+    """refused where the kernels would write it, and right where they write a copy of the gradient or where it only lies beside it"""
+    (bucket,) = _draw([(5000,)], torch.float32)
+    bucket[4000] = 2.0
+    before = bucket.clone()
+    (p,) = _parameters([bucket])
+    with pytest.raises(RuntimeError, match="norm shares memory"):
+        fma.clip_grads_with_norm_([p], 1.0, bucket[4000])
+    assert torch.equal(bucket, before)
+    (strided,) = _parameters([bucket[::2]])
+    fma.clip_grads_with_norm_([strided], 1.0, bucket[4000])
+    _check_scaled([strided.grad], [before[::2]], 2.0, 1.0)
+    bucket.copy_(before)
+    parts = _parameters([bucket[:4000], bucket[4001:]])
+    fma.clip_grads_with_norm_(parts, 1.0, bucket[4000])
+    _check_scaled([q.grad for q in parts], [before[:4000], before[4001:]], 2.0, 1.0)
+    assert bucket[4000] == 2.0
