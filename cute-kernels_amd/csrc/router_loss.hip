@@ -7,7 +7,6 @@
 // A token belongs to L neighbouring lanes, each of which holds NV neighbouring logits; L * NV is the first power of two from E on, so that
 // a wavefront takes 64 / L tokens at a time and a lane meets the same experts in every token: sums over tokens stay in its registers until
 // the workgroup ends. Partial sums go to a workspace and are joined in a fixed order in 64 bits: the same bits on every run.
-//
 #include "common.h"
 
 #include <type_traits>
@@ -357,10 +356,10 @@ struct Partial {
     double* term;  // what each workgroup of the join contributes to the balance
 };
 
-// Bound by vector instructions where there are many choices and logits: 131072 tokens of 256 experts, 8 choices, take 49 us (fp32, 2.7 TB/s; bf16 as
-// long), 35 instructions a logit that issue in 72 % of the cycles of two wavefronts per SIMD. Three of them (768 threads) gain 5 % there, 10 % with 16
-// choices, and lose 3 % with 160 or 161 experts, whose registers no longer suffice. With two
-// choices both kernels take 45 us, 56 with eight.
+// Bound by vector instructions where there are many choices and logits: 131072 tokens of 256 experts, 8 choices, take 46 to 49 us (fp32, 2.8 TB/s;
+// bf16 47 to 51), 35 instructions a logit (bf16 38) that issue in 70 % of the cycles of two wavefronts per SIMD. Three of them (768 threads) gain 5 %
+// there, 10 % with 16 choices, and lose 3 % with 160 or 161 experts, whose registers no longer suffice. With two choices this kernel and the join
+// take 46 us, with eight 59, with sixteen 79.
 template <typename T, int L, int NV, bool VEC>
 __global__ __launch_bounds__(fwd_threads(NV)) void router_loss_kernel(const T* __restrict__ logits, const uint8_t* __restrict__ mask, int64_t T_,
                                                                   int E, uint32_t k, Partial part) {
@@ -560,8 +559,9 @@ __global__ __launch_bounds__(kWave) void router_loss_finish_kernel(Partial part,
     table[E] = (float)inv_n;
 }
 
-// One pass over logits and gradient, the softmax formed again. HBM-bound from some megabytes on: 131072 tokens of 256 experts in fp32 53 us, 5.0 TB/s;
-// 32768 of 128 in bf16 6.9 us, of which a launch is 5.
+// One pass over logits and gradient, the softmax formed again. HBM-bound from some megabytes on: 131072 tokens of 256 experts in fp32 take 53 us, 5.0
+// TB/s, with logits from memory, and 43 behind a forward pass that left part of them in the last-level cache; in bf16 29 us, 4.6 TB/s, where vector
+// instructions come near the bound as well (26 a logit); 32768 of 128 in bf16 take 7 us, of which a launch is 5.
 template <typename T, int L, int NV, bool VEC>
 __global__ __launch_bounds__(kBwdThreads) void router_loss_bwd_kernel(const T* __restrict__ logits, const uint8_t* __restrict__ mask, int64_t T_,
                                                                       int E, const float* __restrict__ table,
@@ -633,7 +633,7 @@ int64_t compute_units() { return num_compute_units() > 0 ? num_compute_units() :
 
 // Logits per lane: 16 where eight would take more than a wavefront, and in the forward pass from 33 on, whose sorting and sums then need one step
 // less between lanes (8 choices, both kernels of the forward pass, us against eight a lane: 131072 tokens of 256 experts, fp32 57 / 69; of 128, bf16
-// 33 / 35; of 64, fp32 20 / 21. The backward pass of the first: 64 / 53, of 65536 of 160, fp16, 13 / 15).
+// 33 / 35; of 64, fp32 20 / 21. The backward pass of the first, its logits from memory: 64 / 53, of 65536 of 160, fp16, 13 / 15).
 int values_per_lane(int64_t E, bool forward) { return E > (forward ? 32 : 512) ? 16 : 8; }
 int lanes_per_token(int64_t E, bool forward) {
     int L = 1;

@@ -22,8 +22,10 @@ namespace {
 
 constexpr int kThreads = 256;
 constexpr int kWaves = kThreads / kWave;
-// Threads of the forward pass per compute unit, each with its share of a row and of the next one. us with 512 to 1024 / 2048, bf16:
-// [16384, 4096] 87 / 94, [16384, 2048] 48 / 56, [8188, 2880] with a full gate 41 / 52; a workgroup per row, which ends with it, 110, 60 and 63.
+// Threads of the forward pass per compute unit, each with its share of a row and of the next one. us with 512 / 1024 / 2048, inputs from memory, bf16:
+// [16384, 4096] 116 / 89 / 99, [16384, 2048] 51 / 51 / 51, [8188, 2880] with a full gate 57 / 41 / 45; fp32 [16384, 4096] - / 195 / 186, the least of 27
+// launches 181 / 182. Within a training step, which leaves part of a row's tensors in the last-level cache, the first is 96 / 98 (the least 86 / 96) with
+// 1024 / 2048, the third 41 / 45. A workgroup per row, which ends with it, took 110, 60 and 63.
 constexpr int kFwdThreadsPerCU = 1024;
 // teams of a workgroup: those of one wavefront meet at no barrier, four of them make a workgroup
 constexpr int teams_of(int team) { return team == kWave ? 4 : 1; }
@@ -416,8 +418,8 @@ __device__ __forceinline__ int64_t team_index() {
     else return (int64_t)blockIdx.x * teams_of(TEAM) + __builtin_amdgcn_readfirstlane((int)(threadIdx.x / TEAM));
 }
 
-// HBM-bound, each tensor touched once: bf16 [16384, 4096] 88 us, 6.1 TB/s, [8188, 2880] with a full gate 41 us, 5.8, [4096, 16384] 90 us, 6.0,
-// [32768, 512] 26 us, 5.2; [16384, 1031] element by element 106 us, 1.3.
+// HBM-bound, each tensor touched once: bf16 [16384, 4096] 89 us, 6.0 TB/s (86 to 96 in a training step), [8188, 2880] with a full gate 41 us, 5.7,
+// [4096, 16384] 90 us, 6.0, [32768, 512] 26 us, 5.2; fp32 [16384, 4096] 195 us, 5.5; bf16 [16384, 1031] element by element 106 us, 1.3.
 template <typename T, bool ELEM, int TEAM, int VPT, Mode MODE>
 __global__ __launch_bounds__(TEAM * teams_of(TEAM)) void sandwich_fwd_kernel(const FwdArgs<T> k) {
     constexpr int N = Wide<T>::N;
@@ -486,8 +488,9 @@ __global__ __launch_bounds__(TEAM * teams_of(TEAM)) void sandwich_fwd_kernel(con
     }
 }
 
-// HBM-bound as well; with the sums over rows, bf16 [16384, 4096] 135 us, 6.0 TB/s, [8188, 2880] with a full gate 71 us, 5.3, [4096, 16384] 160 us, 5.0
-// (rows of more than 1024 vectors have no next row on the way and form r^ three times), [32768, 512] 41 us, 4.9; [16384, 1031] 159 us, 1.3.
+// HBM-bound as well; with the sums over rows, bf16 [16384, 4096] 135 us, 6.0 TB/s, [8188, 2880] with a full gate 71 us, 5.3, [4096, 16384] 160 us,
+// 5.0 (rows of more than 1024 vectors have no next row on the way and form r^ three times), [32768, 512] 41 us, 4.9; fp32 [16384, 4096] 274 us,
+// 5.9; bf16 [16384, 1031] element by element 159 us, 1.3.
 template <typename T, bool ELEM, int TEAM, int VPT, Mode MODE>
 __global__ __launch_bounds__(TEAM * teams_of(TEAM)) void sandwich_bwd_kernel(const BwdArgs<T> k) {
     constexpr int N = Wide<T>::N, kTeams = teams_of(TEAM);
@@ -896,10 +899,10 @@ int forward(const void* x, const void* residual, const void* post_weight, const 
 }
 
 template <typename T>
-int backward(const void* x, const void* stream, const void* post_weight, const void* weight, const void* gate, const void* d_out,
+int backward(const void* x, const void* residual, const void* post_weight, const void* weight, const void* gate, const void* d_out,
              const void* d_stream, const float* stats, void* dx, void* d_residual, void* d_gate, void* d_post_weight, void* d_weight,
              const Shape& s, float a, void* workspace, hipStream_t st) {
-    const BwdArgs<T> k{(const T*)x, (const T*)stream, (const T*)post_weight, (const T*)weight, (const T*)gate, (const T*)d_out, (const T*)d_stream,
+    const BwdArgs<T> k{(const T*)x, (const T*)residual, (const T*)post_weight, (const T*)weight, (const T*)gate, (const T*)d_out, (const T*)d_stream,
                        stats, (T*)dx, (T*)d_residual, (T*)d_gate, Partial{}, s, Split{}, 1.0f / (float)s.H, a, d_weight != nullptr,
                        d_post_weight != nullptr || (s.mode == kChannel && d_gate)};
     return launch_bwd<T>(k, (T*)d_weight, (T*)d_post_weight, workspace, st);

@@ -1,5 +1,5 @@
-"""Calls of fma_grad_norm, fma_scale_grads (and its form for 64-bit norms) and fma_clip_grad_norm of libfma_hip.so. They take lists of tensors that may be a few hundred, and
-are no operators of the dispatcher, which would look at each of them twice more."""
+"""Calls of fma_grad_norm, fma_scale_grads (and its form for 64-bit norms) and fma_clip_grad_norm of libfma_hip.so. They take lists of tensors
+that may be a few hundred, and are no operators of the dispatcher, which would look at each of them twice more."""
 
 from array import array
 
@@ -86,7 +86,7 @@ def scale_grads_cuda(grads: list[torch.Tensor], max_norm: float, norm: torch.Ten
         return
     table, lib = _Table(grads, True), _lib.load()
     assert norm.numel() == 1, "total_norm should be a scalar"
-    # (every type but float32 as 64 bits, which hold it)
+    # (a norm of any other type than float32 goes as 64 bits)
     dtype, scale = (torch.float32, lib.fma_scale_grads) if norm.dtype is torch.float32 else (torch.float64, lib.fma_scale_grads_norm64)
     norm = norm.to(device=table.device, dtype=dtype)
     with _lib.on_device(table.device):

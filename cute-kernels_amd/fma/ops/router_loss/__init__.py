@@ -46,7 +46,8 @@ def router_loss(
     With p = softmax(logits) per token, f_e the share of all choices that fall on expert e (a token chooses its num_experts_per_tok largest
     logits, the lowest expert first among equal ones) and P_e the mean of p_e over the tokens, the balance loss is E sum_e f_e P_e: 1 if both
     are even. The z loss is the mean of logsumexp(logits)^2. Both are float32 scalars, computed in float32 with sums over tokens joined in
-    64 bits, and have gradients by the logits (f counts as a constant; no second derivatives). The tokens per expert are uint32 [E].
+    64 bits, and have gradients by the logits (f counts as a constant; no second derivatives). The tokens per expert are uint32 [E]. A token that
+    counts and has no finite softmax (a NaN, +infinity, or nothing but -infinity) makes both losses NaN, and its own gradients.
 
     mask: bool, one entry per token, False for tokens that do not count (padding): their logits are not looked at, whatever they are, and
     have gradient 0. Its shape is that of the logits without E; to logits [T, E] also any other of T entries, such as [batch, sequence] with

@@ -507,7 +507,8 @@ int fma_swiglu_experts_fp8_bwd(const void* dy, const void* gates, const void* id
  * p_t = softmax(logits_t), N tokens counted and c_e those among whose top_k largest logits expert e is (equal logits: the lowest expert
  * first, NaN above everything):
  *   balance = E / (top_k N^2) sum_e c_e sum_t p_te,   z = 1 / N sum_t logsumexp(logits_t)^2,   counts[e] = c_e
- * balance, z: one float; counts: E uint32; table: E + 1 floats for the backward call. Without tokens all are 0. T < 2^31, E <= FMA_MAX_GROUPS.
+ * balance, z: one float; counts: E uint32; table: E + 1 floats for the backward call. Without tokens all are 0. A counted token without a finite
+ * softmax (NaN, +infinity, nothing but -infinity) makes both losses and its gradients NaN. T < 2^31, E <= FMA_MAX_GROUPS.
  * workspace: 8-byte aligned, no initialisation. Sums over tokens have a fixed order. No counterpart in the reference.
  * Backward: logits_grad [T, E] (0 in rows that are not counted) for the gradients *balance_grad and *z_grad (device; NULL: 0). */
 int64_t fma_router_loss_workspace_bytes(int64_t T, int64_t E);
@@ -523,8 +524,9 @@ int fma_router_loss_bwd(const void* logits, const uint8_t* mask, int64_t T, int6
  * gate_width H or 1 and gate_rows a divisor of B: row i serves the B / gate_rows rows of x from i * B / gate_rows on. stats: 2 * B floats for
  * the backward call (1 / rms of x, then of the stream) or NULL. fp32 arithmetic, one rounding each; out is formed from the unrounded stream.
  * B < 2^31, H <= FMA_MAX_NORM_HIDDEN. No counterpart in the reference (its fused_residual_add_rmsnorm is the case without the first norm).
- * Backward (B > 0), from the forward call's inputs and stats (the stream is formed again, unrounded): out_grad and stream_grad may each be NULL (zero); gate_grad, post_weight_grad and weight_grad, shaped and typed like what
- * they belong to, are computed unless NULL. workspace: 16-byte aligned, no initialisation. Sums over rows have a fixed order. */
+ * Backward (B > 0), from the forward call's inputs and stats (the stream is formed again, unrounded): out_grad and stream_grad may each be
+ * NULL (zero); gate_grad, post_weight_grad and weight_grad, shaped and typed like what they belong to, are computed unless NULL.
+ * workspace: 16-byte aligned, no initialisation. Sums over rows have a fixed order. */
 int fma_sandwich_rmsnorm_fwd(const void* x, const void* residual, const void* post_weight, const void* weight, const void* gate,
                              int64_t gate_rows, int64_t gate_width, void* out, void* stream_out, float* stats, int64_t B, int64_t H, float eps,
                              float multiplier, int dtype, void* stream);
@@ -546,8 +548,8 @@ int fma_grad_norm(void* const* tensors, const int64_t* sizes, const int32_t* dty
                   void* workspace, int64_t workspace_bytes, void* stream);
 /* Every element times min(1, max_norm / (*norm + 1e-6)); with a factor of one nothing is touched. The factor is formed in 64 bits, its digits
  * and the product are rounded to float32 (below float32's normal numbers too, the factor keeps all its digits), the product then to the
- * tensor's type. The tensors must not overlap, neither each other nor the norm. fma_scale_grads_norm64 is the same by a norm in 64 bits (8-byte aligned), and
- * fma_clip_grad_norm fma_grad_norm and this with the norm as it is in 64 bits. */
+ * tensor's type. The tensors must overlap neither each other nor the norm. fma_scale_grads_norm64 is the same by a norm in 64 bits (8-byte
+ * aligned), and fma_clip_grad_norm fma_grad_norm and this with the norm as it is in 64 bits. */
 int fma_scale_grads(void* const* tensors, const int64_t* sizes, const int32_t* dtypes, int64_t count, const float* norm, double max_norm,
                     void* stream);
 int fma_scale_grads_norm64(void* const* tensors, const int64_t* sizes, const int32_t* dtypes, int64_t count, const double* norm,
